@@ -8,6 +8,8 @@ GPU decode:        interleaved_rans_decode, InterleavedRANSDecoder,
                    CudaInterleavedRANS, DeviceMatrix.decode
 Fused GEMV:        DeviceMatrix.gemv, entropy_coded_matmul, EntropyCodedLinear
 Plain 4-bit:       Packed4Matrix (the CACHED store and the HBM-bound control)
+4-bit KV cache:    KV4Cache, kv4_extend / kv4_release (block tables and slot
+                   maps), kv4_append / kv4_gather, kv4_attention
 """
 from .codec import (EncodedMatrix, InterleavedEncodedTile, InterleavedRANSEncoder, RANSTable,  # noqa: F401
                     encode_matrix, interleaved_rans_encode, pack_reference_tiles, choose_tile_cols)
@@ -32,4 +34,8 @@ def __getattr__(name):
     if name in ("SmartDecoder", "DecodeMode", "DecodedWeights"):
         from . import strategies
         return getattr(strategies, name)
+    if name in ("KV4Cache", "KV4Step", "kv4_pages", "kv4_extend", "kv4_release", "kv4_append", "kv4_gather",
+                "kv4_attention"):
+        from . import kv4
+        return getattr(kv4, name)
     raise AttributeError(name)

@@ -27,6 +27,7 @@ ERRORS = {
 STATUS_CORRUPT = 1
 STATUS_TIMEOUT = 2
 STATUS_BADARG = 4
+STATUS_NO_PAGES = 8
 FLAG_CONSTANT = 1
 TILE_ROWS = 8
 NOALLOC_SCRATCH_BYTES = 4 << 20
@@ -69,6 +70,13 @@ EXPORTS = (
     "ecq_decode_attention_workspace_bytes",
     "ecq_decode_attention_splits",
     "ecq_decode_attention_f16",
+    "ecq_kv4_page_bytes",
+    "ecq_kv4_extend",
+    "ecq_kv4_release",
+    "ecq_kv4_append",
+    "ecq_kv4_gather",
+    "ecq_kv4_attention_workspace_bytes",
+    "ecq_kv4_attention",
 )
 
 
@@ -151,6 +159,17 @@ def _declare(L: ctypes.CDLL) -> None:
         "ecq_decode_attention_workspace_bytes": (c_int64, [c_int32, c_int32]),
         "ecq_decode_attention_splits": (c_int32, [c_int32, c_int32]),
         "ecq_decode_attention_f16": (c_int32, [P, P, P, P, c_int32, c_int32, c_int32, c_int64, c_int32, P, c_int64, P]),
+        "ecq_kv4_page_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+        "ecq_kv4_extend": (c_int32, [P, P, P, P, c_int64, c_int32, c_int32, c_int32, P, c_int32, P, P, P, P, P, c_int32,
+                                     P, P]),
+        "ecq_kv4_release": (c_int32, [P, P, P, P, c_int64, c_int32, c_int32, c_int32, P, c_int32, P, P, P, P]),
+        "ecq_kv4_append": (c_int32, [P, c_int64, c_int64, P, c_int64, c_int64, c_int32, P, c_int64, c_int32, c_int32,
+                                     c_int32, c_int32, P, c_int32, P, P]),
+        "ecq_kv4_gather": (c_int32, [P, P, c_int32, P, c_int64, c_int32, c_int32, c_int32, c_int32, P, c_int32, P, P]),
+        "ecq_kv4_attention_workspace_bytes": (c_int64, [c_int32] * 7),
+        "ecq_kv4_attention": (c_int32, [P, c_int64, c_int64, P, c_int64, c_int64, c_int32, P, c_int64, c_int32, c_int32,
+                                        c_int32, c_int32, c_int32, P, c_int64, c_int32, P, P, c_int32, c_int32, c_int32,
+                                        ctypes.c_float, P, c_int64, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -1,0 +1,321 @@
+"""A paged KV cache held in 4 bits, for serving many requests: block tables and
+slot maps built on the GPU, K and V rows stored and read back, and attention
+over the cache (include/ecq_kv4.h has the pool's layout).
+
+One serving step of a layer stack::
+
+    step = cache.extend(new_lens, max_tokens)      # once: pages, slots, positions
+    for layer in ...:                              # k, v, q of the step's tokens
+        cache.append(layer, k, v, step.slots)
+        o = cache.attention(layer, q, step.q_starts, max_q)
+    cache.release(done)                            # pages of finished requests
+
+``KV4Cache`` holds the tensors; the ``kv4_*`` functions under it take plain
+tensors. Calls run on the current stream of the tensors' device, allocate only
+their results and workspaces (from torch's allocator, so they can be captured
+into CUDA graphs) and do not synchronise. Bad values that only the device sees
+set bits of the ``status`` word.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from ._lib import EcqError, check, lib
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_stream = torch.cuda.current_stream
+
+
+class KV4Step(NamedTuple):
+    """What ``kv4_extend`` returns (int32 tensors)."""
+
+    seq_lens: torch.Tensor    # [batch] lengths with the new tokens
+    q_starts: torch.Tensor    # [batch + 1] first new token of each request, then their number
+    slots: torch.Tensor       # [max_tokens] slot of each new token, -1 behind the last
+    positions: torch.Tensor   # [max_tokens] position of each new token in its request, -1 behind the last
+    free_count: torch.Tensor  # [1] pages left on the free stack
+
+
+def _same_device(first: torch.Tensor, **others) -> None:
+    if not first.is_cuda:
+        raise ValueError("the 4-bit KV cache runs on CUDA tensors only")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+
+
+def _int32(name: str, t: torch.Tensor, shape=None) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+
+
+def _table(block_table: torch.Tensor, batch: int) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError(f"block_table must be int32 [{batch}, pages per request]")
+    if block_table.shape[1] < 1 or block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table needs contiguous rows of at least one page")
+
+
+def _status(status) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise ValueError("status must be int32 [1]")
+    return status.data_ptr()
+
+
+def _page_size(pages: torch.Tensor, head_dim: int, group_size: int) -> int:
+    """The tokens per page of a pool, from its shape."""
+    if pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous():
+        raise ValueError("pages must be contiguous uint8 [pages, kv_heads, page bytes]")
+    block = check(lib().ecq_kv4_page_bytes(head_dim, 16, group_size), f"head_dim {head_dim}, group_size {group_size}")
+    size, rest = divmod(pages.shape[2], block)
+    if rest or size not in (1, 2, 4, 8, 16):
+        raise ValueError(f"pages of {pages.shape[2]} bytes do not hold 16, 32, 64, 128 or 256 tokens of {block // 16} bytes")
+    return 16 * size
+
+
+def _rows(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 3 or t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, head_dim]")
+    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        raise ValueError(f"{name}: head_dim must be contiguous, rows 16-byte aligned")
+
+
+def kv4_pages(n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, group_size: int = 64,
+              device="cuda") -> torch.Tensor:
+    """An empty pool: uint8 [n_pages, kv_heads, page bytes]."""
+    per = check(lib().ecq_kv4_page_bytes(head_dim, page_size, group_size),
+                f"head_dim {head_dim}, page_size {page_size}, group_size {group_size}")
+    if n_pages < 1 or kv_heads < 1 or n_pages * page_size >= 1 << 31:
+        raise ValueError("a pool has at least one page and head, and fewer than 2^31 slots")
+    return torch.zeros(n_pages, kv_heads, per, dtype=torch.uint8, device=device)
+
+
+def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               free_count: torch.Tensor, page_size: int, max_tokens: int, *, seq_lens_out: torch.Tensor | None = None,
+               free_count_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> KV4Step:
+    """The bookkeeping of a step on the GPU: request b grows from seq_lens[b]
+    by new_lens[b] tokens (int32 [batch]). Pages that it did not have yet are
+    popped off the end of free_pages[:free_count] into its row of block_table
+    (in place); lengths and count come back as new tensors, or in
+    ``seq_lens_out`` / ``free_count_out``, which may be the inputs. At most
+    ``max_tokens`` new tokens: ``slots`` and ``positions`` have that length,
+    filled with -1 behind the last, so a captured step keeps its shapes. All
+    or nothing: if pages, room or lengths do not suffice nothing changes, every
+    slot is -1 and ``status`` says so."""
+    _same_device(seq_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count,
+                 seq_lens_out=seq_lens_out, free_count_out=free_count_out, status=status)
+    batch = seq_lens.numel()
+    _int32("seq_lens", seq_lens, (batch,))
+    _int32("new_lens", new_lens, (batch,))
+    _int32("free_pages", free_pages, (free_pages.numel(),))
+    _int32("free_count", free_count, (1,))
+    _table(block_table, batch)
+    if max_tokens < 0:
+        raise ValueError("max_tokens is negative")
+    lens_out = torch.empty_like(seq_lens) if seq_lens_out is None else seq_lens_out
+    count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
+    _int32("seq_lens_out", lens_out, (batch,))
+    _int32("free_count_out", count_out, (1,))
+    out = torch.empty(batch + 1 + 2 * max_tokens, dtype=torch.int32, device=seq_lens.device)
+    starts, slots, positions = out[:batch + 1], out[batch + 1:batch + 1 + max_tokens], out[batch + 1 + max_tokens:]
+    with torch.cuda.device(seq_lens.device):
+        check(lib().ecq_kv4_extend(seq_lens.data_ptr(), new_lens.data_ptr(), lens_out.data_ptr(),
+                                   block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, page_size,
+                                   free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                                   count_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                                   max_tokens, _status(status), _stream().cuda_stream), "kv4_extend")
+    return KV4Step(lens_out, starts, slots, positions, count_out)
+
+
+def kv4_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                free_count: torch.Tensor, page_size: int, *, seq_lens_out: torch.Tensor | None = None,
+                free_count_out: torch.Tensor | None = None,
+                status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Push the pages of the requests where ``done`` (bool [batch]) on
+    free_pages (in place) and set their lengths to 0. Returns the lengths and
+    the count of free pages, as new tensors or in the ``_out`` ones."""
+    _same_device(seq_lens, done=done, block_table=block_table, free_pages=free_pages, free_count=free_count,
+                 seq_lens_out=seq_lens_out, free_count_out=free_count_out, status=status)
+    batch = seq_lens.numel()
+    _int32("seq_lens", seq_lens, (batch,))
+    if done.dtype not in (torch.bool, torch.uint8) or tuple(done.shape) != (batch,) or not done.is_contiguous():
+        raise ValueError(f"done must be contiguous bool [{batch}]")
+    _int32("free_pages", free_pages, (free_pages.numel(),))
+    _int32("free_count", free_count, (1,))
+    _table(block_table, batch)
+    lens_out = torch.empty_like(seq_lens) if seq_lens_out is None else seq_lens_out
+    count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
+    _int32("seq_lens_out", lens_out, (batch,))
+    _int32("free_count_out", count_out, (1,))
+    with torch.cuda.device(seq_lens.device):
+        check(lib().ecq_kv4_release(done.data_ptr(), seq_lens.data_ptr(), lens_out.data_ptr(), block_table.data_ptr(),
+                                    block_table.stride(0), block_table.shape[1], batch, page_size,
+                                    free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                                    count_out.data_ptr(), _status(status), _stream().cuda_stream), "kv4_release")
+    return lens_out, count_out
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, *, group_size: int = 64,
+               status: torch.Tensor | None = None) -> None:
+    """Store rows k, v [tokens, kv_heads, head_dim] (float16 or bfloat16, any
+    strides with contiguous 16-byte aligned rows) in 4 bits at slots [tokens]
+    (int32, distinct; negative: not stored). slots may be longer than k, as a
+    padded step's are: the rest is not looked at."""
+    _rows("k", k)
+    _rows("v", v)
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v must have one shape and type")
+    _same_device(k, v=v, pages=pages, slots=slots, status=status)
+    tokens, heads, dim = k.shape
+    page_size = _page_size(pages, dim, group_size)
+    if pages.shape[1] != heads:
+        raise ValueError(f"k has {heads} heads, the pool {pages.shape[1]}")
+    _int32("slots", slots)
+    if slots.dim() != 1 or slots.numel() < tokens:
+        raise ValueError(f"slots must have at least {tokens} entries")
+    with torch.cuda.device(k.device):
+        check(lib().ecq_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                   _DTYPES[k.dtype], pages.data_ptr(), pages.shape[0], heads, dim, page_size,
+                                   group_size, slots.data_ptr(), tokens, _status(status), _stream().cuda_stream),
+              "kv4_append")
+
+
+def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, *, group_size: int = 64,
+               dtype: torch.dtype = torch.float16,
+               status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows at slots [n] (int32) as k, v [n, kv_heads, head_dim] of dtype:
+    code * scale + zero, rounded once; zeros for negative slots."""
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be float16 or bfloat16")
+    _same_device(pages, slots=slots, status=status)
+    page_size = _page_size(pages, head_dim, group_size)
+    _int32("slots", slots)
+    n = slots.numel()
+    k = torch.empty(n, pages.shape[1], head_dim, dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    with torch.cuda.device(pages.device):
+        check(lib().ecq_kv4_gather(k.data_ptr(), v.data_ptr(), _DTYPES[dtype], pages.data_ptr(), pages.shape[0],
+                                   pages.shape[1], head_dim, page_size, group_size, slots.data_ptr(), n,
+                                   _status(status), _stream().cuda_stream), "kv4_gather")
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  q_starts: torch.Tensor | None = None, max_q: int = 1, *, group_size: int = 64,
+                  scale: float | None = None, out: torch.Tensor | None = None,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q . k * scale) v over the cache, for new tokens whose rows are in
+    it already (``kv4_append`` before it).
+
+    q [tokens, heads, head_dim] (float16 or bfloat16; heads a multiple of the
+    pool's), seq_lens int32 [batch] with the new tokens counted, block_table
+    int32 [batch, pages]. q_starts int32 [batch + 1] says which tokens are
+    whose, at most max_q for one request; None: one each. They are the last of
+    their request, each sees the tokens up to its own. scale: 1 / sqrt(head_dim)
+    by default. Rows that see nothing (length 0) are 0; rows at or behind
+    q_starts[-1] are left as they were in ``out``."""
+    _rows("q", q)
+    _same_device(q, pages=pages, block_table=block_table, seq_lens=seq_lens, q_starts=q_starts, out=out, status=status)
+    tokens, heads, dim = q.shape
+    page_size = _page_size(pages, dim, group_size)
+    kv_heads = pages.shape[1]
+    if heads % kv_heads or heads < kv_heads:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} cache heads evenly")
+    batch = seq_lens.numel()
+    _int32("seq_lens", seq_lens, (batch,))
+    _table(block_table, batch)
+    if q_starts is not None:
+        _int32("q_starts", q_starts, (batch + 1,))
+    elif tokens != batch or max_q != 1:
+        raise ValueError("without q_starts every request has one query")
+    if max_q < 1:
+        raise ValueError("max_q must be at least 1")
+    if out is None:
+        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and type")
+    elif out.numel() and (out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8):
+        raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
+    L = lib()
+    need = check(L.ecq_kv4_attention_workspace_bytes(batch, heads, kv_heads, dim, max_q, block_table.shape[1], page_size),
+                 "kv4_attention")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    with torch.cuda.device(q.device):
+        check(L.ecq_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                  _DTYPES[q.dtype], pages.data_ptr(), pages.shape[0], heads, kv_heads, dim, page_size,
+                                  group_size, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                                  seq_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), batch, tokens,
+                                  max_q, dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _status(status),
+                                  _stream().cuda_stream), "kv4_attention")
+    return out
+
+
+class KV4Cache:
+    """The 4-bit KV cache of a layer stack: one pool per layer, and one block
+    table, length vector and free stack for all of them."""
+
+    def __init__(self, layers: int, n_pages: int, kv_heads: int, head_dim: int, max_batch: int, max_len: int,
+                 page_size: int = 64, group_size: int = 64, device="cuda"):
+        self.head_dim, self.page_size, self.group_size = head_dim, page_size, group_size
+        self.pages = [kv4_pages(n_pages, kv_heads, head_dim, page_size, group_size, device) for _ in range(layers)]
+        dev = self.pages[0].device
+        if not 1 <= max_batch <= 8192 or max_len < 1:
+            raise ValueError("a cache holds 1 to 8192 requests of at least one token")
+        self.max_len = max_len
+        self.seq_lens = torch.zeros(max_batch, dtype=torch.int32, device=dev)
+        self.block_table = torch.full((max_batch, -(-max_len // page_size)), -1, dtype=torch.int32, device=dev)
+        # popped from the end: page 0 goes first
+        self.free_pages = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.free_count = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of all layers' pools."""
+        return sum(p.numel() for p in self.pages)
+
+    def extend(self, new_lens: torch.Tensor, max_tokens: int) -> KV4Step:
+        """``kv4_extend`` of the cache's requests, lengths and count in place."""
+        return kv4_extend(self.seq_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size,
+                          max_tokens, seq_lens_out=self.seq_lens, free_count_out=self.free_count, status=self.status)
+
+    def release(self, done: torch.Tensor) -> None:
+        """``kv4_release`` of the requests where ``done`` (bool [max_batch])."""
+        kv4_release(done, self.seq_lens, self.block_table, self.free_pages, self.free_count, self.page_size,
+                    seq_lens_out=self.seq_lens, free_count_out=self.free_count, status=self.status)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """``kv4_append`` into a layer's pool."""
+        kv4_append(k, v, self.pages[layer], slots, group_size=self.group_size, status=self.status)
+
+    def gather(self, layer: int, slots: torch.Tensor,
+               dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+        """``kv4_gather`` from a layer's pool."""
+        return kv4_gather(self.pages[layer], slots, self.head_dim, group_size=self.group_size, dtype=dtype,
+                          status=self.status)
+
+    def attention(self, layer: int, q: torch.Tensor, q_starts: torch.Tensor | None = None, max_q: int = 1,
+                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``kv4_attention`` over a layer's pool."""
+        return kv4_attention(q, self.pages[layer], self.block_table, self.seq_lens, q_starts, max_q,
+                             group_size=self.group_size, scale=scale, out=out, status=self.status)
+
+    def check(self) -> None:
+        """Synchronise and raise if a call found bad values or too few pages."""
+        s = int(self.status.item())
+        if s:
+            self.status.zero_()
+            what = [w for bit, w in ((_lib.STATUS_NO_PAGES, "the free pages did not suffice"),
+                                     (_lib.STATUS_BADARG, "a length, slot or page number is out of range"),
+                                     (_lib.STATUS_TIMEOUT, "a bounded wait gave up")) if s & bit]
+            raise EcqError("4-bit KV cache: " + ", ".join(what or [f"status {s}"]))
+
+
+__all__ = ["KV4Cache", "KV4Step", "kv4_pages", "kv4_extend", "kv4_release", "kv4_append", "kv4_gather", "kv4_attention"]
