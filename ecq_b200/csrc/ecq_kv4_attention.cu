@@ -1,6 +1,33 @@
-// ecq_kv4_attention.cu -- attention over the 4-bit KV cache. One CTA per query
-// token and head; its warps take every 4th key, each with a running maximum
-// and sum, and are joined in shared memory.
+// ecq_kv4_attention.cu -- attention of a few query rows over the 4-bit KV
+// cache (ecq_kv4.h has the layout).
+//
+// Mathematics. With codes c, scales s and zeros z per group G of channels,
+//   q . k_j = sum_G s_jG (sum_{d in G} q_d c_jd) + z_jG (sum_{d in G} q_d)
+//   o_d     = sum_j (p_j s_jG) c_jd + sum_j p_j z_jG
+// so the codes go to the tensor cores as they are: a nibble in the low bits of
+// an fp16 is the subnormal c 2^-24, exact, and one in the next four bits is
+// c 2^-20; an AND (and a shift by 8 for half of them) makes two operands, where
+// scaling every channel would cost a conversion and an fma each. Scales and
+// zeros come in per token and group, in fp32. The products are
+//   S^T[16 tokens x 8 rows] = K codes x q^T   and   o^T[16 d x 8 rows] = V codes^T x (p s)
+// with query rows (tokens x heads that share a cache head) as the narrow side:
+// mma.sync m16n8k16 holds 8 rows of keys' work at full use, where a tcgen05
+// tile would be 64 or 128 rows, of which a decode step has 1 to 8.
+// p s is fp16 twice (value and remainder: 22 bits), so V's side keeps fp32
+// accuracy; q is scaled to its row's largest power of two and exact in fp16.
+//
+// What bounds it: the cache's bytes for long contexts; below that the ~250
+// instructions per 16 tokens and head, and for short ones launches and merges.
+//
+// Layout of the work. The (request, cache head, row tile, 16-token block) space
+// is flattened and cut into one even range per CTA (one wave of CTAs), from the
+// lengths on the device, so ragged batches balance and no host knows them.
+// Within a range block f belongs to warp f % kWarps. Each warp streams its
+// blocks through a ring of its own with cp.async.bulk, one copy per block, and
+// keeps its own running maximum and sum; at the end of a (request, head, tile)
+// the CTA joins its warps in shared memory. Where a range's end cuts one, its
+// parts go to the workspace and a second kernel joins them in order, so results
+// do not depend on timing.
 #include <cuda_runtime.h>
 
 #include "ecq_kv4.cuh"
@@ -11,98 +38,645 @@ using namespace ecq_kv4;
 using ecq_dev::launch_pdl;
 using ecq_dev::pdl_launch_dependents;
 using ecq_dev::pdl_wait;
+using ecq_dev::smem_addr;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+// 16-row tiles need the registers of two 8-row ones
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 2 : 1; }
+// Weights are exp2(score - reference); the reference is raised when a score
+// passes it by more than this, so weights are at most 4 and weight * scale
+// (at most 4 * 131008 / 15) is finite in fp16. Few blocks raise it, and the
+// others need no reduction over the block's tokens.
+constexpr float kSlack = 2.f;
+constexpr float kNoMax = -1e30f;
 
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__host__ __device__ constexpr int ring_slots(int dim, int groups) {
+    const int room = 110 * 1024 - kWarps * 8 * (dim + 4) * 4;
+    const int n = room / (kWarps * block_bytes(dim, groups));
+    return n < 6 ? n : 6;
+}
+
+struct Args {
+    const void* q;
+    void* out;
+    const uint8_t* pages;
+    const int32_t *table, *lens, *starts;
+    float* parts;     // per CTA two parts: one that starts inside a pair, one that starts a pair and does not end it
+    int4* cuts;       // per CTA: request, pair, CTAs that follow; x < 0: none
+    int32_t* status;
+    int64_t q_token, q_head, o_token, o_head, n_pages, table_stride;
+    int kv_heads, share, page_shift, max_pages, batch, total_q;
+    float scale;
+};
+
+// One request's part of the work.
+struct Request {
+    int first_q, rows, len, blocks, tiles, pairs;
+};
+
+template <int TR>  // rows per tile
+__device__ __forceinline__ Request request(const Args& a, int b) {
+    Request r;
+    int lo = b, hi = b + 1;
+    if (a.starts) {
+        lo = a.starts[b];
+        hi = a.starts[b + 1];
+        if (lo < 0 || hi < lo || hi > a.total_q) {
+            raise_status(a.status, ECQ_STATUS_BADARG);
+            lo = hi = 0;
+        }
+    }
+    r.len = a.lens[b];
+    const long long room = static_cast<long long>(a.max_pages) << a.page_shift;
+    if (r.len > room) {
+        raise_status(a.status, ECQ_STATUS_BADARG);
+        r.len = static_cast<int>(room);
+    }
+    r.len = max(r.len, 0);
+    r.first_q = lo;
+    r.rows = (hi - lo) * a.share;
+    r.tiles = (r.rows + TR - 1) / TR;
+    r.pairs = r.tiles * a.kv_heads;
+    // a request without keys has one (masked) block, so that its rows are written
+    r.blocks = r.rows ? max((r.len + kBlockTokens - 1) / kBlockTokens, 1) : 0;
+    return r;
+}
+
+__device__ __forceinline__ long long block_sum(long long v, long long* s) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v += s[w];
+    return v;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+template <int N>  // words
+__device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t addr) {
+    if constexpr (N == 4) {
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+    } else if constexpr (N == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    } else {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    }
+}
+
+__device__ __forceinline__ float2 cvt2(uint32_t u, __half) { return f2(u); }
+__device__ __forceinline__ float2 cvt2(uint32_t u, __nv_bfloat16) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
 __device__ __forceinline__ void store(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(kWarps * 32) attention_kernel(
-    const T* __restrict__ q, int64_t q_token, int64_t q_head, T* __restrict__ out, int64_t o_token, int64_t o_head,
-    const uint8_t* __restrict__ pages, int64_t n_pages, int kv_heads, int share, int page_shift,
-    const int32_t* __restrict__ table, int64_t table_stride, int max_pages, const int32_t* __restrict__ lens,
-    const int32_t* __restrict__ starts, int batch, float scale, int32_t* status) {
-    constexpr int E = D / 32;
-    __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][D];
+// The query rows of one tile as B operands, and what their scores need.
+template <int D, int G, int NT>
+struct Rows {
+    uint32_t b[NT][D / 16][2];
+    float sums[NT][G][2];  // of the lane's two columns, times 2^-24
+    float factor[NT][2];   // scale log2(e) 2^24 / the row's power of two
+    int limit[NT][2];      // keys that the column's row sees
+    int least;             // the smallest limit of rows that exist
+};
+
+template <typename T, int D, int G, int NT>
+__device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, const Request& rq, int head, int tile) {
+    const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
+    const int queries = rq.rows / a.share;
+    R.least = rq.len;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = (tile * NT + nt) * 8 + n;
+        const bool in = row < rq.rows;
+        const int i = row / a.share;
+        const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
+                       static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
+        float x[D / 32][8];
+        float top = 0.f;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (in) u = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = cvt2(us[e], T());
+                x[w][2 * e] = f.x;
+                x[w][2 * e + 1] = f.y;
+                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // rows are brought to [2^11, 2^12): elements down to 2^-25 of the largest, and a sixteenth of
+        // them, are normal or exact subnormal fp16
+        const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
+        const float up = __int_as_float((11 - ex + 127) << 23), down = __int_as_float((ex - 11 + 127) << 23);
+        float sums[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) sums[g] = 0.f;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[w][e] = __half2float(__float2half_rn(x[w][e] * up));
+                sums[w * 32 * G / D] += x[w][e];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                R.b[nt][2 * w + h][0] = h2(x[w][2 * h], x[w][4 + 2 * h]);
+                R.b[nt][2 * w + h][1] = h2(x[w][1 + 2 * h] * 0.0625f, x[w][5 + 2 * h] * 0.0625f);
+            }
+        }
+        const float factor = a.scale * 1.4426950408889634f * (down * 16777216.f);
+        // query i sees keys up to len - queries + i
+        const int limit = in ? rq.len - queries + i + 1 : rq.len;
+        int least = max(limit, 0);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+        R.least = min(R.least, least);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // column 2t + c is row 2t + c of the tile: lane 4 (2t + c) has it
+            const int from = 4 * (2 * t + c);
+            R.factor[nt][c] = __shfl_sync(0xffffffffu, factor, from);
+            R.limit[nt][c] = __shfl_sync(0xffffffffu, limit, from);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                R.sums[nt][g][c] = __shfl_sync(0xffffffffu, sums[g], from) * 5.9604644775390625e-8f;
+        }
+    }
+}
+
+// Running softmax of one warp over its blocks.
+template <int D, int G, int NT>
+struct State {
+    float o[NT][D / 16][4];
+    float zero[NT][G][2];
+    float m[NT][2], l[NT][2];
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[nt][c] = kNoMax;
+                l[nt][c] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) zero[nt][g][c] = 0.f;
+            }
+        }
+    }
+};
+
+// The block's token that row i (< 8) of the products stands for. Even rows are
+// tokens 0..3, odd ones 5, 4, 7, 6: neighbouring rows' K words, and the V words
+// that a lane's four quads take at once, lie in both halves of the banks.
+__device__ __forceinline__ int token_of(int i) { return (i & 1) ? 4 + ((i >> 1) ^ 1) : i >> 1; }
+
+// One block of 16 tokens at shared address blk; `first`: its first token.
+template <int D, int G, int NT, bool kMask>
+__device__ __forceinline__ void block(State<D, G, NT>& S, const Rows<D, G, NT>& R, uint32_t blk, int first, int len) {
+    constexpr int W = D / 32;
+    const int lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
+    const int tok = token_of(r);
+    uint32_t k0[W], k1[W], kp[2][G], vp[2][G];
+    lds<W>(k0, blk + tok * (D / 2) + t * (D / 8));
+    lds<W>(k1, blk + (tok + 8) * (D / 2) + t * (D / 8));
+    lds<G>(kp[0], blk + k_params_at(D) + tok * 4 * G);
+    lds<G>(kp[1], blk + k_params_at(D) + (tok + 8) * 4 * G);
+    lds<G>(vp[0], blk + v_params_at(D, G) + tok * 4 * G);
+    lds<G>(vp[1], blk + v_params_at(D, G) + (tok + 8) * 4 * G);
+    if (kMask) {  // tokens behind the request's last have never been written
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (first + tok + 8 * i >= len)
+#pragma unroll
+                for (int g = 0; g < G; ++g) kp[i][g] = vp[i][g] = 0;
+    }
+    uint32_t hi[NT][G][2], lo[NT][G][2];
+    {
+        float acc[NT][G][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[nt][g][c] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t x0 = h ? k0[w] >> 8 : k0[w], x1 = h ? k1[w] >> 8 : k1[w];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma(acc[nt][w * 32 * G / D], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u,
+                        x1 & 0x00f000f0u, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
+            }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 p = f2(kp[i][g]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        s[2 * i + c] = fmaf(p.x, acc[nt][g][2 * i + c], fmaf(p.y, R.sums[nt][g][c], s[2 * i + c]));
+                }
+            bool seen[4] = {true, true, true, true};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                s[c] *= R.factor[nt][c & 1];
+                if (kMask) {
+                    seen[c] = first + tok + 8 * (c >> 1) < R.limit[nt][c & 1];
+                    if (!seen[c]) s[c] = -INFINITY;
+                }
+            }
+            float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+            if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + kSlack || top[1] > S.m[nt][1] + kSlack)) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = fmaxf(top[c], S.m[nt][c]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    const float keep = exp2_fast(S.m[nt][c] - x);
+                    S.m[nt][c] = x;
+                    S.l[nt][c] *= keep;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) S.zero[nt][g][c] *= keep;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        S.o[nt][i][c] *= keep;
+                        S.o[nt][i][c + 2] *= keep;
+                    }
+                }
+            }
+            float p[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                p[c] = exp2_fast(s[c] - S.m[nt][c & 1]);
+                S.l[nt][c & 1] += p[c];
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 v = f2(vp[i][g]);
+                    float w[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float x = p[2 * i + c];
+                        // a key out of sight may hold anything: 0 times it would not do
+                        w[c] = kMask && !seen[2 * i + c] ? 0.f : x * v.x;
+                        S.zero[nt][g][c] += kMask && !seen[2 * i + c] ? 0.f : x * v.y;
+                    }
+                    const uint32_t u = h2(w[0], w[1]);
+                    const float2 back = f2(u);
+                    hi[nt][g][i] = transpose(u);
+                    lo[nt][g][i] = transpose(h2(w[0] - back.x, w[1] - back.y));
+                }
+        }
+    }
+    constexpr int VW = D / 64;  // words of a lane's chunk of a V row
+    uint32_t v[4][VW];
+    const int ta = token_of(2 * t), tb = token_of(2 * t + 1);
+    const uint32_t vc = blk + v_codes_at(D) + r * (D / 16);
+    lds<VW>(v[0], vc + ta * (D / 2));
+    lds<VW>(v[1], vc + tb * (D / 2));
+    lds<VW>(v[2], vc + (ta + 8) * (D / 2));
+    lds<VW>(v[3], vc + (tb + 8) * (D / 2));
+#pragma unroll
+    for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t pick = half ? 0x7632u : 0x5410u;
+            const uint32_t x = __byte_perm(v[0][w], v[1][w], pick), y = __byte_perm(v[2][w], v[3][w], pick);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int mt = 4 * w + 2 * half + j, g = mt * 16 * G / D;
+                const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
+                const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma(S.o[nt][mt], a0, a1, a2, a3, hi[nt][g][0], hi[nt][g][1]);
+                    mma(S.o[nt][mt], a0, a1, a2, a3, lo[nt][g][0], lo[nt][g][1]);
+                }
+            }
+        }
+}
+
+template <int D, int TR>
+__host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
+
+template <typename T, int D, int G, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a) {
+    constexpr int TR = 8 * NT, NS = ring_slots(D, G), BB = block_bytes(D, G), OS = D + 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long s_sum[kWarps];
+    __shared__ long long s_before;
+    __shared__ int s_request;
+    __shared__ uint64_t s_bar[kWarps][NS];
+    __shared__ float s_m[kWarps][8], s_l[kWarps][8];
+    float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * BB);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+    if (lane < NS) ecq_dev::mbar_init(smem_addr(&s_bar[warp][lane]), 1);
+    ecq_dev::fence_proxy_async();
     pdl_launch_dependents();
     pdl_wait();
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int b = t, i = 0, n = 1;
-    if (starts) {
-        if (t >= starts[batch]) return;
-        int lo = 0, hi = batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (starts[mid] <= t) lo = mid;
-            else hi = mid;
+
+    // this CTA's range of the flattened blocks
+    long long total = 0;
+    for (int b = threadIdx.x; b < a.batch; b += kThreads) {
+        const Request r = request<TR>(a, b);
+        total += static_cast<long long>(r.blocks) * r.pairs;
+    }
+    total = block_sum(total, s_sum);
+    const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
+    if (threadIdx.x == 0) a.cuts[cta] = make_int4(-1, 0, 0, 0);
+    if (cta >= ctas) return;
+    const long long f0 = total * cta / ctas, f1 = total * (cta + 1) / ctas;
+    // the request that f0 lies in
+    long long before = 0;
+    for (int base = 0;; base += kThreads) {
+        const int b = base + threadIdx.x;
+        long long mine = 0;
+        if (b < a.batch) {
+            const Request r = request<TR>(a, b);
+            mine = static_cast<long long>(r.blocks) * r.pairs;
         }
-        b = lo;
-        i = t - starts[b];
-        n = starts[b + 1] - starts[b];
-    }
-    int len = lens[b];
-    const long long room = static_cast<long long>(max_pages) << page_shift;
-    if (len > room) {
-        if (threadIdx.x == 0) raise_status(status, ECQ_STATUS_BADARG);
-        len = static_cast<int>(room);
-    }
-    const int keys = min(len, len - n + i + 1);
-    const int page_size = 1 << page_shift;
-    float qv[E], m = -INFINITY, l = 0.f, o[E];
+        long long incl = mine;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = to_float(q[t * q_token + h * q_head + lane + 32 * e]) * scale;
-        o[e] = 0.f;
-    }
-    for (int j = warp; j < keys; j += kWarps) {
-        const int page = table[b * table_stride + (j >> page_shift)];
-        if (page < 0 || page >= n_pages) {
-            if (lane == 0) raise_status(status, ECQ_STATUS_BADARG);
-            continue;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
         }
-        const int at = j & (page_size - 1), tok = at % kBlockTokens;
-        const uint8_t* blk = pages + ((static_cast<int64_t>(page) * kv_heads + h / share) * (page_size / kBlockTokens) +
-                                      at / kBlockTokens) * block_bytes(D, G);
-        float dot = 0.f, vv[E];
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        if (threadIdx.x == 0) s_request = -1;
+        __syncthreads();
+        long long start = before + incl - mine;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = lane + 32 * e;
-            const int nk = ((d % 32) / 8) * (D / 4) + (d / 32) * 8 + d % 8, nv = (d % 8) * (D / 8) + d / 8;
-            const int ck = blk[tok * (D / 2) + nk / 2] >> (4 * (nk % 2)) & 15;
-            const int cv = blk[v_codes_at(D) + tok * (D / 2) + nv / 2] >> (4 * (nv % 2)) & 15;
-            const int g = d / (D / G);
-            const float2 pk = __half22float2(*reinterpret_cast<const __half2*>(blk + k_params_at(D) + (tok * G + g) * 4));
-            const float2 pv = __half22float2(*reinterpret_cast<const __half2*>(blk + v_params_at(D, G) + (tok * G + g) * 4));
-            dot = fmaf(qv[e], fmaf(static_cast<float>(ck), pk.x, pk.y), dot);
-            vv[e] = fmaf(static_cast<float>(cv), pv.x, pv.y);
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) start += s_sum[w];
+            before += s_sum[w];
+        }
+        if (mine && start <= f0 && f0 < start + mine) {
+            s_request = b;
+            s_before = start;
+        }
+        __syncthreads();
+        if (s_request >= 0) break;
+    }
+
+    // where this warp fetches next; the same in all its lanes
+    int fb = s_request;
+    Request fr = request<TR>(a, fb);
+    long long f_next = f0 + warp;
+    long long f_base = s_before;  // first block of request fb
+    int f_pair, f_blk;
+    int f_page = -1;
+    uint32_t f_ok = 0;            // per ring slot: the block is there
+    int issued = 0;
+    const int blocks_per_page_shift = a.page_shift - 4;
+    auto look = [&]() {  // page of block f_next, for the next fetch
+        if (f_next >= f1) return;
+        while (f_next - f_base >= static_cast<long long>(fr.blocks) * fr.pairs) {
+            f_base += static_cast<long long>(fr.blocks) * fr.pairs;
+            fr = request<TR>(a, ++fb);
+        }
+        const int at = static_cast<int>(f_next - f_base);
+        f_pair = at / fr.blocks;
+        f_blk = at - f_pair * fr.blocks;
+        f_page = -1;
+        if (f_blk * kBlockTokens < fr.len) {
+            f_page = __ldg(a.table + fb * a.table_stride + (f_blk >> blocks_per_page_shift));
+            if (f_page < 0) f_page = INT32_MAX;
+        }
+    };
+    const uint32_t ring = smem_addr(smem) + warp * NS * BB;
+    auto fetch = [&]() {
+        if (f_next >= f1) return;
+        const int slot = issued % NS;
+        const bool there = f_page >= 0 && f_page < a.n_pages;
+        if (lane == 0) {
+            const uint32_t bar = smem_addr(&s_bar[warp][slot]);
+            if (there) {
+                const int in_page = f_blk & ((1 << blocks_per_page_shift) - 1);
+                const uint8_t* src = a.pages + (((static_cast<int64_t>(f_page) * a.kv_heads + f_pair / fr.tiles)
+                                                 << blocks_per_page_shift) + in_page) * BB;
+                ecq_dev::mbar_expect_tx(bar, BB);
+                ecq_dev::bulk_copy_g2s(ring + slot * BB, src, BB, bar);
+            } else {
+                if (f_page >= 0) raise_status(a.status, ECQ_STATUS_BADARG);
+                ecq_dev::mbar_expect_tx(bar, 0);
+            }
+        }
+        f_ok = (f_ok & ~(1u << slot)) | (there ? 1u << slot : 0u);
+        ++issued;
+        f_next += kWarps;
+        look();
+    };
+    __syncwarp();
+    look();
+#pragma unroll 1
+    for (int i = 0; i < NS; ++i) fetch();
+
+    // segment by segment
+    int b = s_request, taken = 0;
+    bool late = false;  // a copy did not come: nothing more is fetched or read
+    Request rq = request<TR>(a, b);
+    long long base = s_before;
+    Rows<D, G, NT> rows;
+    State<D, G, NT> st;
+#pragma unroll 1
+    for (long long f = f0; f < f1;) {
+        while (f - base >= static_cast<long long>(rq.blocks) * rq.pairs) {
+            base += static_cast<long long>(rq.blocks) * rq.pairs;
+            rq = request<TR>(a, ++b);
+        }
+        const int at = static_cast<int>(f - base), pair = at / rq.blocks, blk0 = at - pair * rq.blocks;
+        const int head = pair / rq.tiles, tile = pair - head * rq.tiles;
+        const long long pair_end = base + static_cast<long long>(pair + 1) * rq.blocks;
+        const long long end = min(pair_end, f1);
+        load_rows<T, D, G, NT>(rows, a, rq, head, tile);
+        st.reset();
+        // this warp's first block in [f, end)
+        const int skip = static_cast<int>((f0 + warp - f) % kWarps + kWarps) % kWarps;
+        const int n = static_cast<int>(end - f);
+#pragma unroll 1
+        for (int i = skip; i < n; i += kWarps) {
+            const int slot = taken % NS;
+            if (!late && !ecq_dev::mbar_wait(smem_addr(&s_bar[warp][slot]), (taken / NS) & 1)) {
+                late = true;
+                f_next = f1;
+                if (lane == 0) raise_status(a.status, ECQ_STATUS_TIMEOUT);
+            }
+            if (__any_sync(0xffffffffu, late)) {
+                late = true;
+                f_next = f1;
+                continue;
+            }
+            const int first = (blk0 + i) * kBlockTokens;
+            if (f_ok >> slot & 1u) {
+                if (first + kBlockTokens <= rows.least) block<D, G, NT, false>(st, rows, ring + slot * BB, first, rq.len);
+                else block<D, G, NT, true>(st, rows, ring + slot * BB, first, rq.len);
+            }
+            __syncwarp();
+            ++taken;
+            fetch();
+        }
+        // join the warps
+        const bool whole = blk0 == 0 && end == pair_end;
+        float* part = a.parts + (2 * static_cast<size_t>(cta) + (blk0 == 0)) * part_floats<D, TR>();
+        if (!whole && blk0 == 0 && threadIdx.x == 0) {
+            // the CTA whose range holds the pair's last block
+            long long last = ((pair_end - 1) * ctas) / total;
+            while (total * (last + 1) / ctas <= pair_end - 1) ++last;
+            while (total * last / ctas > pair_end - 1) --last;
+            a.cuts[cta] = make_int4(b, pair, static_cast<int>(last) - cta, 0);
         }
 #pragma unroll
-        for (int x = 16; x; x >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, x);
-        const float mx = fmaxf(m, dot), keep = expf(m - mx), p = expf(dot - mx);
-        l = fmaf(l, keep, p);
+        for (int nt = 0; nt < NT; ++nt) {
+            const int t = lane & 3, r = lane >> 2;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], keep, p * vv[e]);
-        m = mx;
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = o[e];
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
-    for (int w = 0; w < kWarps; ++w) {
-        const float a = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - M);
-        L = fmaf(a, s_l[w], L);
-        O = fmaf(a, s_o[w][threadIdx.x], O);
+                for (int o = 4; o < 32; o <<= 1) {
+                    st.l[nt][c] += __shfl_xor_sync(0xffffffffu, st.l[nt][c], o);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) st.zero[nt][g][c] += __shfl_xor_sync(0xffffffffu, st.zero[nt][g][c], o);
+                }
+                if (r == 0) {
+                    s_m[warp][2 * t + c] = st.m[nt][c];
+                    s_l[warp][2 * t + c] = st.l[nt][c];
+                }
+                float* dst = s_o + (warp * 8 + 2 * t + c) * OS + r;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const float z = st.zero[nt][i * 16 * G / D][c];
+                    dst[16 * i] = fmaf(st.o[nt][i][c], 16777216.f, z);
+                    dst[16 * i + 8] = fmaf(st.o[nt][i][c + 2], 1048576.f, z);
+                }
+            }
+            __syncthreads();
+            for (int x = threadIdx.x; x < 8 * D; x += kThreads) {
+                const int row = x / D, d = x % D, tr = nt * 8 + row;
+                float M = kNoMax, L = 0.f, O = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float k = exp2_fast(s_m[w][row] - M);
+                    L = fmaf(k, s_l[w][row], L);
+                    O = fmaf(k, s_o[(w * 8 + row) * OS + d], O);
+                }
+                if (whole) {
+                    const int qr = tile * TR + tr;
+                    if (qr < rq.rows) {
+                        const int i = qr / a.share;
+                        store(static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
+                                  static_cast<int64_t>(head * a.share + qr - i * a.share) * a.o_head + d,
+                              L == 0.f ? 0.f : O / L);
+                    }
+                } else {
+                    part[TR * 2 + tr * D + d] = O;
+                    if (d == 0) {
+                        part[2 * tr] = M;
+                        part[2 * tr + 1] = L;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        f = end;
     }
-    store(out + t * o_token + h * o_head + threadIdx.x, L == 0.f ? 0.f : O / L);
+    if (late)  // let the copies in flight land before the shared memory is given back
+        for (; taken < issued; ++taken) ecq_dev::mbar_wait(smem_addr(&s_bar[warp][taken % NS]), (taken / NS) & 1);
+}
+
+// CTA i joins the parts of the pair that range i starts and does not end.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
+    constexpr int TR = 8 * NT;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int4 cut = a.cuts[blockIdx.x];
+    if (cut.x < 0) return;
+    const Request rq = request<TR>(a, cut.x);
+    const int head = cut.y / rq.tiles, tile = cut.y - head * rq.tiles;
+    const float* first = a.parts + (2 * static_cast<size_t>(blockIdx.x) + 1) * part_floats<D, TR>();
+    const float* rest = a.parts + 2 * (static_cast<size_t>(blockIdx.x) + 1) * part_floats<D, TR>();
+    for (int x = threadIdx.x; x < TR * D; x += kThreads) {
+        const int tr = x / D, d = x % D, qr = tile * TR + tr;
+        if (qr >= rq.rows) break;
+        float M = first[2 * tr];
+        for (int c = 0; c < cut.z; ++c) M = fmaxf(M, rest[2 * c * part_floats<D, TR>() + 2 * tr]);
+        float k = exp2_fast(first[2 * tr] - M), L = k * first[2 * tr + 1], O = k * first[TR * 2 + tr * D + d];
+        for (int c = 0; c < cut.z; ++c) {
+            const float* p = rest + 2 * c * part_floats<D, TR>();
+            k = exp2_fast(p[2 * tr] - M);
+            L = fmaf(k, p[2 * tr + 1], L);
+            O = fmaf(k, p[TR * 2 + tr * D + d], O);
+        }
+        const int i = qr / a.share;
+        store(static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
+                  static_cast<int64_t>(head * a.share + qr - i * a.share) * a.o_head + d,
+              L == 0.f ? 0.f : O / L);
+    }
+}
+
+int grid_ctas(int nt) { return ctas_per_sm(nt) * ecq_dev::sm_count_cached(); }
+
+// 16-row tiles where a request may have more than 8 rows: one pass over the
+// keys for twice the rows.
+int row_tiles_of_8(int share, int max_q) { return static_cast<int64_t>(share) * max_q > 8 ? 2 : 1; }
+
+template <typename L, int NT>
+int32_t launch(const Args& a, cudaStream_t stream) {
+    using T = typename L::T;
+    constexpr int smem = kWarps * ring_slots(L::D, L::G) * block_bytes(L::D, L::G) + kWarps * 8 * (L::D + 4) * 4;
+    const auto kernel = attention_kernel<T, L::D, L::G, NT>;
+    if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
+    const dim3 grid(grid_ctas(NT));
+    cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a);
+    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, NT>, grid, dim3(kThreads), 0, stream, a);
+    return result(rc);
 }
 
 }  // namespace
@@ -114,7 +688,8 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || max_q < 1 || max_pages < 1)
         return ECQ_ERR_ARG;
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
-    return 0;
+    const int nt = row_tiles_of_8(heads / kv_heads, max_q);
+    return grid_ctas(nt) * (16 + 2 * 4 * 8ll * nt * (head_dim + 2));
 }
 
 int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -135,17 +710,34 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (total_q == 0) return ECQ_OK;
     if (!q || !out || !aligned(q, 16) || !aligned(out, 8)) return ECQ_ERR_ARG;
     if (((q_token_stride | q_head_stride) & 7) || ((out_token_stride | out_head_stride) & 3)) return ECQ_ERR_ARG;
-    if (workspace_bytes < need || (need > 0 && !workspace)) return ECQ_ERR_WORKSPACE;
+    if (workspace_bytes < need || !workspace || !aligned(workspace, 16)) return ECQ_ERR_WORKSPACE;
+    Args a;
+    a.q = q;
+    a.out = out;
+    a.pages = static_cast<const uint8_t*>(pages);
+    a.table = static_cast<const int32_t*>(block_table);
+    a.lens = static_cast<const int32_t*>(seq_lens);
+    a.starts = static_cast<const int32_t*>(q_starts);
+    a.cuts = static_cast<int4*>(workspace);
+    a.parts = reinterpret_cast<float*>(a.cuts + grid_ctas(row_tiles_of_8(heads / kv_heads, max_q)));
+    a.status = static_cast<int32_t*>(status);
+    a.q_token = q_token_stride;
+    a.q_head = q_head_stride;
+    a.o_token = out_token_stride;
+    a.o_head = out_head_stride;
+    a.n_pages = n_pages;
+    a.table_stride = table_stride;
+    a.kv_heads = kv_heads;
+    a.share = heads / kv_heads;
+    a.page_shift = log2i(page_size);
+    a.max_pages = max_pages;
+    a.batch = batch;
+    a.total_q = total_q;
+    a.scale = scale;
+    const int nt = row_tiles_of_8(a.share, max_q);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
-        using T = typename L::T;
-        return result(launch_pdl(attention_kernel<T, L::D, L::G>, dim3(total_q, heads), dim3(kWarps * 32), 0,
-                                 static_cast<cudaStream_t>(stream), static_cast<const T*>(q), q_token_stride,
-                                 q_head_stride, static_cast<T*>(out), out_token_stride, out_head_stride,
-                                 static_cast<const uint8_t*>(pages), n_pages, kv_heads, heads / kv_heads,
-                                 log2i(page_size), static_cast<const int32_t*>(block_table), table_stride, max_pages,
-                                 static_cast<const int32_t*>(seq_lens), static_cast<const int32_t*>(q_starts), batch,
-                                 scale, static_cast<int32_t*>(status)));
+        return nt == 2 ? launch<L, 2>(a, static_cast<cudaStream_t>(stream)) : launch<L, 1>(a, static_cast<cudaStream_t>(stream));
     });
 }
 
