@@ -465,51 +465,63 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     }
 
     // where this warp fetches next; the same in all its lanes
+    const int shift = a.page_shift - 4;  // blocks per page
+    const int page_bytes = BB << shift;
+    const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
     int fb = s_request;
     Request fr = request<TR>(a, fb);
-    long long f_next = f0 + warp;
-    long long f_base = s_before;  // first block of request fb
-    int f_pair, f_blk;
-    int f_page = -1;
-    uint32_t f_ok = 0;            // per ring slot: the block is there
-    int issued = 0;
-    const int blocks_per_page_shift = a.page_shift - 4;
-    auto look = [&]() {  // page of block f_next, for the next fetch
-        if (f_next >= f1) return;
-        while (f_next - f_base >= static_cast<long long>(fr.blocks) * fr.pairs) {
-            f_base += static_cast<long long>(fr.blocks) * fr.pairs;
-            fr = request<TR>(a, ++fb);
+    int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
+    int f_blk, f_tile, f_head, f_page = -1;
+    {
+        const long long at = f0 - s_before;
+        const int pair = static_cast<int>(at / fr.blocks);
+        f_blk = static_cast<int>(at - static_cast<long long>(pair) * fr.blocks) + warp;
+        f_head = pair / fr.tiles;
+        f_tile = pair - f_head * fr.tiles;
+    }
+    const int32_t* f_row = a.table + fb * a.table_stride;
+    const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
+    uint32_t f_ok = 0;  // per ring slot: the block is there
+    int f_slot = 0, issued = 0;
+    auto look = [&]() {  // the page of the next block, one fetch ahead of its use
+        if (f_left <= 0) return;
+        while (f_blk >= fr.blocks) {
+            f_blk -= fr.blocks;
+            if (++f_tile == fr.tiles) {
+                f_tile = 0;
+                if (++f_head == a.kv_heads) {
+                    f_head = 0;
+                    do fr = request<TR>(a, ++fb);
+                    while (fr.blocks == 0);
+                    f_row = a.table + fb * a.table_stride;
+                }
+                f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
+            }
         }
-        const int at = static_cast<int>(f_next - f_base);
-        f_pair = at / fr.blocks;
-        f_blk = at - f_pair * fr.blocks;
+        // below 0: there is nothing to fetch (the one block of a request without keys)
         f_page = -1;
-        if (f_blk * kBlockTokens < fr.len) {
-            f_page = __ldg(a.table + fb * a.table_stride + (f_blk >> blocks_per_page_shift));
-            if (f_page < 0) f_page = INT32_MAX;
-        }
+        if (f_blk * kBlockTokens < fr.len) f_page = __ldg(f_row + (f_blk >> shift)) & INT32_MAX;
     };
-    const uint32_t ring = smem_addr(smem) + warp * NS * BB;
+    const uint32_t ring = smem_addr(smem) + warp * NS * BB, bars = smem_addr(&s_bar[warp][0]);
     auto fetch = [&]() {
-        if (f_next >= f1) return;
-        const int slot = issued % NS;
+        if (f_left <= 0) return;
         const bool there = f_page >= 0 && f_page < a.n_pages;
         if (lane == 0) {
-            const uint32_t bar = smem_addr(&s_bar[warp][slot]);
+            const uint32_t bar = bars + 8 * f_slot;
             if (there) {
-                const int in_page = f_blk & ((1 << blocks_per_page_shift) - 1);
-                const uint8_t* src = a.pages + (((static_cast<int64_t>(f_page) * a.kv_heads + f_pair / fr.tiles)
-                                                 << blocks_per_page_shift) + in_page) * BB;
                 ecq_dev::mbar_expect_tx(bar, BB);
-                ecq_dev::bulk_copy_g2s(ring + slot * BB, src, BB, bar);
+                ecq_dev::bulk_copy_g2s(ring + f_slot * BB, f_src + f_page * pool_row + (f_blk & ((1 << shift) - 1)) * BB,
+                                       BB, bar);
             } else {
                 if (f_page >= 0) raise_status(a.status, ECQ_STATUS_BADARG);
                 ecq_dev::mbar_expect_tx(bar, 0);
             }
         }
-        f_ok = (f_ok & ~(1u << slot)) | (there ? 1u << slot : 0u);
+        f_ok = (f_ok & ~(1u << f_slot)) | (there ? 1u << f_slot : 0u);
+        f_slot = f_slot + 1 == NS ? 0 : f_slot + 1;
         ++issued;
-        f_next += kWarps;
+        --f_left;
+        f_blk += kWarps;
         look();
     };
     __syncwarp();
@@ -518,7 +530,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     for (int i = 0; i < NS; ++i) fetch();
 
     // segment by segment
-    int b = s_request, taken = 0;
+    int b = s_request, taken = 0, slot = 0;
+    uint32_t phase = 0;
     bool late = false;  // a copy did not come: nothing more is fetched or read
     Request rq = request<TR>(a, b);
     long long base = s_before;
@@ -541,15 +554,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         const int n = static_cast<int>(end - f);
 #pragma unroll 1
         for (int i = skip; i < n; i += kWarps) {
-            const int slot = taken % NS;
-            if (!late && !ecq_dev::mbar_wait(smem_addr(&s_bar[warp][slot]), (taken / NS) & 1)) {
+            if (late || __any_sync(0xffffffffu, !ecq_dev::mbar_wait(bars + 8 * slot, phase))) {
+                if (!late && lane == 0) raise_status(a.status, ECQ_STATUS_TIMEOUT);
                 late = true;
-                f_next = f1;
-                if (lane == 0) raise_status(a.status, ECQ_STATUS_TIMEOUT);
-            }
-            if (__any_sync(0xffffffffu, late)) {
-                late = true;
-                f_next = f1;
+                f_left = 0;
                 continue;
             }
             const int first = (blk0 + i) * kBlockTokens;
@@ -559,6 +567,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             }
             __syncwarp();
             ++taken;
+            if (++slot == NS) {
+                slot = 0;
+                phase ^= 1;
+            }
             fetch();
         }
         // join the warps
@@ -627,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         f = end;
     }
     if (late)  // let the copies in flight land before the shared memory is given back
-        for (; taken < issued; ++taken) ecq_dev::mbar_wait(smem_addr(&s_bar[warp][taken % NS]), (taken / NS) & 1);
+        for (; taken < issued; ++taken) ecq_dev::mbar_wait(bars + 8 * (taken % NS), (taken / NS) & 1);
 }
 
 // CTA i joins the parts of the pair that range i starts and does not end.
