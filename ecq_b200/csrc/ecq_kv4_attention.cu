@@ -19,11 +19,11 @@
 // What bounds it: the cache's bytes for long contexts; below that the ~250
 // instructions per 16 tokens and head, and for short ones launches and merges.
 //
-// Layout of the work. The (request, cache head, row tile, 16-token block) space
+// Layout of the work. The (request, cache head, row tile, 32-token unit) space
 // is flattened and cut into one even range per CTA (one wave of CTAs), from the
 // lengths on the device, so ragged batches balance and no host knows them.
-// Within a range block f belongs to warp f % kWarps. Each warp streams its
-// blocks through a ring of its own with cp.async.bulk, one copy per block, and
+// Within a range unit f belongs to warp f % kWarps. Each warp streams its
+// units through a ring of its own with cp.async.bulk and
 // keeps its own running maximum and sum; at the end of a (request, head, tile)
 // the CTA joins its warps in shared memory. Where a range's end cuts one, its
 // parts go to the workspace and a second kernel joins them in order, so results
@@ -41,6 +41,9 @@ using ecq_dev::pdl_wait;
 using ecq_dev::smem_addr;
 
 constexpr int kWarps = 8;
+// A warp takes two blocks of tokens at a time: what it costs to fetch and to
+// wait for them, and the look at the running maximum, are paid once.
+constexpr int kUnit = 2, kUnitTokens = kUnit * kBlockTokens;
 constexpr int kThreads = kWarps * 32;
 // 16-row tiles need the registers of two 8-row ones
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 2 : 1; }
@@ -53,8 +56,8 @@ constexpr float kNoMax = -1e30f;
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups) {
     const int room = 110 * 1024 - kWarps * 8 * (dim + 4) * 4;
-    const int n = room / (kWarps * block_bytes(dim, groups));
-    return n < 6 ? n : 6;
+    const int n = room / (kWarps * kUnit * block_bytes(dim, groups));
+    return n < 4 ? n : 4;
 }
 
 struct Args {
@@ -72,7 +75,7 @@ struct Args {
 
 // One request's part of the work.
 struct Request {
-    int first_q, rows, len, blocks, tiles, pairs;
+    int first_q, rows, len, units, tiles, pairs;
 };
 
 template <int TR>  // rows per tile
@@ -98,8 +101,8 @@ __device__ __forceinline__ Request request(const Args& a, int b) {
     r.rows = (hi - lo) * a.share;
     r.tiles = (r.rows + TR - 1) / TR;
     r.pairs = r.tiles * a.kv_heads;
-    // a request without keys has one (masked) block, so that its rows are written
-    r.blocks = r.rows ? max((r.len + kBlockTokens - 1) / kBlockTokens, 1) : 0;
+    // a request without keys has one (empty) unit, so that its rows are written
+    r.units = r.rows ? max((r.len + kUnitTokens - 1) / kUnitTokens, 1) : 0;
     return r;
 }
 
@@ -122,6 +125,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -138,14 +148,17 @@ __device__ __forceinline__ uint32_t h2(float a, float b) {
 }
 __device__ __forceinline__ float2 f2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-template <int N>  // words
+// N words at shared address addr + kAt
+template <int N, int kAt>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t addr) {
     if constexpr (N == 4) {
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(addr), "n"(kAt));
     } else if constexpr (N == 2) {
-        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr), "n"(kAt));
     } else {
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+        asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(w[0]) : "r"(addr), "n"(kAt));
     }
 }
 
@@ -268,137 +281,157 @@ struct State {
 // that a lane's four quads take at once, lie in both halves of the banks.
 __device__ __forceinline__ int token_of(int i) { return (i & 1) ? 4 + ((i >> 1) ^ 1) : i >> 1; }
 
-// One block of 16 tokens at shared address blk; `first`: its first token.
-template <int D, int G, int NT, bool kMask>
-__device__ __forceinline__ void block(State<D, G, NT>& S, const Rows<D, G, NT>& R, uint32_t blk, int first, int len) {
-    constexpr int W = D / 32;
-    const int lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
-    const int tok = token_of(r);
-    uint32_t k0[W], k1[W], kp[2][G], vp[2][G];
-    lds<W>(k0, blk + tok * (D / 2) + t * (D / 8));
-    lds<W>(k1, blk + (tok + 8) * (D / 2) + t * (D / 8));
-    lds<G>(kp[0], blk + k_params_at(D) + tok * 4 * G);
-    lds<G>(kp[1], blk + k_params_at(D) + (tok + 8) * 4 * G);
-    lds<G>(vp[0], blk + v_params_at(D, G) + tok * 4 * G);
-    lds<G>(vp[1], blk + v_params_at(D, G) + (tok + 8) * 4 * G);
-    if (kMask) {  // tokens behind the request's last have never been written
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (first + tok + 8 * i >= len)
-#pragma unroll
-                for (int g = 0; g < G; ++g) kp[i][g] = vp[i][g] = 0;
+// Where a lane's words lie in a block, from the block's start.
+template <int D, int G>
+struct Lane {
+    uint32_t k, params, va, vb;
+    __device__ __forceinline__ Lane() {
+        const int lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
+        k = token_of(r) * (D / 2) + t * (D / 8);
+        params = k_params_at(D) + token_of(r) * 4 * G;
+        va = v_codes_at(D) + token_of(2 * t) * (D / 2) + r * (D / 16);
+        vb = v_codes_at(D) + token_of(2 * t + 1) * (D / 2) + r * (D / 16);
     }
-    uint32_t hi[NT][G][2], lo[NT][G][2];
-    {
+};
+
+// U blocks of 16 tokens at shared address at, the first of which is token
+// `first` of the request.
+template <int D, int G, int NT, int U, bool kMask>
+__device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
+                                       int first) {
+    constexpr int W = D / 32, BB = block_bytes(D, G);
+    const int tok = token_of((threadIdx.x & 31) >> 2);
+    float s[U][NT][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        uint32_t k0[W], k1[W], kp[2][G];
+        lds<W, 0>(k0, at + u * BB + me.k);
+        lds<W, 8 * (D / 2)>(k1, at + u * BB + me.k);
+        lds<G, 0>(kp[0], at + u * BB + me.params);
+        lds<G, 32 * G>(kp[1], at + u * BB + me.params);
         float acc[NT][G][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[nt][g][c] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t x0 = h ? k0[w] >> 8 : k0[w], x1 = h ? k1[w] >> 8 : k1[w];
+                const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+                const int g = w * 32 * G / D;
+                const bool fresh = h == 0 && (w == 0 || g != (w - 1) * 32 * G / D);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma(acc[nt][w * 32 * G / D], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u,
-                        x1 & 0x00f000f0u, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (fresh) mma_first(acc[nt][g], a0, a1, a2, a3, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
+                    else mma(acc[nt][g], a0, a1, a2, a3, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
+                }
             }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int i = 0; i < 2; ++i) {
+                float x[2] = {0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int g = 0; g < G; ++g) {
                     const float2 p = f2(kp[i][g]);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        s[2 * i + c] = fmaf(p.x, acc[nt][g][2 * i + c], fmaf(p.y, R.sums[nt][g][c], s[2 * i + c]));
-                }
-            bool seen[4] = {true, true, true, true};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[c] *= R.factor[nt][c & 1];
-                if (kMask) {
-                    seen[c] = first + tok + 8 * (c >> 1) < R.limit[nt][c & 1];
-                    if (!seen[c]) s[c] = -INFINITY;
-                }
-            }
-            float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
-            if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + kSlack || top[1] > S.m[nt][1] + kSlack)) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float x = fmaxf(top[c], S.m[nt][c]);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                    const float keep = exp2_fast(S.m[nt][c] - x);
-                    S.m[nt][c] = x;
-                    S.l[nt][c] *= keep;
-#pragma unroll
-                    for (int g = 0; g < G; ++g) S.zero[nt][g][c] *= keep;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        S.o[nt][i][c] *= keep;
-                        S.o[nt][i][c + 2] *= keep;
+                    for (int c = 0; c < 2; ++c) {
+                        x[c] = g ? fmaf(p.y, R.sums[nt][g][c], x[c]) : p.y * R.sums[nt][g][c];
+                        x[c] = fmaf(p.x, acc[nt][g][2 * i + c], x[c]);
                     }
                 }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    // a token out of sight, or behind the last, may hold anything: it is chosen away, not computed away
+                    s[u][nt][2 * i + c] = kMask && first + 16 * u + tok + 8 * i >= R.limit[nt][c]
+                                              ? -INFINITY
+                                              : x[c] * R.factor[nt][c];
+                }
             }
-            float p[4];
+    }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                p[c] = exp2_fast(s[c] - S.m[nt][c & 1]);
-                S.l[nt][c & 1] += p[c];
+    for (int nt = 0; nt < NT; ++nt) {
+        float top[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            top[c] = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+            for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][nt][c], s[u][nt][c + 2]));
+        }
+        if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + kSlack || top[1] > S.m[nt][1] + kSlack)) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = fmaxf(top[c], S.m[nt][c]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                const float keep = exp2_fast(S.m[nt][c] - x);
+                S.m[nt][c] = x;
+                S.l[nt][c] *= keep;
+#pragma unroll
+                for (int g = 0; g < G; ++g) S.zero[nt][g][c] *= keep;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    S.o[nt][i][c] *= keep;
+                    S.o[nt][i][c + 2] *= keep;
+                }
             }
+        }
+    }
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+    for (int u = 0; u < U; ++u) {
+        uint32_t vp[2][G], hi[NT][G][2], lo[NT][G][2];
+        lds<G, 64 * G>(vp[0], at + u * BB + me.params);
+        lds<G, 96 * G>(vp[1], at + u * BB + me.params);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float p[2];
+                bool gone[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    p[c] = exp2_fast(s[u][nt][2 * i + c] - S.m[nt][c]);
+                    gone[c] = kMask && first + 16 * u + tok + 8 * i >= R.limit[nt][c];
+                    S.l[nt][c] += p[c];
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
                     const float2 v = f2(vp[i][g]);
                     float w[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float x = p[2 * i + c];
-                        // a key out of sight may hold anything: 0 times it would not do
-                        w[c] = kMask && !seen[2 * i + c] ? 0.f : x * v.x;
-                        S.zero[nt][g][c] += kMask && !seen[2 * i + c] ? 0.f : x * v.y;
+                        w[c] = gone[c] ? 0.f : p[c] * v.x;
+                        S.zero[nt][g][c] = gone[c] ? S.zero[nt][g][c] : fmaf(p[c], v.y, S.zero[nt][g][c]);
                     }
-                    const uint32_t u = h2(w[0], w[1]);
-                    const float2 back = f2(u);
-                    hi[nt][g][i] = transpose(u);
+                    const uint32_t h = h2(w[0], w[1]);
+                    const float2 back = f2(h);
+                    hi[nt][g][i] = transpose(h);
                     lo[nt][g][i] = transpose(h2(w[0] - back.x, w[1] - back.y));
                 }
-        }
-    }
-    constexpr int VW = D / 64;  // words of a lane's chunk of a V row
-    uint32_t v[4][VW];
-    const int ta = token_of(2 * t), tb = token_of(2 * t + 1);
-    const uint32_t vc = blk + v_codes_at(D) + r * (D / 16);
-    lds<VW>(v[0], vc + ta * (D / 2));
-    lds<VW>(v[1], vc + tb * (D / 2));
-    lds<VW>(v[2], vc + (ta + 8) * (D / 2));
-    lds<VW>(v[3], vc + (tb + 8) * (D / 2));
+            }
+        constexpr int VW = D / 64;  // words of a lane's chunk of a V row
+        uint32_t v[4][VW];
+        lds<VW, 0>(v[0], at + u * BB + me.va);
+        lds<VW, 0>(v[1], at + u * BB + me.vb);
+        lds<VW, 8 * (D / 2)>(v[2], at + u * BB + me.va);
+        lds<VW, 8 * (D / 2)>(v[3], at + u * BB + me.vb);
 #pragma unroll
-    for (int w = 0; w < VW; ++w)
+        for (int w = 0; w < VW; ++w)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint32_t pick = half ? 0x7632u : 0x5410u;
-            const uint32_t x = __byte_perm(v[0][w], v[1][w], pick), y = __byte_perm(v[2][w], v[3][w], pick);
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t pick = half ? 0x7632u : 0x5410u;
+                const uint32_t x = __byte_perm(v[0][w], v[1][w], pick), y = __byte_perm(v[2][w], v[3][w], pick);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int mt = 4 * w + 2 * half + j, g = mt * 16 * G / D;
-                const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
-                const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
+                for (int j = 0; j < 2; ++j) {
+                    const int mt = 4 * w + 2 * half + j, g = mt * 16 * G / D;
+                    const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
+                    const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma(S.o[nt][mt], a0, a1, a2, a3, hi[nt][g][0], hi[nt][g][1]);
-                    mma(S.o[nt][mt], a0, a1, a2, a3, lo[nt][g][0], lo[nt][g][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma(S.o[nt][mt], a0, a1, a2, a3, hi[nt][g][0], hi[nt][g][1]);
+                        mma(S.o[nt][mt], a0, a1, a2, a3, lo[nt][g][0], lo[nt][g][1]);
+                    }
                 }
             }
-        }
+    }
 }
 
 template <int D, int TR>
@@ -406,14 +439,14 @@ __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a) {
-    constexpr int TR = 8 * NT, NS = ring_slots(D, G), BB = block_bytes(D, G), OS = D + 4;
+    constexpr int TR = 8 * NT, NS = ring_slots(D, G), BB = block_bytes(D, G), UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
     __shared__ long long s_before;
     __shared__ int s_request;
     __shared__ uint64_t s_bar[kWarps][NS];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-    float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * BB);
+    float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * UB);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
     if (lane < NS) ecq_dev::mbar_init(smem_addr(&s_bar[warp][lane]), 1);
     ecq_dev::fence_proxy_async();
@@ -424,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     long long total = 0;
     for (int b = threadIdx.x; b < a.batch; b += kThreads) {
         const Request r = request<TR>(a, b);
-        total += static_cast<long long>(r.blocks) * r.pairs;
+        total += static_cast<long long>(r.units) * r.pairs;
     }
     total = block_sum(total, s_sum);
     const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
@@ -438,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         long long mine = 0;
         if (b < a.batch) {
             const Request r = request<TR>(a, b);
-            mine = static_cast<long long>(r.blocks) * r.pairs;
+            mine = static_cast<long long>(r.units) * r.pairs;
         }
         long long incl = mine;
 #pragma unroll
@@ -471,57 +504,69 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     int fb = s_request;
     Request fr = request<TR>(a, fb);
     int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
-    int f_blk, f_tile, f_head, f_page = -1;
+    int f_unit, f_tile, f_head, f_page[kUnit];
     {
         const long long at = f0 - s_before;
-        const int pair = static_cast<int>(at / fr.blocks);
-        f_blk = static_cast<int>(at - static_cast<long long>(pair) * fr.blocks) + warp;
+        const int pair = static_cast<int>(at / fr.units);
+        f_unit = static_cast<int>(at - static_cast<long long>(pair) * fr.units) + warp;
         f_head = pair / fr.tiles;
         f_tile = pair - f_head * fr.tiles;
     }
     const int32_t* f_row = a.table + fb * a.table_stride;
     const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
-    uint32_t f_ok = 0;  // per ring slot: the block is there
+    uint32_t f_ok = 0;  // two bits per ring slot: the blocks that are there
     int f_slot = 0, issued = 0;
-    auto look = [&]() {  // the page of the next block, one fetch ahead of its use
+    auto look = [&]() {  // the pages of the next unit, one fetch ahead of their use
         if (f_left <= 0) return;
-        while (f_blk >= fr.blocks) {
-            f_blk -= fr.blocks;
+        while (f_unit >= fr.units) {
+            f_unit -= fr.units;
             if (++f_tile == fr.tiles) {
                 f_tile = 0;
                 if (++f_head == a.kv_heads) {
                     f_head = 0;
                     do fr = request<TR>(a, ++fb);
-                    while (fr.blocks == 0);
+                    while (fr.units == 0);
                     f_row = a.table + fb * a.table_stride;
                 }
                 f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
             }
         }
-        // below 0: there is nothing to fetch (the one block of a request without keys)
-        f_page = -1;
-        if (f_blk * kBlockTokens < fr.len) f_page = __ldg(f_row + (f_blk >> shift)) & INT32_MAX;
+        // pages of the unit's blocks; below 0: no tokens there (the end of a request)
+#pragma unroll
+        for (int u = 0; u < kUnit; ++u) {
+            const int blk = f_unit * kUnit + u;
+            f_page[u] = -1;
+            if (blk * kBlockTokens < fr.len) f_page[u] = __ldg(f_row + (blk >> shift)) & INT32_MAX;
+        }
     };
-    const uint32_t ring = smem_addr(smem) + warp * NS * BB, bars = smem_addr(&s_bar[warp][0]);
+    const uint32_t ring = smem_addr(smem) + warp * NS * UB, bars = smem_addr(&s_bar[warp][0]);
     auto fetch = [&]() {
         if (f_left <= 0) return;
-        const bool there = f_page >= 0 && f_page < a.n_pages;
+        uint32_t there = 0;
+#pragma unroll
+        for (int u = 0; u < kUnit; ++u) there |= f_page[u] >= 0 && f_page[u] < a.n_pages ? 1u << u : 0u;
         if (lane == 0) {
-            const uint32_t bar = bars + 8 * f_slot;
-            if (there) {
-                ecq_dev::mbar_expect_tx(bar, BB);
-                ecq_dev::bulk_copy_g2s(ring + f_slot * BB, f_src + f_page * pool_row + (f_blk & ((1 << shift) - 1)) * BB,
-                                       BB, bar);
+            const uint32_t bar = bars + 8 * f_slot, dst = ring + f_slot * UB;
+            const int in_page = (f_unit * kUnit) & ((1 << shift) - 1);
+            if (shift && there == (1u << kUnit) - 1u) {  // one page has them all
+                ecq_dev::mbar_expect_tx(bar, UB);
+                ecq_dev::bulk_copy_g2s(dst, f_src + f_page[0] * pool_row + in_page * BB, UB, bar);
             } else {
-                if (f_page >= 0) raise_status(a.status, ECQ_STATUS_BADARG);
-                ecq_dev::mbar_expect_tx(bar, 0);
+                ecq_dev::mbar_expect_tx(bar, __popc(there) * BB);
+#pragma unroll
+                for (int u = 0; u < kUnit; ++u) {
+                    if (there >> u & 1u)
+                        ecq_dev::bulk_copy_g2s(dst + u * BB, f_src + f_page[u] * pool_row + (shift ? in_page + u : 0) * BB, BB,
+                                               bar);
+                    else if (f_page[u] >= 0) raise_status(a.status, ECQ_STATUS_BADARG);
+                }
             }
         }
-        f_ok = (f_ok & ~(1u << f_slot)) | (there ? 1u << f_slot : 0u);
+        f_ok = (f_ok & ~(3u << 2 * f_slot)) | there << 2 * f_slot;
         f_slot = f_slot + 1 == NS ? 0 : f_slot + 1;
         ++issued;
         --f_left;
-        f_blk += kWarps;
+        f_unit += kWarps;
         look();
     };
     __syncwarp();
@@ -537,15 +582,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     long long base = s_before;
     Rows<D, G, NT> rows;
     State<D, G, NT> st;
+    const Lane<D, G> me;
 #pragma unroll 1
     for (long long f = f0; f < f1;) {
-        while (f - base >= static_cast<long long>(rq.blocks) * rq.pairs) {
-            base += static_cast<long long>(rq.blocks) * rq.pairs;
+        while (f - base >= static_cast<long long>(rq.units) * rq.pairs) {
+            base += static_cast<long long>(rq.units) * rq.pairs;
             rq = request<TR>(a, ++b);
         }
-        const int at = static_cast<int>(f - base), pair = at / rq.blocks, blk0 = at - pair * rq.blocks;
+        const int at = static_cast<int>(f - base), pair = at / rq.units, unit0 = at - pair * rq.units;
         const int head = pair / rq.tiles, tile = pair - head * rq.tiles;
-        const long long pair_end = base + static_cast<long long>(pair + 1) * rq.blocks;
+        const long long pair_end = base + static_cast<long long>(pair + 1) * rq.units;
         const long long end = min(pair_end, f1);
         load_rows<T, D, G, NT>(rows, a, rq, head, tile);
         st.reset();
@@ -560,10 +606,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 f_left = 0;
                 continue;
             }
-            const int first = (blk0 + i) * kBlockTokens;
-            if (f_ok >> slot & 1u) {
-                if (first + kBlockTokens <= rows.least) block<D, G, NT, false>(st, rows, ring + slot * BB, first, rq.len);
-                else block<D, G, NT, true>(st, rows, ring + slot * BB, first, rq.len);
+            const int first = (unit0 + i) * kUnitTokens;
+            const uint32_t ok = f_ok >> 2 * slot & 3u, at = ring + slot * UB;
+            if (ok == 3u && first + kUnitTokens <= rows.least) {
+                blocks<D, G, NT, kUnit, false>(st, rows, me, at, first);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kUnit; ++u)
+                    if (ok >> u & 1u) blocks<D, G, NT, 1, true>(st, rows, me, at + u * BB, first + u * kBlockTokens);
             }
             __syncwarp();
             ++taken;
@@ -574,9 +624,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             fetch();
         }
         // join the warps
-        const bool whole = blk0 == 0 && end == pair_end;
-        float* part = a.parts + (2 * static_cast<size_t>(cta) + (blk0 == 0)) * part_floats<D, TR>();
-        if (!whole && blk0 == 0 && threadIdx.x == 0) {
+        const bool whole = unit0 == 0 && end == pair_end;
+        float* part = a.parts + (2 * static_cast<size_t>(cta) + (unit0 == 0)) * part_floats<D, TR>();
+        if (!whole && unit0 == 0 && threadIdx.x == 0) {
             // the CTA whose range holds the pair's last block
             long long last = ((pair_end - 1) * ctas) / total;
             while (total * (last + 1) / ctas <= pair_end - 1) ++last;
@@ -682,7 +732,7 @@ int row_tiles_of_8(int share, int max_q) { return static_cast<int64_t>(share) * 
 template <typename L, int NT>
 int32_t launch(const Args& a, cudaStream_t stream) {
     using T = typename L::T;
-    constexpr int smem = kWarps * ring_slots(L::D, L::G) * block_bytes(L::D, L::G) + kWarps * 8 * (L::D + 4) * 4;
+    constexpr int smem = kWarps * ring_slots(L::D, L::G) * kUnit * block_bytes(L::D, L::G) + kWarps * 8 * (L::D + 4) * 4;
     const auto kernel = attention_kernel<T, L::D, L::G, NT>;
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
     const dim3 grid(grid_ctas(NT));
