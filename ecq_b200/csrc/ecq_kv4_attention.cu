@@ -173,7 +173,7 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2
 template <int D, int G, int NT>
 struct Rows {
     uint32_t b[NT][D / 16][2];
-    float sums[NT][G][2];  // of the lane's two columns, times 2^-24
+    uint32_t sums[NT][2];  // B operand that takes (scale, zero) pairs: (0, sum of the group's q), high and low part
     float factor[NT][2];   // scale log2(e) 2^24 / the row's power of two
     int limit[NT][2];      // keys that the column's row sees
     int least;             // the smallest limit of rows that exist
@@ -208,10 +208,16 @@ __device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, cons
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // rows are brought to [2^11, 2^12): elements down to 2^-25 of the largest, and a sixteenth of
-        // them, are normal or exact subnormal fp16
+        // rows are brought to [2^14, 2^15): elements down to 2^-28 of the largest, and a sixteenth of them, keep
+        // their bits in fp16. A negative scale turns the row's sign; with none every score is 0.
         const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
-        const float up = __int_as_float((11 - ex + 127) << 23), down = __int_as_float((ex - 11 + 127) << 23);
+        float up = __int_as_float((14 - ex + 127) << 23);
+        float factor = fabsf(a.scale) * 1.4426950408889634f * (__int_as_float((ex - 14 + 127) << 23) * 16777216.f);
+        if (a.scale < 0.f) up = -up;
+        if (factor == 0.f) {
+            up = 0.f;
+            factor = 1.f;
+        }
         float sums[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) sums[g] = 0.f;
@@ -228,26 +234,27 @@ __device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, cons
                 R.b[nt][2 * w + h][1] = h2(x[w][1 + 2 * h] * 0.0625f, x[w][5 + 2 * h] * 0.0625f);
             }
         }
-        const float factor = a.scale * 1.4426950408889634f * (down * 16777216.f);
         // query i sees keys up to len - queries + i
         const int limit = in ? rq.len - queries + i + 1 : rq.len;
         int least = max(limit, 0);
 #pragma unroll
         for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
         R.least = min(R.least, least);
+        float mine = 0.f;  // lane t has group t's sum (at most 2^22), times 2^-24
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+            if (t == g) mine = sums[g] * 5.9604644775390625e-8f;
         }
+        const float high = __half2float(__float2half_rn(mine));
+        R.sums[nt][0] = h2(0.f, high);
+        R.sums[nt][1] = h2(0.f, mine - high);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {  // column 2t + c is row 2t + c of the tile: lane 4 (2t + c) has it
             const int from = 4 * (2 * t + c);
             R.factor[nt][c] = __shfl_sync(0xffffffffu, factor, from);
             R.limit[nt][c] = __shfl_sync(0xffffffffu, limit, from);
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-                R.sums[nt][g][c] = __shfl_sync(0xffffffffu, sums[g], from) * 5.9604644775390625e-8f;
         }
     }
 }
@@ -256,8 +263,8 @@ __device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, cons
 template <int D, int G, int NT>
 struct State {
     float o[NT][D / 16][4];
-    float zero[NT][G][2];
-    float m[NT][2], l[NT][2];
+    float sums[NT][4];  // lanes of row r < G: sum p zero of group r; of row G: sum p (columns 2t, 2t + 1; [2], [3] unused)
+    float m[NT][2];
     __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -266,12 +273,8 @@ struct State {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                m[nt][c] = kNoMax;
-                l[nt][c] = 0.f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) zero[nt][g][c] = 0.f;
-            }
+            for (int c = 0; c < 4; ++c) sums[nt][c] = 0.f;
+            m[nt][0] = m[nt][1] = kNoMax;
         }
     }
 };
@@ -284,15 +287,31 @@ __device__ __forceinline__ int token_of(int i) { return (i & 1) ? 4 + ((i >> 1) 
 // Where a lane's words lie in a block, from the block's start.
 template <int D, int G>
 struct Lane {
-    uint32_t k, params, va, vb;
+    uint32_t k, k_params, k_pair, va, vb, va_params, vb_params, va_pair, vb_pair;
     __device__ __forceinline__ Lane() {
         const int lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
+        const int a = token_of(2 * t), b = token_of(2 * t + 1), g = min(r, G - 1);
         k = token_of(r) * (D / 2) + t * (D / 8);
-        params = k_params_at(D) + token_of(r) * 4 * G;
-        va = v_codes_at(D) + token_of(2 * t) * (D / 2) + r * (D / 16);
-        vb = v_codes_at(D) + token_of(2 * t + 1) * (D / 2) + r * (D / 16);
+        k_params = k_params_at(D) + token_of(r) * 4 * G;
+        k_pair = k_params + 4 * min(t, G - 1);
+        va = v_codes_at(D) + a * (D / 2) + r * (D / 16);
+        vb = v_codes_at(D) + b * (D / 2) + r * (D / 16);
+        va_params = v_params_at(D, G) + a * 4 * G;
+        vb_params = v_params_at(D, G) + b * 4 * G;
+        va_pair = va_params + 4 * g;
+        vb_pair = vb_params + 4 * g;
     }
 };
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2_rn(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t fma2h(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
 
 // U blocks of 16 tokens at shared address at, the first of which is token
 // `first` of the request.
@@ -300,16 +319,23 @@ template <int D, int G, int NT, int U, bool kMask>
 __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
                                        int first) {
     constexpr int W = D / 32, BB = block_bytes(D, G);
-    const int tok = token_of((threadIdx.x & 31) >> 2);
+    const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
     float s[U][NT][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t k0[W], k1[W], kp[2][G];
+        uint32_t k0[W], k1[W], kp[2][G], pair[2][1];
         lds<W, 0>(k0, at + u * BB + me.k);
         lds<W, 8 * (D / 2)>(k1, at + u * BB + me.k);
-        lds<G, 0>(kp[0], at + u * BB + me.params);
-        lds<G, 32 * G>(kp[1], at + u * BB + me.params);
+        lds<G, 0>(kp[0], at + u * BB + me.k_params);
+        lds<G, 32 * G>(kp[1], at + u * BB + me.k_params);
+        lds<1, 0>(pair[0], at + u * BB + me.k_pair);
+        lds<1, 32 * G>(pair[1], at + u * BB + me.k_pair);
+        // sum over the groups of zero * (sum of q): the pairs (scale, zero) as they lie are an A operand (lanes past the
+        // last group meet zeros in B). Then, per group, the codes.
         float acc[NT][G][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            mma_first(s[u][nt], pair[0][0], pair[1][0], pair[0][0], pair[1][0], R.sums[nt][0], R.sums[nt][1]);
 #pragma unroll
         for (int w = 0; w < W; ++w)
 #pragma unroll
@@ -325,27 +351,23 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                 }
             }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float x[2] = {0.f, 0.f};
+            for (int g = 0; g < G; ++g) {
+                const float scale = f2(kp[i][g]).x;
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float2 p = f2(kp[i][g]);
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        x[c] = g ? fmaf(p.y, R.sums[nt][g][c], x[c]) : p.y * R.sums[nt][g][c];
-                        x[c] = fmaf(p.x, acc[nt][g][2 * i + c], x[c]);
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    // a token out of sight, or behind the last, may hold anything: it is chosen away, not computed away
-                    s[u][nt][2 * i + c] = kMask && first + 16 * u + tok + 8 * i >= R.limit[nt][c]
-                                              ? -INFINITY
-                                              : x[c] * R.factor[nt][c];
-                }
+                    for (int c = 0; c < 2; ++c) s[u][nt][2 * i + c] = fmaf(scale, acc[nt][g][2 * i + c], s[u][nt][2 * i + c]);
             }
+        if (kMask) {
+            // a token out of sight, or behind the last, may hold anything: it is chosen away, not computed away
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (first + 16 * u + tok + 8 * (c >> 1) >= R.limit[nt][c & 1]) s[u][nt][c] = -INFINITY;
+        }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -355,6 +377,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             top[c] = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
             for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][nt][c], s[u][nt][c + 2]));
+            top[c] *= R.factor[nt][c];
         }
         if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + kSlack || top[1] > S.m[nt][1] + kSlack)) {
 #pragma unroll
@@ -364,9 +387,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                 for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
                 const float keep = exp2_fast(S.m[nt][c] - x);
                 S.m[nt][c] = x;
-                S.l[nt][c] *= keep;
-#pragma unroll
-                for (int g = 0; g < G; ++g) S.zero[nt][g][c] *= keep;
+                S.sums[nt][c] *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     S.o[nt][i][c] *= keep;
@@ -377,36 +398,59 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t vp[2][G], hi[NT][G][2], lo[NT][G][2];
-        lds<G, 64 * G>(vp[0], at + u * BB + me.params);
-        lds<G, 96 * G>(vp[1], at + u * BB + me.params);
+        uint32_t sa[2][G], sb[2][G], za[2][1], zb[2][1];
+        lds<G, 0>(sa[0], at + u * BB + me.va_params);
+        lds<G, 0>(sb[0], at + u * BB + me.vb_params);
+        lds<G, 32 * G>(sa[1], at + u * BB + me.va_params);
+        lds<G, 32 * G>(sb[1], at + u * BB + me.vb_params);
+        lds<1, 0>(za[0], at + u * BB + me.va_pair);
+        lds<1, 0>(zb[0], at + u * BB + me.vb_pair);
+        lds<1, 32 * G>(za[1], at + u * BB + me.va_pair);
+        lds<1, 32 * G>(zb[1], at + u * BB + me.vb_pair);
+        // rows of A: the groups' zeros, then ones (the sum of the weights)
+        uint32_t z[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2; ++i) {
+            z[i] = __byte_perm(za[i][0], zb[i][0], 0x7632);
+            if (kMask) {  // where a zero is not finite its scale is not either, and that reaches the rows that see the token
+                if ((z[i] & 0x7c00u) == 0x7c00u) z[i] &= 0xffff0000u;
+                if ((z[i] & 0x7c000000u) == 0x7c000000u) z[i] &= 0xffffu;
+            }
+            z[i] = r == G ? 0x3c003c00u : z[i];
+        }
+        uint32_t hi[NT][G][2], lo[NT][G][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            uint32_t ph[2], pl[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float p[2];
-                bool gone[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    p[c] = exp2_fast(s[u][nt][2 * i + c] - S.m[nt][c]);
-                    gone[c] = kMask && first + 16 * u + tok + 8 * i >= R.limit[nt][c];
-                    S.l[nt][c] += p[c];
-                }
+                for (int c = 0; c < 2; ++c) p[c] = exp2_fast(fmaf(s[u][nt][2 * i + c], R.factor[nt][c], -S.m[nt][c]));
+                const uint32_t x = h2(p[0], p[1]);
+                const float2 back = f2(x);
+                ph[i] = transpose(x);
+                pl[i] = transpose(h2(p[0] - back.x, p[1] - back.y));
+            }
+            mma(S.sums[nt], z[0], 0u, z[1], 0u, ph[0], ph[1]);
+            mma(S.sums[nt], z[0], 0u, z[1], 0u, pl[0], pl[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const float2 v = f2(vp[i][g]);
-                    float w[2];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        w[c] = gone[c] ? 0.f : p[c] * v.x;
-                        S.zero[nt][g][c] = gone[c] ? S.zero[nt][g][c] : fmaf(p[c], v.y, S.zero[nt][g][c]);
+                    // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
+                    const uint32_t sc = __byte_perm(sa[i][g], sb[i][g], 0x5410);
+                    uint32_t h = mul2(ph[i], sc);
+                    uint32_t l = fma2h(pl[i], sc, fma2h(ph[i], sc, h ^ 0x80008000u));
+                    if (kMask) {  // weight 0: 0, whatever the scale is
+                        const uint32_t keep = (ph[i] & 0xffffu ? 0xffffu : 0u) | (ph[i] & 0xffff0000u ? 0xffff0000u : 0u);
+                        h &= keep;
+                        l &= keep;
                     }
-                    const uint32_t h = h2(w[0], w[1]);
-                    const float2 back = f2(h);
-                    hi[nt][g][i] = transpose(h);
-                    lo[nt][g][i] = transpose(h2(w[0] - back.x, w[1] - back.y));
+                    hi[nt][g][i] = h;
+                    lo[nt][g][i] = l;
                 }
-            }
+        }
         constexpr int VW = D / 64;  // words of a lane's chunk of a V row
         uint32_t v[4][VW];
         lds<VW, 0>(v[0], at + u * BB + me.va);
@@ -638,22 +682,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             const int t = lane & 3, r = lane >> 2;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                float z[G];
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    st.l[nt][c] += __shfl_xor_sync(0xffffffffu, st.l[nt][c], o);
-#pragma unroll
-                    for (int g = 0; g < G; ++g) st.zero[nt][g][c] += __shfl_xor_sync(0xffffffffu, st.zero[nt][g][c], o);
-                }
-                if (r == 0) {
-                    s_m[warp][2 * t + c] = st.m[nt][c];
-                    s_l[warp][2 * t + c] = st.l[nt][c];
-                }
+                for (int g = 0; g < G; ++g) z[g] = __shfl_sync(0xffffffffu, st.sums[nt][c], 4 * g + t);
+                if (r == 0) s_m[warp][2 * t + c] = st.m[nt][c];
+                if (r == G) s_l[warp][2 * t + c] = st.sums[nt][c];
                 float* dst = s_o + (warp * 8 + 2 * t + c) * OS + r;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const float z = st.zero[nt][i * 16 * G / D][c];
-                    dst[16 * i] = fmaf(st.o[nt][i][c], 16777216.f, z);
-                    dst[16 * i + 8] = fmaf(st.o[nt][i][c + 2], 1048576.f, z);
+                    dst[16 * i] = fmaf(st.o[nt][i][c], 16777216.f, z[i * 16 * G / D]);
+                    dst[16 * i + 8] = fmaf(st.o[nt][i][c + 2], 1048576.f, z[i * 16 * G / D]);
                 }
             }
             __syncthreads();
