@@ -40,13 +40,13 @@ using ecq_dev::pdl_launch_dependents;
 using ecq_dev::pdl_wait;
 using ecq_dev::smem_addr;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 // A warp takes two blocks of tokens at a time: what it costs to fetch and to
 // wait for them, and the look at the running maximum, are paid once.
 constexpr int kUnit = 2, kUnitTokens = kUnit * kBlockTokens;
 constexpr int kThreads = kWarps * 32;
 // 16-row tiles need the registers of two 8-row ones
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 2 : 1; }
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 // Weights are exp2(score - reference); the reference is raised when a score
 // passes it by more than this, so weights are at most 4 and weight * scale
 // (at most 4 * 131008 / 15) is finite in fp16. Few blocks raise it, and the
@@ -55,7 +55,7 @@ constexpr float kSlack = 2.f;
 constexpr float kNoMax = -1e30f;
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups) {
-    const int room = 110 * 1024 - kWarps * 8 * (dim + 4) * 4;
+    const int room = 74 * 1024 - kWarps * 8 * (dim + 4) * 4;
     const int n = room / (kWarps * kUnit * block_bytes(dim, groups));
     return n < 4 ? n : 4;
 }
@@ -120,14 +120,14 @@ __device__ __forceinline__ long long block_sum(long long v, long long* s) {
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -332,33 +332,31 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
         lds<1, 32 * G>(pair[1], at + u * BB + me.k_pair);
         // sum over the groups of zero * (sum of q): the pairs (scale, zero) as they lie are an A operand (lanes past the
         // last group meet zeros in B). Then, per group, the codes.
-        float acc[NT][G][4];
+        constexpr int A = G > 2 ? G : 2;  // accumulators: neighbouring steps go to different ones
+        float acc[NT][A][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             mma_first(s[u][nt], pair[0][0], pair[1][0], pair[0][0], pair[1][0], R.sums[nt][0], R.sums[nt][1]);
 #pragma unroll
-        for (int w = 0; w < W; ++w)
+        for (int i = 0; i < 2 * W; ++i) {
+            const int n = i % A, step = n * (2 * W / A) + i / A, w = step / 2, h = step % 2;
+            const uint32_t x0 = h ? k0[w] >> 8 : k0[w], x1 = h ? k1[w] >> 8 : k1[w];
+            const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t x0 = h ? k0[w] >> 8 : k0[w], x1 = h ? k1[w] >> 8 : k1[w];
-                const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-                const int g = w * 32 * G / D;
-                const bool fresh = h == 0 && (w == 0 || g != (w - 1) * 32 * G / D);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (fresh) mma_first(acc[nt][g], a0, a1, a2, a3, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
-                    else mma(acc[nt][g], a0, a1, a2, a3, R.b[nt][2 * w + h][0], R.b[nt][2 * w + h][1]);
-                }
+            for (int nt = 0; nt < NT; ++nt) {
+                if (i < A) mma_first(acc[nt][n], a0, a1, a2, a3, R.b[nt][step][0], R.b[nt][step][1]);
+                else mma(acc[nt][n], a0, a1, a2, a3, R.b[nt][step][0], R.b[nt][step][1]);
             }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const float scale = f2(kp[i][g]).x;
+            for (int n = 0; n < A; ++n) {
+                const float scale = f2(kp[i][n * G / A]).x;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) s[u][nt][2 * i + c] = fmaf(scale, acc[nt][g][2 * i + c], s[u][nt][2 * i + c]);
+                    for (int c = 0; c < 2; ++c) s[u][nt][2 * i + c] = fmaf(scale, acc[nt][n][2 * i + c], s[u][nt][2 * i + c]);
             }
         if (kMask) {
             // a token out of sight, or behind the last, may hold anything: it is chosen away, not computed away
@@ -458,23 +456,32 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
         lds<VW, 8 * (D / 2)>(v[2], at + u * BB + me.va);
         lds<VW, 8 * (D / 2)>(v[3], at + u * BB + me.vb);
 #pragma unroll
-        for (int w = 0; w < VW; ++w)
+        for (int w = 0; w < VW; ++w) {
+            uint32_t x[4][4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t pick = half ? 0x7632u : 0x5410u;
-                const uint32_t x = __byte_perm(v[0][w], v[1][w], pick), y = __byte_perm(v[2][w], v[3][w], pick);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t pick = j & 2 ? 0x7632u : 0x5410u;
+                uint32_t a = __byte_perm(v[0][w], v[1][w], pick), b = __byte_perm(v[2][w], v[3][w], pick);
+                if (j & 1) {
+                    a >>= 8;
+                    b >>= 8;
+                }
+                x[j][0] = a & 0x000f000fu;
+                x[j][1] = a & 0x00f000f0u;
+                x[j][2] = b & 0x000f000fu;
+                x[j][3] = b & 0x00f000f0u;
+            }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int mt = 4 * w + 2 * half + j, g = mt * 16 * G / D;
-                    const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
-                    const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma(S.o[nt][mt], a0, a1, a2, a3, hi[nt][g][0], hi[nt][g][1]);
-                        mma(S.o[nt][mt], a0, a1, a2, a3, lo[nt][g][0], lo[nt][g][1]);
+                        const int mt = 4 * w + j, g = mt * 16 * G / D;
+                        const uint32_t(&p)[2] = part ? lo[nt][g] : hi[nt][g];
+                        mma(S.o[nt][mt], x[j][0], x[j][1], x[j][2], x[j][3], p[0], p[1]);
                     }
-                }
-            }
+        }
     }
 }
 
@@ -488,34 +495,39 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     __shared__ long long s_sum[kWarps];
     __shared__ long long s_before;
     __shared__ int s_request;
+    __shared__ Request s_own;
     __shared__ uint64_t s_bar[kWarps][NS];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
     float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * UB);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+    const int lane = threadIdx.x & 31, cta = blockIdx.x;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // the compiler sees that it is one for the warp
     if (lane < NS) ecq_dev::mbar_init(smem_addr(&s_bar[warp][lane]), 1);
     ecq_dev::fence_proxy_async();
     pdl_launch_dependents();
     pdl_wait();
 
-    // this CTA's range of the flattened blocks
-    long long total = 0;
+    // this CTA's range of the flattened units, and the request that it starts in
+    long long total = 0, mine = 0;
+    Request own = {};
     for (int b = threadIdx.x; b < a.batch; b += kThreads) {
-        const Request r = request<TR>(a, b);
-        total += static_cast<long long>(r.units) * r.pairs;
+        own = request<TR>(a, b);
+        mine = static_cast<long long>(own.units) * own.pairs;
+        total += mine;
     }
     total = block_sum(total, s_sum);
     const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
     if (threadIdx.x == 0) a.cuts[cta] = make_int4(-1, 0, 0, 0);
     if (cta >= ctas) return;
     const long long f0 = total * cta / ctas, f1 = total * (cta + 1) / ctas;
-    // the request that f0 lies in
     long long before = 0;
-    for (int base = 0;; base += kThreads) {
-        const int b = base + threadIdx.x;
-        long long mine = 0;
-        if (b < a.batch) {
-            const Request r = request<TR>(a, b);
-            mine = static_cast<long long>(r.units) * r.pairs;
+    for (int first = 0; first < a.batch; first += kThreads) {
+        const int b = first + threadIdx.x;
+        if (a.batch > kThreads) {  // more than one round: not the last one's any more
+            mine = 0;
+            if (b < a.batch) {
+                own = request<TR>(a, b);
+                mine = static_cast<long long>(own.units) * own.pairs;
+            }
         }
         long long incl = mine;
 #pragma unroll
@@ -536,17 +548,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         if (mine && start <= f0 && f0 < start + mine) {
             s_request = b;
             s_before = start;
+            s_own = own;
         }
         __syncthreads();
         if (s_request >= 0) break;
     }
+    if (s_request < 0) return;  // lengths that change meanwhile: no range, but no endless search either
 
     // where this warp fetches next; the same in all its lanes
     const int shift = a.page_shift - 4;  // blocks per page
     const int page_bytes = BB << shift;
     const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
     int fb = s_request;
-    Request fr = request<TR>(a, fb);
+    Request fr = s_own;
     int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
     int f_unit, f_tile, f_head, f_page[kUnit];
     {
@@ -558,8 +572,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     }
     const int32_t* f_row = a.table + fb * a.table_stride;
     const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
-    uint32_t f_ok = 0;  // two bits per ring slot: the blocks that are there
-    int f_slot = 0, issued = 0;
+    uint32_t f_bad = 0;  // a bit per ring slot and block: its page number is out of range
+    int f_slot = 0;
     auto look = [&]() {  // the pages of the next unit, one fetch ahead of their use
         if (f_left <= 0) return;
         while (f_unit >= fr.units) {
@@ -568,47 +582,56 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 f_tile = 0;
                 if (++f_head == a.kv_heads) {
                     f_head = 0;
-                    do fr = request<TR>(a, ++fb);
-                    while (fr.units == 0);
+                    do {
+                        if (++fb >= a.batch) {
+                            f_left = 0;
+                            return;
+                        }
+                        fr = request<TR>(a, fb);
+                    } while (fr.units == 0);
                     f_row = a.table + fb * a.table_stride;
                 }
                 f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
             }
         }
-        // pages of the unit's blocks; below 0: no tokens there (the end of a request)
+        if (shift) {  // a page has the whole unit
+            f_page[0] = -1;  // nothing there: the one unit of a request without keys
+            if (fr.len) f_page[0] = __ldg(f_row + (f_unit * kUnit >> shift)) & INT32_MAX;
+        } else {
 #pragma unroll
-        for (int u = 0; u < kUnit; ++u) {
-            const int blk = f_unit * kUnit + u;
-            f_page[u] = -1;
-            if (blk * kBlockTokens < fr.len) f_page[u] = __ldg(f_row + (blk >> shift)) & INT32_MAX;
+            for (int u = 0; u < kUnit; ++u) {
+                f_page[u] = -1;
+                if ((f_unit * kUnit + u) * kBlockTokens < fr.len) f_page[u] = __ldg(f_row + f_unit * kUnit + u) & INT32_MAX;
+            }
         }
     };
     const uint32_t ring = smem_addr(smem) + warp * NS * UB, bars = smem_addr(&s_bar[warp][0]);
     auto fetch = [&]() {
         if (f_left <= 0) return;
-        uint32_t there = 0;
-#pragma unroll
-        for (int u = 0; u < kUnit; ++u) there |= f_page[u] >= 0 && f_page[u] < a.n_pages ? 1u << u : 0u;
-        if (lane == 0) {
-            const uint32_t bar = bars + 8 * f_slot, dst = ring + f_slot * UB;
-            const int in_page = (f_unit * kUnit) & ((1 << shift) - 1);
-            if (shift && there == (1u << kUnit) - 1u) {  // one page has them all
+        const uint32_t bar = bars + 8 * f_slot, dst = ring + f_slot * UB;
+        f_bad &= ~(3u << 2 * f_slot);
+        if (shift && static_cast<uint32_t>(f_page[0]) < a.n_pages) {
+            if (lane == 0) {
                 ecq_dev::mbar_expect_tx(bar, UB);
-                ecq_dev::bulk_copy_g2s(dst, f_src + f_page[0] * pool_row + in_page * BB, UB, bar);
-            } else {
+                ecq_dev::bulk_copy_g2s(dst, f_src + f_page[0] * pool_row + ((f_unit * kUnit) & ((1 << shift) - 1)) * BB, UB, bar);
+            }
+        } else {
+            uint32_t there = 0;
+#pragma unroll
+            for (int u = 0; u < kUnit; ++u) {
+                const int page = shift ? f_page[0] : f_page[u];
+                if (page >= 0 && page < a.n_pages) there |= 1u << u;
+                else if (page >= 0) f_bad |= 1u << (2 * f_slot + u);
+            }
+            if (lane == 0) {
                 ecq_dev::mbar_expect_tx(bar, __popc(there) * BB);
 #pragma unroll
-                for (int u = 0; u < kUnit; ++u) {
-                    if (there >> u & 1u)
-                        ecq_dev::bulk_copy_g2s(dst + u * BB, f_src + f_page[u] * pool_row + (shift ? in_page + u : 0) * BB, BB,
-                                               bar);
-                    else if (f_page[u] >= 0) raise_status(a.status, ECQ_STATUS_BADARG);
-                }
+                for (int u = 0; u < kUnit; ++u)
+                    if (there >> u & 1u) ecq_dev::bulk_copy_g2s(dst + u * BB, f_src + f_page[u] * pool_row, BB, bar);
+                if (f_bad) raise_status(a.status, ECQ_STATUS_BADARG);
             }
         }
-        f_ok = (f_ok & ~(3u << 2 * f_slot)) | there << 2 * f_slot;
         f_slot = f_slot + 1 == NS ? 0 : f_slot + 1;
-        ++issued;
         --f_left;
         f_unit += kWarps;
         look();
@@ -619,10 +642,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     for (int i = 0; i < NS; ++i) fetch();
 
     // segment by segment
-    int b = s_request, taken = 0, slot = 0;
+    int b = s_request, slot = 0;
     uint32_t phase = 0;
     bool late = false;  // a copy did not come: nothing more is fetched or read
-    Request rq = request<TR>(a, b);
+    Request rq = s_own;
     long long base = s_before;
     Rows<D, G, NT> rows;
     State<D, G, NT> st;
@@ -631,7 +654,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     for (long long f = f0; f < f1;) {
         while (f - base >= static_cast<long long>(rq.units) * rq.pairs) {
             base += static_cast<long long>(rq.units) * rq.pairs;
-            rq = request<TR>(a, ++b);
+            if (++b >= a.batch) return;
+            rq = request<TR>(a, b);
         }
         const int at = static_cast<int>(f - base), pair = at / rq.units, unit0 = at - pair * rq.units;
         const int head = pair / rq.tiles, tile = pair - head * rq.tiles;
@@ -651,16 +675,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 continue;
             }
             const int first = (unit0 + i) * kUnitTokens;
-            const uint32_t ok = f_ok >> 2 * slot & 3u, at = ring + slot * UB;
-            if (ok == 3u && first + kUnitTokens <= rows.least) {
-                blocks<D, G, NT, kUnit, false>(st, rows, me, at, first);
-            } else {
+            const uint32_t at = ring + slot * UB;
+            if (f_bad >> 2 * slot & 3u) {  // keys of a bad page are left out
 #pragma unroll 1
                 for (int u = 0; u < kUnit; ++u)
-                    if (ok >> u & 1u) blocks<D, G, NT, 1, true>(st, rows, me, at + u * BB, first + u * kBlockTokens);
+                    if (!(f_bad >> (2 * slot + u) & 1u)) blocks<D, G, NT, 1, true>(st, rows, me, at + u * BB, first + u * kBlockTokens);
+            } else if (first + kUnitTokens <= rows.least) {
+                blocks<D, G, NT, kUnit, false>(st, rows, me, at, first);
+            } else {
+                blocks<D, G, NT, kUnit, true>(st, rows, me, at, first);
             }
             __syncwarp();
-            ++taken;
             if (++slot == NS) {
                 slot = 0;
                 phase ^= 1;
@@ -726,38 +751,94 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         }
         f = end;
     }
-    if (late)  // let the copies in flight land before the shared memory is given back
-        for (; taken < issued; ++taken) ecq_dev::mbar_wait(bars + 8 * (taken % NS), (taken / NS) & 1);
+    if (late) {
+        // let the copies in flight land before the shared memory is given back (a slot without one waits in vain)
+        for (int i = 0; i < NS; ++i) ecq_dev::mbar_wait(bars + 8 * i, i < slot ? phase ^ 1u : phase);
+    }
 }
 
-// CTA i joins the parts of the pair that range i starts and does not end.
+// CTA i joins the parts of the pair that range i starts and does not end. A
+// row's parts are dealt to kJoinWarps / rows warps, whose sums meet in shared
+// memory: few rows with many parts (one long request) are the slow case, and
+// loads of the same thread would queue up behind one another.
+constexpr int kJoinWarps = 32;
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
-    constexpr int TR = 8 * NT;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
+    constexpr int TR = 8 * NT, kDeal = kJoinWarps / TR, V = D / 32, PF = part_floats<D, TR>();
+    __shared__ float s_o[kDeal][TR][D], s_l[kDeal][TR], s_m[kDeal][TR];
     pdl_launch_dependents();
     pdl_wait();
     const int4 cut = a.cuts[blockIdx.x];
     if (cut.x < 0) return;
+    const int lane = threadIdx.x & 31, row = (threadIdx.x >> 5) % TR, deal = (threadIdx.x >> 5) / TR;
+    // the first part is the range's second one, the others the first ones of the ranges that follow: part c is at c * 2 PF
+    // from there, but for the first
+    const float* parts = a.parts + 2 * static_cast<size_t>(blockIdx.x) * PF;
+    const int n = cut.z + 1;
+    float M = kNoMax, L = 0.f, o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = 0.f;
+    for (int c0 = deal; c0 < n; c0 += 4 * kDeal) {  // four parts at a time
+        float m[4], l[4], x[4][V];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + j * kDeal;
+            m[j] = kNoMax;
+            l[j] = 0.f;
+            if (c < n) {
+                const float* p = parts + (c ? 2 * static_cast<size_t>(c) * PF : PF);
+                m[j] = p[2 * row];
+                l[j] = p[2 * row + 1];
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[j][v] = p[2 * TR + row * D + V * lane + v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[j][v] = 0.f;
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, m[j]);
+        const float keep = exp2_fast(M - top);
+        M = top;
+        L *= keep;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= keep;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float k = exp2_fast(m[j] - top);
+            L = fmaf(k, l[j], L);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] = fmaf(k, x[j][v], o[v]);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_o[deal][row][V * lane + v] = o[v];
+    if (lane == 0) {
+        s_m[deal][row] = M;
+        s_l[deal][row] = L;
+    }
+    __syncthreads();
     const Request rq = request<TR>(a, cut.x);
+    if (rq.rows == 0) return;
     const int head = cut.y / rq.tiles, tile = cut.y - head * rq.tiles;
-    const float* first = a.parts + (2 * static_cast<size_t>(blockIdx.x) + 1) * part_floats<D, TR>();
-    const float* rest = a.parts + 2 * (static_cast<size_t>(blockIdx.x) + 1) * part_floats<D, TR>();
-    for (int x = threadIdx.x; x < TR * D; x += kThreads) {
+    for (int x = threadIdx.x; x < TR * D; x += kJoinWarps * 32) {
         const int tr = x / D, d = x % D, qr = tile * TR + tr;
         if (qr >= rq.rows) break;
-        float M = first[2 * tr];
-        for (int c = 0; c < cut.z; ++c) M = fmaxf(M, rest[2 * c * part_floats<D, TR>() + 2 * tr]);
-        float k = exp2_fast(first[2 * tr] - M), L = k * first[2 * tr + 1], O = k * first[TR * 2 + tr * D + d];
-        for (int c = 0; c < cut.z; ++c) {
-            const float* p = rest + 2 * c * part_floats<D, TR>();
-            k = exp2_fast(p[2 * tr] - M);
-            L = fmaf(k, p[2 * tr + 1], L);
-            O = fmaf(k, p[TR * 2 + tr * D + d], O);
+        float top = kNoMax, sum = 0.f, val = 0.f;
+#pragma unroll
+        for (int k = 0; k < kDeal; ++k) top = fmaxf(top, s_m[k][tr]);
+#pragma unroll
+        for (int k = 0; k < kDeal; ++k) {
+            const float w = exp2_fast(s_m[k][tr] - top);
+            sum = fmaf(w, s_l[k][tr], sum);
+            val = fmaf(w, s_o[k][tr][d], val);
         }
         const int i = qr / a.share;
         store(static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
                   static_cast<int64_t>(head * a.share + qr - i * a.share) * a.o_head + d,
-              L == 0.f ? 0.f : O / L);
+              sum == 0.f ? 0.f : val / sum);
     }
 }
 
@@ -775,7 +856,7 @@ int32_t launch(const Args& a, cudaStream_t stream) {
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
     const dim3 grid(grid_ctas(NT));
     cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a);
-    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, NT>, grid, dim3(kThreads), 0, stream, a);
+    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, NT>, grid, dim3(kJoinWarps * 32), 0, stream, a);
     return result(rc);
 }
 
