@@ -75,7 +75,7 @@ struct Args {
 
 // One request's part of the work.
 struct Request {
-    int first_q, rows, len, units, tiles, pairs;
+    int first_q, queries, rows, len, units, tiles, pairs;
 };
 
 template <int TR>  // rows per tile
@@ -98,7 +98,8 @@ __device__ __forceinline__ Request request(const Args& a, int b) {
     }
     r.len = max(r.len, 0);
     r.first_q = lo;
-    r.rows = (hi - lo) * a.share;
+    r.queries = hi - lo;
+    r.rows = r.queries * a.share;
     r.tiles = (r.rows + TR - 1) / TR;
     r.pairs = r.tiles * a.kv_heads;
     // a request without keys has one (empty) unit, so that its rows are written
@@ -166,8 +167,34 @@ __device__ __forceinline__ float2 cvt2(uint32_t u, __half) { return f2(u); }
 __device__ __forceinline__ float2 cvt2(uint32_t u, __nv_bfloat16) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
-__device__ __forceinline__ void store(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) { return h2(a, b); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// V neighbouring channels
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&x)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1], T()), pack2(x[2], x[3], T()));
+    else *reinterpret_cast<uint32_t*>(p) = pack2(x[0], x[1], T());
+}
+template <int V>
+__device__ __forceinline__ void load(float (&x)[V], const float* p) {
+    if constexpr (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        x[0] = v.x, x[1] = v.y;
+    }
+}
+// Row `row` of a (request, head): its channels V * lane .. in the output.
+template <typename T, int V>
+__device__ __forceinline__ T* out_row(const Args& a, const Request& rq, int head, int row) {
+    const int i = row / a.share;
+    return static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
+           static_cast<int64_t>(head * a.share + row - i * a.share) * a.o_head + V * (threadIdx.x & 31);
+}
 
 // The query rows of one tile as B operands, and what their scores need.
 template <int D, int G, int NT>
@@ -179,25 +206,38 @@ struct Rows {
     int least;             // the smallest limit of rows that exist
 };
 
-template <typename T, int D, int G, int NT>
-__device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, const Request& rq, int head, int tile) {
+// A lane's share of the tile's rows as they lie in memory: the loads are issued
+// early and set_rows makes the operands of them.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& a, const Request& rq, int head, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
-    const int queries = rq.rows / a.share;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = (tile * NT + nt) * 8 + n, i = row / a.share;
+        const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
+                       static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+            raw[nt][w] = make_uint4(0, 0, 0, 0);
+            if (row < rq.rows) raw[nt][w] = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
+        }
+    }
+}
+
+template <typename T, int D, int G, int NT>
+__device__ __forceinline__ void set_rows(Rows<D, G, NT>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
+                                         const Request& rq, int tile) {
+    const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
     R.least = rq.len;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int row = (tile * NT + nt) * 8 + n;
         const bool in = row < rq.rows;
-        const int i = row / a.share;
-        const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
-                       static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
         float x[D / 32][8];
         float top = 0.f;
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (in) u = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
-            const uint32_t us[4] = {u.x, u.y, u.z, u.w};
+            const uint32_t us[4] = {raw[nt][w].x, raw[nt][w].y, raw[nt][w].z, raw[nt][w].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float2 f = cvt2(us[e], T());
@@ -235,7 +275,7 @@ __device__ __forceinline__ void load_rows(Rows<D, G, NT>& R, const Args& a, cons
             }
         }
         // query i sees keys up to len - queries + i
-        const int limit = in ? rq.len - queries + i + 1 : rq.len;
+        const int limit = in ? rq.len - rq.queries + row / a.share + 1 : rq.len;
         int least = max(limit, 0);
 #pragma unroll
         for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -279,27 +319,23 @@ struct State {
     }
 };
 
-// The block's token that row i (< 8) of the products stands for. Even rows are
-// tokens 0..3, odd ones 5, 4, 7, 6: neighbouring rows' K words, and the V words
-// that a lane's four quads take at once, lie in both halves of the banks.
-__device__ __forceinline__ int token_of(int i) { return (i & 1) ? 4 + ((i >> 1) ^ 1) : i >> 1; }
+// The block's token that row i (< 8) of the products stands for. Rows 2t and
+// 2t + 1 are tokens t and t + 4, so that what a lane reads for the second lies
+// at a constant from the first.
+__device__ __forceinline__ int token_of(int i) { return (i >> 1) + 4 * (i & 1); }
 
 // Where a lane's words lie in a block, from the block's start.
 template <int D, int G>
 struct Lane {
-    uint32_t k, k_params, k_pair, va, vb, va_params, vb_params, va_pair, vb_pair;
+    uint32_t k, k_params, k_pair, v, v_params, v_pair;
     __device__ __forceinline__ Lane() {
         const int lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
-        const int a = token_of(2 * t), b = token_of(2 * t + 1), g = min(r, G - 1);
         k = token_of(r) * (D / 2) + t * (D / 8);
         k_params = k_params_at(D) + token_of(r) * 4 * G;
         k_pair = k_params + 4 * min(t, G - 1);
-        va = v_codes_at(D) + a * (D / 2) + r * (D / 16);
-        vb = v_codes_at(D) + b * (D / 2) + r * (D / 16);
-        va_params = v_params_at(D, G) + a * 4 * G;
-        vb_params = v_params_at(D, G) + b * 4 * G;
-        va_pair = va_params + 4 * g;
-        vb_pair = vb_params + 4 * g;
+        v = v_codes_at(D) + t * (D / 2) + r * (D / 16);
+        v_params = v_params_at(D, G) + t * 4 * G;
+        v_pair = v_params + 4 * min(r, G - 1);
     }
 };
 
@@ -308,17 +344,21 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t fma2h(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t neg2(uint32_t a) {
+    const __half2 r = __hneg2(*reinterpret_cast<const __half2*>(&a));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// U blocks of 16 tokens at shared address at, the first of which is token
-// `first` of the request.
-template <int D, int G, int NT, int U, bool kMask>
+// A unit's blocks at shared address at; first[u]: the request's token that
+// block u starts with (used with kMask; beyond all limits: leave it out).
+template <int D, int G, int NT, bool kMask>
 __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
-                                       int first) {
-    constexpr int W = D / 32, BB = block_bytes(D, G);
+                                       const int (&first)[kUnit]) {
+    constexpr int U = kUnit, W = D / 32, BB = block_bytes(D, G);
     const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
     float s[U][NT][4];
 #pragma unroll
@@ -364,7 +404,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (first + 16 * u + tok + 8 * (c >> 1) >= R.limit[nt][c & 1]) s[u][nt][c] = -INFINITY;
+                    if (first[u] + tok + 8 * (c >> 1) >= R.limit[nt][c & 1]) s[u][nt][c] = -INFINITY;
         }
     }
 #pragma unroll
@@ -397,14 +437,14 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         uint32_t sa[2][G], sb[2][G], za[2][1], zb[2][1];
-        lds<G, 0>(sa[0], at + u * BB + me.va_params);
-        lds<G, 0>(sb[0], at + u * BB + me.vb_params);
-        lds<G, 32 * G>(sa[1], at + u * BB + me.va_params);
-        lds<G, 32 * G>(sb[1], at + u * BB + me.vb_params);
-        lds<1, 0>(za[0], at + u * BB + me.va_pair);
-        lds<1, 0>(zb[0], at + u * BB + me.vb_pair);
-        lds<1, 32 * G>(za[1], at + u * BB + me.va_pair);
-        lds<1, 32 * G>(zb[1], at + u * BB + me.vb_pair);
+        lds<G, 0>(sa[0], at + u * BB + me.v_params);
+        lds<G, 16 * G>(sb[0], at + u * BB + me.v_params);
+        lds<G, 32 * G>(sa[1], at + u * BB + me.v_params);
+        lds<G, 48 * G>(sb[1], at + u * BB + me.v_params);
+        lds<1, 0>(za[0], at + u * BB + me.v_pair);
+        lds<1, 16 * G>(zb[0], at + u * BB + me.v_pair);
+        lds<1, 32 * G>(za[1], at + u * BB + me.v_pair);
+        lds<1, 48 * G>(zb[1], at + u * BB + me.v_pair);
         // rows of A: the groups' zeros, then ones (the sum of the weights)
         uint32_t z[2];
 #pragma unroll
@@ -439,7 +479,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                     // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
                     const uint32_t sc = __byte_perm(sa[i][g], sb[i][g], 0x5410);
                     uint32_t h = mul2(ph[i], sc);
-                    uint32_t l = fma2h(pl[i], sc, fma2h(ph[i], sc, h ^ 0x80008000u));
+                    uint32_t l = fma2h(pl[i], sc, fma2h(ph[i], sc, neg2(h)));
                     if (kMask) {  // weight 0: 0, whatever the scale is
                         const uint32_t keep = (ph[i] & 0xffffu ? 0xffffu : 0u) | (ph[i] & 0xffff0000u ? 0xffff0000u : 0u);
                         h &= keep;
@@ -451,10 +491,10 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
         }
         constexpr int VW = D / 64;  // words of a lane's chunk of a V row
         uint32_t v[4][VW];
-        lds<VW, 0>(v[0], at + u * BB + me.va);
-        lds<VW, 0>(v[1], at + u * BB + me.vb);
-        lds<VW, 8 * (D / 2)>(v[2], at + u * BB + me.va);
-        lds<VW, 8 * (D / 2)>(v[3], at + u * BB + me.vb);
+        lds<VW, 0>(v[0], at + u * BB + me.v);
+        lds<VW, 4 * (D / 2)>(v[1], at + u * BB + me.v);
+        lds<VW, 8 * (D / 2)>(v[2], at + u * BB + me.v);
+        lds<VW, 12 * (D / 2)>(v[3], at + u * BB + me.v);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
             uint32_t x[4][4];
@@ -518,7 +558,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
     if (threadIdx.x == 0) a.cuts[cta] = make_int4(-1, 0, 0, 0);
     if (cta >= ctas) return;
-    const long long f0 = total * cta / ctas, f1 = total * (cta + 1) / ctas;
+    // the first `longer` ranges have one unit more
+    const long long each = total / ctas, longer = total - each * ctas;
+    const long long f0 = each * cta + min(static_cast<long long>(cta), longer), f1 = f0 + each + (cta < longer);
     long long before = 0;
     for (int first = 0; first < a.batch; first += kThreads) {
         const int b = first + threadIdx.x;
@@ -559,17 +601,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     const int shift = a.page_shift - 4;  // blocks per page
     const int page_bytes = BB << shift;
     const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
-    int fb = s_request;
-    Request fr = s_own;
-    int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
-    int f_unit, f_tile, f_head, f_page[kUnit];
+    int b = s_request, head, tile, unit0;
+    Request rq = s_own;
     {
         const long long at = f0 - s_before;
-        const int pair = static_cast<int>(at / fr.units);
-        f_unit = static_cast<int>(at - static_cast<long long>(pair) * fr.units) + warp;
-        f_head = pair / fr.tiles;
-        f_tile = pair - f_head * fr.tiles;
+        const int pair = static_cast<int>(at / rq.units);
+        unit0 = static_cast<int>(at - static_cast<long long>(pair) * rq.units);
+        head = pair / rq.tiles;
+        tile = pair - head * rq.tiles;
     }
+    uint4 raw[NT][D / 32];
+    load_rows<T, D, NT>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
+    int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + warp, f_page[kUnit];
+    int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
+    Request fr = rq;
     const int32_t* f_row = a.table + fb * a.table_stride;
     const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
     uint32_t f_bad = 0;  // a bit per ring slot and block: its page number is out of range
@@ -641,67 +686,86 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 #pragma unroll 1
     for (int i = 0; i < NS; ++i) fetch();
 
-    // segment by segment
-    int b = s_request, slot = 0;
+    // segment by segment: what the range has of one (request, head, tile)
+    int slot = 0;
     uint32_t phase = 0;
     bool late = false;  // a copy did not come: nothing more is fetched or read
-    Request rq = s_own;
-    long long base = s_before;
     Rows<D, G, NT> rows;
     State<D, G, NT> st;
     const Lane<D, G> me;
 #pragma unroll 1
     for (long long f = f0; f < f1;) {
-        while (f - base >= static_cast<long long>(rq.units) * rq.pairs) {
-            base += static_cast<long long>(rq.units) * rq.pairs;
-            if (++b >= a.batch) return;
-            rq = request<TR>(a, b);
-        }
-        const int at = static_cast<int>(f - base), pair = at / rq.units, unit0 = at - pair * rq.units;
-        const int head = pair / rq.tiles, tile = pair - head * rq.tiles;
-        const long long pair_end = base + static_cast<long long>(pair + 1) * rq.units;
-        const long long end = min(pair_end, f1);
-        load_rows<T, D, G, NT>(rows, a, rq, head, tile);
+        const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), f1 - f));
+        set_rows<T, D, G, NT>(rows, raw, a, rq, tile);
         st.reset();
-        // this warp's first block in [f, end)
-        const int skip = static_cast<int>((f0 + warp - f) % kWarps + kWarps) % kWarps;
-        const int n = static_cast<int>(end - f);
-#pragma unroll 1
-        for (int i = skip; i < n; i += kWarps) {
+        // this warp's first unit in [f, f + n)
+        int i = (warp - static_cast<int>((f - f0) % kWarps) + kWarps) % kWarps;
+        auto wait = [&]() {
             if (late || __any_sync(0xffffffffu, !ecq_dev::mbar_wait(bars + 8 * slot, phase))) {
                 if (!late && lane == 0) raise_status(a.status, ECQ_STATUS_TIMEOUT);
                 late = true;
                 f_left = 0;
-                continue;
+                i = n;
             }
-            const int first = (unit0 + i) * kUnitTokens;
-            const uint32_t at = ring + slot * UB;
-            if (f_bad >> 2 * slot & 3u) {  // keys of a bad page are left out
-#pragma unroll 1
-                for (int u = 0; u < kUnit; ++u)
-                    if (!(f_bad >> (2 * slot + u) & 1u)) blocks<D, G, NT, 1, true>(st, rows, me, at + u * BB, first + u * kBlockTokens);
-            } else if (first + kUnitTokens <= rows.least) {
-                blocks<D, G, NT, kUnit, false>(st, rows, me, at, first);
-            } else {
-                blocks<D, G, NT, kUnit, true>(st, rows, me, at, first);
-            }
+            return !late;
+        };
+        auto done = [&]() {
             __syncwarp();
             if (++slot == NS) {
                 slot = 0;
                 phase ^= 1;
             }
+            i += kWarps;
             fetch();
+        };
+        // units that every row sees, then (or between, where a page number is bad) those with a mask
+        const int seen = rows.least / kUnitTokens - unit0;
+#pragma unroll 1
+        while (i < n) {
+            int first[kUnit] = {};
+#pragma unroll 1
+            while (i < min(n, seen) && !(f_bad >> 2 * slot & 3u)) {
+                if (!wait()) break;
+                blocks<D, G, NT, false>(st, rows, me, ring + slot * UB, first);
+                done();
+            }
+            if (i >= n || !wait()) break;
+#pragma unroll
+            for (int u = 0; u < kUnit; ++u)
+                first[u] = f_bad >> (2 * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
+            blocks<D, G, NT, true>(st, rows, me, ring + slot * UB, first);
+            done();
         }
-        // join the warps
-        const bool whole = unit0 == 0 && end == pair_end;
-        float* part = a.parts + (2 * static_cast<size_t>(cta) + (unit0 == 0)) * part_floats<D, TR>();
-        if (!whole && unit0 == 0 && threadIdx.x == 0) {
-            // the CTA whose range holds the pair's last block
-            long long last = ((pair_end - 1) * ctas) / total;
-            while (total * (last + 1) / ctas <= pair_end - 1) ++last;
-            while (total * last / ctas > pair_end - 1) --last;
-            a.cuts[cta] = make_int4(b, pair, static_cast<int>(last) - cta, 0);
+        // the next segment's rows are on their way while the warps join
+        const Request now = rq;
+        const int b_now = b, head_now = head, tile_now = tile;
+        const bool starts = unit0 == 0, ends = unit0 + n == rq.units;
+        const long long rest = rq.units - unit0 - n;
+        f += n;
+        unit0 = 0;
+        if (++tile == rq.tiles) {
+            tile = 0;
+            if (++head == a.kv_heads) head = 0;
         }
+        if (f < f1) {
+            if (head == 0 && tile == 0) {
+                do {
+                    if (++b >= a.batch) break;
+                    rq = request<TR>(a, b);
+                } while (rq.units == 0);
+                if (b >= a.batch) late = true;
+            }
+            if (late) f = f1;
+            else load_rows<T, D, NT>(raw, a, rq, head, tile);
+        }
+        float* part = a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
+        if (starts && !ends && threadIdx.x == 0) {
+            // how many of the ranges that follow it takes to the pair's end
+            const long long k = max(longer - cta - 1, 0ll);
+            const long long more = rest <= k * (each + 1) ? (rest + each) / (each + 1) : k + (rest - k * (each + 1) + each - 1) / each;
+            a.cuts[cta] = make_int4(b_now, head_now * now.tiles + tile_now, static_cast<int>(more), 0);
+        }
+        constexpr int V = D / 32;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int t = lane & 3, r = lane >> 2;
@@ -720,28 +784,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 }
             }
             __syncthreads();
-            for (int x = threadIdx.x; x < 8 * D; x += kThreads) {
-                const int row = x / D, d = x % D, tr = nt * 8 + row;
-                float M = kNoMax, L = 0.f, O = 0.f;
+#pragma unroll
+            for (int row = warp; row < 8; row += kWarps) {
+                float M = kNoMax, L = 0.f, o[V];
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
 #pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = 0.f;
+#pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float k = exp2_fast(s_m[w][row] - M);
+                    float x[V];
+                    load<V>(x, s_o + (w * 8 + row) * OS + V * lane);
                     L = fmaf(k, s_l[w][row], L);
-                    O = fmaf(k, s_o[(w * 8 + row) * OS + d], O);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] = fmaf(k, x[v], o[v]);
                 }
-                if (whole) {
-                    const int qr = tile * TR + tr;
-                    if (qr < rq.rows) {
-                        const int i = qr / a.share;
-                        store(static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
-                                  static_cast<int64_t>(head * a.share + qr - i * a.share) * a.o_head + d,
-                              L == 0.f ? 0.f : O / L);
-                    }
+                const int tr = nt * 8 + row, qr = tile_now * TR + tr;
+                if (qr >= now.rows) continue;
+                if (starts && ends) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] = L == 0.f ? 0.f : o[v] / L;
+                    store<T, V>(out_row<T, V>(a, now, head_now, qr), o);
                 } else {
-                    part[TR * 2 + tr * D + d] = O;
-                    if (d == 0) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) part[TR * 2 + tr * D + V * lane + v] = o[v];
+                    if (lane == 0) {
                         part[2 * tr] = M;
                         part[2 * tr + 1] = L;
                     }
@@ -749,7 +817,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             }
             __syncthreads();
         }
-        f = end;
     }
     if (late) {
         // let the copies in flight land before the shared memory is given back (a slot without one waits in vain)
@@ -766,7 +833,8 @@ constexpr int kJoinWarps = 32;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
     constexpr int TR = 8 * NT, kDeal = kJoinWarps / TR, V = D / 32, PF = part_floats<D, TR>();
-    __shared__ float s_o[kDeal][TR][D], s_l[kDeal][TR], s_m[kDeal][TR];
+    __shared__ __align__(16) float s_o[kDeal][TR][D];
+    __shared__ float s_l[kDeal][TR], s_m[kDeal][TR];
     pdl_launch_dependents();
     pdl_wait();
     const int4 cut = a.cuts[blockIdx.x];
@@ -790,8 +858,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
                 const float* p = parts + (c ? 2 * static_cast<size_t>(c) * PF : PF);
                 m[j] = p[2 * row];
                 l[j] = p[2 * row + 1];
-#pragma unroll
-                for (int v = 0; v < V; ++v) x[j][v] = p[2 * TR + row * D + V * lane + v];
+                load<V>(x[j], p + 2 * TR + row * D + V * lane);
             } else {
 #pragma unroll
                 for (int v = 0; v < V; ++v) x[j][v] = 0.f;
@@ -823,23 +890,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
     const Request rq = request<TR>(a, cut.x);
     if (rq.rows == 0) return;
     const int head = cut.y / rq.tiles, tile = cut.y - head * rq.tiles;
-    for (int x = threadIdx.x; x < TR * D; x += kJoinWarps * 32) {
-        const int tr = x / D, d = x % D, qr = tile * TR + tr;
-        if (qr >= rq.rows) break;
-        float top = kNoMax, sum = 0.f, val = 0.f;
+    const int tr = threadIdx.x >> 5, qr = tile * TR + tr;
+    if (tr >= TR || qr >= rq.rows) return;
+    float top = kNoMax, sum = 0.f, val[V];
 #pragma unroll
-        for (int k = 0; k < kDeal; ++k) top = fmaxf(top, s_m[k][tr]);
+    for (int k = 0; k < kDeal; ++k) top = fmaxf(top, s_m[k][tr]);
 #pragma unroll
-        for (int k = 0; k < kDeal; ++k) {
-            const float w = exp2_fast(s_m[k][tr] - top);
-            sum = fmaf(w, s_l[k][tr], sum);
-            val = fmaf(w, s_o[k][tr][d], val);
-        }
-        const int i = qr / a.share;
-        store(static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
-                  static_cast<int64_t>(head * a.share + qr - i * a.share) * a.o_head + d,
-              sum == 0.f ? 0.f : val / sum);
+    for (int v = 0; v < V; ++v) val[v] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kDeal; ++k) {
+        const float w = exp2_fast(s_m[k][tr] - top);
+        float x[V];
+        load<V>(x, s_o[k][tr] + V * lane);
+        sum = fmaf(w, s_l[k][tr], sum);
+#pragma unroll
+        for (int v = 0; v < V; ++v) val[v] = fmaf(w, x[v], val[v]);
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) val[v] = sum == 0.f ? 0.f : val[v] / sum;
+    store<T, V>(out_row<T, V>(a, rq, head, qr), val);
 }
 
 int grid_ctas(int nt) { return ctas_per_sm(nt) * ecq_dev::sm_count_cached(); }
