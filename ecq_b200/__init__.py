@@ -19,23 +19,20 @@ PROB_SCALE = 1 << PROB_BITS
 RANS_BYTE_L = 1 << 23
 
 
+# GPU-side modules import torch; they are loaded when one of their names is first used
+_LAZY = {
+    "device": ("DeviceMatrix", "Packed4Matrix", "device_info"),
+    "interleaved": ("interleaved_rans_decode", "InterleavedRANSDecoder", "CudaInterleavedRANS", "verify_interleaved_roundtrip"),
+    "ops": ("entropy_coded_matmul", "EntropyCodedLinear", "rans_gemv", "rans_matmul"),
+    "strategies": ("SmartDecoder", "DecodeMode", "DecodedWeights"),
+    "kv4": ("KV4Cache", "KV4Step", "kv4_pages", "kv4_extend", "kv4_release", "kv4_append", "kv4_gather", "kv4_attention"),
+}
+
+
 def __getattr__(name):
-    # GPU-side modules import torch; load them on first use
-    if name in ("DeviceMatrix", "Packed4Matrix", "device_info"):
-        from . import device
-        return getattr(device, name)
-    if name in ("interleaved_rans_decode", "InterleavedRANSDecoder", "CudaInterleavedRANS",
-                "verify_interleaved_roundtrip"):
-        from . import interleaved
-        return getattr(interleaved, name)
-    if name in ("entropy_coded_matmul", "EntropyCodedLinear", "rans_gemv", "rans_matmul"):
-        from . import ops
-        return getattr(ops, name)
-    if name in ("SmartDecoder", "DecodeMode", "DecodedWeights"):
-        from . import strategies
-        return getattr(strategies, name)
-    if name in ("KV4Cache", "KV4Step", "kv4_pages", "kv4_extend", "kv4_release", "kv4_append", "kv4_gather",
-                "kv4_attention"):
-        from . import kv4
-        return getattr(kv4, name)
+    for module, names in _LAZY.items():
+        if name in names:
+            from importlib import import_module
+            value = globals()[name] = getattr(import_module(f".{module}", __name__), name)
+            return value
     raise AttributeError(name)

@@ -18,6 +18,7 @@ set bits of the ``status`` word.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -26,7 +27,9 @@ from . import _lib
 from ._lib import EcqError, check, lib
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
-_stream = torch.cuda.current_stream
+_I32 = torch.int32
+_U8 = torch.uint8
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without an object for it
 
 
 class KV4Step(NamedTuple):
@@ -39,52 +42,88 @@ class KV4Step(NamedTuple):
     free_count: torch.Tensor  # [1] pages left on the free stack
 
 
-def _same_device(first: torch.Tensor, **others) -> None:
-    if not first.is_cuda:
+# A step of a small model is a few microseconds of GPU time per call, so the
+# checks are written to cost little: plain comparisons, device numbers instead
+# of device objects, sizes from a cache.
+
+def _device(first: torch.Tensor, names: str, *others) -> int:
+    """The device number that all tensors share."""
+    d = first.get_device()
+    if d < 0:
         raise ValueError("the 4-bit KV cache runs on CUDA tensors only")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+    for i, t in enumerate(others):
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"{names.split()[i]} is on {t.device}, not on {first.device}")
+    return d
 
 
-def _int32(name: str, t: torch.Tensor, shape=None) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+def _on(device: int, fn, *args) -> int:
+    """fn(*args, stream) with `device` current (a launch needs that)."""
+    if torch.cuda.current_device() == device:
+        return fn(*args, _raw_stream(device))
+    with torch.cuda.device(device):
+        return fn(*args, _raw_stream(device))
 
 
-def _table(block_table: torch.Tensor, batch: int) -> None:
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+def _int32(name: str, t: torch.Tensor, n: int | None = None) -> None:
+    if t.dtype != _I32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 with one dimension")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, not {t.shape[0]}")
+
+
+def _table(block_table: torch.Tensor, batch: int) -> tuple[int, int]:
+    """Row stride and columns."""
+    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.shape[0] != batch:
         raise ValueError(f"block_table must be int32 [{batch}, pages per request]")
-    if block_table.shape[1] < 1 or block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
+    stride, cols = block_table.stride(), block_table.shape[1]
+    if batch == 1:  # a single row's stride says nothing
+        stride = (max(stride[0], cols), stride[1])
+    if cols < 1 or (stride[1] != 1 and cols > 1) or stride[0] < cols:
         raise ValueError("block_table needs contiguous rows of at least one page")
+    return stride[0], cols
 
 
 def _status(status) -> int | None:
     if status is None:
         return None
-    if status.dtype != torch.int32 or status.numel() < 1:
+    if status.dtype != _I32 or status.numel() < 1:
         raise ValueError("status must be int32 [1]")
     return status.data_ptr()
 
 
-def _page_size(pages: torch.Tensor, head_dim: int, group_size: int) -> int:
-    """The tokens per page of a pool, from its shape."""
-    if pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous():
-        raise ValueError("pages must be contiguous uint8 [pages, kv_heads, page bytes]")
+@lru_cache(maxsize=256)
+def _tokens_per_page(page_bytes: int, head_dim: int, group_size: int) -> int:
     block = check(lib().ecq_kv4_page_bytes(head_dim, 16, group_size), f"head_dim {head_dim}, group_size {group_size}")
-    size, rest = divmod(pages.shape[2], block)
+    size, rest = divmod(page_bytes, block)
     if rest or size not in (1, 2, 4, 8, 16):
-        raise ValueError(f"pages of {pages.shape[2]} bytes do not hold 16, 32, 64, 128 or 256 tokens of {block // 16} bytes")
+        raise ValueError(f"pages of {page_bytes} bytes do not hold 16, 32, 64, 128 or 256 tokens of {block // 16} bytes")
     return 16 * size
 
 
-def _rows(name: str, t: torch.Tensor) -> None:
-    if t.dim() != 3 or t.dtype not in _DTYPES:
+def _page_size(pages: torch.Tensor, head_dim: int, group_size: int) -> int:
+    """The tokens per page of a pool, from its shape."""
+    if pages.dtype != _U8 or pages.dim() != 3 or not pages.is_contiguous():
+        raise ValueError("pages must be contiguous uint8 [pages, kv_heads, page bytes]")
+    return _tokens_per_page(pages.shape[2], head_dim, group_size)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, heads: int, kv_heads: int, head_dim: int, max_q: int, max_pages: int, page_size: int,
+                     device: int) -> int:
+    return check(lib().ecq_kv4_attention_workspace_bytes(batch, heads, kv_heads, head_dim, max_q, max_pages, page_size),
+                 "kv4_attention")
+
+
+def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """Dtype code and the strides of tokens and heads."""
+    code = _DTYPES.get(t.dtype)
+    if t.dim() != 3 or code is None:
         raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, head_dim]")
-    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+    token, head, last = t.stride()
+    if t.numel() and (last != 1 or token % 8 or head % 8 or t.data_ptr() % 16):
         raise ValueError(f"{name}: head_dim must be contiguous, rows 16-byte aligned")
+    return code, token, head
 
 
 def kv4_pages(n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, group_size: int = 64,
@@ -109,28 +148,29 @@ def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     filled with -1 behind the last, so a captured step keeps its shapes. All
     or nothing: if pages, room or lengths do not suffice nothing changes, every
     slot is -1 and ``status`` says so."""
-    _same_device(seq_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count,
-                 seq_lens_out=seq_lens_out, free_count_out=free_count_out, status=status)
-    batch = seq_lens.numel()
-    _int32("seq_lens", seq_lens, (batch,))
-    _int32("new_lens", new_lens, (batch,))
-    _int32("free_pages", free_pages, (free_pages.numel(),))
-    _int32("free_count", free_count, (1,))
-    _table(block_table, batch)
+    device = _device(seq_lens, "new_lens block_table free_pages free_count seq_lens_out free_count_out status", new_lens,
+                     block_table, free_pages, free_count, seq_lens_out, free_count_out, status)
+    batch = seq_lens.shape[0] if seq_lens.dim() else 0
+    _int32("seq_lens", seq_lens, batch)
+    _int32("new_lens", new_lens, batch)
+    _int32("free_pages", free_pages)
+    _int32("free_count", free_count, 1)
+    stride, cols = _table(block_table, batch)
     if max_tokens < 0:
         raise ValueError("max_tokens is negative")
-    lens_out = torch.empty_like(seq_lens) if seq_lens_out is None else seq_lens_out
-    count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
-    _int32("seq_lens_out", lens_out, (batch,))
-    _int32("free_count_out", count_out, (1,))
-    out = torch.empty(batch + 1 + 2 * max_tokens, dtype=torch.int32, device=seq_lens.device)
-    starts, slots, positions = out[:batch + 1], out[batch + 1:batch + 1 + max_tokens], out[batch + 1 + max_tokens:]
-    with torch.cuda.device(seq_lens.device):
-        check(lib().ecq_kv4_extend(seq_lens.data_ptr(), new_lens.data_ptr(), lens_out.data_ptr(),
-                                   block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, page_size,
-                                   free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-                                   count_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                                   max_tokens, _status(status), _stream().cuda_stream), "kv4_extend")
+    out = torch.empty(2 * batch + 2 + 2 * max_tokens, dtype=_I32, device=seq_lens.device)
+    starts, slots, positions, lens_out, count_out = out.split_with_sizes((batch + 1, max_tokens, max_tokens, batch, 1))
+    if seq_lens_out is not None:
+        _int32("seq_lens_out", seq_lens_out, batch)
+        lens_out = seq_lens_out
+    if free_count_out is not None:
+        _int32("free_count_out", free_count_out, 1)
+        count_out = free_count_out
+    at = out.data_ptr()
+    check(_on(device, lib().ecq_kv4_extend, seq_lens.data_ptr(), new_lens.data_ptr(), lens_out.data_ptr(),
+              block_table.data_ptr(), stride, cols, batch, page_size, free_pages.data_ptr(), free_pages.shape[0],
+              free_count.data_ptr(), count_out.data_ptr(), at, at + 4 * (batch + 1), at + 4 * (batch + 1 + max_tokens),
+              max_tokens, _status(status)), "kv4_extend")
     return KV4Step(lens_out, starts, slots, positions, count_out)
 
 
@@ -141,24 +181,22 @@ def kv4_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.T
     """Push the pages of the requests where ``done`` (bool [batch]) on
     free_pages (in place) and set their lengths to 0. Returns the lengths and
     the count of free pages, as new tensors or in the ``_out`` ones."""
-    _same_device(seq_lens, done=done, block_table=block_table, free_pages=free_pages, free_count=free_count,
-                 seq_lens_out=seq_lens_out, free_count_out=free_count_out, status=status)
-    batch = seq_lens.numel()
-    _int32("seq_lens", seq_lens, (batch,))
-    if done.dtype not in (torch.bool, torch.uint8) or tuple(done.shape) != (batch,) or not done.is_contiguous():
+    device = _device(seq_lens, "done block_table free_pages free_count seq_lens_out free_count_out status", done,
+                     block_table, free_pages, free_count, seq_lens_out, free_count_out, status)
+    batch = seq_lens.shape[0] if seq_lens.dim() else 0
+    _int32("seq_lens", seq_lens, batch)
+    if done.dtype not in (torch.bool, _U8) or done.dim() != 1 or done.shape[0] != batch or not done.is_contiguous():
         raise ValueError(f"done must be contiguous bool [{batch}]")
-    _int32("free_pages", free_pages, (free_pages.numel(),))
-    _int32("free_count", free_count, (1,))
-    _table(block_table, batch)
+    _int32("free_pages", free_pages)
+    _int32("free_count", free_count, 1)
+    stride, cols = _table(block_table, batch)
     lens_out = torch.empty_like(seq_lens) if seq_lens_out is None else seq_lens_out
     count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
-    _int32("seq_lens_out", lens_out, (batch,))
-    _int32("free_count_out", count_out, (1,))
-    with torch.cuda.device(seq_lens.device):
-        check(lib().ecq_kv4_release(done.data_ptr(), seq_lens.data_ptr(), lens_out.data_ptr(), block_table.data_ptr(),
-                                    block_table.stride(0), block_table.shape[1], batch, page_size,
-                                    free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-                                    count_out.data_ptr(), _status(status), _stream().cuda_stream), "kv4_release")
+    _int32("seq_lens_out", lens_out, batch)
+    _int32("free_count_out", count_out, 1)
+    check(_on(device, lib().ecq_kv4_release, done.data_ptr(), seq_lens.data_ptr(), lens_out.data_ptr(),
+              block_table.data_ptr(), stride, cols, batch, page_size, free_pages.data_ptr(), free_pages.shape[0],
+              free_count.data_ptr(), count_out.data_ptr(), _status(status)), "kv4_release")
     return lens_out, count_out
 
 
@@ -168,23 +206,21 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slots: tor
     strides with contiguous 16-byte aligned rows) in 4 bits at slots [tokens]
     (int32, distinct; negative: not stored). slots may be longer than k, as a
     padded step's are: the rest is not looked at."""
-    _rows("k", k)
-    _rows("v", v)
+    code, k_token, k_head = _rows("k", k)
+    _, v_token, v_head = _rows("v", v)
     if k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v must have one shape and type")
-    _same_device(k, v=v, pages=pages, slots=slots, status=status)
+    device = _device(k, "v pages slots status", v, pages, slots, status)
     tokens, heads, dim = k.shape
     page_size = _page_size(pages, dim, group_size)
     if pages.shape[1] != heads:
         raise ValueError(f"k has {heads} heads, the pool {pages.shape[1]}")
     _int32("slots", slots)
-    if slots.dim() != 1 or slots.numel() < tokens:
+    if slots.shape[0] < tokens:
         raise ValueError(f"slots must have at least {tokens} entries")
-    with torch.cuda.device(k.device):
-        check(lib().ecq_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                   _DTYPES[k.dtype], pages.data_ptr(), pages.shape[0], heads, dim, page_size,
-                                   group_size, slots.data_ptr(), tokens, _status(status), _stream().cuda_stream),
-              "kv4_append")
+    check(_on(device, lib().ecq_kv4_append, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, code,
+              pages.data_ptr(), pages.shape[0], heads, dim, page_size, group_size, slots.data_ptr(), tokens,
+              _status(status)), "kv4_append")
 
 
 def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, *, group_size: int = 64,
@@ -192,18 +228,16 @@ def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, *, group
                status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows at slots [n] (int32) as k, v [n, kv_heads, head_dim] of dtype:
     code * scale + zero, rounded once; zeros for negative slots."""
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("dtype must be float16 or bfloat16")
-    _same_device(pages, slots=slots, status=status)
+    device = _device(pages, "slots status", slots, status)
     page_size = _page_size(pages, head_dim, group_size)
     _int32("slots", slots)
-    n = slots.numel()
-    k = torch.empty(n, pages.shape[1], head_dim, dtype=dtype, device=pages.device)
-    v = torch.empty_like(k)
-    with torch.cuda.device(pages.device):
-        check(lib().ecq_kv4_gather(k.data_ptr(), v.data_ptr(), _DTYPES[dtype], pages.data_ptr(), pages.shape[0],
-                                   pages.shape[1], head_dim, page_size, group_size, slots.data_ptr(), n,
-                                   _status(status), _stream().cuda_stream), "kv4_gather")
+    n, heads = slots.shape[0], pages.shape[1]
+    k, v = torch.empty((2, n, heads, head_dim), dtype=dtype, device=pages.device).unbind()
+    check(_on(device, lib().ecq_kv4_gather, k.data_ptr(), v.data_ptr(), code, pages.data_ptr(), pages.shape[0], heads,
+              head_dim, page_size, group_size, slots.data_ptr(), n, _status(status)), "kv4_gather")
     return k, v
 
 
@@ -221,39 +255,37 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     their request, each sees the tokens up to its own. scale: 1 / sqrt(head_dim)
     by default. Rows that see nothing (length 0) are 0; rows at or behind
     q_starts[-1] are left as they were in ``out``."""
-    _rows("q", q)
-    _same_device(q, pages=pages, block_table=block_table, seq_lens=seq_lens, q_starts=q_starts, out=out, status=status)
+    code, q_token, q_head = _rows("q", q)
+    device = _device(q, "pages block_table seq_lens q_starts out status", pages, block_table, seq_lens, q_starts, out, status)
     tokens, heads, dim = q.shape
     page_size = _page_size(pages, dim, group_size)
-    kv_heads = pages.shape[1]
+    n_pages, kv_heads, _ = pages.shape
     if heads % kv_heads or heads < kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} cache heads evenly")
-    batch = seq_lens.numel()
-    _int32("seq_lens", seq_lens, (batch,))
-    _table(block_table, batch)
+    _int32("seq_lens", seq_lens)
+    batch = seq_lens.shape[0]
+    stride, cols = _table(block_table, batch)
     if q_starts is not None:
-        _int32("q_starts", q_starts, (batch + 1,))
+        _int32("q_starts", q_starts, batch + 1)
     elif tokens != batch or max_q != 1:
         raise ValueError("without q_starts every request has one query")
     if max_q < 1:
         raise ValueError("max_q must be at least 1")
     if out is None:
-        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must have q's shape and type")
-    elif out.numel() and (out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8):
-        raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
-    L = lib()
-    need = check(L.ecq_kv4_attention_workspace_bytes(batch, heads, kv_heads, dim, max_q, block_table.shape[1], page_size),
-                 "kv4_attention")
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        check(L.ecq_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                  _DTYPES[q.dtype], pages.data_ptr(), pages.shape[0], heads, kv_heads, dim, page_size,
-                                  group_size, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                                  seq_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), batch, tokens,
-                                  max_q, dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _status(status),
-                                  _stream().cuda_stream), "kv4_attention")
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        o_token, o_head = heads * dim, dim
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and type")
+        o_token, o_head, last = out.stride()
+        if out.numel() and (last != 1 or o_token % 4 or o_head % 4 or out.data_ptr() % 8):
+            raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
+    need = _workspace_bytes(batch, heads, kv_heads, dim, max_q, cols, page_size, device)
+    ws = torch.empty(need, dtype=_U8, device=q.device)
+    check(_on(device, lib().ecq_kv4_attention, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, code,
+              pages.data_ptr(), n_pages, heads, kv_heads, dim, page_size, group_size, block_table.data_ptr(), stride, cols,
+              seq_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), batch, tokens, max_q,
+              dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _status(status)), "kv4_attention")
     return out
 
 
