@@ -22,7 +22,7 @@ OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libecq.so"
 
 SOURCES = ["ecq_device.cu", "ecq_matmul.cu", "ecq_plain4.cu", "ecq_comm.cu", "ecq_glue.cu", "ecq_attention.cu", "ecq_kv4.cu",
-           "ecq_kv4_attention.cu", "ecq_host.cpp"]
+           "ecq_kv4_attention.cu", "ecq_kv4_prompt.cu", "ecq_host.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

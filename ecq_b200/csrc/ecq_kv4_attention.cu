@@ -30,7 +30,7 @@
 // do not depend on timing.
 #include <cuda_runtime.h>
 
-#include "ecq_kv4.cuh"
+#include "ecq_kv4_attention.cuh"
 
 namespace {
 
@@ -60,19 +60,6 @@ __host__ __device__ constexpr int ring_slots(int dim, int groups) {
     return n < 4 ? n : 4;
 }
 
-struct Args {
-    const void* q;
-    void* out;
-    const uint8_t* pages;
-    const int32_t *table, *lens, *starts;
-    float* parts;     // per CTA two parts: one that starts inside a pair, one that starts a pair and does not end it
-    int4* cuts;       // per CTA: request, pair, CTAs that follow; x < 0: none
-    int32_t* status;
-    int64_t q_token, q_head, o_token, o_head, n_pages, table_stride;
-    int kv_heads, share, page_shift, max_pages, batch, total_q;
-    float scale;
-};
-
 // One request's part of the work.
 struct Request {
     int first_q, queries, rows, len, units, tiles, pairs;
@@ -80,26 +67,8 @@ struct Request {
 
 template <int TR>  // rows per tile
 __device__ __forceinline__ Request request(const Args& a, int b) {
-    Request r;
-    int lo = b, hi = b + 1;
-    if (a.starts) {
-        lo = a.starts[b];
-        hi = a.starts[b + 1];
-        if (lo < 0 || hi < lo || hi > a.total_q) {
-            raise_status(a.status, ECQ_STATUS_BADARG);
-            lo = hi = 0;
-        }
-    }
-    r.len = a.lens[b];
-    const long long room = static_cast<long long>(a.max_pages) << a.page_shift;
-    if (r.len > room) {
-        raise_status(a.status, ECQ_STATUS_BADARG);
-        r.len = static_cast<int>(room);
-    }
-    r.len = max(r.len, 0);
-    r.first_q = lo;
-    r.queries = hi - lo;
-    r.rows = r.queries * a.share;
+    const Range x = range_of(a, b);
+    Request r = {x.first_q, x.queries, x.rows > a.most_rows ? 0 : x.rows, x.len, 0, 0, 0};
     r.tiles = (r.rows + TR - 1) / TR;
     r.pairs = r.tiles * a.kv_heads;
     // a request without keys has one (empty) unit, so that its rows are written
@@ -138,17 +107,6 @@ __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 f2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-
 // N words at shared address addr + kAt
 template <int N, int kAt>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t addr) {
@@ -163,15 +121,6 @@ __device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t addr) {
     }
 }
 
-__device__ __forceinline__ float2 cvt2(uint32_t u, __half) { return f2(u); }
-__device__ __forceinline__ float2 cvt2(uint32_t u, __nv_bfloat16) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) { return h2(a, b); }
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 // V neighbouring channels
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&x)[V]) {
@@ -188,14 +137,6 @@ __device__ __forceinline__ void load(float (&x)[V], const float* p) {
         x[0] = v.x, x[1] = v.y;
     }
 }
-// Row `row` of a (request, head): its channels V * lane .. in the output.
-template <typename T, int V>
-__device__ __forceinline__ T* out_row(const Args& a, const Request& rq, int head, int row) {
-    const int i = row / a.share;
-    return static_cast<T*>(a.out) + static_cast<int64_t>(rq.first_q + i) * a.o_token +
-           static_cast<int64_t>(head * a.share + row - i * a.share) * a.o_head + V * (threadIdx.x & 31);
-}
-
 // The query rows of one tile as B operands, and what their scores need.
 template <int D, int G, int NT>
 struct Rows {
@@ -805,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 if (starts && ends) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) o[v] = L == 0.f ? 0.f : o[v] / L;
-                    store<T, V>(out_row<T, V>(a, now, head_now, qr), o);
+                    store<T, V>(out_row<T>(a, now.first_q, head_now, qr) + V * lane, o);
                 } else {
 #pragma unroll
                     for (int v = 0; v < V; ++v) part[TR * 2 + tr * D + V * lane + v] = o[v];
@@ -908,10 +849,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) val[v] = sum == 0.f ? 0.f : val[v] / sum;
-    store<T, V>(out_row<T, V>(a, rq, head, qr), val);
+    store<T, V>(out_row<T>(a, rq.first_q, head, qr) + V * lane, val);
 }
 
 int grid_ctas(int nt) { return ctas_per_sm(nt) * ecq_dev::sm_count_cached(); }
+
+// Requests with up to so many rows (queries times heads that share a cache
+// head) are streamed by attention_kernel, those with more are the prompt
+// kernel's; a call that may have such launches both.
+constexpr int kStreamRows = 64;
 
 // 16-row tiles where a request may have more than 8 rows: one pass over the
 // keys for twice the rows.
@@ -958,6 +904,7 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (static_cast<int64_t>(max_pages) * page_size >= (1ll << 31) - 256) return ECQ_ERR_ARG;
     if (!q_starts && (total_q != batch || max_q != 1)) return ECQ_ERR_ARG;
     if (total_q == 0) return ECQ_OK;
+    if (static_cast<int64_t>(total_q) * (heads / kv_heads) >= (1ll << 31)) return ECQ_ERR_UNSUPPORTED;
     if (!q || !out || !aligned(q, 16) || !aligned(out, 8)) return ECQ_ERR_ARG;
     if (((q_token_stride | q_head_stride) & 7) || ((out_token_stride | out_head_stride) & 3)) return ECQ_ERR_ARG;
     if (workspace_bytes < need || !workspace || !aligned(workspace, 16)) return ECQ_ERR_WORKSPACE;
@@ -984,6 +931,12 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     a.batch = batch;
     a.total_q = total_q;
     a.scale = scale;
+    const bool prompts = static_cast<int64_t>(a.share) * max_q > kStreamRows;
+    a.most_rows = prompts ? kStreamRows : INT32_MAX;
+    if (prompts) {
+        const int32_t rc = launch_prompt(a, dtype, head_dim, head_dim / group_size, max_q, static_cast<cudaStream_t>(stream));
+        if (rc != ECQ_OK) return rc;
+    }
     const int nt = row_tiles_of_8(a.share, max_q);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);

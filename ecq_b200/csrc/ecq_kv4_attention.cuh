@@ -1,0 +1,77 @@
+// ecq_kv4_attention.cuh -- what the attention kernels over the 4-bit KV cache
+// share: their arguments, a request's part of the work, conversions and the
+// launch of the one for prompts.
+#pragma once
+
+#include "ecq_kv4.cuh"
+
+namespace ecq_kv4 {
+
+struct Args {
+    const void* q;
+    void* out;
+    const uint8_t* pages;
+    const int32_t *table, *lens, *starts;
+    float* parts;     // per CTA two parts: one that starts inside a pair, one that starts a pair and does not end it
+    int4* cuts;       // per CTA: request, pair, CTAs that follow; x < 0: none
+    int32_t* status;
+    int64_t q_token, q_head, o_token, o_head, n_pages, table_stride;
+    int kv_heads, share, page_shift, max_pages, batch, total_q;
+    int most_rows;    // requests with more rows (queries times share) are the prompt kernel's
+    float scale;
+};
+
+// A request's queries and keys, as far as they are sound.
+struct Range {
+    int first_q, queries, rows, len;
+};
+__device__ __forceinline__ Range range_of(const Args& a, int b) {
+    int lo = b, hi = b + 1;
+    if (a.starts) {
+        lo = a.starts[b];
+        hi = a.starts[b + 1];
+        if (lo < 0 || hi < lo || hi > a.total_q) {
+            raise_status(a.status, ECQ_STATUS_BADARG);
+            lo = hi = 0;
+        }
+    }
+    int len = a.lens[b];
+    const long long room = static_cast<long long>(a.max_pages) << a.page_shift;
+    if (len > room) {
+        raise_status(a.status, ECQ_STATUS_BADARG);
+        len = static_cast<int>(room);
+    }
+    return {lo, hi - lo, (hi - lo) * a.share, max(len, 0)};
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+__device__ __forceinline__ float2 cvt2(uint32_t u, __half) { return f2(u); }
+__device__ __forceinline__ float2 cvt2(uint32_t u, __nv_bfloat16) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) { return h2(a, b); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Row `row` of a (request, head) in the output.
+template <typename T>
+__device__ __forceinline__ T* out_row(const Args& a, int first_q, int head, int row) {
+    const int i = row / a.share;
+    return static_cast<T*>(a.out) + static_cast<int64_t>(first_q + i) * a.o_token +
+           static_cast<int64_t>(head * a.share + row - i * a.share) * a.o_head;
+}
+
+int32_t launch_prompt(const Args& a, int dtype, int head_dim, int groups, int max_q, cudaStream_t stream);
+
+}  // namespace ecq_kv4

@@ -1,0 +1,605 @@
+// ecq_kv4_prompt.cu -- attention of many query rows (prompt chunks) over the
+// 4-bit KV cache, on the tcgen05 tensor cores.
+//
+// A CTA takes 256 rows (queries x heads that share a cache head) of one
+// (request, cache head) as two tiles of 128 and walks the keys 64 at a time:
+//   loader   one warp copies the packed blocks of 16 tokens into a ring
+//            (cp.async.bulk, a lane per block, its page number read one step
+//            ahead);
+//   decoders four warps turn codes into fp16 K [64 x D] and V^T [D x 64] in the
+//            tensor core's K-major, no-swizzle layout: code * scale + zero,
+//            rounded once to fp16, shared by all 256 rows;
+//   MMA      one thread issues S = Q K^T (A = Q in tensor memory) and O += P V
+//            (A = P in tensor memory) for the two tiles in turn, so that one
+//            tile's softmax runs beside the other's products;
+//   softmax  four warps per tile, a thread per row: S from tensor memory, running
+//            maximum (raised only when a score passes it by 2^8: then the row's
+//            O is rescaled), exp2, P as fp16 over S's place, sums in fp32.
+// Tensor memory (512 columns): Q, S and O of both tiles.
+//
+// fp16 for K, V and P costs a relative 2^-11 on each, next to the output's own
+// rounding; q is brought to its row's power of two and keeps its bits. What
+// bounds it: the exponentials (16 a cycle and SM) and the products take the
+// same time per step at D = 128; the decoding of K and V runs beside them.
+//
+// Masks. Keys beyond a row's own are chosen away in S. A V row whose scale or
+// zero is not finite would reach rows that do not see it (0 * NaN), so it
+// enters as 0 and the first such token per group of channels is remembered:
+// rows that see it get NaN there at the end. Keys of a page whose number is bad
+// are left out.
+//
+// Every wait is bounded and looks at a flag that a wait sets which gave up; all
+// roles then leave, and tensor memory is given back after the products in
+// flight.
+#include <cuda_runtime.h>
+
+#include "ecq_kv4_attention.cuh"
+
+namespace {
+
+using namespace ecq_kv4;
+using ecq_dev::bulk_copy_g2s;
+using ecq_dev::fence_proxy_async;
+using ecq_dev::mbar_expect_tx;
+using ecq_dev::mbar_init;
+using ecq_dev::smem_addr;
+
+constexpr int kKeys = 64;                       // keys a step
+constexpr int kTileBlocks = kKeys / kBlockTokens;
+constexpr int kRows = 128, kCtaRows = 2 * kRows;
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
+constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 2) * 32;
+constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
+constexpr int kRing = 4;
+constexpr uint32_t kTmemColumns = 512;
+constexpr float kSlack = 8.f;  // P is at most 2^8
+constexpr float kNoMax = -1e30f;
+
+template <int D, int G>
+struct Smem {
+    static constexpr int kPacked = kTileBlocks * block_bytes(D, G);
+    // K: core columns of 8 channels, 64 keys of 16 bytes each; 32 more bytes put a warp's stores in different banks
+    static constexpr uint32_t kLboK = kKeys * 16 + 32, kBytesK = D / 8 * kLboK;
+    static constexpr uint32_t kLboV = D * 16, kBytesV = kKeys / 8 * kLboV;
+    static constexpr int kRingAt = 0, kAtK = kRing * kPacked, kAtV = kAtK + 2 * kBytesK, kBytes = kAtV + 2 * kBytesV;
+};
+
+// Tensor memory columns of tile x
+template <int D>
+struct Tmem {
+    static __device__ constexpr uint32_t q(int x) { return x * (D / 2); }
+    static __device__ constexpr uint32_t s(int x) { return 128 + x * kKeys; }
+    static __device__ constexpr uint32_t o(int x) { return 256 + x * 128; }
+};
+
+struct Control {
+    uint64_t packed_full[kRing], packed_empty[kRing];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    uint32_t tmem, gave_up;
+    uint32_t hidden[8];  // by step: a bit per block where nothing is, or a bad page (the loader is at most 5 steps ahead of a softmax)
+    int poison[4];           // per group: the first token whose V is not finite
+};
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ uint64_t kmajor(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>((lbo >> 4) & 0x3fffu) << 16) |
+           (static_cast<uint64_t>((sbo >> 4) & 0x3fffu) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* v) {  // 32 columns of this thread's lane
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t lds1(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint4 lds4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint2 lds2(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+
+// Waits for a phase of bar; false (and everybody told) after the limit, or
+// where another wait gave up.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, int32_t* status) {
+    if (ecq_dev::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = ecq_dev::global_timer_ns();
+    for (;;) {
+        if (ecq_dev::mbar_try_wait(bar, parity)) return true;
+        if (*gave_up) return false;
+        if (ecq_dev::global_timer_ns() - t0 > ecq_dev::kWaitLimitNs) {
+            *gave_up = 1u;
+            raise_status(status, ECQ_STATUS_TIMEOUT);
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t hfma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t hadd(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// code * scale + zero of the nibbles at bits 0..3 (low) or 4..7 of both halves
+// of x: a nibble in the mantissa of 1024 is 1024 + code (or 1024 + 16 code),
+// what takes that off is exact, and the fma rounds once.
+__device__ __forceinline__ uint32_t value_low(uint32_t x, uint32_t scale, uint32_t zero) {
+    return hfma(hadd((x & 0x000f000fu) | 0x64006400u, 0xe400e400u), scale, zero);
+}
+__device__ __forceinline__ uint32_t value_high(uint32_t x, uint32_t scale, uint32_t zero) {
+    return hfma(hfma((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u), scale, zero);
+}
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const int tiles) {
+    using S = Smem<D, G>;
+    using M = Tmem<D>;
+    constexpr int BB = block_bytes(D, G);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Control ctl;
+    const int lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    volatile uint32_t* gave_up = &ctl.gave_up;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(smem_addr(&ctl.packed_full[i]), kTileBlocks);
+            mbar_init(smem_addr(&ctl.packed_empty[i]), kDecodeWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&ctl.k_full[i]), kDecodeWarps * 32);
+            mbar_init(smem_addr(&ctl.v_full[i]), kDecodeWarps * 32);
+            mbar_init(smem_addr(&ctl.k_empty[i]), 1);
+            mbar_init(smem_addr(&ctl.v_empty[i]), 1);
+            mbar_init(smem_addr(&ctl.q_full[i]), kRows);
+            mbar_init(smem_addr(&ctl.s_full[i]), 1);
+            mbar_init(smem_addr(&ctl.p_full[i]), kRows);
+            mbar_init(smem_addr(&ctl.o_full[i]), 1);
+        }
+        mbar_init(smem_addr(&ctl.drained), 1);
+        ctl.gave_up = 0u;
+        for (int g = 0; g < 4; ++g) ctl.poison[g] = INT32_MAX;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&ctl.tmem)),
+                     "r"(kTmemColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tmem = ctl.tmem;
+    ecq_dev::pdl_launch_dependents();  // after the allocation: the next kernel may want tensor memory too
+    ecq_dev::pdl_wait();
+
+    // the last tiles, which see the most keys, first
+    const int per_tile = a.kv_heads * a.batch;
+    const int tile = tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
+    const int b = static_cast<int>(blockIdx.x % per_tile) / a.kv_heads, head = static_cast<int>(blockIdx.x % per_tile) % a.kv_heads;
+    const Range rq = range_of(a, b);
+    if (tile == tiles - 1 && threadIdx.x == 0 && rq.rows > a.most_rows && rq.queries > 0 &&
+        (rq.rows - 1) / kCtaRows >= tiles)
+        raise_status(a.status, ECQ_STATUS_BADARG);  // more queries than the call said: their rows are not computed
+    const bool work = rq.rows > a.most_rows && tile * kCtaRows < rq.rows;
+    // steps of the two tiles
+    int n[2] = {0, 0};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int first = tile * kCtaRows + x * kRows, last = min(rq.rows, first + kRows) - 1;
+        if (work && first < rq.rows) n[x] = (max(rq.len - rq.queries + last / a.share + 1, 0) + kKeys - 1) / kKeys;
+    }
+    const int steps = max(n[0], n[1]);
+    const uint32_t base = smem_addr(smem);
+
+    if (!work) {
+        // nothing of this request: straight to the end
+    } else if (warp < kSoftmaxWarps) {
+        // ---------------------------------------------------------------- softmax: a thread per row
+        const int x = warp / 4, row = tile * kCtaRows + x * kRows + (warp & 3) * 32 + lane;
+        const bool in = row < rq.rows;
+        const int i = row / a.share;
+        const uint32_t mine = tmem + ((warp & 3) << 21);  // lanes 32 (warp % 4) ..
+        const int limit = in ? rq.len - rq.queries + i + 1 : 0;
+        // q, in the order of a K row's decoded nibbles: of 8 channels 0 4 1 5 2 6 3 7
+        float factor;
+        {
+            const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
+                           static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head;
+            uint4 raw[D / 8];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                raw[c] = make_uint4(0, 0, 0, 0);
+                if (in) raw[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = cvt2(w[e], T());
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            }
+            const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
+            float up = __int_as_float((10 - ex + 127) << 23);
+            factor = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 10 + 127) << 23);
+            if (a.scale < 0.f) up = -up;
+            if (factor == 0.f) {
+                up = 0.f;
+                factor = 1.f;
+            }
+#pragma unroll
+            for (int part = 0; part < D / 64; ++part) {
+                uint32_t v[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    // decoded K: core column 4 w + t holds channels 32 w + 8 t ..: the natural order of groups of 8
+                    const uint4 u = raw[8 * part + c];
+                    const float2 f0 = cvt2(u.x, T()), f1 = cvt2(u.y, T()), f2 = cvt2(u.z, T()), f3 = cvt2(u.w, T());
+                    v[4 * c] = pack2(f0.x * up, f2.x * up, __half());
+                    v[4 * c + 1] = pack2(f0.y * up, f2.y * up, __half());
+                    v[4 * c + 2] = pack2(f1.x * up, f3.x * up, __half());
+                    v[4 * c + 3] = pack2(f1.y * up, f3.y * up, __half());
+                }
+                tmem_st(mine + M::q(x) + 32 * part, v);
+            }
+            wait_st();
+            before_sync();
+            mbar_arrive(smem_addr(&ctl.q_full[x]));
+        }
+        float m = kNoMax;
+        uint64_t l[2] = {0ull, 0ull};  // two pairs of sums
+        const uint64_t f2x = ecq_dev::pack2(__float_as_uint(factor), __float_as_uint(factor));
+        bool ok = true;
+#pragma unroll 1
+        for (int j = 0; j < n[x]; ++j) {
+            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.s_full[x]), j & 1, gave_up, a.status));
+            if (!ok) break;
+            after_sync();
+            uint32_t s[kKeys];
+            tmem_ld(mine + M::s(x), s);
+            tmem_ld(mine + M::s(x) + 32, s + 32);
+            wait_ld();
+            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
+            const int left = limit - j * kKeys;  // keys of this step that the row sees
+            if (__any_sync(0xffffffffu, left < kKeys) || hidden) {
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k)
+                    if (k >= left || (hidden >> (k / kBlockTokens) & 1u)) s[k] = 0xff800000u;
+            }
+            float top = __uint_as_float(s[0]);
+#pragma unroll
+            for (int k = 1; k < kKeys; ++k) top = fmaxf(top, __uint_as_float(s[k]));
+            top *= factor;
+            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                const float next = fmaxf(top, m), keep = exp2_fast(m - next);
+                m = next;
+                const uint64_t k2 = ecq_dev::pack2(__float_as_uint(keep), __float_as_uint(keep));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) l[u] = ecq_dev::fma2(l[u], k2, 0ull);
+                if (j) {  // the products so far are done: their completion came with S
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld(mine + M::o(x) + c, o);
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_st(mine + M::o(x) + c, o);
+                    }
+                }
+            }
+            const uint64_t m2 = ecq_dev::pack2(__float_as_uint(-m), __float_as_uint(-m));
+#pragma unroll
+            for (int k = 0; k < kKeys; k += 2) {
+                float e0, e1;
+                ecq_dev::unpack2(ecq_dev::fma2(ecq_dev::pack2(s[k], s[k + 1]), f2x, m2), e0, e1);
+                e0 = exp2_fast(e0);
+                e1 = exp2_fast(e1);
+                l[k / 2 % 2] = ecq_dev::add2(l[k / 2 % 2], ecq_dev::pack2(__float_as_uint(e0), __float_as_uint(e1)));
+                s[k / 2] = pack2(e0, e1, __half());
+            }
+            tmem_st(mine + M::s(x), s);
+            wait_st();
+            before_sync();
+            mbar_arrive(smem_addr(&ctl.p_full[x]));
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float e0, e1;
+            ecq_dev::unpack2(l[u], e0, e1);
+            sum += e0 + e1;
+        }
+        if (ok && n[x]) {
+            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.o_full[x]), 0, gave_up, a.status));
+            after_sync();
+        }
+        if (ok) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* dst = out_row<T>(a, rq.first_q, head, in ? row : 0);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (n[x]) {
+                    tmem_ld(mine + M::o(x) + c, o);
+                    wait_ld();
+                }
+                if (limit > ctl.poison[c * G / D]) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0x7fc00000u;
+                }
+                if (in) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = sum == 0.f ? 0.f : __uint_as_float(o[e + k]) * inv;
+                        *reinterpret_cast<uint2*>(dst + c + e) = make_uint2(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()));
+                    }
+                }
+            }
+        }
+    } else if (warp < kMmaWarp) {
+        // ---------------------------------------------------------------- decoders
+        const int tid = threadIdx.x - kSoftmaxWarps * 32;
+#pragma unroll 1
+        for (int j = 0; j < steps; ++j) {
+            const int slot = j % kRing, stage = j & 1;
+            bool ok = wait_for(smem_addr(&ctl.packed_full[slot]), (j / kRing) & 1, gave_up, a.status);
+            if (j >= 2) ok = wait_for(smem_addr(&ctl.k_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const uint32_t packed = base + S::kRingAt + slot * S::kPacked;
+            // K: key tid / 4 (and 32 more), a quarter of its channels
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int key = tid / 4 + 32 * half, t = tid & 3;
+                const uint32_t blk = packed + (key / kBlockTokens) * BB;
+                uint32_t w[D / 32], p[G];
+                const uint32_t at = blk + (key % kBlockTokens) * (D / 2) + t * (D / 8);
+                if constexpr (D == 128) {
+                    const uint4 u = lds4(at);
+                    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                } else {
+                    const uint2 u = lds2(at);
+                    w[0] = u.x, w[1] = u.y;
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) p[g] = lds1(blk + k_params_at(D) + (key % kBlockTokens) * 4 * G + 4 * g);
+                const uint32_t dst = base + S::kAtK + stage * S::kBytesK + (key / 8) * 128 + (key % 8) * 16;
+#pragma unroll
+                for (int q = 0; q < D / 32; ++q) {
+                    const uint32_t pg = p[q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
+                    const uint32_t y = w[q] >> 8;
+                    sts4(dst + (4 * q + t) * S::kLboK, value_low(w[q], sc, z), value_high(w[q], sc, z), value_low(y, sc, z),
+                         value_high(y, sc, z));
+                }
+            }
+            fence_proxy_async();
+            mbar_arrive(smem_addr(&ctl.k_full[stage]));
+            if (j >= 2) ok = wait_for(smem_addr(&ctl.v_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            // V: eight keys (a core column) of chunk r, one word (8 channels) of each at a time
+            constexpr int kWords = D / 64;              // words of a chunk
+            constexpr int kItems = kKeys / 8 * 8 * kWords;
+            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
+            const bool ragged = (j + 1) * kKeys > rq.len || hidden;
+            if (tid < kItems) {
+                const int wd = tid % kWords, r = tid / kWords % 8, kc = tid / kWords / 8;
+                const uint32_t blk = packed + (kc / 2) * BB;
+                const int tok = (kc & 1) * 8;
+                constexpr int kGroups = G * 64 / D > 0 ? G * 64 / D : 1;  // groups that a word's channels lie in
+                const int g0 = wd * 64 * G / D;
+                uint32_t w[8], sc[kGroups][4], z[kGroups][4];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = lds1(blk + v_codes_at(D) + (tok + k) * (D / 2) + r * (D / 16) + 4 * wd);
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    uint32_t p[8], probe = 0u;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        p[k] = lds1(blk + v_params_at(D, G) + (tok + k) * 4 * G + 4 * (g0 + g));
+                        if (ragged && (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u))) p[k] = 0u;
+                        probe = hfma(p[k], 0u, probe);  // 0, or NaN once something is not finite
+                    }
+                    if (probe & 0x7fff7fffu) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if ((p[k] & 0x7c00u) == 0x7c00u || (p[k] & 0x7c000000u) == 0x7c000000u) {
+                                p[k] = 0u;
+                                atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + k);
+                            }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        sc[g][k] = __byte_perm(p[2 * k], p[2 * k + 1], 0x5410);
+                        z[g][k] = __byte_perm(p[2 * k], p[2 * k + 1], 0x7632);
+                    }
+                }
+                const uint32_t dst = base + S::kAtV + stage * S::kBytesV + kc * S::kLboV + wd * 1024 + r * 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // nibbles 4 h .. 4 h + 3: channels 8 (8 wd + 4 h + i) + r
+                    uint32_t v[4][4];
+                    const int g = kGroups == 1 ? 0 : h * kGroups / 2;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t pair = __byte_perm(w[2 * k], w[2 * k + 1], h ? 0x7632 : 0x5410), y = pair >> 8;
+                        v[0][k] = value_low(pair, sc[g][k], z[g][k]);
+                        v[1][k] = value_high(pair, sc[g][k], z[g][k]);
+                        v[2][k] = value_low(y, sc[g][k], z[g][k]);
+                        v[3][k] = value_high(y, sc[g][k], z[g][k]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sts4(dst + (4 * h + e) * 128, v[e][0], v[e][1], v[e][2], v[e][3]);
+                }
+            }
+            fence_proxy_async();
+            mbar_arrive(smem_addr(&ctl.v_full[stage]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&ctl.packed_empty[slot]));
+        }
+    } else if (warp == kMmaWarp) {
+        // ---------------------------------------------------------------- products
+        if (lane == 0 && steps) {
+            // D fp32, A and B fp16, both K-major; N >> 3 at bit 17, M = 128 >> 4 at bit 24
+            constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
+            constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
+            auto scores = [&](int x, int j) {
+                const uint32_t k = base + S::kAtK + (j & 1) * S::kBytesK;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma_ts(tmem + M::s(x), tmem + M::q(x) + 8 * i, kmajor(k + 2 * i * S::kLboK, S::kLboK, 128), kIdescS, i != 0);
+                commit(smem_addr(&ctl.s_full[x]));
+            };
+            bool ok = wait_for(smem_addr(&ctl.k_full[0]), 0, gave_up, a.status);
+            for (int x = 0; x < 2 && ok; ++x) {
+                if (!n[x]) continue;
+                ok = wait_for(smem_addr(&ctl.q_full[x]), 0, gave_up, a.status);
+                after_sync();
+                if (ok) scores(x, 0);
+            }
+            if (ok) commit(smem_addr(&ctl.k_empty[0]));
+#pragma unroll 1
+            for (int j = 0; j < steps && ok; ++j) {
+                const int next = (j + 1) & 1;
+                ok = wait_for(smem_addr(&ctl.v_full[j & 1]), (j >> 1) & 1, gave_up, a.status);
+                if (ok && j + 1 < steps) ok = wait_for(smem_addr(&ctl.k_full[next]), ((j + 1) >> 1) & 1, gave_up, a.status);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || j >= n[x]) continue;
+                    ok = wait_for(smem_addr(&ctl.p_full[x]), j & 1, gave_up, a.status);
+                    if (!ok) continue;
+                    after_sync();
+                    const uint32_t v = base + S::kAtV + (j & 1) * S::kBytesV;
+#pragma unroll
+                    for (int i = 0; i < kKeys / 16; ++i)
+                        mma_ts(tmem + M::o(x), tmem + M::s(x) + 8 * i, kmajor(v + 2 * i * S::kLboV, S::kLboV, 128), kIdescO,
+                               (j | i) != 0);
+                    if (j + 1 == n[x]) commit(smem_addr(&ctl.o_full[x]));
+                    else scores(x, j + 1);
+                }
+                if (!ok) break;
+                commit(smem_addr(&ctl.v_empty[j & 1]));
+                if (j + 1 < steps) commit(smem_addr(&ctl.k_empty[next]));
+            }
+            // nothing is in flight when tensor memory is given back
+            commit(smem_addr(&ctl.drained));
+            ecq_dev::mbar_wait(smem_addr(&ctl.drained), 0);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- loader: a lane per block of the step
+        if (lane < kTileBlocks) {
+            const int shift = a.page_shift - 4;
+            const int64_t page_bytes = static_cast<int64_t>(BB) << shift;
+            const int32_t* row = a.table + b * a.table_stride;
+            auto page_of = [&](int j) {  // -1: no such tokens
+                const int blk = j * kTileBlocks + lane;
+                return j < steps && blk * kBlockTokens < rq.len ? __ldg(row + (blk >> shift)) & INT32_MAX : -1;
+            };
+            constexpr uint32_t kLanes = (1u << kTileBlocks) - 1u;
+            int page = page_of(0), j = 0;
+#pragma unroll 1
+            for (; j < steps; ++j) {
+                const int slot = j % kRing;
+                const uint32_t bar = smem_addr(&ctl.packed_full[slot]);
+                bool ok = true;
+                if (j >= kRing) ok = wait_for(smem_addr(&ctl.packed_empty[slot]), (j / kRing - 1) & 1, gave_up, a.status);
+                if (!__all_sync(kLanes, ok)) break;
+                const bool there = page >= 0 && page < a.n_pages;
+                if (page >= a.n_pages) raise_status(a.status, ECQ_STATUS_BADARG);
+                const uint32_t hidden = __ballot_sync(kLanes, !there);
+                if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]) = hidden;
+                __syncwarp(kLanes);
+                if (there) {
+                    const int blk = j * kTileBlocks + lane;
+                    mbar_expect_tx(bar, BB);
+                    bulk_copy_g2s(base + S::kRingAt + slot * S::kPacked + lane * BB,
+                                  a.pages + (static_cast<int64_t>(page) * a.kv_heads + head) * page_bytes +
+                                      (blk & ((1 << shift) - 1)) * BB,
+                                  BB, bar);
+                } else {
+                    mbar_expect_tx(bar, 0);
+                }
+                page = page_of(j + 1);
+            }
+            // no copy is in flight when the shared memory is given back
+            for (int i = max(j - kRing, 0); i < j; ++i) ecq_dev::mbar_wait(smem_addr(&ctl.packed_full[i % kRing]), (i / kRing) & 1);
+        }
+        __syncwarp();
+    }
+    before_sync();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+    }
+}
+
+}  // namespace
+
+namespace ecq_kv4 {
+
+int32_t launch_prompt(const Args& a, int dtype, int head_dim, int groups, int max_q, cudaStream_t stream) {
+    const int64_t tiles = (static_cast<int64_t>(a.share) * max_q + kCtaRows - 1) / kCtaRows;
+    const int64_t ctas = tiles * a.kv_heads * a.batch;
+    if (ctas > INT32_MAX) return ECQ_ERR_UNSUPPORTED;
+    return by_layout(dtype, head_dim, groups, [&](auto layout) {
+        using L = decltype(layout);
+        const auto kernel = prompt_kernel<typename L::T, L::D, L::G>;
+        // more than half of the shared memory, whatever is used: one CTA per SM, as tensor memory has room for one
+        const int smem = Smem<L::D, L::G>::kBytes > 120 * 1024 ? Smem<L::D, L::G>::kBytes : 120 * 1024;
+        if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
+        return result(ecq_dev::launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, a,
+                                          static_cast<int>(tiles)));
+    });
+}
+
+}  // namespace ecq_kv4

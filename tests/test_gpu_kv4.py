@@ -284,14 +284,20 @@ def reference(q, pages, table, lens, starts, page, dim, g, scale=None):
     return out, s_abs.double(), v_abs.double()
 
 
-def check_attention(got, want, s_abs, v_abs, dtype):
+def check_attention(got, want, s_abs, v_abs, dtype, rounded=False):
     """Scores are sums of at most 256 products in fp32 (each step 2^-24 of what is
     summed: 2^-16 of sum |q||k|); an error e of a score is a factor 1 +- e of its
     weight, and of the sum: 2 e of the largest |v|. Weights (2^-20: two fp16 parts,
-    exp2) and their fp32 sums add 2^-16 of it. Then one rounding to the type."""
-    tol = (torch.finfo(dtype).eps / 2) * want.abs() + (2 * 2.0 ** -16 * s_abs + 2 * 2.0 ** -16) * v_abs + 2.0 ** -24
+    exp2) and their fp32 sums add 2^-16 of it. Then one rounding to the type.
+    ``rounded``: the prompt kernel's K, V and weights are fp16, 2^-11 of each: 2^-11
+    of sum |q||k| in a score, and 2^-11 of the largest |v| twice."""
+    k, v = (2.0 ** -11, 2 * 2.0 ** -11) if rounded else (0.0, 0.0)
+    tol = (torch.finfo(dtype).eps / 2) * want.abs() + (2 * (2.0 ** -16 + k) * s_abs + 2 * 2.0 ** -16 + v) * v_abs + 2.0 ** -24
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+STREAM_ROWS = 64  # requests with more rows (queries times heads that share a cache head) go to the prompt kernel
 
 
 def attend_case(lens, new, heads, share, dim, g, page, dtype, seed=1, q_scale=1.0, **kw):
@@ -307,7 +313,9 @@ def attend_case(lens, new, heads, share, dim, g, page, dtype, seed=1, q_scale=1.
     torch.cuda.synchronize()
     assert status.item() == 0
     want, s_abs, v_abs = reference(q, pages, table, lens, starts, page, dim, g, kw.get("scale"))
-    check_attention(got, want, s_abs, v_abs, dtype)
+    for b, n in enumerate(new):
+        at = slice(starts[b], starts[b + 1])
+        check_attention(got[at], want[at], s_abs[at], v_abs[at], dtype, n * share > STREAM_ROWS)
     return q, pages, table, starts, got
 
 
@@ -329,6 +337,71 @@ def test_attention_head_layouts(heads, share):
 @pytest.mark.parametrize("lens,new", [([5], [5]), ([1, 40, 40, 0, 200], [1, 2, 0, 0, 7]), ([33, 47], [33, 17]), ([90, 300], [64, 1])])
 def test_attention_of_several_tokens_is_causal(dtype, dim, g, lens, new):
     attend_case(lens, new, 2, 3, dim, g, 16, dtype, seed=sum(new))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,g", LAYOUTS)
+@pytest.mark.parametrize("lens,new,page", [([65], [65], 16), ([64, 200], [64, 129], 16), ([300, 5, 64], [257, 1, 64], 64)])
+def test_attention_of_prompts(dtype, dim, g, lens, new, page):
+    attend_case(lens, new, 2, 2, dim, g, page, dtype, seed=sum(new))
+
+
+@pytest.mark.parametrize("share,new,lens", [
+    (1, [65, 128, 129, 600], [65, 1000, 129, 700]), (4, [17, 32, 33, 64, 65, 1, 0], [17, 500, 33, 64, 129, 77, 30]),
+    (8, [130], [1500]), (7, [40, 9, 10], [41, 400, 10]), (64, [2, 1, 5], [100, 64, 5]), (3, [300], [300])])
+def test_attention_of_prompts_head_layouts(share, new, lens):
+    attend_case(lens, new, 2, share, 128, 64, 32, torch.float16, seed=share)
+    attend_case(lens, new, 1, share, 64, 32, 128, torch.bfloat16, seed=share + 1, scale=-0.2)
+
+
+def test_attention_of_prompts_longer_than_the_request_and_scales():
+    # more queries than tokens: the first ones see nothing
+    lens, new = [50, 0], [70, 80]
+    pages, table = fill(lens, 1, 64, 32, 16, 3)
+    q = torch.randn(150, 2, 64, device="cuda").half()
+    got = ecq.kv4_attention(q, pages, table, i32(lens), i32([0, 70, 150]), 80, group_size=32)
+    want, s_abs, v_abs = reference(q, pages, table, lens, [0, 70, 150], 16, 64, 32)
+    check_attention(got, want, s_abs, v_abs, torch.float16, True)
+    assert not bool(got[:20].any()) and not bool(got[70:].any()) and bool(got[20:70].any())
+    for kw in (dict(scale=0.0), dict(q_scale=30.0), dict(q_scale=1e-6, scale=3e5)):
+        attend_case([400], [150], 1, 2, 128, 64, 64, torch.bfloat16, **kw)
+
+
+def test_tokens_that_are_not_numbers_reach_only_rows_that_see_them():
+    # a row of NaN at position 45 of a 70-token prompt: earlier queries are as without it
+    for n, share in ((70, 2), (9, 2), (1, 1)):
+        x = torch.randn(2, 70, 1, 64, device="cuda").half()
+        pages, clean = ecq.kv4_pages(5, 1, 64, 16, 32), ecq.kv4_pages(5, 1, 64, 16, 32)
+        slots, table = torch.arange(70, dtype=torch.int32, device="cuda"), torch.arange(5, dtype=torch.int32, device="cuda")[None]
+        q = torch.randn(n, share, 64, device="cuda").half()
+        ecq.kv4_append(x[0], x[1], clean, slots, group_size=32)
+        for which in (0, 1):
+            y = x.clone()
+            y[which, 66, 0, 3] = float("nan")
+            ecq.kv4_append(y[0], y[1], pages, slots, group_size=32)
+            starts = i32([0, n])
+            got, want = (ecq.kv4_attention(q, p, table, i32([70]), starts, n, group_size=32) for p in (pages, clean))
+            first = max(0, 66 - (70 - n))  # the first query that sees token 66
+            assert torch.equal(got[:first], want[:first])
+            seen = got[first:]
+            if which == 0:
+                assert bool(seen.isnan().all())
+            else:  # the value's group of channels
+                assert bool(seen[..., :32].isnan().all()) and torch.equal(seen[..., 32:], want[first:, :, 32:])
+
+
+def test_prompts_with_bad_pages_leave_their_keys_out():
+    lens, new, dim, g, page = [200, 130], [100, 100], 64, 32, 16
+    q, pages, table, starts, want = attend_case(lens, new, 1, 2, dim, g, page, torch.float16)
+    bad, status = table.clone(), i32([0])
+    bad[1, 8] = 2 ** 31 - 1  # tokens 128 and 129 of request 1: its last two queries lose them
+    got = ecq.kv4_attention(q, pages, bad, i32(lens), i32(starts), 100, group_size=g, status=status)
+    assert status.item() == BADARG
+    assert torch.equal(got[:198], want[:198])
+    short, s_abs, v_abs = reference(q, pages, table, [200, 128], [0, 100, 198], page, dim, g)
+    check_attention(got[:198], short[:198], s_abs[:198], v_abs[:198], torch.float16, True)
+    k = reference(q[198:], pages, table[1:], [128], [0, 1], page, dim, g)
+    check_attention(got[198:199], k[0][:1], k[1][:1], k[2][:1], torch.float16, True)
 
 
 def test_attention_of_long_contexts():
