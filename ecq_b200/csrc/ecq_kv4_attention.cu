@@ -47,11 +47,14 @@ constexpr int kUnit = 2, kUnitTokens = kUnit * kBlockTokens;
 constexpr int kThreads = kWarps * 32;
 // 16-row tiles need the registers of two 8-row ones
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-// Weights are exp2(score - reference); the reference is raised when a score
-// passes it by more than this, so weights are at most 4 and weight * scale
-// (at most 4 * 131008 / 15) is finite in fp16. Few blocks raise it, and the
-// others need no reduction over the block's tokens.
-constexpr float kSlack = 2.f;
+// Weights are exp2(score - reference + kLift). The reference is raised when a
+// score passes it by more than kSlack, so few blocks raise it and the others
+// need no reduction over their tokens. The lift keeps the weights of keys far
+// below the largest (most of a long context) out of fp16's subnormals, whose
+// step of 2^-24 would be felt in sums of thousands of them. weight * scale
+// then overflows fp16 from a scale of 16: that is seen (kDrop).
+constexpr float kSlack = 2.f, kLift = 10.f;
+constexpr float kDrop = 10.f;  // the reference goes up by so much where weight * scale is infinite
 constexpr float kNoMax = -1e30f;
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups) {
@@ -101,6 +104,14 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void add4(float (&o)[4], const float (&t)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const uint64_t x = ecq_dev::add2(ecq_dev::pack2(__float_as_uint(o[i]), __float_as_uint(o[i + 1])),
+                                         ecq_dev::pack2(__float_as_uint(t[i]), __float_as_uint(t[i + 1])));
+        ecq_dev::unpack2(x, o[i], o[i + 1]);
+    }
 }
 __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     uint32_t y;
@@ -244,7 +255,7 @@ __device__ __forceinline__ void set_rows(Rows<D, G, NT>& R, const uint4 (&raw)[N
 template <int D, int G, int NT>
 struct State {
     float o[NT][D / 16][4];
-    float sums[NT][4];  // lanes of row r < G: sum p zero of group r; of row G: sum p (columns 2t, 2t + 1; [2], [3] unused)
+    float sums[NT][2];  // columns 2t, 2t + 1; lanes of row r < G: sum p zero of group r; of row G: sum p
     float m[NT][2];
     __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -253,8 +264,7 @@ struct State {
             for (int i = 0; i < D / 16; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sums[nt][c] = 0.f;
+            sums[nt][0] = sums[nt][1] = 0.f;
             m[nt][0] = m[nt][1] = kNoMax;
         }
     }
@@ -287,6 +297,10 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t fma2h(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
                               *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t neg2(uint32_t a) {
@@ -358,10 +372,10 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][nt][c], s[u][nt][c + 2]));
             top[c] *= R.factor[nt][c];
         }
-        if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + kSlack || top[1] > S.m[nt][1] + kSlack)) {
+        if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + (kSlack + kLift) || top[1] > S.m[nt][1] + (kSlack + kLift))) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float x = fmaxf(top[c], S.m[nt][c]);
+                float x = fmaxf(top[c] - kLift, S.m[nt][c]);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
                 const float keep = exp2_fast(S.m[nt][c] - x);
@@ -375,95 +389,136 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             }
         }
     }
+    uint32_t hi[U][NT][G][2], lo[U][NT][G][2];
+    for (;;) {
+        uint32_t ph[U][NT][2], pl[U][NT][2], most = 0u;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        uint32_t sa[2][G], sb[2][G], za[2][1], zb[2][1];
-        lds<G, 0>(sa[0], at + u * BB + me.v_params);
-        lds<G, 16 * G>(sb[0], at + u * BB + me.v_params);
-        lds<G, 32 * G>(sa[1], at + u * BB + me.v_params);
-        lds<G, 48 * G>(sb[1], at + u * BB + me.v_params);
-        lds<1, 0>(za[0], at + u * BB + me.v_pair);
-        lds<1, 16 * G>(zb[0], at + u * BB + me.v_pair);
-        lds<1, 32 * G>(za[1], at + u * BB + me.v_pair);
-        lds<1, 48 * G>(zb[1], at + u * BB + me.v_pair);
-        // rows of A: the groups' zeros, then ones (the sum of the weights)
-        uint32_t z[2];
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            z[i] = __byte_perm(za[i][0], zb[i][0], 0x7632);
-            if (kMask) {  // where a zero is not finite its scale is not either, and that reaches the rows that see the token
-                if ((z[i] & 0x7c00u) == 0x7c00u) z[i] &= 0xffff0000u;
-                if ((z[i] & 0x7c000000u) == 0x7c000000u) z[i] &= 0xffffu;
-            }
-            z[i] = r == G ? 0x3c003c00u : z[i];
-        }
-        uint32_t hi[NT][G][2], lo[NT][G][2];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            uint32_t ph[2], pl[2];
+                for (int i = 0; i < 2; ++i) {
+                    float p[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float p[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) p[c] = exp2_fast(fmaf(s[u][nt][2 * i + c], R.factor[nt][c], -S.m[nt][c]));
-                const uint32_t x = h2(p[0], p[1]);
-                const float2 back = f2(x);
-                ph[i] = transpose(x);
-                pl[i] = transpose(h2(p[0] - back.x, p[1] - back.y));
-            }
-            mma(S.sums[nt], z[0], 0u, z[1], 0u, ph[0], ph[1]);
-            mma(S.sums[nt], z[0], 0u, z[1], 0u, pl[0], pl[1]);
+                    for (int c = 0; c < 2; ++c) p[c] = exp2_fast(fmaf(s[u][nt][2 * i + c], R.factor[nt][c], -S.m[nt][c]));
+                    const uint32_t x = h2(p[0], p[1]);
+                    const float2 back = f2(x);
+                    ph[u][nt][i] = transpose(x);
+                    pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
+                }
+            uint32_t sa[2][G], sb[2][G];
+            lds<G, 0>(sa[0], at + u * BB + me.v_params);
+            lds<G, 16 * G>(sb[0], at + u * BB + me.v_params);
+            lds<G, 32 * G>(sa[1], at + u * BB + me.v_params);
+            lds<G, 48 * G>(sb[1], at + u * BB + me.v_params);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
                     const uint32_t sc = __byte_perm(sa[i][g], sb[i][g], 0x5410);
-                    uint32_t h = mul2(ph[i], sc);
-                    uint32_t l = fma2h(pl[i], sc, fma2h(ph[i], sc, neg2(h)));
-                    if (kMask) {  // weight 0: 0, whatever the scale is
-                        const uint32_t keep = (ph[i] & 0xffffu ? 0xffffu : 0u) | (ph[i] & 0xffff0000u ? 0xffff0000u : 0u);
-                        h &= keep;
-                        l &= keep;
-                    }
-                    hi[nt][g][i] = h;
-                    lo[nt][g][i] = l;
-                }
-        }
-        constexpr int VW = D / 64;  // words of a lane's chunk of a V row
-        uint32_t v[4][VW];
-        lds<VW, 0>(v[0], at + u * BB + me.v);
-        lds<VW, 4 * (D / 2)>(v[1], at + u * BB + me.v);
-        lds<VW, 8 * (D / 2)>(v[2], at + u * BB + me.v);
-        lds<VW, 12 * (D / 2)>(v[3], at + u * BB + me.v);
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            uint32_t x[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t pick = j & 2 ? 0x7632u : 0x5410u;
-                uint32_t a = __byte_perm(v[0][w], v[1][w], pick), b = __byte_perm(v[2][w], v[3][w], pick);
-                if (j & 1) {
-                    a >>= 8;
-                    b >>= 8;
-                }
-                x[j][0] = a & 0x000f000fu;
-                x[j][1] = a & 0x00f000f0u;
-                x[j][2] = b & 0x000f000fu;
-                x[j][3] = b & 0x00f000f0u;
-            }
-#pragma unroll
-            for (int part = 0; part < 2; ++part)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const int mt = 4 * w + j, g = mt * 16 * G / D;
-                        const uint32_t(&p)[2] = part ? lo[nt][g] : hi[nt][g];
-                        mma(S.o[nt][mt], x[j][0], x[j][1], x[j][2], x[j][3], p[0], p[1]);
+                        // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
+                        const uint32_t w = ph[u][nt][i];
+                        uint32_t h = mul2(w, sc);
+                        uint32_t l = fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h)));
+                        if (kMask) {  // weight 0: 0, whatever the scale is
+                            const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
+                            h &= keep;
+                            l &= keep;
+                        }
+                        hi[u][nt][g][i] = h;
+                        lo[u][nt][g][i] = l;
+                        most = max2(most, h);  // not negative, and a NaN passes by
                     }
+                }
         }
+        if (!__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
+            // rows of A: the groups' zeros, then ones (the sum of the weights)
+            float sums[NT][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint32_t za[2][1], zb[2][1], z[2];
+                lds<1, 0>(za[0], at + u * BB + me.v_pair);
+                lds<1, 16 * G>(zb[0], at + u * BB + me.v_pair);
+                lds<1, 32 * G>(za[1], at + u * BB + me.v_pair);
+                lds<1, 48 * G>(zb[1], at + u * BB + me.v_pair);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    z[i] = __byte_perm(za[i][0], zb[i][0], 0x7632);
+                    if (kMask) {  // where a zero is not finite its scale is not either, and that reaches the rows that see the token
+                        if ((z[i] & 0x7c00u) == 0x7c00u) z[i] &= 0xffff0000u;
+                        if ((z[i] & 0x7c000000u) == 0x7c000000u) z[i] &= 0xffffu;
+                    }
+                    z[i] = r == G ? 0x3c003c00u : z[i];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
+                    else mma(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
+                    mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                S.sums[nt][0] += sums[nt][0];
+                S.sums[nt][1] += sums[nt][1];
+            }
+            break;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                S.m[nt][c] += kDrop;
+                S.sums[nt][c] *= 0.0009765625f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    S.o[nt][i][c] *= 0.0009765625f;
+                    S.o[nt][i][c + 2] *= 0.0009765625f;
+                }
+            }
     }
+    // The unit's part of o starts from 0 and is added with a rounded fp32 sum: codes are 0..15 and the zeros take about 7.5
+    // of that away again, so what a running sum loses to the tensor core's truncation would be many times as much in o.
+    constexpr int VW = D / 64;  // words of a lane's chunk of a V row
+    uint32_t v[U][4][VW];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        lds<VW, 0>(v[u][0], at + u * BB + me.v);
+        lds<VW, 4 * (D / 2)>(v[u][1], at + u * BB + me.v);
+        lds<VW, 8 * (D / 2)>(v[u][2], at + u * BB + me.v);
+        lds<VW, 12 * (D / 2)>(v[u][3], at + u * BB + me.v);
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t pick = half ? 0x7632u : 0x5410u;
+            float t[2][NT][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t x = __byte_perm(v[u][0][w], v[u][1][w], pick), y = __byte_perm(v[u][2][w], v[u][3][w], pick);
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int g = (4 * w + 2 * half + j) * 16 * G / D;
+                        const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
+                        const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t(&p)[2] = part ? lo[u][nt][g] : hi[u][nt][g];
+                            if (u == 0 && part == 0) mma_first(t[j][nt], a0, a1, a2, a3, p[0], p[1]);
+                            else mma(t[j][nt], a0, a1, a2, a3, p[0], p[1]);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) add4(S.o[nt][4 * w + 2 * half + j], t[j][nt]);
+        }
 }
 
 template <int D, int TR>

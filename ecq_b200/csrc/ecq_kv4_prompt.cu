@@ -52,7 +52,9 @@ constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 2) * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kRing = 4;
 constexpr uint32_t kTmemColumns = 512;
-constexpr float kSlack = 8.f;  // P is at most 2^8
+// P is exp2(score - reference + kLift), at most 2^15; the lift keeps the weights of keys far below the largest out of
+// fp16's subnormals
+constexpr float kSlack = 8.f, kLift = 7.f;
 constexpr float kNoMax = -1e30f;
 
 template <int D, int G>
@@ -318,8 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
 #pragma unroll
             for (int k = 1; k < kKeys; ++k) top = fmaxf(top, __uint_as_float(s[k]));
             top *= factor;
-            if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                const float next = fmaxf(top, m), keep = exp2_fast(m - next);
+            if (__any_sync(0xffffffffu, top > m + (kSlack + kLift))) {
+                const float next = fmaxf(top - kLift, m), keep = exp2_fast(m - next);
                 m = next;
                 const uint64_t k2 = ecq_dev::pack2(__float_as_uint(keep), __float_as_uint(keep));
 #pragma unroll
