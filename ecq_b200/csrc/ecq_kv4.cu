@@ -26,6 +26,7 @@ using ecq_dev::pdl_wait;
 // latency.
 // ---------------------------------------------------------------------------
 constexpr int kTableThreads = 512;
+constexpr int kRun = 4;  // outputs that a thread takes in a row
 
 struct Totals {
     long long tokens;  // sums of 2^13 lengths below 2^31
@@ -157,19 +158,37 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
         const int held = (s_len[b] + page_size - 1) >> page_shift;
         table[b * table_stride + held + (j - s_page[b])] = free_pages[count - 1 - j];
     }
-    for (int i = tid; i < max_tokens; i += threads) {
-        int slot = -1, pos = -1;
-        if (i < total) {
-            const int b = owner(s_tok, batch, i);
-            pos = s_len[b] + (i - s_tok[b]);
-            const int col = pos >> page_shift, held = (s_len[b] + page_size - 1) >> page_shift;
-            // a page of this step comes off the stack again: the table entry is another thread's write
-            const int page = col < held ? table[b * table_stride + col] : free_pages[count - 1 - (s_page[b] + col - held)];
-            const long long at = (static_cast<long long>(page) << page_shift) + (pos & (page_size - 1));
-            slot = page < 0 || at > 0x7fffffffll ? -1 : static_cast<int>(at);
+    // a thread takes kRun tokens in a row: one search, and mostly one page, for all of them
+    for (int i0 = tid * kRun; i0 < max_tokens; i0 += threads * kRun) {
+        int b = 0, held = 0, next = -1, page = -1, have = -1;
+        if (i0 < total) b = owner(s_tok, batch, i0);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const int i = i0 + k;
+            int slot = -1, pos = -1;
+            if (i < total) {
+                if (i >= next) {  // the first token, or the next request that has any
+                    if (next >= 0) do ++b;
+                        while ((b + 1 < batch ? s_tok[b + 1] : total) <= i);
+                    next = b + 1 < batch ? s_tok[b + 1] : total;
+                    held = (s_len[b] + page_size - 1) >> page_shift;
+                    have = -1;
+                }
+                pos = s_len[b] + (i - s_tok[b]);
+                const int col = pos >> page_shift;
+                if (col != have) {
+                    have = col;
+                    // a page of this step comes off the stack again: the table entry is another thread's write
+                    page = col < held ? table[b * table_stride + col] : free_pages[count - 1 - (s_page[b] + col - held)];
+                }
+                const long long at = (static_cast<long long>(page) << page_shift) + (pos & (page_size - 1));
+                slot = page < 0 || at > 0x7fffffffll ? -1 : static_cast<int>(at);
+            }
+            if (i < max_tokens) {
+                slots[i] = slot;
+                positions[i] = pos;
+            }
         }
-        slots[i] = slot;
-        positions[i] = pos;
     }
 }
 
@@ -225,9 +244,16 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
     const int pages = static_cast<int>(pages_sum);
     if (tid == 0) *count_out = count + pages;
     for (int b = tid; b < batch; b += threads) lens_out[b] = s_len[b];
-    for (int j = tid; j < pages; j += threads) {
-        const int b = owner(s_page, batch, j);
-        free_pages[count + j] = table[b * table_stride + (j - s_page[b])];
+    for (int j0 = tid * kRun; j0 < pages; j0 += threads * kRun) {
+        int b = owner(s_page, batch, j0);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const int j = j0 + k;
+            if (j < pages) {
+                while (b + 1 < batch && s_page[b + 1] <= j) ++b;  // the last request that starts at or before j: the one with it
+                free_pages[count + j] = table[b * table_stride + (j - s_page[b])];
+            }
+        }
     }
 }
 
@@ -237,9 +263,9 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
 // 128, two at 64. Minimum and maximum of a group go over its g / 8 lanes by
 // shuffles. A K lane's 8 channels are one 32-bit word of codes; V words want
 // every 8th channel, which an 8 x 8 transposition of nibbles over 8 lanes
-// gives (3 shuffles). Bound by memory for prompts, by latency for steps; the
-// division is IEEE so that a value on the border between two codes goes the
-// same way everywhere.
+// gives (3 shuffles). Bound by latency for steps and by instructions for
+// prompts. Codes are those of the IEEE quotient, so that a value on the border
+// between two codes goes the same way everywhere.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
@@ -289,17 +315,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x, int lane) {
     return x;
 }
 
-// This thread's row: token and head, whether V, and which 8 channels.
+// This thread's row: token (of head blockIdx.y), whether V, and which 8 channels.
 template <int D>
 struct RowLane {
     static constexpr int kUnit = D / 4;  // lanes per token and head
-    int64_t unit;
-    int c;       // channels 8c .. 8c + 7
+    static constexpr int kTokens = kRowThreads / kUnit;
+    int token, c;  // channels 8c .. 8c + 7
     bool is_v;
-    __device__ explicit RowLane() {
-        const int64_t i = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
-        unit = i / kUnit;
-        const int l = static_cast<int>(i % kUnit);
+    __device__ __forceinline__ RowLane() {
+        const int l = threadIdx.x % kUnit;
+        token = static_cast<int>(blockIdx.x) * kTokens + threadIdx.x / kUnit;
         is_v = l >= D / 8;
         c = l % (D / 8);
     }
@@ -326,8 +351,7 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const T* __restrict
     pdl_launch_dependents();
     const RowLane<D> me;
     pdl_wait();
-    const int64_t token = me.unit / heads;
-    const int head = static_cast<int>(me.unit - token * heads);
+    const int token = me.token, head = blockIdx.y;
     const bool in = token < tokens;
     const int32_t slot = in ? slots[token] : -1;
     const bool keep = slot >= 0 && slot < n_slots;
@@ -357,12 +381,26 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const T* __restrict
     }
     const __half zero = __float2half_rn(lo), scale = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
     const float z = __half2float(zero), s = __half2float(scale);
+    // (x - zero) / scale by the reciprocal; where that comes so near to the border between two codes that the rounded
+    // quotient might fall on the other side, the division itself decides. 1.5 2^23 + q holds q rounded to even in its
+    // low bits. A NaN's code is 0 (fmaxf takes the other operand).
+    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+    constexpr float kInt = 12582912.f;
     uint32_t word = 0;
+    bool near = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        // fmaxf takes the other operand of a NaN: codes of a NaN group are 0
-        const float t = s == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f);
-        word |= static_cast<uint32_t>(t) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float q = fminf(fmaxf((x[i] - z) * inv, 0.f), 15.f), y = q + kInt;
+        near |= fabsf(q - (y - kInt)) > 0.49999f;
+        word = word * 16u + (__float_as_uint(y) - 0x4b400000u);
+    }
+    if (near) {
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = s == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f);
+            word |= static_cast<uint32_t>(t) << (4 * i);
+        }
     }
     const uint32_t turned = transpose8(word, threadIdx.x & 31);
     if (!keep) return;
@@ -384,8 +422,7 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, 
     pdl_launch_dependents();
     const RowLane<D> me;
     pdl_wait();
-    const int64_t token = me.unit / heads;
-    const int head = static_cast<int>(me.unit - token * heads);
+    const int token = me.token, head = blockIdx.y;
     const bool in = token < tokens;
     const int32_t slot = in ? slots[token] : -1;
     const bool have = slot >= 0 && slot < n_slots;
@@ -408,7 +445,7 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, 
     for (int i = 0; i < 4; ++i)
         o[i] = from_float2<T>(fmaf(static_cast<float>((word >> (8 * i)) & 15u), par.x, par.y),
                               fmaf(static_cast<float>((word >> (8 * i + 4)) & 15u), par.x, par.y));
-    T* row = (me.is_v ? v : k) + me.unit * D + 8 * me.c;
+    T* row = (me.is_v ? v : k) + (static_cast<int64_t>(token) * heads + head) * D + 8 * me.c;
     *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
@@ -486,13 +523,12 @@ int32_t ecq_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_str
     if (tokens == 0) return ECQ_OK;
     if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16)) return ECQ_ERR_ARG;
     if ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return ECQ_ERR_ARG;
-    const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 4);
-    const int64_t blocks = (threads + kRowThreads - 1) / kRowThreads;
-    if (blocks > 0x7fffffff) return ECQ_ERR_UNSUPPORTED;
+    const int per_block = kRowThreads / (head_dim / 4);
+    const dim3 grid((tokens + per_block - 1) / per_block, kv_heads);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
         using T = typename L::T;
-        return result(launch_pdl(append_kernel<T, L::D, L::G>, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0,
+        return result(launch_pdl(append_kernel<T, L::D, L::G>, grid, dim3(kRowThreads), 0,
                                  static_cast<cudaStream_t>(stream), static_cast<const T*>(k), k_token_stride,
                                  k_head_stride, static_cast<const T*>(v), v_token_stride, v_head_stride,
                                  static_cast<uint8_t*>(pages), n_pages * page_size, kv_heads, log2i(page_size),
@@ -508,13 +544,12 @@ int32_t ecq_kv4_gather(void* k, void* v, int32_t dtype, const void* pages, int64
     if (tokens < 0 || !pool_ok(pages, n_pages, kv_heads, page_size)) return ECQ_ERR_ARG;
     if (tokens == 0) return ECQ_OK;
     if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16)) return ECQ_ERR_ARG;
-    const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 4);
-    const int64_t blocks = (threads + kRowThreads - 1) / kRowThreads;
-    if (blocks > 0x7fffffff) return ECQ_ERR_UNSUPPORTED;
+    const int per_block = kRowThreads / (head_dim / 4);
+    const dim3 grid((tokens + per_block - 1) / per_block, kv_heads);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
         using T = typename L::T;
-        return result(launch_pdl(gather_kernel<T, L::D, L::G>, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0,
+        return result(launch_pdl(gather_kernel<T, L::D, L::G>, grid, dim3(kRowThreads), 0,
                                  static_cast<cudaStream_t>(stream), static_cast<T*>(k), static_cast<T*>(v),
                                  static_cast<const uint8_t*>(pages), n_pages * page_size, kv_heads, log2i(page_size),
                                  static_cast<const int32_t*>(slots), tokens, static_cast<int32_t*>(status)));

@@ -52,7 +52,7 @@ int32_t by_layout(int dtype, int dim, int groups, F&& f) {
 }
 
 inline bool pool_ok(const void* pages, int64_t n_pages, int kv_heads, int page_size) {
-    return pages && aligned(pages, 16) && n_pages >= 1 && kv_heads >= 1 && n_pages <= ((1ll << 31) - 1) / page_size;
+    return pages && aligned(pages, 16) && n_pages >= 1 && kv_heads >= 1 && kv_heads <= 65535 && n_pages <= ((1ll << 31) - 1) / page_size;
 }
 inline int32_t result(cudaError_t rc) { return rc == cudaSuccess ? ECQ_OK : (cudaGetLastError(), ECQ_ERR_CUDA); }
 
