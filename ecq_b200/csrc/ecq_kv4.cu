@@ -269,15 +269,28 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Packed minimum that passes NaN on.
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+template <>
+__device__ __forceinline__ uint32_t min2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+// x / 15, correctly rounded: the product with the rounded reciprocal is within
+// a unit of the quotient, and one step with the exact remainder rounds it
+// (Markstein's theorem).
+__device__ __forceinline__ float fifteenth(float x) {
+    constexpr float r = 1.f / 15.f;
+    const float q = x * r;
+    return fmaf(fmaf(-q, 15.f, x), r, q);
 }
 
 template <typename T>
@@ -315,8 +328,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x, int lane) {
     return x;
 }
 
-// This thread's row: token (of head blockIdx.y), whether V, and which 8 channels.
-template <int D>
+// This thread's rows: tokens token, token + kTokens, ... (of head blockIdx.y),
+// whether V, and which 8 channels. kPer rows a thread: their loads overlap.
+template <int D, int kPer>
 struct RowLane {
     static constexpr int kUnit = D / 4;  // lanes per token and head
     static constexpr int kTokens = kRowThreads / kUnit;
@@ -324,11 +338,31 @@ struct RowLane {
     bool is_v;
     __device__ __forceinline__ RowLane() {
         const int l = threadIdx.x % kUnit;
-        token = static_cast<int>(blockIdx.x) * kTokens + threadIdx.x / kUnit;
+        token = static_cast<int>(blockIdx.x) * (kTokens * kPer) + threadIdx.x / kUnit;
         is_v = l >= D / 8;
         c = l % (D / 8);
     }
 };
+// The slots of the thread's rows; -1: none. One beyond the pool is reported.
+template <int D, int kPer>
+__device__ __forceinline__ void row_slots(int (&slot)[kPer], const RowLane<D, kPer>& me, const int32_t* slots, int tokens,
+                                          int64_t n_slots, int32_t* status) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int token = me.token + i * me.kTokens;
+        slot[i] = token < tokens ? slots[token] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (slot[i] >= n_slots) {
+            if (blockIdx.y == 0 && me.c == 0) raise_status(status, ECQ_STATUS_BADARG);
+            slot[i] = -1;
+        }
+}
+__device__ __forceinline__ int64_t block_of(int slot, int heads, int page_shift) {
+    return (static_cast<int64_t>(slot >> page_shift) * heads + blockIdx.y) * (1 << page_shift) / kBlockTokens +
+           (slot & ((1 << page_shift) - 1)) / kBlockTokens;
+}
 
 // Where the lane's word of codes and its group's pair lie in the token's block.
 template <int D, int G>
@@ -341,7 +375,7 @@ __device__ __forceinline__ int params_at(bool is_v, int tok, int c) {
     return (is_v ? v_params_at(D, G) : k_params_at(D)) + tok * 4 * G + (c * 8 / (D / G)) * 4;
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int kPer>
 __global__ void __launch_bounds__(kRowThreads) append_kernel(const T* __restrict__ k, int64_t k_token, int64_t k_head,
                                                             const T* __restrict__ v, int64_t v_token, int64_t v_head,
                                                             uint8_t* __restrict__ pages, int64_t n_slots, int heads,
@@ -349,104 +383,130 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const T* __restrict
                                                             int tokens, int32_t* status) {
     constexpr int kGroupLanes = D / G / 8;
     pdl_launch_dependents();
-    const RowLane<D> me;
+    const RowLane<D, kPer> me;
+    const int64_t step = me.is_v ? v_token : k_token;
+    const T* src = (me.is_v ? v + blockIdx.y * v_head : k + blockIdx.y * k_head) + me.token * step + 8 * me.c;
     pdl_wait();
-    const int token = me.token, head = blockIdx.y;
-    const bool in = token < tokens;
-    const int32_t slot = in ? slots[token] : -1;
-    const bool keep = slot >= 0 && slot < n_slots;
-    if (in && slot >= n_slots && head == 0 && me.c == 0) raise_status(status, ECQ_STATUS_BADARG);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (keep) {
-        const T* row = me.is_v ? v + token * v_token + head * v_head : k + token * k_token + head * k_head;
-        const uint4 u = *reinterpret_cast<const uint4*>(row + 8 * me.c);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    int slot[kPer];
+    row_slots(slot, me, slots, tokens, n_slots, status);
+    uint4 raw[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (slot[i] >= 0) raw[i] = *reinterpret_cast<const uint4*>(src + i * me.kTokens * step);
+    }
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) {
+        const uint32_t w[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+        // (minimum, minus maximum) of the group as one packed minimum
+        const uint32_t lo2 = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3]));
+        const uint32_t hi2 = min2<T>(min2<T>(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), min2<T>(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+        uint32_t ends = min2<T>(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
+#pragma unroll
+        for (int o = 1; o < kGroupLanes; o <<= 1) ends = min2<T>(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+        const float2 e = to_float2<T>(ends);
+        const bool wide = e.x < -65504.f || e.y < -65504.f;
+        // a NaN is neither wide nor changed by what follows
+        const float lo = wide ? fmaxf(e.x, -65504.f) : e.x, hi = wide ? fminf(-e.y, 65504.f) : -e.y;
+        const __half zero = __float2half_rn(lo), scale = __float2half_rn(fifteenth(hi - lo));
+        const float z = __half2float(zero), s = __half2float(scale);
+        float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = to_float2<T>(w[i]);
-            x[2 * i] = min_nan(max_nan(f.x, -65504.f), 65504.f);
-            x[2 * i + 1] = min_nan(max_nan(f.y, -65504.f), 65504.f);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
+        }
+        // (x - zero) / (15 scale), held to 0..1, by the reciprocal (its roundings: under 2^-20 of it); where 15 of that come
+        // so near to the border between two codes that the rounded quotient might fall on the other side, the division
+        // itself decides. 1.5 2^23 + q holds q rounded to even in its low bits. A NaN's code is 0 (.sat).
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s * 15.f));
+        if (s == 0.f) inv = 0.f;
+        constexpr float kInt = 12582912.f;
+        uint32_t word = 0;
+        float far = 0.f;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const float t = __saturatef((x[i] - z) * inv), y = fmaf(t, 15.f, kInt);
+            far = fmaxf(far, fabsf(fmaf(t, 15.f, kInt - y)));
+            word = word * 16u + __float_as_uint(y);
+        }
+        word -= 0x4b400000u * 0x11111111u;  // the bits of 1.5 2^23, eight times
+        if (far > 0.49997f) {
+            word = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float t = s == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f);
+                word |= static_cast<uint32_t>(t) << (4 * i);
+            }
+        }
+        const uint32_t turned = transpose8(word, threadIdx.x & 31);
+        if (slot[n] >= 0) {
+            const int tok = slot[n] % kBlockTokens;
+            uint8_t* blk = pages + block_of(slot[n], heads, page_shift) * block_bytes(D, G);
+            *reinterpret_cast<uint32_t*>(blk + code_at<D, G>(me.is_v, tok, me.c)) = me.is_v ? turned : word;
+            if (me.c % kGroupLanes == 0)
+                *reinterpret_cast<__half2*>(blk + params_at<D, G>(me.is_v, tok, me.c)) = __halves2half2(scale, zero);
         }
     }
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = min_nan(lo, x[i]);
-        hi = max_nan(hi, x[i]);
-    }
-#pragma unroll
-    for (int o = 1; o < kGroupLanes; o <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const __half zero = __float2half_rn(lo), scale = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
-    const float z = __half2float(zero), s = __half2float(scale);
-    // (x - zero) / scale by the reciprocal; where that comes so near to the border between two codes that the rounded
-    // quotient might fall on the other side, the division itself decides. 1.5 2^23 + q holds q rounded to even in its
-    // low bits. A NaN's code is 0 (fmaxf takes the other operand).
-    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
-    constexpr float kInt = 12582912.f;
-    uint32_t word = 0;
-    bool near = false;
-#pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        const float q = fminf(fmaxf((x[i] - z) * inv, 0.f), 15.f), y = q + kInt;
-        near |= fabsf(q - (y - kInt)) > 0.49999f;
-        word = word * 16u + (__float_as_uint(y) - 0x4b400000u);
-    }
-    if (near) {
-        word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = s == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f);
-            word |= static_cast<uint32_t>(t) << (4 * i);
-        }
-    }
-    const uint32_t turned = transpose8(word, threadIdx.x & 31);
-    if (!keep) return;
-    const int page_size = 1 << page_shift, at = slot & (page_size - 1);
-    uint8_t* blk = pages + ((static_cast<int64_t>(slot >> page_shift) * heads + head) * (page_size / kBlockTokens) +
-                            at / kBlockTokens) * block_bytes(D, G);
-    const int tok = at % kBlockTokens;
-    *reinterpret_cast<uint32_t*>(blk + code_at<D, G>(me.is_v, tok, me.c)) = me.is_v ? turned : word;
-    if (me.c % kGroupLanes == 0)
-        *reinterpret_cast<__half2*>(blk + params_at<D, G>(me.is_v, tok, me.c)) = __halves2half2(scale, zero);
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int kPer>
 __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, T* __restrict__ v,
                                                             const uint8_t* __restrict__ pages, int64_t n_slots,
                                                             int heads, int page_shift,
                                                             const int32_t* __restrict__ slots, int tokens,
                                                             int32_t* status) {
     pdl_launch_dependents();
-    const RowLane<D> me;
+    const RowLane<D, kPer> me;
+    const int64_t step = static_cast<int64_t>(heads) * D;
+    T* dst = (me.is_v ? v : k) + me.token * step + blockIdx.y * D + 8 * me.c;
     pdl_wait();
-    const int token = me.token, head = blockIdx.y;
-    const bool in = token < tokens;
-    const int32_t slot = in ? slots[token] : -1;
-    const bool have = slot >= 0 && slot < n_slots;
-    if (in && slot >= n_slots && head == 0 && me.c == 0) raise_status(status, ECQ_STATUS_BADARG);
-    uint32_t word = 0;
-    float2 par = make_float2(0.f, 0.f);
-    if (have) {
-        const int page_size = 1 << page_shift, at = slot & (page_size - 1);
-        const uint8_t* blk = pages + ((static_cast<int64_t>(slot >> page_shift) * heads + head) *
-                                      (page_size / kBlockTokens) + at / kBlockTokens) * block_bytes(D, G);
-        const int tok = at % kBlockTokens;
-        word = *reinterpret_cast<const uint32_t*>(blk + code_at<D, G>(me.is_v, tok, me.c));
-        par = __half22float2(*reinterpret_cast<const __half2*>(blk + params_at<D, G>(me.is_v, tok, me.c)));
-    }
-    const uint32_t turned = transpose8(word, threadIdx.x & 31);
-    if (!in) return;
-    if (me.is_v) word = turned;
-    uint32_t o[4];
+    int slot[kPer];
+    row_slots(slot, me, slots, tokens, n_slots, status);
+    uint32_t word[kPer], par[kPer];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        o[i] = from_float2<T>(fmaf(static_cast<float>((word >> (8 * i)) & 15u), par.x, par.y),
-                              fmaf(static_cast<float>((word >> (8 * i + 4)) & 15u), par.x, par.y));
-    T* row = (me.is_v ? v : k) + (static_cast<int64_t>(token) * heads + head) * D + 8 * me.c;
-    *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
+    for (int i = 0; i < kPer; ++i) {
+        word[i] = par[i] = 0u;
+        if (slot[i] >= 0) {
+            const int tok = slot[i] % kBlockTokens;
+            const uint8_t* blk = pages + block_of(slot[i], heads, page_shift) * block_bytes(D, G);
+            word[i] = *reinterpret_cast<const uint32_t*>(blk + code_at<D, G>(me.is_v, tok, me.c));
+            par[i] = *reinterpret_cast<const uint32_t*>(blk + params_at<D, G>(me.is_v, tok, me.c));
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) {
+        const uint32_t turned = transpose8(word[n], threadIdx.x & 31), x = me.is_v ? turned : word[n];
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&par[n]));
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // a code in the low bits of 2^23, less that, is exact
+            const uint32_t c = (x >> (4 * i)) & 15u;
+            f[i] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, p.x, p.y);
+        }
+        if (me.token + n * me.kTokens < tokens)
+            *reinterpret_cast<uint4*>(dst + n * me.kTokens * step) =
+                make_uint4(from_float2<T>(f[0], f[1]), from_float2<T>(f[2], f[3]), from_float2<T>(f[4], f[5]),
+                           from_float2<T>(f[6], f[7]));
+    }
+}
+
+// Rows a thread takes: one while one round of CTAs covers them (a step: the
+// shortest way), four above (a prompt: loads overlap, addresses are shared).
+int rows_per_thread(int tokens, int kv_heads, int head_dim) {
+    const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 4);
+    return threads <= 2048ll * ecq_dev::sm_count_cached() ? 1 : 4;
+}
+dim3 row_grid(int tokens, int kv_heads, int head_dim, int per) {
+    const int block = kRowThreads / (head_dim / 4) * per;
+    return dim3((tokens + block - 1) / block, kv_heads);
 }
 
 bool table_args_ok(int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_size, int32_t free_capacity) {
@@ -523,13 +583,13 @@ int32_t ecq_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_str
     if (tokens == 0) return ECQ_OK;
     if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16)) return ECQ_ERR_ARG;
     if ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return ECQ_ERR_ARG;
-    const int per_block = kRowThreads / (head_dim / 4);
-    const dim3 grid((tokens + per_block - 1) / per_block, kv_heads);
+    const int per = rows_per_thread(tokens, kv_heads, head_dim);
+    const dim3 grid = row_grid(tokens, kv_heads, head_dim, per);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
         using T = typename L::T;
-        return result(launch_pdl(append_kernel<T, L::D, L::G>, grid, dim3(kRowThreads), 0,
-                                 static_cast<cudaStream_t>(stream), static_cast<const T*>(k), k_token_stride,
+        const auto kernel = per == 1 ? append_kernel<T, L::D, L::G, 1> : append_kernel<T, L::D, L::G, 4>;
+        return result(launch_pdl(kernel, grid, dim3(kRowThreads), 0, static_cast<cudaStream_t>(stream), static_cast<const T*>(k), k_token_stride,
                                  k_head_stride, static_cast<const T*>(v), v_token_stride, v_head_stride,
                                  static_cast<uint8_t*>(pages), n_pages * page_size, kv_heads, log2i(page_size),
                                  static_cast<const int32_t*>(slots), tokens, static_cast<int32_t*>(status)));
@@ -544,13 +604,13 @@ int32_t ecq_kv4_gather(void* k, void* v, int32_t dtype, const void* pages, int64
     if (tokens < 0 || !pool_ok(pages, n_pages, kv_heads, page_size)) return ECQ_ERR_ARG;
     if (tokens == 0) return ECQ_OK;
     if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16)) return ECQ_ERR_ARG;
-    const int per_block = kRowThreads / (head_dim / 4);
-    const dim3 grid((tokens + per_block - 1) / per_block, kv_heads);
+    const int per = rows_per_thread(tokens, kv_heads, head_dim);
+    const dim3 grid = row_grid(tokens, kv_heads, head_dim, per);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
         using T = typename L::T;
-        return result(launch_pdl(gather_kernel<T, L::D, L::G>, grid, dim3(kRowThreads), 0,
-                                 static_cast<cudaStream_t>(stream), static_cast<T*>(k), static_cast<T*>(v),
+        const auto kernel = per == 1 ? gather_kernel<T, L::D, L::G, 1> : gather_kernel<T, L::D, L::G, 4>;
+        return result(launch_pdl(kernel, grid, dim3(kRowThreads), 0, static_cast<cudaStream_t>(stream), static_cast<T*>(k), static_cast<T*>(v),
                                  static_cast<const uint8_t*>(pages), n_pages * page_size, kv_heads, log2i(page_size),
                                  static_cast<const int32_t*>(slots), tokens, static_cast<int32_t*>(status)));
     });
