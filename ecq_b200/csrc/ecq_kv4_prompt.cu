@@ -9,13 +9,16 @@
 //   decoders four warps turn codes into fp16 K [64 x D] and V^T [D x 64] in the
 //            tensor core's K-major, no-swizzle layout: code * scale + zero,
 //            rounded once to fp16, shared by all 256 rows;
-//   MMA      one thread issues S = Q K^T (A = Q in tensor memory) and O += P V
-//            (A = P in tensor memory) for the two tiles in turn, so that one
-//            tile's softmax runs beside the other's products;
-//   softmax  four warps per tile, a thread per row: S from tensor memory, running
-//            maximum (raised only when a score passes it by 2^8: then the row's
-//            O is rescaled), exp2, P as fp16 over S's place, sums in fp32.
-// Tensor memory (512 columns): Q, S and O of both tiles.
+//   MMA      one warp issues S = Q K^T and O += P V for both tiles;
+//   softmax  four warps per tile, a thread per row: S from tensor memory (its
+//            place is free for the next step's scores at once), running maximum
+//            (raised only when a score passes it by 2^8: then the row's O is
+//            rescaled), exp2, P as fp16 to tensor memory, sums in fp32.
+// So the next scores and the last step's O += P V are made while the
+// exponentials of a step are computed. Tensor memory is full (512 columns): Q
+// of the first tile, S, P and O of both; the second tile's Q lies in shared
+// memory (its scores then read both operands there: 384 cycles a step instead
+// of 256).
 //
 // fp16 for K, V and P costs a relative 2^-11 on each, next to the output's own
 // rounding; q is brought to its row's power of two and keeps its bits. What
@@ -49,7 +52,7 @@ constexpr int kTileBlocks = kKeys / kBlockTokens;
 constexpr int kRows = 128, kCtaRows = 2 * kRows;
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
 constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 2) * 32;
-constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
+constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;  // the loader is the one behind it
 constexpr int kRing = 4;
 constexpr uint32_t kTmemColumns = 512;
 // P is exp2(score - reference + kLift), at most 2^15; the lift keeps the weights of keys far below the largest out of
@@ -63,21 +66,23 @@ struct Smem {
     // K: core columns of 8 channels, 64 keys of 16 bytes each; 32 more bytes put a warp's stores in different banks
     static constexpr uint32_t kLboK = kKeys * 16 + 32, kBytesK = D / 8 * kLboK;
     static constexpr uint32_t kLboV = D * 16, kBytesV = kKeys / 8 * kLboV;
-    static constexpr int kRingAt = 0, kAtK = kRing * kPacked, kAtV = kAtK + 2 * kBytesK, kBytes = kAtV + 2 * kBytesV;
+    static constexpr uint32_t kLboQ = kRows * 16, kBytesQ = D / 8 * kLboQ;
+    static constexpr int kRingAt = 0, kAtK = kRing * kPacked, kAtV = kAtK + 2 * kBytesK, kAtQ = kAtV + 2 * kBytesV,
+                         kBytes = kAtQ + kBytesQ;
 };
 
-// Tensor memory columns of tile x
-template <int D>
+// Tensor memory columns (of tile x)
 struct Tmem {
-    static __device__ constexpr uint32_t q(int x) { return x * (D / 2); }
-    static __device__ constexpr uint32_t s(int x) { return 128 + x * kKeys; }
+    static constexpr uint32_t kQ = 0;
+    static __device__ constexpr uint32_t s(int x) { return 64 + x * 64; }
+    static __device__ constexpr uint32_t p(int x) { return 192 + x * 32; }
     static __device__ constexpr uint32_t o(int x) { return 256 + x * 128; }
 };
 
 struct Control {
     uint64_t packed_full[kRing], packed_empty[kRing];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t q_full[2], s_full[2], s_read[2], p_full[2], p_read[2], drained;
     uint32_t tmem, gave_up;
     uint32_t hidden[8];  // by step: a bit per block where nothing is, or a bad page (the loader is at most 5 steps ahead of a softmax)
     int poison[4];           // per group: the first token whose V is not finite
@@ -89,12 +94,24 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
 }
+// The whole warp comes here and one lane issues: what the instruction takes from
+// uniform registers stays in them (issued under a branch on the lane, a product
+// took 90 cycles to issue, which is three times what it takes to run).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ uint64_t kmajor(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -182,7 +199,7 @@ __device__ __forceinline__ uint32_t value_high(uint32_t x, uint32_t scale, uint3
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const int tiles) {
     using S = Smem<D, G>;
-    using M = Tmem<D>;
+    using M = Tmem;
     constexpr int BB = block_bytes(D, G);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Control ctl;
@@ -202,8 +219,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             mbar_init(smem_addr(&ctl.v_empty[i]), 1);
             mbar_init(smem_addr(&ctl.q_full[i]), kRows);
             mbar_init(smem_addr(&ctl.s_full[i]), 1);
+            mbar_init(smem_addr(&ctl.s_read[i]), kRows);
             mbar_init(smem_addr(&ctl.p_full[i]), kRows);
-            mbar_init(smem_addr(&ctl.o_full[i]), 1);
+            mbar_init(smem_addr(&ctl.p_read[i]), 1);
         }
         mbar_init(smem_addr(&ctl.drained), 1);
         ctl.gave_up = 0u;
@@ -219,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     before_sync();
     __syncthreads();
     after_sync();
-    const uint32_t tmem = ctl.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem, 0);
     ecq_dev::pdl_launch_dependents();  // after the allocation: the next kernel may want tensor memory too
     ecq_dev::pdl_wait();
 
@@ -256,13 +274,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
         {
             const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
                            static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head;
-            uint4 raw[D / 8];
             float top = 0.f;
-#pragma unroll
+#pragma unroll 4
             for (int c = 0; c < D / 8; ++c) {
-                raw[c] = make_uint4(0, 0, 0, 0);
-                if (in) raw[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (in) u = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 f = cvt2(w[e], T());
@@ -282,18 +299,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                 uint32_t v[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    // decoded K: core column 4 w + t holds channels 32 w + 8 t ..: the natural order of groups of 8
-                    const uint4 u = raw[8 * part + c];
+                    // core column c of K holds channels 8 c ..
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (in) u = __ldg(reinterpret_cast<const uint4*>(src) + 8 * part + c);
                     const float2 f0 = cvt2(u.x, T()), f1 = cvt2(u.y, T()), f2 = cvt2(u.z, T()), f3 = cvt2(u.w, T());
                     v[4 * c] = pack2(f0.x * up, f2.x * up, __half());
                     v[4 * c + 1] = pack2(f0.y * up, f2.y * up, __half());
                     v[4 * c + 2] = pack2(f1.x * up, f3.x * up, __half());
                     v[4 * c + 3] = pack2(f1.y * up, f3.y * up, __half());
+                    if (x == 1)
+                        sts4(base + S::kAtQ + (8 * part + c) * S::kLboQ + (threadIdx.x - kRows) * 16, v[4 * c], v[4 * c + 1],
+                             v[4 * c + 2], v[4 * c + 3]);
                 }
-                tmem_st(mine + M::q(x) + 32 * part, v);
+                if (x == 0) tmem_st(mine + M::kQ + 32 * part, v);
             }
-            wait_st();
-            before_sync();
+            if (x == 0) {
+                wait_st();
+                before_sync();
+            } else {
+                fence_proxy_async();
+            }
             mbar_arrive(smem_addr(&ctl.q_full[x]));
         }
         float m = kNoMax;
@@ -309,6 +334,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             tmem_ld(mine + M::s(x), s);
             tmem_ld(mine + M::s(x) + 32, s + 32);
             wait_ld();
+            before_sync();
+            mbar_arrive(smem_addr(&ctl.s_read[x]));
+            bool emptied = j == 0;  // P and O are not in use by the last step's product
             const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
             const int left = limit - j * kKeys;  // keys of this step that the row sees
             if (__any_sync(0xffffffffu, left < kKeys) || hidden) {
@@ -326,7 +354,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                 const uint64_t k2 = ecq_dev::pack2(__float_as_uint(keep), __float_as_uint(keep));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) l[u] = ecq_dev::fma2(l[u], k2, 0ull);
-                if (j) {  // the products so far are done: their completion came with S
+                if (j) {
+                    ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (j - 1) & 1, gave_up, a.status));
+                    if (!ok) break;
+                    after_sync();
+                    emptied = true;
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -348,7 +380,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                 l[k / 2 % 2] = ecq_dev::add2(l[k / 2 % 2], ecq_dev::pack2(__float_as_uint(e0), __float_as_uint(e1)));
                 s[k / 2] = pack2(e0, e1, __half());
             }
-            tmem_st(mine + M::s(x), s);
+            if (!emptied) {
+                ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (j - 1) & 1, gave_up, a.status));
+                if (!ok) break;
+                after_sync();
+            }
+            tmem_st(mine + M::p(x), s);
             wait_st();
             before_sync();
             mbar_arrive(smem_addr(&ctl.p_full[x]));
@@ -361,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             sum += e0 + e1;
         }
         if (ok && n[x]) {
-            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.o_full[x]), 0, gave_up, a.status));
+            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (n[x] - 1) & 1, gave_up, a.status));
             after_sync();
         }
         if (ok) {
@@ -392,35 +429,58 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------------- decoders
         const int tid = threadIdx.x - kSoftmaxWarps * 32;
+        // K: key tid / 4 (and 32 more), a quarter of its channels. V: eight keys (a core column) of chunk r, one word (8
+        // channels) of each.
+        constexpr int kWords = D / 64;                            // words of a V chunk
+        constexpr int kGroups = G * 64 / D > 0 ? G * 64 / D : 1;  // groups that a word's channels lie in
+        const int t = tid & 3, wd = tid % kWords, r = tid / kWords % 8, kc = tid / kWords / 8, g0 = wd * 64 * G / D;
+        const bool has_v = kc < kKeys / 8;
+        const uint32_t from_k = base + S::kRingAt + (tid / 64) * BB + (tid / 4 % kBlockTokens) * (D / 2) + t * (D / 8);
+        const uint32_t from_kp = base + S::kRingAt + (tid / 64) * BB + k_params_at(D) + (tid / 4 % kBlockTokens) * 4 * G;
+        const uint32_t blk_v = base + S::kRingAt + (has_v ? kc / 2 : 0) * BB, tok_v = (kc & 1) * 8;
+        const uint32_t from_v = blk_v + v_codes_at(D) + tok_v * (D / 2) + r * (D / 16) + 4 * wd;
+        const uint32_t from_vp = blk_v + v_params_at(D, G) + tok_v * 4 * G + 4 * g0;
+        const uint32_t to_k = base + S::kAtK + (tid / 32) * 128 + (tid / 4 % 8) * 16 + t * S::kLboK;
+        const uint32_t to_v = base + S::kAtV + kc * S::kLboV + wd * 1024 + r * 16;
 #pragma unroll 1
         for (int j = 0; j < steps; ++j) {
             const int slot = j % kRing, stage = j & 1;
             bool ok = wait_for(smem_addr(&ctl.packed_full[slot]), (j / kRing) & 1, gave_up, a.status);
-            if (j >= 2) ok = wait_for(smem_addr(&ctl.k_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
-            const uint32_t packed = base + S::kRingAt + slot * S::kPacked;
-            // K: key tid / 4 (and 32 more), a quarter of its channels
+            // all that this thread needs of the step, then the slot is free
+            const uint32_t off = slot * S::kPacked;
+            uint32_t kw[2][D / 32], kp[2][G], w[8], p[kGroups][8];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int key = tid / 4 + 32 * half, t = tid & 3;
-                const uint32_t blk = packed + (key / kBlockTokens) * BB;
-                uint32_t w[D / 32], p[G];
-                const uint32_t at = blk + (key % kBlockTokens) * (D / 2) + t * (D / 8);
+            for (int half = 0; half < 2; ++half) {  // 32 keys on: two blocks on
                 if constexpr (D == 128) {
-                    const uint4 u = lds4(at);
-                    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                    const uint4 u = lds4(from_k + off + half * 2 * BB);
+                    kw[half][0] = u.x, kw[half][1] = u.y, kw[half][2] = u.z, kw[half][3] = u.w;
                 } else {
-                    const uint2 u = lds2(at);
-                    w[0] = u.x, w[1] = u.y;
+                    const uint2 u = lds2(from_k + off + half * 2 * BB);
+                    kw[half][0] = u.x, kw[half][1] = u.y;
                 }
 #pragma unroll
-                for (int g = 0; g < G; ++g) p[g] = lds1(blk + k_params_at(D) + (key % kBlockTokens) * 4 * G + 4 * g);
-                const uint32_t dst = base + S::kAtK + stage * S::kBytesK + (key / 8) * 128 + (key % 8) * 16;
+                for (int g = 0; g < G; ++g) kp[half][g] = lds1(from_kp + off + half * 2 * BB + 4 * g);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                w[k] = lds1(from_v + off + k * (D / 2));
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) p[g][k] = lds1(from_vp + off + k * 4 * G + 4 * g);
+            }
+            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&ctl.packed_empty[slot]));
+            if (j >= 2) ok = wait_for(smem_addr(&ctl.k_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status);
+            if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t dst = to_k + stage * S::kBytesK + half * 512;
 #pragma unroll
                 for (int q = 0; q < D / 32; ++q) {
-                    const uint32_t pg = p[q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
-                    const uint32_t y = w[q] >> 8;
-                    sts4(dst + (4 * q + t) * S::kLboK, value_low(w[q], sc, z), value_high(w[q], sc, z), value_low(y, sc, z),
+                    const uint32_t pg = kp[half][q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
+                    const uint32_t x = kw[half][q], y = x >> 8;
+                    sts4(dst + 4 * q * S::kLboK, value_low(x, sc, z), value_high(x, sc, z), value_low(y, sc, z),
                          value_high(y, sc, z));
                 }
             }
@@ -428,44 +488,32 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             mbar_arrive(smem_addr(&ctl.k_full[stage]));
             if (j >= 2) ok = wait_for(smem_addr(&ctl.v_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status);
             if (!__all_sync(0xffffffffu, ok)) break;
-            // V: eight keys (a core column) of chunk r, one word (8 channels) of each at a time
-            constexpr int kWords = D / 64;              // words of a chunk
-            constexpr int kItems = kKeys / 8 * 8 * kWords;
-            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
             const bool ragged = (j + 1) * kKeys > rq.len || hidden;
-            if (tid < kItems) {
-                const int wd = tid % kWords, r = tid / kWords % 8, kc = tid / kWords / 8;
-                const uint32_t blk = packed + (kc / 2) * BB;
-                const int tok = (kc & 1) * 8;
-                constexpr int kGroups = G * 64 / D > 0 ? G * 64 / D : 1;  // groups that a word's channels lie in
-                const int g0 = wd * 64 * G / D;
-                uint32_t w[8], sc[kGroups][4], z[kGroups][4];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) w[k] = lds1(blk + v_codes_at(D) + (tok + k) * (D / 2) + r * (D / 16) + 4 * wd);
+            if (has_v) {
+                uint32_t sc[kGroups][4], z[kGroups][4];
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
-                    uint32_t p[8], probe = 0u;
+                    uint32_t probe = 0u;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        p[k] = lds1(blk + v_params_at(D, G) + (tok + k) * 4 * G + 4 * (g0 + g));
-                        if (ragged && (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u))) p[k] = 0u;
-                        probe = hfma(p[k], 0u, probe);  // 0, or NaN once something is not finite
+                        if (ragged && (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u))) p[g][k] = 0u;
+                        probe = hfma(p[g][k], 0u, probe);  // 0, or NaN once something is not finite
                     }
                     if (probe & 0x7fff7fffu) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            if ((p[k] & 0x7c00u) == 0x7c00u || (p[k] & 0x7c000000u) == 0x7c000000u) {
-                                p[k] = 0u;
+                            if ((p[g][k] & 0x7c00u) == 0x7c00u || (p[g][k] & 0x7c000000u) == 0x7c000000u) {
+                                p[g][k] = 0u;
                                 atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + k);
                             }
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        sc[g][k] = __byte_perm(p[2 * k], p[2 * k + 1], 0x5410);
-                        z[g][k] = __byte_perm(p[2 * k], p[2 * k + 1], 0x7632);
+                        sc[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x5410);
+                        z[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x7632);
                     }
                 }
-                const uint32_t dst = base + S::kAtV + stage * S::kBytesV + kc * S::kLboV + wd * 1024 + r * 16;
+                const uint32_t dst = to_v + stage * S::kBytesV;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {  // nibbles 4 h .. 4 h + 3: channels 8 (8 wd + 4 h + i) + r
                     uint32_t v[4][4];
@@ -484,52 +532,55 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             }
             fence_proxy_async();
             mbar_arrive(smem_addr(&ctl.v_full[stage]));
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&ctl.packed_empty[slot]));
         }
     } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------------- products
-        if (lane == 0 && steps) {
+        if (steps) {
             // D fp32, A and B fp16, both K-major; N >> 3 at bit 17, M = 128 >> 4 at bit 24
             constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
             constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
-            auto scores = [&](int x, int j) {
-                const uint32_t k = base + S::kAtK + (j & 1) * S::kBytesK;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma_ts(tmem + M::s(x), tmem + M::q(x) + 8 * i, kmajor(k + 2 * i * S::kLboK, S::kLboK, 128), kIdescS, i != 0);
-                commit(smem_addr(&ctl.s_full[x]));
+            const uint64_t k0 = kmajor(base + S::kAtK, S::kLboK, 128), v0 = kmajor(base + S::kAtV, S::kLboV, 128),
+                           q0 = kmajor(base + S::kAtQ, S::kLboQ, 128);
+            auto wait = [&](uint64_t* bar, int parity) {
+                return __all_sync(0xffffffffu, wait_for(smem_addr(bar), parity, gave_up, a.status)) != 0;
             };
-            bool ok = wait_for(smem_addr(&ctl.k_full[0]), 0, gave_up, a.status);
-            for (int x = 0; x < 2 && ok; ++x) {
-                if (!n[x]) continue;
-                ok = wait_for(smem_addr(&ctl.q_full[x]), 0, gave_up, a.status);
-                after_sync();
-                if (ok) scores(x, 0);
-            }
-            if (ok) commit(smem_addr(&ctl.k_empty[0]));
+            bool ok = true;
 #pragma unroll 1
-            for (int j = 0; j < steps && ok; ++j) {
+            for (int j = -1; j < steps && ok; ++j) {
+                // scores of step j + 1, as soon as those of step j are in registers
                 const int next = (j + 1) & 1;
-                ok = wait_for(smem_addr(&ctl.v_full[j & 1]), (j >> 1) & 1, gave_up, a.status);
-                if (ok && j + 1 < steps) ok = wait_for(smem_addr(&ctl.k_full[next]), ((j + 1) >> 1) & 1, gave_up, a.status);
+                if (j + 1 < steps) ok = wait(&ctl.k_full[next], ((j + 1) >> 1) & 1);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || j + 1 >= n[x]) continue;
+                    ok = j < 0 ? wait(&ctl.q_full[x], 0) : wait(&ctl.s_read[x], j & 1);
+                    if (!ok) continue;
+                    after_sync();
+                    const uint64_t k = k0 + next * (S::kBytesK / 16);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        if (x == 0) mma_ts(tmem + M::s(0), tmem + M::kQ + 8 * i, k + 2 * i * (S::kLboK / 16), kIdescS, i != 0);
+                        else mma_ss(tmem + M::s(1), q0 + 2 * i * (S::kLboQ / 16), k + 2 * i * (S::kLboK / 16), kIdescS, i != 0);
+                    }
+                    commit(smem_addr(&ctl.s_full[x]));
+                }
+                if (!ok) break;
+                if (j + 1 < steps) commit(smem_addr(&ctl.k_empty[next]));
+                if (j < 0) continue;
+                ok = wait(&ctl.v_full[j & 1], (j >> 1) & 1);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (!ok || j >= n[x]) continue;
-                    ok = wait_for(smem_addr(&ctl.p_full[x]), j & 1, gave_up, a.status);
+                    ok = wait(&ctl.p_full[x], j & 1);
                     if (!ok) continue;
                     after_sync();
-                    const uint32_t v = base + S::kAtV + (j & 1) * S::kBytesV;
+                    const uint64_t v = v0 + (j & 1) * (S::kBytesV / 16);
 #pragma unroll
                     for (int i = 0; i < kKeys / 16; ++i)
-                        mma_ts(tmem + M::o(x), tmem + M::s(x) + 8 * i, kmajor(v + 2 * i * S::kLboV, S::kLboV, 128), kIdescO,
-                               (j | i) != 0);
-                    if (j + 1 == n[x]) commit(smem_addr(&ctl.o_full[x]));
-                    else scores(x, j + 1);
+                        mma_ts(tmem + M::o(x), tmem + M::p(x) + 8 * i, v + 2 * i * (S::kLboV / 16), kIdescO, (j | i) != 0);
+                    commit(smem_addr(&ctl.p_read[x]));
                 }
-                if (!ok) break;
-                commit(smem_addr(&ctl.v_empty[j & 1]));
-                if (j + 1 < steps) commit(smem_addr(&ctl.k_empty[next]));
+                if (ok) commit(smem_addr(&ctl.v_empty[j & 1]));
             }
             // nothing is in flight when tensor memory is given back
             commit(smem_addr(&ctl.drained));
