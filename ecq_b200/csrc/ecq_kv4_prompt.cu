@@ -6,14 +6,17 @@
 //   loader   one warp copies the packed blocks of 16 tokens into a ring
 //            (cp.async.bulk, a lane per block, its page number read one step
 //            ahead);
-//   decoders four warps turn codes into fp16 K [64 x D] and V^T [D x 64] in the
-//            tensor core's K-major, no-swizzle layout: code * scale + zero,
-//            rounded once to fp16, shared by all 256 rows;
+//   decoders four warps turn codes into fp16 K [64 x D] and four into V^T [D x
+//            64], in the tensor core's K-major, no-swizzle layout: code * scale +
+//            zero, rounded once to fp16, shared by all 256 rows;
 //   MMA      one warp issues S = Q K^T and O += P V for both tiles;
-//   softmax  four warps per tile, a thread per row: S from tensor memory (its
-//            place is free for the next step's scores at once), running maximum
-//            (raised only when a score passes it by 2^8: then the row's O is
-//            rescaled), exp2, P as fp16 to tensor memory, sums in fp32.
+//   softmax  eight warps per tile, two threads per row with 32 keys each: S from
+//            tensor memory (its place is free for the next step's scores at
+//            once), running maximum (the two threads exchange theirs; it is
+//            raised only when a score passes it by 2^8, and the row's O is
+//            rescaled then), exp2, P as fp16 to tensor memory, sums in fp32. With
+//            one thread per row the warps' own latencies took twice the time of
+//            the exponentials.
 // So the next scores and the last step's O += P V are made while the
 // exponentials of a step are computed. Tensor memory is full (512 columns): Q
 // of the first tile, S, P and O of both; the second tile's Q lies in shared
@@ -35,6 +38,7 @@
 // roles then leave, and tensor memory is given back after the products in
 // flight.
 #include <cuda_runtime.h>
+#include <stddef.h>
 
 #include "ecq_kv4_attention.cuh"
 
@@ -50,8 +54,9 @@ using ecq_dev::smem_addr;
 constexpr int kKeys = 64;                       // keys a step
 constexpr int kTileBlocks = kKeys / kBlockTokens;
 constexpr int kRows = 128, kCtaRows = 2 * kRows;
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
+constexpr int kSoftmaxWarps = 16, kDecodeWarps = 8;  // decoders: four for K, four for V
 constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 2) * 32;
+constexpr int kHalf = kKeys / 2;                // keys of a step that a softmax thread takes
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;  // the loader is the one behind it
 constexpr int kRing = 4;
 constexpr uint32_t kTmemColumns = 512;
@@ -83,8 +88,10 @@ struct Control {
     uint64_t packed_full[kRing], packed_empty[kRing];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t q_full[2], s_full[2], s_read[2], p_full[2], p_read[2], drained;
+    uint64_t pair[8];        // of the two warps that share 32 rows
+    float top[2][2][2 * kRows], sum[2][2 * kRows];  // by step parity and half: a row's maximum; by half: its sum
     uint32_t tmem, gave_up;
-    uint32_t hidden[8];  // by step: a bit per block where nothing is, or a bad page (the loader is at most 5 steps ahead of a softmax)
+    uint32_t hidden[8];  // by step: a bit per block where nothing is, or a bad page (the loader is at most 6 steps ahead of a softmax)
     int poison[4];           // per group: the first token whose V is not finite
 };
 
@@ -129,6 +136,14 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* v) {  // 32 col
         : "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -137,6 +152,13 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t* v) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
         "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -161,9 +183,9 @@ __device__ __forceinline__ uint2 lds2(uint32_t addr) {
 }
 
 // Waits for a phase of bar; false (and everybody told) after the limit, or
-// where another wait gave up.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, int32_t* status) {
-    if (ecq_dev::mbar_try_wait(bar, parity)) return true;
+// where another wait gave up. (A time hint at the wait makes it a loop of
+// sleeps, which cost a third of the speed.)
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, int32_t* status) {
     const uint64_t t0 = ecq_dev::global_timer_ns();
     for (;;) {
         if (ecq_dev::mbar_try_wait(bar, parity)) return true;
@@ -174,6 +196,9 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
             return false;
         }
     }
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, int32_t* status) {
+    return ecq_dev::mbar_try_wait(bar, parity) || wait_longer(bar, parity, gave_up, status);
 }
 
 __device__ __forceinline__ uint32_t hfma(uint32_t a, uint32_t b, uint32_t c) {
@@ -203,27 +228,29 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     constexpr int BB = block_bytes(D, G);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Control ctl;
+    const uint32_t bars = smem_addr(&ctl);  // once: each look at a shared variable's address costs three instructions
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     volatile uint32_t* gave_up = &ctl.gave_up;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
-            mbar_init(smem_addr(&ctl.packed_full[i]), kTileBlocks);
-            mbar_init(smem_addr(&ctl.packed_empty[i]), kDecodeWarps);
+            mbar_init((bars + offsetof(Control, packed_full) + 8 * (i)), kTileBlocks);
+            mbar_init((bars + offsetof(Control, packed_empty) + 8 * (i)), kDecodeWarps);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&ctl.k_full[i]), kDecodeWarps * 32);
-            mbar_init(smem_addr(&ctl.v_full[i]), kDecodeWarps * 32);
-            mbar_init(smem_addr(&ctl.k_empty[i]), 1);
-            mbar_init(smem_addr(&ctl.v_empty[i]), 1);
-            mbar_init(smem_addr(&ctl.q_full[i]), kRows);
-            mbar_init(smem_addr(&ctl.s_full[i]), 1);
-            mbar_init(smem_addr(&ctl.s_read[i]), kRows);
-            mbar_init(smem_addr(&ctl.p_full[i]), kRows);
-            mbar_init(smem_addr(&ctl.p_read[i]), 1);
+            mbar_init((bars + offsetof(Control, k_full) + 8 * (i)), kDecodeWarps * 16);
+            mbar_init((bars + offsetof(Control, v_full) + 8 * (i)), kDecodeWarps * 16);
+            mbar_init((bars + offsetof(Control, k_empty) + 8 * (i)), 1);
+            mbar_init((bars + offsetof(Control, v_empty) + 8 * (i)), 1);
+            mbar_init((bars + offsetof(Control, q_full) + 8 * (i)), 2 * kRows);
+            mbar_init((bars + offsetof(Control, s_full) + 8 * (i)), 1);
+            mbar_init((bars + offsetof(Control, s_read) + 8 * (i)), 2 * kRows);
+            mbar_init((bars + offsetof(Control, p_full) + 8 * (i)), 2 * kRows);
+            mbar_init((bars + offsetof(Control, p_read) + 8 * (i)), 1);
         }
-        mbar_init(smem_addr(&ctl.drained), 1);
+        mbar_init((bars + offsetof(Control, drained)), 1);
+        for (int i = 0; i < 8; ++i) mbar_init((bars + offsetof(Control, pair) + 8 * (i)), 2);
         ctl.gave_up = 0u;
         for (int g = 0; g < 4; ++g) ctl.poison[g] = INT32_MAX;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -257,14 +284,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
         const int first = tile * kCtaRows + x * kRows, last = min(rq.rows, first + kRows) - 1;
         if (work && first < rq.rows) n[x] = (max(rq.len - rq.queries + last / a.share + 1, 0) + kKeys - 1) / kKeys;
     }
+    // one for the warp, as the compiler can see: the products' operands stay in uniform registers
+    n[0] = __shfl_sync(0xffffffffu, n[0], 0);
+    n[1] = __shfl_sync(0xffffffffu, n[1], 0);
     const int steps = max(n[0], n[1]);
     const uint32_t base = smem_addr(smem);
 
     if (!work) {
         // nothing of this request: straight to the end
     } else if (warp < kSoftmaxWarps) {
-        // ---------------------------------------------------------------- softmax: a thread per row
-        const int x = warp / 4, row = tile * kCtaRows + x * kRows + (warp & 3) * 32 + lane;
+        // ---------------------------------------------------------------- softmax: two threads per row
+        const int x = warp / 8, h = warp / 4 & 1, here = x * kRows + (warp & 3) * 32 + lane, row = tile * kCtaRows + x * kRows + (warp & 3) * 32 + lane;
         const bool in = row < rq.rows;
         const int i = row / a.share;
         const uint32_t mine = tmem + ((warp & 3) << 21);  // lanes 32 (warp % 4) ..
@@ -296,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             }
 #pragma unroll
             for (int part = 0; part < D / 64; ++part) {
+                if (part != h % (D / 64)) continue;
                 uint32_t v[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
@@ -308,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                     v[4 * c + 2] = pack2(f1.x * up, f3.x * up, __half());
                     v[4 * c + 3] = pack2(f1.y * up, f3.y * up, __half());
                     if (x == 1)
-                        sts4(base + S::kAtQ + (8 * part + c) * S::kLboQ + (threadIdx.x - kRows) * 16, v[4 * c], v[4 * c + 1],
+                        sts4(base + S::kAtQ + (8 * part + c) * S::kLboQ + (here - kRows) * 16, v[4 * c], v[4 * c + 1],
                              v[4 * c + 2], v[4 * c + 3]);
                 }
                 if (x == 0) tmem_st(mine + M::kQ + 32 * part, v);
@@ -319,35 +350,47 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             } else {
                 fence_proxy_async();
             }
-            mbar_arrive(smem_addr(&ctl.q_full[x]));
+            mbar_arrive((bars + offsetof(Control, q_full) + 8 * (x)));
         }
         float m = kNoMax;
         uint64_t l[2] = {0ull, 0ull};  // two pairs of sums
         const uint64_t f2x = ecq_dev::pack2(__float_as_uint(factor), __float_as_uint(factor));
+        const uint32_t pair = (bars + offsetof(Control, pair) + 8 * (x * 4 + (warp & 3)));
         bool ok = true;
+        auto wait = [&](uint32_t bar, int parity) {
+            ok = __all_sync(0xffffffffu, wait_for(bar, parity, gave_up, a.status));
+            return ok;
+        };
+        int j = 0;
 #pragma unroll 1
-        for (int j = 0; j < n[x]; ++j) {
-            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.s_full[x]), j & 1, gave_up, a.status));
-            if (!ok) break;
+        for (; j < n[x]; ++j) {
+            if (!wait((bars + offsetof(Control, s_full) + 8 * (x)), j & 1)) break;
             after_sync();
-            uint32_t s[kKeys];
-            tmem_ld(mine + M::s(x), s);
-            tmem_ld(mine + M::s(x) + 32, s + 32);
+            uint32_t s[kHalf];
+            tmem_ld(mine + M::s(x) + kHalf * h, s);
             wait_ld();
             before_sync();
-            mbar_arrive(smem_addr(&ctl.s_read[x]));
-            bool emptied = j == 0;  // P and O are not in use by the last step's product
-            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
-            const int left = limit - j * kKeys;  // keys of this step that the row sees
-            if (__any_sync(0xffffffffu, left < kKeys) || hidden) {
+            mbar_arrive((bars + offsetof(Control, s_read) + 8 * (x)));
+            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]) >> (h * kTileBlocks / 2);
+            const int left = limit - j * kKeys - h * kHalf;  // of this thread's keys those that the row sees
+            if (__any_sync(0xffffffffu, left < kHalf) || hidden) {
 #pragma unroll
-                for (int k = 0; k < kKeys; ++k)
+                for (int k = 0; k < kHalf; ++k)
                     if (k >= left || (hidden >> (k / kBlockTokens) & 1u)) s[k] = 0xff800000u;
             }
-            float top = __uint_as_float(s[0]);
+            float t[4];
 #pragma unroll
-            for (int k = 1; k < kKeys; ++k) top = fmaxf(top, __uint_as_float(s[k]));
-            top *= factor;
+            for (int k = 0; k < 4; ++k) t[k] = __uint_as_float(s[k]);
+#pragma unroll
+            for (int k = 4; k < kHalf; ++k) t[k & 3] = fmaxf(t[k & 3], __uint_as_float(s[k]));
+            float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * factor;
+            volatile float* tops = &ctl.top[j & 1][0][0];
+            tops[h * 2 * kRows + here] = top;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair);
+            if (!wait(pair, j & 1)) break;
+            top = fmaxf(top, tops[(h ^ 1) * 2 * kRows + here]);
+            bool emptied = j == 0;  // P and O are not in use by the last step's product
             if (__any_sync(0xffffffffu, top > m + (kSlack + kLift))) {
                 const float next = fmaxf(top - kLift, m), keep = exp2_fast(m - next);
                 m = next;
@@ -355,24 +398,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
 #pragma unroll
                 for (int u = 0; u < 2; ++u) l[u] = ecq_dev::fma2(l[u], k2, 0ull);
                 if (j) {
-                    ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (j - 1) & 1, gave_up, a.status));
-                    if (!ok) break;
+                    if (!wait((bars + offsetof(Control, p_read) + 8 * (x)), (j - 1) & 1)) break;
                     after_sync();
                     emptied = true;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld(mine + M::o(x) + c, o);
+                    for (int c = 0; c < D / 2; c += 16) {  // this thread's half of the channels
+                        uint32_t o[16];
+                        tmem_ld16(mine + M::o(x) + h * (D / 2) + c, o);
                         wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                        tmem_st(mine + M::o(x) + c, o);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_st16(mine + M::o(x) + h * (D / 2) + c, o);
                     }
                 }
             }
             const uint64_t m2 = ecq_dev::pack2(__float_as_uint(-m), __float_as_uint(-m));
 #pragma unroll
-            for (int k = 0; k < kKeys; k += 2) {
+            for (int k = 0; k < kHalf; k += 2) {
                 float e0, e1;
                 ecq_dev::unpack2(ecq_dev::fma2(ecq_dev::pack2(s[k], s[k + 1]), f2x, m2), e0, e1);
                 e0 = exp2_fast(e0);
@@ -381,14 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                 s[k / 2] = pack2(e0, e1, __half());
             }
             if (!emptied) {
-                ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (j - 1) & 1, gave_up, a.status));
-                if (!ok) break;
+                if (!wait((bars + offsetof(Control, p_read) + 8 * (x)), (j - 1) & 1)) break;
                 after_sync();
             }
-            tmem_st(mine + M::p(x), s);
+            tmem_st16(mine + M::p(x) + kHalf / 2 * h, s);
             wait_st();
             before_sync();
-            mbar_arrive(smem_addr(&ctl.p_full[x]));
+            mbar_arrive((bars + offsetof(Control, p_full) + 8 * (x)));
         }
         float sum = 0.f;
 #pragma unroll
@@ -398,26 +439,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             sum += e0 + e1;
         }
         if (ok && n[x]) {
-            ok = __all_sync(0xffffffffu, wait_for(smem_addr(&ctl.p_read[x]), (n[x] - 1) & 1, gave_up, a.status));
+            volatile float* sums = &ctl.sum[0][0];
+            sums[h * 2 * kRows + here] = sum;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair);
+            if (wait(pair, j & 1)) {
+                sum += sums[(h ^ 1) * 2 * kRows + here];
+                wait((bars + offsetof(Control, p_read) + 8 * (x)), (j - 1) & 1);
+            }
             after_sync();
         }
         if (ok) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             T* dst = out_row<T>(a, rq.first_q, head, in ? row : 0);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
+            for (int c = h * (D / 2); c < (h + 1) * (D / 2); c += 16) {
+                uint32_t o[16];
                 if (n[x]) {
-                    tmem_ld(mine + M::o(x) + c, o);
+                    tmem_ld16(mine + M::o(x) + c, o);
                     wait_ld();
                 }
                 if (limit > ctl.poison[c * G / D]) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0x7fc00000u;
+                    for (int e = 0; e < 16; ++e) o[e] = 0x7fc00000u;
                 }
                 if (in) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
+                    for (int e = 0; e < 16; e += 4) {
                         float v[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) v[k] = sum == 0.f ? 0.f : __uint_as_float(o[e + k]) * inv;
@@ -429,109 +477,122 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------------- decoders
         const int tid = threadIdx.x - kSoftmaxWarps * 32;
-        // K: key tid / 4 (and 32 more), a quarter of its channels. V: eight keys (a core column) of chunk r, one word (8
-        // channels) of each.
-        constexpr int kWords = D / 64;                            // words of a V chunk
-        constexpr int kGroups = G * 64 / D > 0 ? G * 64 / D : 1;  // groups that a word's channels lie in
-        const int t = tid & 3, wd = tid % kWords, r = tid / kWords % 8, kc = tid / kWords / 8, g0 = wd * 64 * G / D;
-        const bool has_v = kc < kKeys / 8;
-        const uint32_t from_k = base + S::kRingAt + (tid / 64) * BB + (tid / 4 % kBlockTokens) * (D / 2) + t * (D / 8);
-        const uint32_t from_kp = base + S::kRingAt + (tid / 64) * BB + k_params_at(D) + (tid / 4 % kBlockTokens) * 4 * G;
-        const uint32_t blk_v = base + S::kRingAt + (has_v ? kc / 2 : 0) * BB, tok_v = (kc & 1) * 8;
-        const uint32_t from_v = blk_v + v_codes_at(D) + tok_v * (D / 2) + r * (D / 16) + 4 * wd;
-        const uint32_t from_vp = blk_v + v_params_at(D, G) + tok_v * 4 * G + 4 * g0;
-        const uint32_t to_k = base + S::kAtK + (tid / 32) * 128 + (tid / 4 % 8) * 16 + t * S::kLboK;
-        const uint32_t to_v = base + S::kAtV + kc * S::kLboV + wd * 1024 + r * 16;
+        if (warp < kSoftmaxWarps + kDecodeWarps / 2) {
+            // K: key tid / 4 (and 32 more), a quarter of its channels
+            const int t = tid & 3;
+            const uint32_t from = base + S::kRingAt + (tid / 64) * BB + (tid / 4 % kBlockTokens) * (D / 2) + t * (D / 8);
+            const uint32_t from_p = base + S::kRingAt + (tid / 64) * BB + k_params_at(D) + (tid / 4 % kBlockTokens) * 4 * G;
+            const uint32_t to = base + S::kAtK + (tid / 32) * 128 + (tid / 4 % 8) * 16 + t * S::kLboK;
 #pragma unroll 1
-        for (int j = 0; j < steps; ++j) {
-            const int slot = j % kRing, stage = j & 1;
-            bool ok = wait_for(smem_addr(&ctl.packed_full[slot]), (j / kRing) & 1, gave_up, a.status);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            // all that this thread needs of the step, then the slot is free
-            const uint32_t off = slot * S::kPacked;
-            uint32_t kw[2][D / 32], kp[2][G], w[8], p[kGroups][8];
+            for (int j = 0; j < steps; ++j) {
+                const int slot = j % kRing, stage = j & 1;
+                if (!__all_sync(0xffffffffu, wait_for((bars + offsetof(Control, packed_full) + 8 * (slot)), (j / kRing) & 1, gave_up, a.status))) break;
+                // all that this thread needs of the step, then the slot is free
+                const uint32_t off = slot * S::kPacked;
+                uint32_t w[2][D / 32], p[2][G];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {  // 32 keys on: two blocks on
-                if constexpr (D == 128) {
-                    const uint4 u = lds4(from_k + off + half * 2 * BB);
-                    kw[half][0] = u.x, kw[half][1] = u.y, kw[half][2] = u.z, kw[half][3] = u.w;
-                } else {
-                    const uint2 u = lds2(from_k + off + half * 2 * BB);
-                    kw[half][0] = u.x, kw[half][1] = u.y;
-                }
-#pragma unroll
-                for (int g = 0; g < G; ++g) kp[half][g] = lds1(from_kp + off + half * 2 * BB + 4 * g);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                w[k] = lds1(from_v + off + k * (D / 2));
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) p[g][k] = lds1(from_vp + off + k * 4 * G + 4 * g);
-            }
-            const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&ctl.packed_empty[slot]));
-            if (j >= 2) ok = wait_for(smem_addr(&ctl.k_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status);
-            if (!__all_sync(0xffffffffu, ok)) break;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t dst = to_k + stage * S::kBytesK + half * 512;
-#pragma unroll
-                for (int q = 0; q < D / 32; ++q) {
-                    const uint32_t pg = kp[half][q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
-                    const uint32_t x = kw[half][q], y = x >> 8;
-                    sts4(dst + 4 * q * S::kLboK, value_low(x, sc, z), value_high(x, sc, z), value_low(y, sc, z),
-                         value_high(y, sc, z));
-                }
-            }
-            fence_proxy_async();
-            mbar_arrive(smem_addr(&ctl.k_full[stage]));
-            if (j >= 2) ok = wait_for(smem_addr(&ctl.v_empty[stage]), ((j >> 1) - 1) & 1, gave_up, a.status);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            const bool ragged = (j + 1) * kKeys > rq.len || hidden;
-            if (has_v) {
-                uint32_t sc[kGroups][4], z[kGroups][4];
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    uint32_t probe = 0u;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if (ragged && (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u))) p[g][k] = 0u;
-                        probe = hfma(p[g][k], 0u, probe);  // 0, or NaN once something is not finite
-                    }
-                    if (probe & 0x7fff7fffu) {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if ((p[g][k] & 0x7c00u) == 0x7c00u || (p[g][k] & 0x7c000000u) == 0x7c000000u) {
-                                p[g][k] = 0u;
-                                atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + k);
-                            }
+                for (int half = 0; half < 2; ++half) {  // 32 keys on: two blocks on
+                    if constexpr (D == 128) {
+                        const uint4 u = lds4(from + off + half * 2 * BB);
+                        w[half][0] = u.x, w[half][1] = u.y, w[half][2] = u.z, w[half][3] = u.w;
+                    } else {
+                        const uint2 u = lds2(from + off + half * 2 * BB);
+                        w[half][0] = u.x, w[half][1] = u.y;
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        sc[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x5410);
-                        z[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x7632);
+                    for (int g = 0; g < G; ++g) p[half][g] = lds1(from_p + off + half * 2 * BB + 4 * g);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive((bars + offsetof(Control, packed_empty) + 8 * (slot)));
+                if (j >= 2 && !__all_sync(0xffffffffu, wait_for((bars + offsetof(Control, k_empty) + 8 * (stage)), ((j >> 1) - 1) & 1, gave_up, a.status)))
+                    break;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t dst = to + stage * S::kBytesK + half * 512;
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        const uint32_t pg = p[half][q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
+                        const uint32_t u = w[half][q], y = u >> 8;
+                        sts4(dst + 4 * q * S::kLboK, value_low(u, sc, z), value_high(u, sc, z), value_low(y, sc, z),
+                             value_high(y, sc, z));
                     }
                 }
-                const uint32_t dst = to_v + stage * S::kBytesV;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // nibbles 4 h .. 4 h + 3: channels 8 (8 wd + 4 h + i) + r
-                    uint32_t v[4][4];
-                    const int g = kGroups == 1 ? 0 : h * kGroups / 2;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t pair = __byte_perm(w[2 * k], w[2 * k + 1], h ? 0x7632 : 0x5410), y = pair >> 8;
-                        v[0][k] = value_low(pair, sc[g][k], z[g][k]);
-                        v[1][k] = value_high(pair, sc[g][k], z[g][k]);
-                        v[2][k] = value_low(y, sc[g][k], z[g][k]);
-                        v[3][k] = value_high(y, sc[g][k], z[g][k]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sts4(dst + (4 * h + e) * 128, v[e][0], v[e][1], v[e][2], v[e][3]);
-                }
+                fence_proxy_async();
+                mbar_arrive((bars + offsetof(Control, k_full) + 8 * (stage)));
             }
-            fence_proxy_async();
-            mbar_arrive(smem_addr(&ctl.v_full[stage]));
+        } else {
+            // V: eight keys (a core column) of chunk r, one word (8 channels) of each
+            constexpr int kWords = D / 64;                            // words of a V chunk
+            constexpr int kGroups = G * 64 / D > 0 ? G * 64 / D : 1;  // groups that a word's channels lie in
+            const int id = tid - kDecodeWarps / 2 * 32;
+            const int wd = id % kWords, r = id / kWords % 8, kc = id / kWords / 8, g0 = wd * 64 * G / D;
+            const bool has = kc < kKeys / 8;
+            const uint32_t blk = base + S::kRingAt + (has ? kc / 2 : 0) * BB, tok = (kc & 1) * 8;
+            const uint32_t from = blk + v_codes_at(D) + tok * (D / 2) + r * (D / 16) + 4 * wd;
+            const uint32_t from_p = blk + v_params_at(D, G) + tok * 4 * G + 4 * g0;
+            const uint32_t to = base + S::kAtV + kc * S::kLboV + wd * 1024 + r * 16;
+#pragma unroll 1
+            for (int j = 0; j < steps; ++j) {
+                const int slot = j % kRing, stage = j & 1;
+                if (!__all_sync(0xffffffffu, wait_for((bars + offsetof(Control, packed_full) + 8 * (slot)), (j / kRing) & 1, gave_up, a.status))) break;
+                const uint32_t off = slot * S::kPacked;
+                uint32_t w[8], p[kGroups][8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    w[k] = lds1(from + off + k * (D / 2));
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) p[g][k] = lds1(from_p + off + k * 4 * G + 4 * g);
+                }
+                const uint32_t hidden = *reinterpret_cast<volatile uint32_t*>(&ctl.hidden[j & 7]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive((bars + offsetof(Control, packed_empty) + 8 * (slot)));
+                if (j >= 2 && !__all_sync(0xffffffffu, wait_for((bars + offsetof(Control, v_empty) + 8 * (stage)), ((j >> 1) - 1) & 1, gave_up, a.status)))
+                    break;
+                const bool ragged = (j + 1) * kKeys > rq.len || hidden;
+                if (has) {
+                    uint32_t sc[kGroups][4], z[kGroups][4];
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        uint32_t probe = 0u;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (ragged && (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u))) p[g][k] = 0u;
+                            probe = hfma(p[g][k], 0u, probe);  // 0, or NaN once something is not finite
+                        }
+                        if (probe & 0x7fff7fffu) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if ((p[g][k] & 0x7c00u) == 0x7c00u || (p[g][k] & 0x7c000000u) == 0x7c000000u) {
+                                    p[g][k] = 0u;
+                                    atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + k);
+                                }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            sc[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x5410);
+                            z[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x7632);
+                        }
+                    }
+                    const uint32_t dst = to + stage * S::kBytesV;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // nibbles 4 h .. 4 h + 3: channels 8 (8 wd + 4 h + i) + r
+                        uint32_t v[4][4];
+                        const int g = kGroups == 1 ? 0 : h * kGroups / 2;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t both = __byte_perm(w[2 * k], w[2 * k + 1], h ? 0x7632 : 0x5410), y = both >> 8;
+                            v[0][k] = value_low(both, sc[g][k], z[g][k]);
+                            v[1][k] = value_high(both, sc[g][k], z[g][k]);
+                            v[2][k] = value_low(y, sc[g][k], z[g][k]);
+                            v[3][k] = value_high(y, sc[g][k], z[g][k]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sts4(dst + (4 * h + e) * 128, v[e][0], v[e][1], v[e][2], v[e][3]);
+                    }
+                }
+                fence_proxy_async();
+                mbar_arrive((bars + offsetof(Control, v_full) + 8 * (stage)));
+            }
         }
     } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------------- products
@@ -541,19 +602,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
             const uint64_t k0 = kmajor(base + S::kAtK, S::kLboK, 128), v0 = kmajor(base + S::kAtV, S::kLboV, 128),
                            q0 = kmajor(base + S::kAtQ, S::kLboQ, 128);
-            auto wait = [&](uint64_t* bar, int parity) {
-                return __all_sync(0xffffffffu, wait_for(smem_addr(bar), parity, gave_up, a.status)) != 0;
+            auto wait = [&](uint32_t bar, int parity) {
+                return __all_sync(0xffffffffu, wait_for(bar, parity, gave_up, a.status)) != 0;
             };
             bool ok = true;
 #pragma unroll 1
             for (int j = -1; j < steps && ok; ++j) {
                 // scores of step j + 1, as soon as those of step j are in registers
                 const int next = (j + 1) & 1;
-                if (j + 1 < steps) ok = wait(&ctl.k_full[next], ((j + 1) >> 1) & 1);
+                if (j + 1 < steps) ok = wait(bars + offsetof(Control, k_full) + 8 * next, ((j + 1) >> 1) & 1);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (!ok || j + 1 >= n[x]) continue;
-                    ok = j < 0 ? wait(&ctl.q_full[x], 0) : wait(&ctl.s_read[x], j & 1);
+                    ok = j < 0 ? wait(bars + offsetof(Control, q_full) + 8 * x, 0) : wait(bars + offsetof(Control, s_read) + 8 * x, j & 1);
                     if (!ok) continue;
                     after_sync();
                     const uint64_t k = k0 + next * (S::kBytesK / 16);
@@ -562,29 +623,29 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                         if (x == 0) mma_ts(tmem + M::s(0), tmem + M::kQ + 8 * i, k + 2 * i * (S::kLboK / 16), kIdescS, i != 0);
                         else mma_ss(tmem + M::s(1), q0 + 2 * i * (S::kLboQ / 16), k + 2 * i * (S::kLboK / 16), kIdescS, i != 0);
                     }
-                    commit(smem_addr(&ctl.s_full[x]));
+                    commit((bars + offsetof(Control, s_full) + 8 * (x)));
                 }
                 if (!ok) break;
-                if (j + 1 < steps) commit(smem_addr(&ctl.k_empty[next]));
+                if (j + 1 < steps) commit((bars + offsetof(Control, k_empty) + 8 * (next)));
                 if (j < 0) continue;
-                ok = wait(&ctl.v_full[j & 1], (j >> 1) & 1);
+                ok = wait(bars + offsetof(Control, v_full) + 8 * (j & 1), (j >> 1) & 1);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (!ok || j >= n[x]) continue;
-                    ok = wait(&ctl.p_full[x], j & 1);
+                    ok = wait(bars + offsetof(Control, p_full) + 8 * x, j & 1);
                     if (!ok) continue;
                     after_sync();
                     const uint64_t v = v0 + (j & 1) * (S::kBytesV / 16);
 #pragma unroll
                     for (int i = 0; i < kKeys / 16; ++i)
                         mma_ts(tmem + M::o(x), tmem + M::p(x) + 8 * i, v + 2 * i * (S::kLboV / 16), kIdescO, (j | i) != 0);
-                    commit(smem_addr(&ctl.p_read[x]));
+                    commit((bars + offsetof(Control, p_read) + 8 * (x)));
                 }
-                if (ok) commit(smem_addr(&ctl.v_empty[j & 1]));
+                if (ok) commit((bars + offsetof(Control, v_empty) + 8 * (j & 1)));
             }
             // nothing is in flight when tensor memory is given back
-            commit(smem_addr(&ctl.drained));
-            ecq_dev::mbar_wait(smem_addr(&ctl.drained), 0);
+            commit((bars + offsetof(Control, drained)));
+            ecq_dev::mbar_wait((bars + offsetof(Control, drained)), 0);
         }
         __syncwarp();
     } else {
@@ -602,9 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
 #pragma unroll 1
             for (; j < steps; ++j) {
                 const int slot = j % kRing;
-                const uint32_t bar = smem_addr(&ctl.packed_full[slot]);
+                const uint32_t bar = (bars + offsetof(Control, packed_full) + 8 * (slot));
                 bool ok = true;
-                if (j >= kRing) ok = wait_for(smem_addr(&ctl.packed_empty[slot]), (j / kRing - 1) & 1, gave_up, a.status);
+                if (j >= kRing) ok = wait_for((bars + offsetof(Control, packed_empty) + 8 * (slot)), (j / kRing - 1) & 1, gave_up, a.status);
                 if (!__all_sync(kLanes, ok)) break;
                 const bool there = page >= 0 && page < a.n_pages;
                 if (page >= a.n_pages) raise_status(a.status, ECQ_STATUS_BADARG);
@@ -624,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
                 page = page_of(j + 1);
             }
             // no copy is in flight when the shared memory is given back
-            for (int i = max(j - kRing, 0); i < j; ++i) ecq_dev::mbar_wait(smem_addr(&ctl.packed_full[i % kRing]), (i / kRing) & 1);
+            for (int i = max(j - kRing, 0); i < j; ++i) ecq_dev::mbar_wait((bars + offsetof(Control, packed_full) + 8 * (i % kRing)), (i / kRing) & 1);
         }
         __syncwarp();
     }
