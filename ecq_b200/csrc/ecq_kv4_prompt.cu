@@ -71,9 +71,11 @@ struct Smem {
     // K: core columns of 8 channels, 64 keys of 16 bytes each; 32 more bytes put a warp's stores in different banks
     static constexpr uint32_t kLboK = kKeys * 16 + 32, kBytesK = D / 8 * kLboK;
     static constexpr uint32_t kLboV = D * 16, kBytesV = kKeys / 8 * kLboV;
-    static constexpr uint32_t kLboQ = kRows * 16, kBytesQ = D / 8 * kLboQ;
+    // Q of both tiles: the first one's on its way to tensor memory; a tile's output at the end. 16 more bytes a core column:
+    // a warp writes rows
+    static constexpr uint32_t kLboQ = kRows * 16 + 16, kBytesQ = D / 8 * kLboQ;
     static constexpr int kRingAt = 0, kAtK = kRing * kPacked, kAtV = kAtK + 2 * kBytesK, kAtQ = kAtV + 2 * kBytesV,
-                         kBytes = kAtQ + kBytesQ;
+                         kBytes = kAtQ + 2 * kBytesQ;
 };
 
 // Tensor memory columns (of tile x)
@@ -88,8 +90,10 @@ struct Control {
     uint64_t packed_full[kRing], packed_empty[kRing];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t q_full[2], s_full[2], s_read[2], p_full[2], p_read[2], drained;
+    uint64_t rows[2];        // a tile's q is in shared memory
     uint64_t pair[8];        // of the two warps that share 32 rows
     float top[2][2][2 * kRows], sum[2][2 * kRows];  // by step parity and half: a row's maximum; by half: its sum
+    float factor[2 * kRows];
     uint32_t tmem, gave_up;
     uint32_t hidden[8];  // by step: a bit per block where nothing is, or a bad page (the loader is at most 6 steps ahead of a softmax)
     int poison[4];           // per group: the first token whose V is not finite
@@ -233,6 +237,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     volatile uint32_t* gave_up = &ctl.gave_up;
 
+    ecq_dev::pdl_wait();
+    // the last tiles, which see the most keys, first
+    const int per_tile = a.kv_heads * a.batch;
+    const int tile = tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
+    const int b = static_cast<int>(blockIdx.x % per_tile) / a.kv_heads, head = static_cast<int>(blockIdx.x % per_tile) % a.kv_heads;
+    const Range rq = range_of(a, b);
+    if (tile == tiles - 1 && threadIdx.x == 0 && rq.rows > a.most_rows && rq.queries > 0 &&
+        (rq.rows - 1) / kCtaRows >= tiles)
+        raise_status(a.status, ECQ_STATUS_BADARG);  // more queries than the call said: their rows are not computed
+    const bool work = rq.rows > a.most_rows && tile * kCtaRows < rq.rows;
+    if (!work) {
+        ecq_dev::pdl_launch_dependents();
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
             mbar_init((bars + offsetof(Control, packed_full) + 8 * (i)), kTileBlocks);
@@ -249,7 +267,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             mbar_init((bars + offsetof(Control, p_full) + 8 * (i)), 2 * kRows);
             mbar_init((bars + offsetof(Control, p_read) + 8 * (i)), 1);
         }
-        mbar_init((bars + offsetof(Control, drained)), 1);
+        mbar_init(bars + offsetof(Control, drained), 1);
+        for (int i = 0; i < 2; ++i) mbar_init(bars + offsetof(Control, rows) + 8 * i, kSoftmaxWarps / 2);
         for (int i = 0; i < 8; ++i) mbar_init((bars + offsetof(Control, pair) + 8 * (i)), 2);
         ctl.gave_up = 0u;
         for (int g = 0; g < 4; ++g) ctl.poison[g] = INT32_MAX;
@@ -266,23 +285,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem, 0);
     ecq_dev::pdl_launch_dependents();  // after the allocation: the next kernel may want tensor memory too
-    ecq_dev::pdl_wait();
 
-    // the last tiles, which see the most keys, first
-    const int per_tile = a.kv_heads * a.batch;
-    const int tile = tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
-    const int b = static_cast<int>(blockIdx.x % per_tile) / a.kv_heads, head = static_cast<int>(blockIdx.x % per_tile) % a.kv_heads;
-    const Range rq = range_of(a, b);
-    if (tile == tiles - 1 && threadIdx.x == 0 && rq.rows > a.most_rows && rq.queries > 0 &&
-        (rq.rows - 1) / kCtaRows >= tiles)
-        raise_status(a.status, ECQ_STATUS_BADARG);  // more queries than the call said: their rows are not computed
-    const bool work = rq.rows > a.most_rows && tile * kCtaRows < rq.rows;
     // steps of the two tiles
     int n[2] = {0, 0};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int first = tile * kCtaRows + x * kRows, last = min(rq.rows, first + kRows) - 1;
-        if (work && first < rq.rows) n[x] = (max(rq.len - rq.queries + last / a.share + 1, 0) + kKeys - 1) / kKeys;
+        if (first < rq.rows) n[x] = (max(rq.len - rq.queries + last / a.share + 1, 0) + kKeys - 1) / kKeys;
     }
     // one for the warp, as the compiler can see: the products' operands stay in uniform registers
     n[0] = __shfl_sync(0xffffffffu, n[0], 0);
@@ -290,80 +299,88 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     const int steps = max(n[0], n[1]);
     const uint32_t base = smem_addr(smem);
 
-    if (!work) {
-        // nothing of this request: straight to the end
-    } else if (warp < kSoftmaxWarps) {
+    if (warp < kSoftmaxWarps) {
         // ---------------------------------------------------------------- softmax: two threads per row
         const int x = warp / 8, h = warp / 4 & 1, here = x * kRows + (warp & 3) * 32 + lane, row = tile * kCtaRows + x * kRows + (warp & 3) * 32 + lane;
         const bool in = row < rq.rows;
         const int i = row / a.share;
         const uint32_t mine = tmem + ((warp & 3) << 21);  // lanes 32 (warp % 4) ..
         const int limit = in ? rq.len - rq.queries + i + 1 : 0;
-        // q, in the order of a K row's decoded nibbles: of 8 channels 0 4 1 5 2 6 3 7
-        float factor;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, int parity) {
+            ok = __all_sync(0xffffffffu, wait_for(bar, parity, gave_up, a.status));
+            return ok;
+        };
+        // q: a group of D / 8 lanes takes a row (all loads at once), brings it to its power of two and writes it to shared
+        // memory in the order of a K row's decoded nibbles: of 8 channels 0 4 1 5 2 6 3 7
         {
-            const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
-                           static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head;
-            float top = 0.f;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (in) u = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 16 / kAtOnce;  // 16 rows a warp
+            const int c = lane % kLanes;
+            uint4 u[kLoads];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = cvt2(w[e], T());
-                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            for (int e = 0; e < kLoads; ++e) {
+                const int at = (warp & 7) * 16 + e * kAtOnce + lane / kLanes, qr = tile * kCtaRows + x * kRows + at;
+                u[e] = make_uint4(0, 0, 0, 0);
+                if (qr < rq.rows) {
+                    const int qi = qr / a.share;
+                    const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + qi) * a.q_token +
+                                   static_cast<int64_t>(head * a.share + qr - qi * a.share) * a.q_head;
+                    u[e] = __ldg(reinterpret_cast<const uint4*>(src) + c);
                 }
             }
-            const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
-            float up = __int_as_float((10 - ex + 127) << 23);
-            factor = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 10 + 127) << 23);
-            if (a.scale < 0.f) up = -up;
-            if (factor == 0.f) {
-                up = 0.f;
-                factor = 1.f;
+#pragma unroll
+            for (int e = 0; e < kLoads; ++e) {
+                const int at = (warp & 7) * 16 + e * kAtOnce + lane / kLanes;
+                const float2 f0 = cvt2(u[e].x, T()), f1 = cvt2(u[e].y, T()), f2 = cvt2(u[e].z, T()), f3 = cvt2(u[e].w, T());
+                float top = fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                                  fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
+                float up = __int_as_float((10 - ex + 127) << 23);
+                float f = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 10 + 127) << 23);
+                if (a.scale < 0.f) up = -up;
+                if (f == 0.f) {
+                    up = 0.f;
+                    f = 1.f;
+                }
+                if (c == 0) ctl.factor[x * kRows + at] = f;
+                sts4(base + S::kAtQ + x * S::kBytesQ + c * S::kLboQ + at * 16, pack2(f0.x * up, f2.x * up, __half()),
+                     pack2(f0.y * up, f2.y * up, __half()), pack2(f1.x * up, f3.x * up, __half()),
+                     pack2(f1.y * up, f3.y * up, __half()));
             }
+            if (x == 1) {
+                fence_proxy_async();
+                mbar_arrive(bars + offsetof(Control, q_full) + 8);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + offsetof(Control, rows) + 8 * x);
+            wait(bars + offsetof(Control, rows) + 8 * x, 0);
+        }
+        const float factor = *reinterpret_cast<volatile float*>(&ctl.factor[here]);
+        if (x == 0 && ok) {  // this thread's half of the row's channels to tensor memory
 #pragma unroll
             for (int part = 0; part < D / 64; ++part) {
                 if (part != h % (D / 64)) continue;
                 uint32_t v[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    // core column c of K holds channels 8 c ..
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (in) u = __ldg(reinterpret_cast<const uint4*>(src) + 8 * part + c);
-                    const float2 f0 = cvt2(u.x, T()), f1 = cvt2(u.y, T()), f2 = cvt2(u.z, T()), f3 = cvt2(u.w, T());
-                    v[4 * c] = pack2(f0.x * up, f2.x * up, __half());
-                    v[4 * c + 1] = pack2(f0.y * up, f2.y * up, __half());
-                    v[4 * c + 2] = pack2(f1.x * up, f3.x * up, __half());
-                    v[4 * c + 3] = pack2(f1.y * up, f3.y * up, __half());
-                    if (x == 1)
-                        sts4(base + S::kAtQ + (8 * part + c) * S::kLboQ + (here - kRows) * 16, v[4 * c], v[4 * c + 1],
-                             v[4 * c + 2], v[4 * c + 3]);
+                    const uint4 u = lds4(base + S::kAtQ + (8 * part + c) * S::kLboQ + here * 16);
+                    v[4 * c] = u.x, v[4 * c + 1] = u.y, v[4 * c + 2] = u.z, v[4 * c + 3] = u.w;
                 }
-                if (x == 0) tmem_st(mine + M::kQ + 32 * part, v);
+                tmem_st(mine + M::kQ + 32 * part, v);
             }
-            if (x == 0) {
-                wait_st();
-                before_sync();
-            } else {
-                fence_proxy_async();
-            }
-            mbar_arrive((bars + offsetof(Control, q_full) + 8 * (x)));
+            wait_st();
+            before_sync();
+            mbar_arrive(bars + offsetof(Control, q_full));
         }
         float m = kNoMax;
         uint64_t l[2] = {0ull, 0ull};  // two pairs of sums
         const uint64_t f2x = ecq_dev::pack2(__float_as_uint(factor), __float_as_uint(factor));
         const uint32_t pair = (bars + offsetof(Control, pair) + 8 * (x * 4 + (warp & 3)));
-        bool ok = true;
-        auto wait = [&](uint32_t bar, int parity) {
-            ok = __all_sync(0xffffffffu, wait_for(bar, parity, gave_up, a.status));
-            return ok;
-        };
         int j = 0;
 #pragma unroll 1
-        for (; j < n[x]; ++j) {
+        for (; ok && j < n[x]; ++j) {
             if (!wait((bars + offsetof(Control, s_full) + 8 * (x)), j & 1)) break;
             after_sync();
             uint32_t s[kHalf];
@@ -451,27 +468,37 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
         }
         if (ok) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* dst = out_row<T>(a, rq.first_q, head, in ? row : 0);
+            // this warp's 32 rows and half of the channels through its part of the tile's q (no product reads that any
+            // more), so that rows are stored together
+            constexpr int kBytesRow = D, kChunks = kBytesRow / 16;
+            const uint32_t mem = base + S::kAtQ + x * S::kBytesQ + (warp & 7) * 32 * kBytesRow;
+            auto chunk = [&](int r, int c) { return mem + r * kBytesRow + ((c ^ (r * kBytesRow / 128)) & (kChunks - 1)) * 16; };
 #pragma unroll 1
-            for (int c = h * (D / 2); c < (h + 1) * (D / 2); c += 16) {
+            for (int c = 0; c < D / 2; c += 16) {
                 uint32_t o[16];
                 if (n[x]) {
-                    tmem_ld16(mine + M::o(x) + c, o);
+                    tmem_ld16(mine + M::o(x) + h * (D / 2) + c, o);
                     wait_ld();
                 }
-                if (limit > ctl.poison[c * G / D]) {
+                if (limit > ctl.poison[(h * (D / 2) + c) * G / D]) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[e] = 0x7fc00000u;
                 }
-                if (in) {
+                uint32_t v[8];
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        float v[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = sum == 0.f ? 0.f : __uint_as_float(o[e + k]) * inv;
-                        *reinterpret_cast<uint2*>(dst + c + e) = make_uint2(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()));
-                    }
-                }
+                for (int e = 0; e < 8; ++e)
+                    v[e] = sum == 0.f ? 0u : pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv, T());
+                sts4(chunk(lane, c / 8), v[0], v[1], v[2], v[3]);
+                sts4(chunk(lane, c / 8 + 1), v[4], v[5], v[6], v[7]);
+            }
+            __syncwarp();
+            constexpr int kLanes = kBytesRow / 8, kAtOnce = 32 / kLanes;  // 8 bytes a lane
+            const int e = lane % kLanes, row0 = tile * kCtaRows + x * kRows + (warp & 3) * 32;
+#pragma unroll 4
+            for (int r = lane / kLanes; r < 32; r += kAtOnce) {
+                const uint2 v = lds2(chunk(r, e / 2) + (e & 1) * 8);
+                if (row0 + r < rq.rows)
+                    *reinterpret_cast<uint2*>(out_row<T>(a, rq.first_q, head, row0 + r) + h * (D / 2) + 4 * e) = v;
             }
         }
     } else if (warp < kMmaWarp) {
@@ -601,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
             constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
             constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
             const uint64_t k0 = kmajor(base + S::kAtK, S::kLboK, 128), v0 = kmajor(base + S::kAtV, S::kLboV, 128),
-                           q0 = kmajor(base + S::kAtQ, S::kLboQ, 128);
+                           q0 = kmajor(base + S::kAtQ + S::kBytesQ, S::kLboQ, 128);
             auto wait = [&](uint32_t bar, int parity) {
                 return __all_sync(0xffffffffu, wait_for(bar, parity, gave_up, a.status)) != 0;
             };
