@@ -34,6 +34,7 @@ import torch.distributed as dist
 from ._lib import check, lib
 from .codec import RANSTable, concat_rows, encode_matrix, split_even, choose_tile_cols
 from .device import DeviceMatrix
+from .kv4 import KV4Cache
 from .ops import rans_gemv
 
 GROUP = 128
@@ -144,19 +145,25 @@ class Llama7BDecoder:
     rank of a tensor-parallel group (tp = world size, rank = this rank)."""
 
     def __init__(self, cfg: Llama7BConfig | None = None, device=None, tp: int = 1, rank: int = 0, seed: int = 3,
-                 group=None, exchange: str = "peer", attention: str = "auto"):
+                 group=None, exchange: str = "peer", attention: str = "auto", kv_cache: str = "fp16"):
         """exchange (tp > 1): "peer" fuses each row-parallel layer's all-reduce
         into its GEMV and the next add + RMSNorm over NVLink peer memory
         (ecq_b200.comm); "nccl" runs GEMV -> NCCL all-reduce -> add + RMSNorm.
         attention: "ecq" runs libecq's split-key decode attention
         (ecq_decode_attention_f16), "sdpa" torch's scaled_dot_product_attention,
         "auto" the first for at most ECQ_ATTENTION_MAX_HEADS heads per rank
-        (where it was measured faster), the second above."""
+        (where it was measured faster), the second above.
+        kv_cache: "fp16" holds the cache as [heads, tokens, head_dim] rows for
+        these; "int4" holds it in 4 bits (ecq_b200.kv4: pages of 64 tokens, a
+        scale and a zero per 64 channels) and runs its attention."""
         self.cfg = cfg = cfg or Llama7BConfig()
         if attention not in ("ecq", "sdpa", "auto"):
             raise ValueError("attention is 'ecq', 'sdpa' or 'auto'")
         if attention == "auto":
             attention = "ecq" if cfg.heads // tp <= ECQ_ATTENTION_MAX_HEADS else "sdpa"
+        if kv_cache not in ("fp16", "int4"):
+            raise ValueError("kv_cache is 'fp16' or 'int4'")
+        self.kv_cache = kv_cache
         self.attention = attention
         self.dev = torch.device(device or "cuda")
         self.tp, self.rank, self.group = tp, rank, group
@@ -226,12 +233,28 @@ class Llama7BDecoder:
         # every layer's cache is drawn for all heads and this rank keeps its
         # heads, so every TP size decodes against the same cache
         shape = (cfg.layers, 2, self.local_heads, cfg.kv_len + 1, D)
-        self.kv = torch.empty(shape, device=self.dev, dtype=torch.float16)
+        if kv_cache == "int4":
+            self.kv = None
+            self.cache = KV4Cache(cfg.layers, -(-(cfg.kv_len + 1) // 64), self.local_heads, D, 1, cfg.kv_len + 1,
+                                  device=self.dev)
+            self.kv_new = torch.empty(2, 1, self.local_heads, D, device=self.dev, dtype=torch.float16)
+            lens = torch.full((1,), cfg.kv_len, device=self.dev, dtype=torch.int32)
+            past = self.cache.extend(lens, cfg.kv_len).slots
+            # the step's token: every step decodes it into the same slot
+            self.slot = self.cache.extend(torch.ones_like(lens), 1).slots
+        else:
+            self.cache = None
+            self.kv = torch.empty(shape, device=self.dev, dtype=torch.float16)
         h0 = rank * self.local_heads
         for li in range(cfg.layers):
             full = torch.randn((2, cfg.heads, cfg.kv_len + 1, D), generator=g, device=self.dev, dtype=torch.float16)
-            self.kv[li].copy_(full[:, h0:h0 + self.local_heads])
-            del full
+            mine = full[:, h0:h0 + self.local_heads]
+            if self.cache is not None:
+                k, v = mine[:, :, :cfg.kv_len].transpose(1, 2)
+                self.cache.append(li, k, v, past)
+            else:
+                self.kv[li].copy_(mine)
+            del full, mine
         pos = cfg.kv_len
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, device=self.dev, dtype=torch.float32) / D))
         ang = pos * inv
@@ -320,13 +343,19 @@ class Llama7BDecoder:
             else:
                 a = self._add_rms(h, d, lw["ln1"])
                 mk("add + rmsnorm")
-            kslot = self.kv[li, 0, :, cfg.kv_len]
-            vslot = self.kv[li, 1, :, cfg.kv_len]
-            # [1, 3L]: q | k | v, q and k rotated, k and v stored into the cache slot
-            qkv = lw["qkv"].m.gemv_rope_kv(a, lw["qkv"].scales, self.cos, self.sin, kslot, vslot, D,
-                                           (cfg.kv_len + 1) * D)
+            # [1, 3L]: q | k | v, q and k rotated, k and v stored into the cache slot (or on their way to it)
+            if self.cache is not None:
+                kslot, vslot, head_stride = self.kv_new[0, 0], self.kv_new[1, 0], D
+            else:
+                kslot, vslot, head_stride = self.kv[li, 0, :, cfg.kv_len], self.kv[li, 1, :, cfg.kv_len], (cfg.kv_len + 1) * D
+            qkv = lw["qkv"].m.gemv_rope_kv(a, lw["qkv"].scales, self.cos, self.sin, kslot, vslot, D, head_stride)
             mk("gemv q|k|v + rope + kv write")
-            if self.attention == "ecq":
+            if self.cache is not None:
+                self.cache.append(li, self.kv_new[0], self.kv_new[1], self.slot)
+                mk("kv write in 4 bits")
+                att = self.cache.attention(li, qkv[:, :L].view(1, nh, D))
+                mk("attention (4-bit cache)")
+            elif self.attention == "ecq":
                 att = self.att_out
                 check(lib().ecq_decode_attention_f16(qkv.data_ptr(), self.kv[li, 0].data_ptr(),
                                                      self.kv[li, 1].data_ptr(), att.data_ptr(), nh, D,
@@ -388,6 +417,8 @@ class Llama7BDecoder:
             for k in ("qkv", "o", "gate_up", "down"):
                 lw[k].m.check()
         self.lm_head.m.check()
+        if self.cache is not None:
+            self.cache.check()
         if self.xch is not None:
             self.xch.check()
 

@@ -635,3 +635,57 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for g, c in zip(got, cases):
         assert all(torch.equal(x, c[4]) for x in g)
+
+
+# -- the decoder ------------------------------------------------------------------
+
+def test_decoder_with_a_4bit_cache_matches_plain_attention_over_its_values():
+    from ecq_b200.model import Llama7BConfig, Llama7BDecoder
+
+    cfg = Llama7BConfig(layers=2, hidden=512, heads=4, head_dim=128, mlp=1024, vocab=1000, kv_len=100)
+    a = Llama7BDecoder(cfg, tp=1, seed=5, kv_cache="int4")
+    fp16 = Llama7BDecoder(cfg, tp=1, seed=5)
+    tok = torch.tensor([17], device="cuda")
+    got = a.step_logits(tok).float()
+    a.check()
+    cache, n = a.cache, cfg.kv_len + 1
+    assert cache.seq_lens.tolist() == [n]
+    pos = torch.arange(n, device="cuda")
+    slots = (cache.block_table[0, pos // 64] * 64 + pos % 64).to(torch.int32)
+    for li in range(cfg.layers):  # the rows are those of the fp16 cache, in 4 bits: half a step of the largest group
+        for half, rows in enumerate(cache.gather(li, slots)):
+            want = fp16.kv[li, half, :, :cfg.kv_len].transpose(0, 1).float()
+            step = (want.amax() - want.amin()) / 15
+            assert float((rows[:-1].float() - want).abs().max()) <= 0.5 * float(step) + 2.0 ** -8
+
+    def plain(layer, q):
+        k, v = cache.gather(layer, slots)
+        return plain_attention(q, k, v, 1).half()
+
+    cache.attention = plain
+    want = a.step_logits(tok).float()
+    assert float((got - want).abs().max() / want.abs().max()) <= 1e-2
+    assert int(torch.argmax(got)) == int(torch.argmax(want))
+
+
+def test_decoder_with_a_4bit_cache_in_a_graph():
+    from ecq_b200.model import Llama7BConfig, Llama7BDecoder
+
+    cfg = Llama7BConfig(layers=2, hidden=512, heads=4, head_dim=128, mlp=1024, vocab=1000, kv_len=64)
+    dec = Llama7BDecoder(cfg, tp=1, seed=6, kv_cache="int4")
+    tok = torch.tensor([3], device="cuda")
+    eager = dec.step(tok)
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        dec.step(tok)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            out = dec.step(tok)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    dec.check()
+    assert int(out) == int(eager)
+    with pytest.raises(ValueError):
+        Llama7BDecoder(cfg, kv_cache="int8")
