@@ -56,9 +56,10 @@ __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; 
 constexpr float kSlack = 2.f, kLift = 10.f;
 constexpr float kDrop = 10.f;  // the reference goes up by so much where weight * scale is infinite
 constexpr float kNoMax = -1e30f;
+constexpr int kMostRanks = 8;  // CTAs that share a pair
 
-__host__ __device__ constexpr int ring_slots(int dim, int groups) {
-    const int room = 74 * 1024 - kWarps * 8 * (dim + 4) * 4;
+__host__ __device__ constexpr int ring_slots(int dim, int groups, int besides) {
+    const int room = 74 * 1024 - kWarps * 8 * (dim + 4) * 4 - besides;
     const int n = room / (kWarps * kUnit * block_bytes(dim, groups));
     return n < 4 ? n : 4;
 }
@@ -132,6 +133,12 @@ __device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t addr) {
     }
 }
 
+template <typename T>
+__device__ __forceinline__ T one(float x);
+template <>
+__device__ __forceinline__ __half one<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 one<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 // V neighbouring channels
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&x)[V]) {
@@ -524,9 +531,9 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
 template <int D, int TR>
 __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
-template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a) {
-    constexpr int TR = 8 * NT, NS = ring_slots(D, G), BB = block_bytes(D, G), UB = kUnit * BB, OS = D + 4;
+template <typename T, int D, int G, int NT, bool kPairs>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a, const int tiles) {
+    constexpr int TR = 8 * NT, NS = ring_slots(D, G, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G), UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
     __shared__ long long s_before;
@@ -535,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     __shared__ uint64_t s_bar[kWarps][NS];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
     float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * UB);
+    float* s_part = s_o + kWarps * 8 * OS;  // kPairs: this CTA's part of the pair
     const int lane = threadIdx.x & 31, cta = blockIdx.x;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // the compiler sees that it is one for the warp
     if (lane < NS) ecq_dev::mbar_init(smem_addr(&s_bar[warp][lane]), 1);
@@ -542,74 +550,94 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     pdl_launch_dependents();
     pdl_wait();
 
-    // this CTA's range of the flattened units, and the request that it starts in
-    long long total = 0, mine = 0;
-    Request own = {};
-    for (int b = threadIdx.x; b < a.batch; b += kThreads) {
-        own = request<TR>(a, b);
-        mine = static_cast<long long>(own.units) * own.pairs;
-        total += mine;
-    }
-    total = block_sum(total, s_sum);
-    const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
-    if (threadIdx.x == 0) a.cuts[cta] = make_int4(-1, 0, 0, 0);
-    if (cta >= ctas) return;
-    // the first `longer` ranges have one unit more
-    const long long each = total / ctas, longer = total - each * ctas;
-    const long long f0 = each * cta + min(static_cast<long long>(cta), longer), f1 = f0 + each + (cta < longer);
-    long long before = 0;
-    for (int first = 0; first < a.batch; first += kThreads) {
-        const int b = first + threadIdx.x;
-        if (a.batch > kThreads) {  // more than one round: not the last one's any more
-            mine = 0;
-            if (b < a.batch) {
-                own = request<TR>(a, b);
-                mine = static_cast<long long>(own.units) * own.pairs;
+    // which units of which pair come first: number unit0 + mine of (request b, head, tile), then every step-th, `range` in all
+    int b, head, tile, unit0 = 0, mine = warp, step = kWarps;
+    long long range, each = 0, longer = 0;
+    Request rq;
+    if constexpr (kPairs) {
+        const int ranks = static_cast<int>(ecq_dev::cluster_size()), pair = cta / ranks;
+        b = pair / (a.kv_heads * tiles);
+        head = pair / tiles - b * a.kv_heads;
+        tile = pair % tiles;
+        rq = request<TR>(a, b);
+        // more queries than the call said: their rows are not computed
+        if (tile == tiles - 1 && rq.tiles > tiles && threadIdx.x == 0) raise_status(a.status, ECQ_STATUS_BADARG);
+        if (tile >= rq.tiles) return;  // the whole cluster
+        mine += static_cast<int>(ecq_dev::cluster_rank()) * kWarps;
+        step *= ranks;
+        range = rq.units;
+    } else {
+        // this CTA's range of the flattened units, and the request that it starts in
+        long long total = 0, weight = 0;
+        Request own = {};
+        for (int r = threadIdx.x; r < a.batch; r += kThreads) {
+            own = request<TR>(a, r);
+            weight = static_cast<long long>(own.units) * own.pairs;
+            total += weight;
+        }
+        total = block_sum(total, s_sum);
+        const long long ctas = min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps);
+        if (threadIdx.x == 0) a.cuts[cta] = make_int4(-1, 0, 0, 0);
+        if (cta >= ctas) return;
+        // the first `longer` ranges have one unit more
+        each = total / ctas;
+        longer = total - each * ctas;
+        const long long f0 = each * cta + min(static_cast<long long>(cta), longer);
+        range = each + (cta < longer);
+        long long before = 0;
+        for (int first = 0; first < a.batch; first += kThreads) {
+            const int r = first + threadIdx.x;
+            if (a.batch > kThreads) {  // more than one round: not the last one's any more
+                weight = 0;
+                if (r < a.batch) {
+                    own = request<TR>(a, r);
+                    weight = static_cast<long long>(own.units) * own.pairs;
+                }
             }
-        }
-        long long incl = mine;
+            long long incl = weight;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-        }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = incl;
-        if (threadIdx.x == 0) s_request = -1;
-        __syncthreads();
-        long long start = before + incl - mine;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = incl;
+            if (threadIdx.x == 0) s_request = -1;
+            __syncthreads();
+            long long start = before + incl - weight;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) start += s_sum[w];
-            before += s_sum[w];
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) start += s_sum[w];
+                before += s_sum[w];
+            }
+            if (weight && start <= f0 && f0 < start + weight) {
+                s_request = r;
+                s_before = start;
+                s_own = own;
+            }
+            __syncthreads();
+            if (s_request >= 0) break;
         }
-        if (mine && start <= f0 && f0 < start + mine) {
-            s_request = b;
-            s_before = start;
-            s_own = own;
-        }
-        __syncthreads();
-        if (s_request >= 0) break;
-    }
-    if (s_request < 0) return;  // lengths that change meanwhile: no range, but no endless search either
-
-    // where this warp fetches next; the same in all its lanes
-    const int shift = a.page_shift - 4;  // blocks per page
-    const int page_bytes = BB << shift;
-    const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
-    int b = s_request, head, tile, unit0;
-    Request rq = s_own;
-    {
+        if (s_request < 0) return;  // lengths that change meanwhile: no range, but no endless search either
+        b = s_request;
+        rq = s_own;
         const long long at = f0 - s_before;
         const int pair = static_cast<int>(at / rq.units);
         unit0 = static_cast<int>(at - static_cast<long long>(pair) * rq.units);
         head = pair / rq.tiles;
         tile = pair - head * rq.tiles;
     }
+
+    // where this warp fetches next; the same in all its lanes
+    const int shift = a.page_shift - 4;  // blocks per page
+    const int page_bytes = BB << shift;
+    const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
+    const Request rq0 = rq;
+    const int head0 = head, tile0 = tile;
     uint4 raw[NT][D / 32];
     load_rows<T, D, NT>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
-    int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + warp, f_page[kUnit];
-    int f_left = f1 - f0 > warp ? static_cast<int>((f1 - f0 - warp + kWarps - 1) / kWarps) : 0;
+    int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + mine, f_page[kUnit];
+    int f_left = range > mine ? static_cast<int>((range - mine + step - 1) / step) : 0;
     Request fr = rq;
     const int32_t* f_row = a.table + fb * a.table_stride;
     const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
@@ -674,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         }
         f_slot = f_slot + 1 == NS ? 0 : f_slot + 1;
         --f_left;
-        f_unit += kWarps;
+        f_unit += step;
         look();
     };
     __syncwarp();
@@ -690,12 +718,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     State<D, G, NT> st;
     const Lane<D, G> me;
 #pragma unroll 1
-    for (long long f = f0; f < f1;) {
-        const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), f1 - f));
+    for (long long f = 0; f < range;) {
+        const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), range - f));
         set_rows<T, D, G, NT>(rows, raw, a, rq, tile);
         st.reset();
         // this warp's first unit in [f, f + n)
-        int i = (warp - static_cast<int>((f - f0) % kWarps) + kWarps) % kWarps;
+        int i = kPairs ? mine : (warp - static_cast<int>(f % kWarps) + kWarps) % kWarps;
         auto wait = [&]() {
             if (late || __any_sync(0xffffffffu, !ecq_dev::mbar_wait(bars + 8 * slot, phase))) {
                 if (!late && lane == 0) raise_status(a.status, ECQ_STATUS_TIMEOUT);
@@ -711,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 slot = 0;
                 phase ^= 1;
             }
-            i += kWarps;
+            i += step;
             fetch();
         };
         // units that every row sees, then (or between, where a page number is bad) those with a mask
@@ -743,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             tile = 0;
             if (++head == a.kv_heads) head = 0;
         }
-        if (f < f1) {
+        if (!kPairs && f < range) {
             if (head == 0 && tile == 0) {
                 do {
                     if (++b >= a.batch) break;
@@ -751,11 +779,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 } while (rq.units == 0);
                 if (b >= a.batch) late = true;
             }
-            if (late) f = f1;
+            if (late) f = range;
             else load_rows<T, D, NT>(raw, a, rq, head, tile);
         }
-        float* part = a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
-        if (starts && !ends && threadIdx.x == 0) {
+        float* part = kPairs ? s_part : a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
+        if (!kPairs && starts && !ends && threadIdx.x == 0) {
             // how many of the ranges that follow it takes to the pair's end
             const long long k = max(longer - cta - 1, 0ll);
             const long long more = rest <= k * (each + 1) ? (rest + each) / (each + 1) : k + (rest - k * (each + 1) + each - 1) / each;
@@ -798,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 }
                 const int tr = nt * 8 + row, qr = tile_now * TR + tr;
                 if (qr >= now.rows) continue;
-                if (starts && ends) {
+                if (!kPairs && starts && ends) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) o[v] = L == 0.f ? 0.f : o[v] / L;
                     store<T, V>(out_row<T>(a, now.first_q, head_now, qr) + V * lane, o);
@@ -813,6 +841,47 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             }
             __syncthreads();
         }
+    }
+    if constexpr (kPairs) {
+        // the cluster's parts: rank r joins rows r, r + ranks, ...
+        constexpr int V = D / 32;
+        const int ranks = static_cast<int>(ecq_dev::cluster_size()), rank = static_cast<int>(ecq_dev::cluster_rank());
+        ecq_dev::cluster_sync();
+#pragma unroll 1
+        for (int tr = rank + warp * ranks; tr < TR; tr += ranks * kWarps) {
+            const int qr = tile0 * TR + tr;
+            if (qr >= rq0.rows) break;
+            float M[kMostRanks], L[kMostRanks], x[kMostRanks][V];
+#pragma unroll
+            for (int k = 0; k < kMostRanks; ++k) {
+                M[k] = kNoMax;
+                L[k] = 0.f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[k][v] = 0.f;
+                if (k < ranks) {
+                    M[k] = ecq_dev::ld_cluster_f32(s_part + 2 * tr, k);
+                    L[k] = ecq_dev::ld_cluster_f32(s_part + 2 * tr + 1, k);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[k][v] = ecq_dev::ld_cluster_f32(s_part + 2 * TR + tr * D + 32 * v + lane, k);
+                }
+            }
+            float top = kNoMax, sum = 0.f, val[V];
+#pragma unroll
+            for (int k = 0; k < kMostRanks; ++k) top = fmaxf(top, M[k]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) val[v] = 0.f;
+#pragma unroll
+            for (int k = 0; k < kMostRanks; ++k) {
+                const float w = exp2_fast(M[k] - top);
+                sum = fmaf(w, L[k], sum);
+#pragma unroll
+                for (int v = 0; v < V; ++v) val[v] = fmaf(w, x[k][v], val[v]);
+            }
+            T* dst = out_row<T>(a, rq0.first_q, head0, qr) + lane;
+#pragma unroll
+            for (int v = 0; v < V; ++v) dst[32 * v] = one<T>(sum == 0.f ? 0.f : val[v] / sum);
+        }
+        ecq_dev::cluster_sync();  // no CTA leaves while another reads its part
     }
     if (late) {
         // let the copies in flight land before the shared memory is given back (a slot without one waits in vain)
@@ -918,14 +987,40 @@ constexpr int kStreamRows = 64;
 // keys for twice the rows.
 int row_tiles_of_8(int share, int max_q) { return static_cast<int64_t>(share) * max_q > 8 ? 2 : 1; }
 
+// CTAs of a cluster for each (request, head, tile); 0: ranges instead. Ranges
+// balance lengths that differ and spread a few long requests over the GPU, at
+// the price of a look at all lengths, and of a second kernel that joins what
+// was cut. Clusters have neither, and are taken where that counts: all of them
+// fit on the GPU at once, and the longest request that the tables have room for
+// is a few rounds of its cluster's warps (7b step, 32 pairs of up to 66 units:
+// 14.4 us with ranges, 10.0 with clusters).
+constexpr int kMostRounds = 6;
+int cluster_ranks(const Args& a, int nt, int tiles) {
+    const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads * tiles;
+    const int64_t units = (static_cast<int64_t>(a.max_pages) << a.page_shift) / kUnitTokens + 1;
+    for (int ranks = kMostRanks; ranks >= 1; ranks /= 2)
+        if (pairs * ranks <= grid_ctas(nt)) return units <= static_cast<int64_t>(kMostRounds) * ranks * kWarps ? ranks : 0;
+    return 0;
+}
+
 template <typename L, int NT>
-int32_t launch(const Args& a, cudaStream_t stream) {
+int32_t launch(const Args& a, int max_q, cudaStream_t stream) {
     using T = typename L::T;
-    constexpr int smem = kWarps * ring_slots(L::D, L::G) * kUnit * block_bytes(L::D, L::G) + kWarps * 8 * (L::D + 4) * 4;
-    const auto kernel = attention_kernel<T, L::D, L::G, NT>;
+    constexpr int UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = 8 * NT * (L::D + 4) * 4;
+    const int64_t most = static_cast<int64_t>(a.share) * max_q;
+    const int tiles = static_cast<int>(((most < a.most_rows ? most : a.most_rows) + 8 * NT - 1) / (8 * NT));
+    if (const int ranks = cluster_ranks(a, NT, tiles)) {
+        constexpr int smem = kWarps * ring_slots(L::D, L::G, part) * UB + join + part;
+        const auto kernel = attention_kernel<T, L::D, L::G, NT, true>;
+        if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
+        const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * tiles * ranks);
+        return result(ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, ranks, a, tiles));
+    }
+    constexpr int smem = kWarps * ring_slots(L::D, L::G, 0) * UB + join;
+    const auto kernel = attention_kernel<T, L::D, L::G, NT, false>;
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
     const dim3 grid(grid_ctas(NT));
-    cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a);
+    cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a, 0);
     if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, NT>, grid, dim3(kJoinWarps * 32), 0, stream, a);
     return result(rc);
 }
@@ -995,7 +1090,8 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     const int nt = row_tiles_of_8(a.share, max_q);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
-        return nt == 2 ? launch<L, 2>(a, static_cast<cudaStream_t>(stream)) : launch<L, 1>(a, static_cast<cudaStream_t>(stream));
+        return nt == 2 ? launch<L, 2>(a, max_q, static_cast<cudaStream_t>(stream))
+                       : launch<L, 1>(a, max_q, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -409,6 +409,28 @@ def test_attention_of_long_contexts():
     attend_case([4099, 17, 9000], [2, 1, 4], 1, 8, 64, 64, 128, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,g", LAYOUTS)
+@pytest.mark.parametrize("lens,new,share", [([1, 300, 0, 77], [1, 1, 1, 1], 4), ([500, 33, 640], [4, 1, 3], 5), ([2000], [1], 1)])
+def test_attention_with_room_for_long_requests(dtype, dim, g, lens, new, share):
+    # tables with room for far more than the requests have: the work is cut into ranges, and cut pairs are joined
+    q, pages, table, starts, got = attend_case(lens, new, 3, share, dim, g, 16, dtype, seed=sum(lens))
+    wide = torch.full((len(lens), 20000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    again = ecq.kv4_attention(q, pages, wide, i32(lens), i32(starts), max(new), group_size=g)
+    want, s_abs, v_abs = reference(q, pages, table, lens, starts, 16, dim, g)
+    check_attention(again, want, s_abs, v_abs, dtype)
+    for _ in range(2):
+        assert torch.equal(again, ecq.kv4_attention(q, pages, wide, i32(lens), i32(starts), max(new), group_size=g))
+
+
+def test_attention_of_many_requests():
+    # more than the threads of a CTA look at in one round
+    rng = random.Random(3)
+    lens = [rng.choice([0, 1, 15, 16, 17, 40]) for _ in range(300)]
+    attend_case(lens, [1] * 300, 2, 2, 64, 32, 16, torch.float16)
+
+
 def test_attention_with_peaked_and_flat_scores():
     attend_case([1000], [1], 2, 4, 128, 64, 16, torch.float16, q_scale=30.0)      # one key takes all
     attend_case([1000], [1], 2, 4, 128, 64, 16, torch.float16, q_scale=0.0)       # the mean of all values
