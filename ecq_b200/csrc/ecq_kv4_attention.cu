@@ -13,8 +13,10 @@
 // with query rows (tokens x heads that share a cache head) as the narrow side:
 // mma.sync m16n8k16 holds 8 rows of keys' work at full use, where a tcgen05
 // tile would be 64 or 128 rows, of which a decode step has 1 to 8.
-// p s is fp16 twice (value and remainder: 22 bits), so V's side keeps fp32
-// accuracy; q is scaled to its row's largest power of two and exact in fp16.
+// For fp16 outputs p and p s are fp16 twice (value and remainder: 22 bits), so
+// V's side keeps fp32 accuracy. For bf16 they are fp16 once: 2^-12 of each
+// weight beside the output's 2^-9, for 30 instructions fewer of 330. q is
+// scaled to its row's largest power of two and exact in fp16.
 //
 // What bounds it: the cache's bytes for long contexts; below that the ~250
 // instructions per 16 tokens and head, and for short ones launches and merges.
@@ -29,6 +31,8 @@
 // parts go to the workspace and a second kernel joins them in order, so results
 // do not depend on timing.
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "ecq_kv4_attention.cuh"
 
@@ -317,7 +321,7 @@ __device__ __forceinline__ uint32_t neg2(uint32_t a) {
 
 // A unit's blocks at shared address at; first[u]: the request's token that
 // block u starts with (used with kMask; beyond all limits: leave it out).
-template <int D, int G, int NT, bool kMask>
+template <int D, int G, int NT, bool kMask, bool kExact>
 __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
                                        const int (&first)[kUnit]) {
     constexpr int U = kUnit, W = D / 32, BB = block_bytes(D, G);
@@ -411,7 +415,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                     const uint32_t x = h2(p[0], p[1]);
                     const float2 back = f2(x);
                     ph[u][nt][i] = transpose(x);
-                    pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
+                    if (kExact) pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
                 }
             uint32_t sa[2][G], sb[2][G];
             lds<G, 0>(sa[0], at + u * BB + me.v_params);
@@ -428,7 +432,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                         // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
                         const uint32_t w = ph[u][nt][i];
                         uint32_t h = mul2(w, sc);
-                        uint32_t l = fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h)));
+                        uint32_t l = kExact ? fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h))) : 0u;
                         if (kMask) {  // weight 0: 0, whatever the scale is
                             const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
                             h &= keep;
@@ -463,7 +467,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                 for (int nt = 0; nt < NT; ++nt) {
                     if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
                     else mma(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
-                    mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
+                    if (kExact) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
                 }
             }
 #pragma unroll
@@ -507,7 +511,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             for (int u = 0; u < U; ++u) {
                 const uint32_t x = __byte_perm(v[u][0][w], v[u][1][w], pick), y = __byte_perm(v[u][2][w], v[u][3][w], pick);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                for (int part = 0; part < (kExact ? 2 : 1); ++part)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int g = (4 * w + 2 * half + j) * 16 * G / D;
@@ -533,6 +537,7 @@ __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
 template <typename T, int D, int G, int NT, bool kPairs>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a, const int tiles) {
+    constexpr bool kExact = std::is_same<T, __half>::value;
     constexpr int TR = 8 * NT, NS = ring_slots(D, G, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G), UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
@@ -750,14 +755,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 #pragma unroll 1
             while (i < min(n, seen) && !(f_bad >> 2 * slot & 3u)) {
                 if (!wait()) break;
-                blocks<D, G, NT, false>(st, rows, me, ring + slot * UB, first);
+                blocks<D, G, NT, false, kExact>(st, rows, me, ring + slot * UB, first);
                 done();
             }
             if (i >= n || !wait()) break;
 #pragma unroll
             for (int u = 0; u < kUnit; ++u)
                 first[u] = f_bad >> (2 * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
-            blocks<D, G, NT, true>(st, rows, me, ring + slot * UB, first);
+            blocks<D, G, NT, true, kExact>(st, rows, me, ring + slot * UB, first);
             done();
         }
         // the next segment's rows are on their way while the warps join

@@ -290,8 +290,10 @@ def check_attention(got, want, s_abs, v_abs, dtype, rounded=False):
     weight, and of the sum: 2 e of the largest |v|. Weights (2^-20: two fp16 parts,
     exp2) and their fp32 sums add 2^-16 of it. Then one rounding to the type.
     ``rounded``: the prompt kernel's K, V and weights are fp16, 2^-11 of each: 2^-11
-    of sum |q||k| in a score, and 2^-11 of the largest |v| twice."""
-    k, v = (2.0 ** -11, 2 * 2.0 ** -11) if rounded else (0.0, 0.0)
+    of sum |q||k| in a score, and 2^-11 of the largest |v| twice. For bf16 the other
+    kernel's weights, and weights times scale, are fp16: 2^-11 each, of codes times
+    scales (at most twice the largest |v|, as are the zeros)."""
+    k, v = (2.0 ** -11, 2 * 2.0 ** -11) if rounded else (0.0, 4 * 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
     tol = (torch.finfo(dtype).eps / 2) * want.abs() + (2 * (2.0 ** -16 + k) * s_abs + 2 * 2.0 ** -16 + v) * v_abs + 2.0 ** -24
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
