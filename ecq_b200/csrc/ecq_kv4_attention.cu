@@ -985,12 +985,23 @@ int grid_ctas(int nt) { return ctas_per_sm(nt) * ecq_dev::sm_count_cached(); }
 
 // Requests with up to so many rows (queries times heads that share a cache
 // head) are streamed by attention_kernel, those with more are the prompt
-// kernel's; a call that may have such launches both.
-constexpr int kStreamRows = 64;
+// kernel's; a call that may have such launches both. A row costs the stream
+// kernel the same wherever it is, the prompt kernel works by 256 rows of a pair
+// on one SM: many pairs fill the GPU with those, few do not. Measured (us,
+// stream / prompt kernel, shared by 4): 128 pairs of 4096 tokens 32 rows
+// 77 / 85, 48 rows 108 / 86; 32 pairs of 8192 96 rows 103 / 146; 8 pairs of
+// 65536 256 rows 456 / 1139: they meet at about 4500 rows of all pairs.
+int stream_rows(int batch, int kv_heads) {
+    const int64_t rows = 4500 / (static_cast<int64_t>(batch) * kv_heads);
+    return rows > 32 ? static_cast<int>(rows) : 32;
+}
 
-// 16-row tiles where a request may have more than 8 rows: one pass over the
-// keys for twice the rows.
-int row_tiles_of_8(int share, int max_q) { return static_cast<int64_t>(share) * max_q > 8 ? 2 : 1; }
+// 16-row tiles (one pass over the keys for twice the rows, at two thirds of the
+// warps) where 8-row tiles would be even in number: 128 pairs of 4096 tokens,
+// 16 rows 49 against 54 us, 32 rows 77 against 89, but 24 rows 77 against 71.
+int row_tiles_of_8(int share, int max_q) {
+    return (static_cast<int64_t>(share) * max_q + 7) / 8 % 2 == 0 ? 2 : 1;
+}
 
 // CTAs of a cluster for each (request, head, tile); 0: ranges instead. Ranges
 // balance lengths that differ and spread a few long requests over the GPU, at
@@ -1086,8 +1097,9 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     a.batch = batch;
     a.total_q = total_q;
     a.scale = scale;
-    const bool prompts = static_cast<int64_t>(a.share) * max_q > kStreamRows;
-    a.most_rows = prompts ? kStreamRows : INT32_MAX;
+    const int most = stream_rows(batch, kv_heads);
+    const bool prompts = static_cast<int64_t>(a.share) * max_q > most;
+    a.most_rows = prompts ? most : INT32_MAX;
     if (prompts) {
         const int32_t rc = launch_prompt(a, dtype, head_dim, head_dim / group_size, max_q, static_cast<cudaStream_t>(stream));
         if (rc != ECQ_OK) return rc;

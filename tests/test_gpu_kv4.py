@@ -299,7 +299,10 @@ def check_attention(got, want, s_abs, v_abs, dtype, rounded=False):
     assert bool((err <= tol).all()), float((err / tol).max())
 
 
-STREAM_ROWS = 64  # requests with more rows (queries times heads that share a cache head) go to the prompt kernel
+def stream_rows(batch, heads):
+    """Requests with more rows (queries times heads that share a cache head) go to
+    the prompt kernel."""
+    return max(32, 4500 // (batch * heads))
 
 
 def attend_case(lens, new, heads, share, dim, g, page, dtype, seed=1, q_scale=1.0, **kw):
@@ -317,7 +320,7 @@ def attend_case(lens, new, heads, share, dim, g, page, dtype, seed=1, q_scale=1.
     want, s_abs, v_abs = reference(q, pages, table, lens, starts, page, dim, g, kw.get("scale"))
     for b, n in enumerate(new):
         at = slice(starts[b], starts[b + 1])
-        check_attention(got[at], want[at], s_abs[at], v_abs[at], dtype, n * share > STREAM_ROWS)
+        check_attention(got[at], want[at], s_abs[at], v_abs[at], dtype, n * share > stream_rows(len(lens), heads))
     return q, pages, table, starts, got
 
 
@@ -345,47 +348,48 @@ def test_attention_of_several_tokens_is_causal(dtype, dim, g, lens, new):
 @pytest.mark.parametrize("dim,g", LAYOUTS)
 @pytest.mark.parametrize("lens,new,page", [([65], [65], 16), ([64, 200], [64, 129], 16), ([300, 5, 64], [257, 1, 64], 64)])
 def test_attention_of_prompts(dtype, dim, g, lens, new, page):
-    attend_case(lens, new, 2, 2, dim, g, page, dtype, seed=sum(new))
+    attend_case(lens, new, 64, 2, dim, g, page, dtype, seed=sum(new))  # 64 heads: the prompt kernel from 32 rows on
 
 
 @pytest.mark.parametrize("share,new,lens", [
     (1, [65, 128, 129, 600], [65, 1000, 129, 700]), (4, [17, 32, 33, 64, 65, 1, 0], [17, 500, 33, 64, 129, 77, 30]),
     (8, [130], [1500]), (7, [40, 9, 10], [41, 400, 10]), (64, [2, 1, 5], [100, 64, 5]), (3, [300], [300])])
 def test_attention_of_prompts_head_layouts(share, new, lens):
-    attend_case(lens, new, 2, share, 128, 64, 32, torch.float16, seed=share)
-    attend_case(lens, new, 1, share, 64, 32, 128, torch.bfloat16, seed=share + 1, scale=-0.2)
+    attend_case(lens, new, 48, share, 128, 64, 32, torch.float16, seed=share)
+    attend_case(lens, new, 80, share, 64, 32, 128, torch.bfloat16, seed=share + 1, scale=-0.2)
 
 
 def test_attention_of_prompts_longer_than_the_request_and_scales():
     # more queries than tokens: the first ones see nothing
     lens, new = [50, 0], [70, 80]
-    pages, table = fill(lens, 1, 64, 32, 16, 3)
-    q = torch.randn(150, 2, 64, device="cuda").half()
+    pages, table = fill(lens, 64, 64, 32, 16, 3)
+    q = torch.randn(150, 128, 64, device="cuda").half()
     got = ecq.kv4_attention(q, pages, table, i32(lens), i32([0, 70, 150]), 80, group_size=32)
     want, s_abs, v_abs = reference(q, pages, table, lens, [0, 70, 150], 16, 64, 32)
     check_attention(got, want, s_abs, v_abs, torch.float16, True)
     assert not bool(got[:20].any()) and not bool(got[70:].any()) and bool(got[20:70].any())
     for kw in (dict(scale=0.0), dict(q_scale=30.0), dict(q_scale=1e-6, scale=3e5)):
-        attend_case([400], [150], 1, 2, 128, 64, 64, torch.bfloat16, **kw)
+        attend_case([400], [150], 128, 2, 128, 64, 64, torch.bfloat16, **kw)
 
 
 def test_tokens_that_are_not_numbers_reach_only_rows_that_see_them():
     # a row of NaN at position 45 of a 70-token prompt: earlier queries are as without it
     for n, share in ((70, 2), (9, 2), (1, 1)):
-        x = torch.randn(2, 70, 1, 64, device="cuda").half()
-        pages, clean = ecq.kv4_pages(5, 1, 64, 16, 32), ecq.kv4_pages(5, 1, 64, 16, 32)
+        x = torch.randn(2, 70, 128, 64, device="cuda").half()
+        pages, clean = ecq.kv4_pages(5, 128, 64, 16, 32), ecq.kv4_pages(5, 128, 64, 16, 32)
         slots, table = torch.arange(70, dtype=torch.int32, device="cuda"), torch.arange(5, dtype=torch.int32, device="cuda")[None]
-        q = torch.randn(n, share, 64, device="cuda").half()
+        q = torch.randn(n, 128 * share, 64, device="cuda").half()
         ecq.kv4_append(x[0], x[1], clean, slots, group_size=32)
         for which in (0, 1):
             y = x.clone()
-            y[which, 66, 0, 3] = float("nan")
+            y[which, 66, 0, 3] = float("nan")  # in one of the heads
             ecq.kv4_append(y[0], y[1], pages, slots, group_size=32)
             starts = i32([0, n])
             got, want = (ecq.kv4_attention(q, p, table, i32([70]), starts, n, group_size=32) for p in (pages, clean))
             first = max(0, 66 - (70 - n))  # the first query that sees token 66
             assert torch.equal(got[:first], want[:first])
-            seen = got[first:]
+            assert torch.equal(got[:, share:], want[:, share:])
+            seen, want = got[first:, :share], want[:, :share]
             if which == 0:
                 assert bool(seen.isnan().all())
             else:  # the value's group of channels
@@ -394,7 +398,7 @@ def test_tokens_that_are_not_numbers_reach_only_rows_that_see_them():
 
 def test_prompts_with_bad_pages_leave_their_keys_out():
     lens, new, dim, g, page = [200, 130], [100, 100], 64, 32, 16
-    q, pages, table, starts, want = attend_case(lens, new, 1, 2, dim, g, page, torch.float16)
+    q, pages, table, starts, want = attend_case(lens, new, 100, 2, dim, g, page, torch.float16)
     bad, status = table.clone(), i32([0])
     bad[1, 8] = 2 ** 31 - 1  # tokens 128 and 129 of request 1: its last two queries lose them
     got = ecq.kv4_attention(q, pages, bad, i32(lens), i32(starts), 100, group_size=g, status=status)
