@@ -168,8 +168,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
             int slot = -1, pos = -1;
             if (i < total) {
                 if (i >= next) {  // the first token, or the next request that has any
-                    if (next >= 0) do ++b;
-                        while ((b + 1 < batch ? s_tok[b + 1] : total) <= i);
+                    while ((b + 1 < batch ? s_tok[b + 1] : total) <= i) ++b;
                     next = b + 1 < batch ? s_tok[b + 1] : total;
                     held = (s_len[b] + page_size - 1) >> page_shift;
                     have = -1;

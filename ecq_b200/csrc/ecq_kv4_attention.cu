@@ -401,7 +401,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
         }
     }
     uint32_t hi[U][NT][G][2], lo[U][NT][G][2];
-    for (;;) {
+    for (int drops = 0;; ++drops) {
         uint32_t ph[U][NT][2], pl[U][NT][2], most = 0u;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -444,7 +444,8 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                     }
                 }
         }
-        if (!__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
+        // two drops bring any finite scale's product below fp16's end; a scale that is infinite stays so
+        if (drops == 2 || !__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
             // rows of A: the groups' zeros, then ones (the sum of the weights)
             float sums[NT][4];
 #pragma unroll

@@ -226,7 +226,7 @@ __device__ __forceinline__ uint32_t value_high(uint32_t x, uint32_t scale, uint3
 }
 
 template <typename T, int D, int G>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const int tiles) {
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     using S = Smem<D, G>;
     using M = Tmem;
     constexpr int BB = block_bytes(D, G);
@@ -238,15 +238,45 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
     volatile uint32_t* gave_up = &ctl.gave_up;
 
     ecq_dev::pdl_wait();
-    // the last tiles, which see the most keys, first
-    const int per_tile = a.kv_heads * a.batch;
-    const int tile = tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
-    const int b = static_cast<int>(blockIdx.x % per_tile) / a.kv_heads, head = static_cast<int>(blockIdx.x % per_tile) % a.kv_heads;
-    const Range rq = range_of(a, b);
-    if (tile == tiles - 1 && threadIdx.x == 0 && rq.rows > a.most_rows && rq.queries > 0 &&
-        (rq.rows - 1) / kCtaRows >= tiles)
-        raise_status(a.status, ECQ_STATUS_BADARG);  // more queries than the call said: their rows are not computed
-    const bool work = rq.rows > a.most_rows && tile * kCtaRows < rq.rows;
+    // this CTA's request and tile: every request has as many tiles as its rows fill, and the grid is as large as all rows
+    // together may need. Last tiles, which see the most keys, come first.
+    const int head = blockIdx.x % a.kv_heads;
+    const int items = gridDim.x / a.kv_heads, item = items - 1 - static_cast<int>(blockIdx.x / a.kv_heads);
+    __shared__ int s_sum[kThreads / 32], s_request, s_tile;
+    if (threadIdx.x == 0) s_request = -1;
+    int before = 0;
+    for (int first = 0; first < a.batch && (before <= item || blockIdx.x == 0); first += kThreads) {
+        const int r = first + threadIdx.x;
+        int mine = 0;
+        if (r < a.batch) {
+            const int rows = range_of(a, r).rows;
+            if (rows > a.most_rows) mine = (rows + kCtaRows - 1) / kCtaRows;
+        }
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int start = before + incl - mine;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) start += s_sum[w];
+            before += s_sum[w];
+        }
+        if (start <= item && item < start + mine) {
+            s_request = r;
+            s_tile = item - start;
+        }
+    }
+    __syncthreads();
+    // more queries than the call said: some rows are not computed
+    if (blockIdx.x == 0 && threadIdx.x == 0 && before > items) raise_status(a.status, ECQ_STATUS_BADARG);
+    const int b = s_request, tile = s_tile;
+    const bool work = b >= 0;
+    const Range rq = range_of(a, max(b, 0));
     if (!work) {
         ecq_dev::pdl_launch_dependents();
         return;
@@ -729,8 +759,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a, const
 namespace ecq_kv4 {
 
 int32_t launch_prompt(const Args& a, int dtype, int head_dim, int groups, int max_q, cudaStream_t stream) {
-    const int64_t tiles = (static_cast<int64_t>(a.share) * max_q + kCtaRows - 1) / kCtaRows;
-    const int64_t ctas = tiles * a.kv_heads * a.batch;
+    // tiles of a request: its rows / 256, rounded up; of all requests at most so many
+    const int64_t each = (static_cast<int64_t>(a.share) * max_q + kCtaRows - 1) / kCtaRows * a.batch;
+    const int64_t all = static_cast<int64_t>(a.share) * a.total_q / kCtaRows + a.batch;
+    const int64_t ctas = (each < all ? each : all) * a.kv_heads;
     if (ctas > INT32_MAX) return ECQ_ERR_UNSUPPORTED;
     return by_layout(dtype, head_dim, groups, [&](auto layout) {
         using L = decltype(layout);
@@ -738,8 +770,7 @@ int32_t launch_prompt(const Args& a, int dtype, int head_dim, int groups, int ma
         // more than half of the shared memory, whatever is used: one CTA per SM, as tensor memory has room for one
         const int smem = Smem<L::D, L::G>::kBytes > 120 * 1024 ? Smem<L::D, L::G>::kBytes : 120 * 1024;
         if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
-        return result(ecq_dev::launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, a,
-                                          static_cast<int>(tiles)));
+        return result(ecq_dev::launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, a));
     });
 }
 

@@ -396,6 +396,27 @@ def test_tokens_that_are_not_numbers_reach_only_rows_that_see_them():
                 assert bool(seen[..., :32].isnan().all()) and torch.equal(seen[..., 32:], want[first:, :, 32:])
 
 
+def test_a_scale_that_is_infinite_ends_and_stays_with_the_rows_that_see_it():
+    # bytes that kv4_append never writes: token 40's V scales are infinite
+    for lens, new, heads in (([100, 60], [1, 1], 2), ([100, 60], [60, 50], 64)):
+        q, pages, table, starts, want = attend_case(lens, new, heads, 2, 64, 32, 16, torch.float16)
+        broken, at = pages.clone(), int(table[0, 2]) * 16 + 8
+        par = broken.view(-1, heads, 16 * 64 + 256)[at // 16, :, 16 * 64 + 128:].view(torch.float16).view(heads, 16, 2, 2)
+        par[:, at % 16, :, 0] = float("inf")
+        got = ecq.kv4_attention(q, broken, table, i32(lens), None if new[0] == 1 else i32(starts), max(new), group_size=32)
+        first = max(0, 40 - (100 - new[0]))  # the first query of request 0 that sees token 40
+        assert torch.equal(got[:first], want[:first]) and torch.equal(got[starts[1]:], want[starts[1]:])
+        assert not bool(got[first:starts[1]].isfinite().any())
+
+
+def test_more_queries_than_max_q_are_reported():
+    for new, heads, said in ((9, 2, 1), (200, 64, 40)):
+        pages, table = fill([300], heads, 64, 32, 16, 3)
+        q, status = torch.randn(new, 2 * heads, 64, device="cuda").half(), i32([0])
+        ecq.kv4_attention(q, pages, table, i32([300]), i32([0, new]), said, group_size=32, status=status)
+        assert status.item() == BADARG
+
+
 def test_prompts_with_bad_pages_leave_their_keys_out():
     lens, new, dim, g, page = [200, 130], [100, 100], 64, 32, 16
     q, pages, table, starts, want = attend_case(lens, new, 100, 2, dim, g, page, torch.float16)
