@@ -1012,26 +1012,40 @@ int row_tiles_of_8(int share, int max_q) {
 // is a few rounds of its cluster's warps (7b step, 32 pairs of up to 66 units:
 // 14.4 us with ranges, 10.0 with clusters).
 constexpr int kMostRounds = 6;
-int cluster_ranks(const Args& a, int nt, int tiles) {
-    const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads * tiles;
-    const int64_t units = (static_cast<int64_t>(a.max_pages) << a.page_shift) / kUnitTokens + 1;
-    for (int ranks = kMostRanks; ranks >= 1; ranks /= 2)
-        if (pairs * ranks <= grid_ctas(nt)) return units <= static_cast<int64_t>(kMostRounds) * ranks * kWarps ? ranks : 0;
-    return 0;
+struct Plan {
+    int most_rows;  // of a request that is streamed
+    bool prompts;   // some may have more
+    int nt;         // 8-row tiles as one
+    int tiles;      // of a streamed request at most
+    int ranks;      // CTAs of a cluster; 0: ranges
+};
+Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page_size) {
+    Plan p;
+    const int64_t rows = static_cast<int64_t>(share) * max_q;
+    p.most_rows = stream_rows(batch, kv_heads);
+    p.prompts = rows > p.most_rows;
+    if (!p.prompts) p.most_rows = INT32_MAX;
+    p.nt = row_tiles_of_8(share, max_q);
+    p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.tiles;
+    const int64_t units = static_cast<int64_t>(max_pages) * page_size / kUnitTokens + 1;
+    p.ranks = kMostRanks;
+    while (p.ranks && pairs * p.ranks > grid_ctas(p.nt)) p.ranks /= 2;
+    if (units > static_cast<int64_t>(kMostRounds) * p.ranks * kWarps) p.ranks = 0;
+    return p;
 }
 
 template <typename L, int NT>
-int32_t launch(const Args& a, int max_q, cudaStream_t stream) {
+int32_t launch(const Args& a, const Plan& plan, cudaStream_t stream) {
     using T = typename L::T;
     constexpr int UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = 8 * NT * (L::D + 4) * 4;
-    const int64_t most = static_cast<int64_t>(a.share) * max_q;
-    const int tiles = static_cast<int>(((most < a.most_rows ? most : a.most_rows) + 8 * NT - 1) / (8 * NT));
-    if (const int ranks = cluster_ranks(a, NT, tiles)) {
+    if (plan.ranks) {
         constexpr int smem = kWarps * ring_slots(L::D, L::G, part) * UB + join + part;
         const auto kernel = attention_kernel<T, L::D, L::G, NT, true>;
         if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
-        const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * tiles * ranks);
-        return result(ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, ranks, a, tiles));
+        const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * plan.tiles * plan.ranks);
+        return result(
+            ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, plan.ranks, a, plan.tiles));
     }
     constexpr int smem = kWarps * ring_slots(L::D, L::G, 0) * UB + join;
     const auto kernel = attention_kernel<T, L::D, L::G, NT, false>;
@@ -1051,8 +1065,8 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || max_q < 1 || max_pages < 1)
         return ECQ_ERR_ARG;
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
-    const int nt = row_tiles_of_8(heads / kv_heads, max_q);
-    return grid_ctas(nt) * (16 + 2 * 4 * 8ll * nt * (head_dim + 2));
+    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size);
+    return p.ranks ? 0 : grid_ctas(p.nt) * (16 + 2 * 4 * 8ll * p.nt * (head_dim + 2));
 }
 
 int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -1074,7 +1088,8 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (static_cast<int64_t>(total_q) * (heads / kv_heads) >= (1ll << 31)) return ECQ_ERR_UNSUPPORTED;
     if (!q || !out || !aligned(q, 16) || !aligned(out, 8)) return ECQ_ERR_ARG;
     if (((q_token_stride | q_head_stride) & 7) || ((out_token_stride | out_head_stride) & 3)) return ECQ_ERR_ARG;
-    if (workspace_bytes < need || !workspace || !aligned(workspace, 16)) return ECQ_ERR_WORKSPACE;
+    if (need && (workspace_bytes < need || !workspace || !aligned(workspace, 16))) return ECQ_ERR_WORKSPACE;
+    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size);
     Args a;
     a.q = q;
     a.out = out;
@@ -1083,7 +1098,7 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     a.lens = static_cast<const int32_t*>(seq_lens);
     a.starts = static_cast<const int32_t*>(q_starts);
     a.cuts = static_cast<int4*>(workspace);
-    a.parts = reinterpret_cast<float*>(a.cuts + grid_ctas(row_tiles_of_8(heads / kv_heads, max_q)));
+    a.parts = reinterpret_cast<float*>(a.cuts + grid_ctas(p.nt));
     a.status = static_cast<int32_t*>(status);
     a.q_token = q_token_stride;
     a.q_head = q_head_stride;
@@ -1098,18 +1113,15 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     a.batch = batch;
     a.total_q = total_q;
     a.scale = scale;
-    const int most = stream_rows(batch, kv_heads);
-    const bool prompts = static_cast<int64_t>(a.share) * max_q > most;
-    a.most_rows = prompts ? most : INT32_MAX;
-    if (prompts) {
+    a.most_rows = p.most_rows;
+    if (p.prompts) {
         const int32_t rc = launch_prompt(a, dtype, head_dim, head_dim / group_size, max_q, static_cast<cudaStream_t>(stream));
         if (rc != ECQ_OK) return rc;
     }
-    const int nt = row_tiles_of_8(a.share, max_q);
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
-        return nt == 2 ? launch<L, 2>(a, max_q, static_cast<cudaStream_t>(stream))
-                       : launch<L, 1>(a, max_q, static_cast<cudaStream_t>(stream));
+        return p.nt == 2 ? launch<L, 2>(a, p, static_cast<cudaStream_t>(stream))
+                         : launch<L, 1>(a, p, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -29,7 +29,9 @@ from ._lib import EcqError, check, lib
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _I32 = torch.int32
 _U8 = torch.uint8
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without an object for it
+# the current stream's handle and the current device, without objects for them
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 class KV4Step(NamedTuple):
@@ -59,7 +61,7 @@ def _device(first: torch.Tensor, names: str, *others) -> int:
 
 def _on(device: int, fn, *args) -> int:
     """fn(*args, stream) with `device` current (a launch needs that)."""
-    if torch.cuda.current_device() == device:
+    if _current_device() == device:
         return fn(*args, _raw_stream(device))
     with torch.cuda.device(device):
         return fn(*args, _raw_stream(device))
@@ -76,12 +78,13 @@ def _table(block_table: torch.Tensor, batch: int) -> tuple[int, int]:
     """Row stride and columns."""
     if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.shape[0] != batch:
         raise ValueError(f"block_table must be int32 [{batch}, pages per request]")
-    stride, cols = block_table.stride(), block_table.shape[1]
-    if batch == 1:  # a single row's stride says nothing
-        stride = (max(stride[0], cols), stride[1])
-    if cols < 1 or (stride[1] != 1 and cols > 1) or stride[0] < cols:
+    cols = block_table.shape[1]
+    stride, last = block_table.stride()
+    if batch == 1 and stride < cols:  # a single row's stride says nothing
+        stride = cols
+    if cols < 1 or (last != 1 and cols > 1) or stride < cols:
         raise ValueError("block_table needs contiguous rows of at least one page")
-    return stride[0], cols
+    return stride, cols
 
 
 def _status(status) -> int | None:
@@ -190,10 +193,17 @@ def kv4_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.T
     _int32("free_pages", free_pages)
     _int32("free_count", free_count, 1)
     stride, cols = _table(block_table, batch)
-    lens_out = torch.empty_like(seq_lens) if seq_lens_out is None else seq_lens_out
-    count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
-    _int32("seq_lens_out", lens_out, batch)
-    _int32("free_count_out", count_out, 1)
+    lens_out, count_out = seq_lens_out, free_count_out
+    if lens_out is None and count_out is None:
+        lens_out, count_out = torch.empty(batch + 1, dtype=_I32, device=seq_lens.device).split_with_sizes((batch, 1))
+    elif lens_out is None:
+        lens_out = torch.empty_like(seq_lens)
+    elif count_out is None:
+        count_out = torch.empty_like(free_count)
+    if seq_lens_out is not None:
+        _int32("seq_lens_out", lens_out, batch)
+    if free_count_out is not None:
+        _int32("free_count_out", count_out, 1)
     check(_on(device, lib().ecq_kv4_release, done.data_ptr(), seq_lens.data_ptr(), lens_out.data_ptr(),
               block_table.data_ptr(), stride, cols, batch, page_size, free_pages.data_ptr(), free_pages.shape[0],
               free_count.data_ptr(), count_out.data_ptr(), _status(status)), "kv4_release")
@@ -272,7 +282,10 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     if max_q < 1:
         raise ValueError("max_q must be at least 1")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        if q.is_contiguous():
+            out = torch.empty_like(q)
+        else:
+            out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
         o_token, o_head = heads * dim, dim
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
@@ -281,11 +294,12 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         if out.numel() and (last != 1 or o_token % 4 or o_head % 4 or out.data_ptr() % 8):
             raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
     need = _workspace_bytes(batch, heads, kv_heads, dim, max_q, cols, page_size, device)
-    ws = torch.empty(need, dtype=_U8, device=q.device)
+    ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
     check(_on(device, lib().ecq_kv4_attention, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, code,
               pages.data_ptr(), n_pages, heads, kv_heads, dim, page_size, group_size, block_table.data_ptr(), stride, cols,
               seq_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), batch, tokens, max_q,
-              dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _status(status)), "kv4_attention")
+              dim ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, _status(status)),
+          "kv4_attention")
     return out
 
 
