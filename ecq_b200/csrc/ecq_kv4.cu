@@ -16,11 +16,12 @@ using ecq_dev::pdl_launch_dependents;
 using ecq_dev::pdl_wait;
 
 // ---------------------------------------------------------------------------
-// Block tables and slot maps. One launch: every CTA of one cluster scans all
-// requests (a few KB from L2) into its own shared memory -- tokens and pages
-// before each request -- and then writes its share of the outputs. The cluster
-// barrier between the two parts is what lets lengths and count be updated in
-// place: nothing is written before every CTA has read. Work per token and per
+// Block tables and slot maps. One launch: every CTA scans all requests (a few
+// KB from L2) into its own shared memory -- tokens and pages before each
+// request -- and then writes its share of the outputs. Where lengths or count
+// are updated in place the CTAs are one cluster, whose barrier between the two
+// parts keeps anything from being written before every CTA has read; otherwise
+// there are more of them. Work per token and per
 // page is found by a binary search in the scanned starts, so one request with
 // all the tokens is spread like many with few. Bound by launch and barrier
 // latency.
@@ -129,8 +130,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     bad = __syncthreads_or(bad || sum.tokens > max_tokens);
     const bool dry = !bad && pages_sum > count;
     ecq_dev::cluster_sync();
-    const int rank = static_cast<int>(ecq_dev::cluster_rank()), ranks = static_cast<int>(ecq_dev::cluster_size());
-    const int tid = rank * kTableThreads + threadIdx.x, threads = ranks * kTableThreads;
+    const int tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads;
     if (bad || dry) {
         if (tid == 0) {
             raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
@@ -228,8 +228,7 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
     bad = __syncthreads_or(bad);
     const bool full = !bad && pages_sum + count > free_capacity;
     ecq_dev::cluster_sync();
-    const int rank = static_cast<int>(ecq_dev::cluster_rank()), ranks = static_cast<int>(ecq_dev::cluster_size());
-    const int tid = rank * kTableThreads + threadIdx.x, threads = ranks * kTableThreads;
+    const int tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads;
     if (bad || full) {
         if (tid == 0) {
             raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
@@ -514,6 +513,15 @@ bool table_args_ok(int64_t table_stride, int32_t max_pages, int32_t batch, int32
     return static_cast<int64_t>(max_pages) * page_size < (1ll << 31) - 256;
 }
 
+// CTAs for so many outputs, kRun to a thread: one, a cluster, or (not in
+// place) several clusters.
+unsigned table_ctas(int64_t outputs, bool in_place) {
+    const int64_t want = (outputs + kTableThreads * kRun - 1) / (kTableThreads * kRun);
+    if (want <= 1) return 1;
+    if (in_place || want <= 8) return 8;
+    return want < 64 ? static_cast<unsigned>((want + 7) / 8 * 8) : 64;
+}
+
 cudaError_t allow(const void* fn, size_t smem) {
     if (smem <= 48 * 1024) return cudaSuccess;
     return ecq_dev::ensure_smem_limit(fn, 112 * 1024) ? cudaSuccess : cudaErrorInvalidValue;
@@ -540,10 +548,10 @@ int32_t ecq_kv4_extend(const void* seq_lens, const void* new_lens, void* seq_len
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
     const size_t smem = static_cast<size_t>(batch) * 12;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(extend_kernel), smem); rc != cudaSuccess) return result(rc);
-    // one CTA while its threads cover the outputs in a few rounds, a cluster of 8 above
-    const unsigned ctas = (max_tokens > 4 * kTableThreads || batch > 2 * kTableThreads) ? 8 : 1;
+    const unsigned ctas = table_ctas(static_cast<int64_t>(max_tokens) + batch,
+                                     seq_lens == seq_lens_out || free_count == free_count_out);
     return result(launch_pdl_cluster(extend_kernel, dim3(ctas), dim3(kTableThreads), smem,
-                                     static_cast<cudaStream_t>(stream), ctas, static_cast<const int32_t*>(seq_lens),
+                                     static_cast<cudaStream_t>(stream), ctas < 8 ? ctas : 8, static_cast<const int32_t*>(seq_lens),
                                      static_cast<const int32_t*>(new_lens), static_cast<int32_t*>(seq_lens_out),
                                      static_cast<int32_t*>(block_table), table_stride, max_pages, batch,
                                      log2i(page_size), static_cast<const int32_t*>(free_pages), free_capacity,
@@ -562,9 +570,10 @@ int32_t ecq_kv4_release(const void* done, const void* seq_lens, void* seq_lens_o
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
     const size_t smem = static_cast<size_t>(batch) * 8;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(release_kernel), smem); rc != cudaSuccess) return result(rc);
-    const unsigned ctas = static_cast<int64_t>(batch) * max_pages > 8 * kTableThreads ? 8 : 1;
+    const unsigned ctas = table_ctas(static_cast<int64_t>(batch) * max_pages / 2,
+                                     seq_lens == seq_lens_out || free_count == free_count_out);
     return result(launch_pdl_cluster(release_kernel, dim3(ctas), dim3(kTableThreads), smem,
-                                     static_cast<cudaStream_t>(stream), ctas, static_cast<const uint8_t*>(done),
+                                     static_cast<cudaStream_t>(stream), ctas < 8 ? ctas : 8, static_cast<const uint8_t*>(done),
                                      static_cast<const int32_t*>(seq_lens), static_cast<int32_t*>(seq_lens_out),
                                      static_cast<const int32_t*>(block_table), table_stride, max_pages, batch,
                                      log2i(page_size), static_cast<int32_t*>(free_pages), free_capacity,
