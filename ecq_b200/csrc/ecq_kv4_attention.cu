@@ -18,7 +18,7 @@
 // weight beside the output's 2^-9, for 30 instructions fewer of 330. q is
 // scaled to its row's largest power of two and exact in fp16.
 //
-// What bounds it: the cache's bytes for long contexts; below that the ~250
+// What bounds it: the cache's bytes for long contexts; below that the ~330
 // instructions per 16 tokens and head, and for short ones launches and merges.
 //
 // Layout of the work. The (request, cache head, row tile, 32-token unit) space
@@ -1010,7 +1010,7 @@ int row_tiles_of_8(int share, int max_q) {
 // was cut. Clusters have neither, and are taken where that counts: all of them
 // fit on the GPU at once, and the longest request that the tables have room for
 // is a few rounds of its cluster's warps (7b step, 32 pairs of up to 66 units:
-// 14.4 us with ranges, 10.0 with clusters).
+// 14.4 us with ranges, 10.5 with clusters).
 constexpr int kMostRounds = 6;
 struct Plan {
     int most_rows;  // of a request that is streamed
