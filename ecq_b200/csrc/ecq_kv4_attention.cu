@@ -14,9 +14,12 @@
 // mma.sync m16n8k16 holds 8 rows of keys' work at full use, where a tcgen05
 // tile would be 64 or 128 rows, of which a decode step has 1 to 8.
 // For fp16 outputs p and p s are fp16 twice (value and remainder: 22 bits), so
-// V's side keeps fp32 accuracy. For bf16 they are fp16 once: 2^-12 of each
-// weight beside the output's 2^-9, for 30 instructions fewer of 330. q is
-// scaled to its row's largest power of two and exact in fp16.
+// V's side keeps fp32 accuracy. With up to 4 rows the remainders take the
+// columns that would be idle: rows n and n + 4 of the narrow side are one row
+// (32 requests of 4-8k tokens, heads shared by 4: 70 -> 65 us). For bf16 they
+// are fp16 once: 2^-12 of each weight beside the output's 2^-9, for 30
+// instructions fewer of 330. q is scaled to its row's largest power of two and
+// exact in fp16.
 //
 // What bounds it: the cache's bytes for long contexts; below that the ~330
 // instructions per 16 tokens and head, and for short ones launches and merges.
@@ -61,6 +64,11 @@ constexpr float kSlack = 2.f, kLift = 10.f;
 constexpr float kDrop = 10.f;  // the reference goes up by so much where weight * scale is infinite
 constexpr float kNoMax = -1e30f;
 constexpr int kMostRanks = 8;  // CTAs that share a pair
+
+// How the weights are held: once, twice, or twice in the columns of a row.
+enum Weights { kOnce, kTwice, kFolded };
+template <int NT, int W>
+__host__ __device__ constexpr int tile_rows() { return W == kFolded ? 4 : 8 * NT; }
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups, int besides) {
     const int room = 74 * 1024 - kWarps * 8 * (dim + 4) * 4 - besides;
@@ -171,12 +179,12 @@ struct Rows {
 
 // A lane's share of the tile's rows as they lie in memory: the loads are issued
 // early and set_rows makes the operands of them.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int W>
 __device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& a, const Request& rq, int head, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int row = (tile * NT + nt) * 8 + n, i = row / a.share;
+        const int row = W == kFolded ? tile * 4 + (n & 3) : (tile * NT + nt) * 8 + n, i = row / a.share;
         const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
                        static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
 #pragma unroll
@@ -187,14 +195,14 @@ __device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& 
     }
 }
 
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int W>
 __device__ __forceinline__ void set_rows(Rows<D, G, NT>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
                                          const Request& rq, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
     R.least = rq.len;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int row = (tile * NT + nt) * 8 + n;
+        const int row = W == kFolded ? tile * 4 + (n & 3) : (tile * NT + nt) * 8 + n;
         const bool in = row < rq.rows;
         float x[D / 32][8];
         float top = 0.f;
@@ -321,7 +329,7 @@ __device__ __forceinline__ uint32_t neg2(uint32_t a) {
 
 // A unit's blocks at shared address at; first[u]: the request's token that
 // block u starts with (used with kMask; beyond all limits: leave it out).
-template <int D, int G, int NT, bool kMask, bool kExact>
+template <int D, int G, int NT, bool kMask, int kWeights>
 __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
                                        const int (&first)[kUnit]) {
     constexpr int U = kUnit, W = D / 32, BB = block_bytes(D, G);
@@ -415,7 +423,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                     const uint32_t x = h2(p[0], p[1]);
                     const float2 back = f2(x);
                     ph[u][nt][i] = transpose(x);
-                    if (kExact) pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
+                    if (kWeights != kOnce) pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
                 }
             uint32_t sa[2][G], sb[2][G];
             lds<G, 0>(sa[0], at + u * BB + me.v_params);
@@ -432,13 +440,13 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                         // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
                         const uint32_t w = ph[u][nt][i];
                         uint32_t h = mul2(w, sc);
-                        uint32_t l = kExact ? fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h))) : 0u;
+                        uint32_t l = kWeights != kOnce ? fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h))) : 0u;
                         if (kMask) {  // weight 0: 0, whatever the scale is
                             const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
                             h &= keep;
                             l &= keep;
                         }
-                        hi[u][nt][g][i] = h;
+                        hi[u][nt][g][i] = kWeights == kFolded && r >= 4 ? l : h;
                         lo[u][nt][g][i] = l;
                         most = max2(most, h);  // not negative, and a NaN passes by
                     }
@@ -466,9 +474,11 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
-                    else mma(sums[nt], z[0], 0u, z[1], 0u, ph[u][nt][0], ph[u][nt][1]);
-                    if (kExact) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
+                    const bool rest = kWeights == kFolded && r >= 4;
+                    const uint32_t p0 = rest ? pl[u][nt][0] : ph[u][nt][0], p1 = rest ? pl[u][nt][1] : ph[u][nt][1];
+                    if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
+                    else mma(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
+                    if (kWeights == kTwice) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
                 }
             }
 #pragma unroll
@@ -512,7 +522,7 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
             for (int u = 0; u < U; ++u) {
                 const uint32_t x = __byte_perm(v[u][0][w], v[u][1][w], pick), y = __byte_perm(v[u][2][w], v[u][3][w], pick);
 #pragma unroll
-                for (int part = 0; part < (kExact ? 2 : 1); ++part)
+                for (int part = 0; part < (kWeights == kTwice ? 2 : 1); ++part)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int g = (4 * w + 2 * half + j) * 16 * G / D;
@@ -536,10 +546,10 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
 template <int D, int TR>
 __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
-template <typename T, int D, int G, int NT, bool kPairs>
+template <typename T, int D, int G, int NT, bool kPairs, int kWeights>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a, const int tiles) {
-    constexpr bool kExact = std::is_same<T, __half>::value;
-    constexpr int TR = 8 * NT, NS = ring_slots(D, G, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G), UB = kUnit * BB, OS = D + 4;
+    constexpr int TR = tile_rows<NT, kWeights>(), NS = ring_slots(D, G, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G),
+                  UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
     __shared__ long long s_before;
@@ -641,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     const Request rq0 = rq;
     const int head0 = head, tile0 = tile;
     uint4 raw[NT][D / 32];
-    load_rows<T, D, NT>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
+    load_rows<T, D, NT, kWeights>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
     int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + mine, f_page[kUnit];
     int f_left = range > mine ? static_cast<int>((range - mine + step - 1) / step) : 0;
     Request fr = rq;
@@ -726,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 #pragma unroll 1
     for (long long f = 0; f < range;) {
         const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), range - f));
-        set_rows<T, D, G, NT>(rows, raw, a, rq, tile);
+        set_rows<T, D, G, NT, kWeights>(rows, raw, a, rq, tile);
         st.reset();
         // this warp's first unit in [f, f + n)
         int i = kPairs ? mine : (warp - static_cast<int>(f % kWarps) + kWarps) % kWarps;
@@ -756,14 +766,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 #pragma unroll 1
             while (i < min(n, seen) && !(f_bad >> 2 * slot & 3u)) {
                 if (!wait()) break;
-                blocks<D, G, NT, false, kExact>(st, rows, me, ring + slot * UB, first);
+                blocks<D, G, NT, false, kWeights>(st, rows, me, ring + slot * UB, first);
                 done();
             }
             if (i >= n || !wait()) break;
 #pragma unroll
             for (int u = 0; u < kUnit; ++u)
                 first[u] = f_bad >> (2 * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
-            blocks<D, G, NT, true, kExact>(st, rows, me, ring + slot * UB, first);
+            blocks<D, G, NT, true, kWeights>(st, rows, me, ring + slot * UB, first);
             done();
         }
         // the next segment's rows are on their way while the warps join
@@ -786,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                 if (b >= a.batch) late = true;
             }
             if (late) f = range;
-            else load_rows<T, D, NT>(raw, a, rq, head, tile);
+            else load_rows<T, D, NT, kWeights>(raw, a, rq, head, tile);
         }
         float* part = kPairs ? s_part : a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
         if (!kPairs && starts && !ends && threadIdx.x == 0) {
@@ -815,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             }
             __syncthreads();
 #pragma unroll
-            for (int row = warp; row < 8; row += kWarps) {
+            for (int row = warp; row < (TR < 8 ? TR : 8); row += kWarps) {
                 float M = kNoMax, L = 0.f, o[V];
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
@@ -824,9 +834,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float k = exp2_fast(s_m[w][row] - M);
-                    float x[V];
+                    float x[V], l = s_l[w][row];
                     load<V>(x, s_o + (w * 8 + row) * OS + V * lane);
-                    L = fmaf(k, s_l[w][row], L);
+                    if (kWeights == kFolded) {
+                        float y[V];
+                        load<V>(y, s_o + (w * 8 + row + 4) * OS + V * lane);
+                        l += s_l[w][row + 4];
+#pragma unroll
+                        for (int v = 0; v < V; ++v) x[v] += y[v];
+                    }
+                    L = fmaf(k, l, L);
 #pragma unroll
                     for (int v = 0; v < V; ++v) o[v] = fmaf(k, x[v], o[v]);
                 }
@@ -901,9 +918,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
 // loads of the same thread would queue up behind one another.
 constexpr int kJoinWarps = 32;
 
-template <typename T, int D, int NT>
+template <typename T, int D, int TR>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
-    constexpr int TR = 8 * NT, kDeal = kJoinWarps / TR, V = D / 32, PF = part_floats<D, TR>();
+    constexpr int kDeal = kJoinWarps / TR, V = D / 32, PF = part_floats<D, TR>();
     __shared__ __align__(16) float s_o[kDeal][TR][D];
     __shared__ float s_l[kDeal][TR], s_m[kDeal][TR];
     pdl_launch_dependents();
@@ -1016,17 +1033,19 @@ struct Plan {
     int most_rows;  // of a request that is streamed
     bool prompts;   // some may have more
     int nt;         // 8-row tiles as one
+    int rows;       // of a tile
     int tiles;      // of a streamed request at most
     int ranks;      // CTAs of a cluster; 0: ranges
 };
-Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page_size) {
+Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page_size, int dtype) {
     Plan p;
     const int64_t rows = static_cast<int64_t>(share) * max_q;
     p.most_rows = stream_rows(batch, kv_heads);
     p.prompts = rows > p.most_rows;
     if (!p.prompts) p.most_rows = INT32_MAX;
     p.nt = row_tiles_of_8(share, max_q);
-    p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + 8 * p.nt - 1) / (8 * p.nt));
+    p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8 * p.nt;
+    p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.tiles;
     const int64_t units = static_cast<int64_t>(max_pages) * page_size / kUnitTokens + 1;
     p.ranks = kMostRanks;
@@ -1035,24 +1054,24 @@ Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page
     return p;
 }
 
-template <typename L, int NT>
+template <typename L, int NT, int W>
 int32_t launch(const Args& a, const Plan& plan, cudaStream_t stream) {
     using T = typename L::T;
-    constexpr int UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = 8 * NT * (L::D + 4) * 4;
+    constexpr int UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = tile_rows<NT, W>() * (L::D + 4) * 4;
     if (plan.ranks) {
         constexpr int smem = kWarps * ring_slots(L::D, L::G, part) * UB + join + part;
-        const auto kernel = attention_kernel<T, L::D, L::G, NT, true>;
+        const auto kernel = attention_kernel<T, L::D, L::G, NT, true, W>;
         if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
         const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * plan.tiles * plan.ranks);
         return result(
             ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, plan.ranks, a, plan.tiles));
     }
     constexpr int smem = kWarps * ring_slots(L::D, L::G, 0) * UB + join;
-    const auto kernel = attention_kernel<T, L::D, L::G, NT, false>;
+    const auto kernel = attention_kernel<T, L::D, L::G, NT, false, W>;
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
     const dim3 grid(grid_ctas(NT));
     cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a, 0);
-    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, NT>, grid, dim3(kJoinWarps * 32), 0, stream, a);
+    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, tile_rows<NT, W>()>, grid, dim3(kJoinWarps * 32), 0, stream, a);
     return result(rc);
 }
 
@@ -1065,7 +1084,8 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || max_q < 1 || max_pages < 1)
         return ECQ_ERR_ARG;
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
-    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size);
+    // the same clusters or ranges for both types: tiles of 4 rows are taken where there is one tile of 8
+    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size, ECQ_KV4_BF16);
     return p.ranks ? 0 : grid_ctas(p.nt) * (16 + 2 * 4 * 8ll * p.nt * (head_dim + 2));
 }
 
@@ -1089,7 +1109,7 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (!q || !out || !aligned(q, 16) || !aligned(out, 8)) return ECQ_ERR_ARG;
     if (((q_token_stride | q_head_stride) & 7) || ((out_token_stride | out_head_stride) & 3)) return ECQ_ERR_ARG;
     if (need && (workspace_bytes < need || !workspace || !aligned(workspace, 16))) return ECQ_ERR_WORKSPACE;
-    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size);
+    const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size, dtype);
     Args a;
     a.q = q;
     a.out = out;
@@ -1120,8 +1140,13 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     }
     return by_layout(dtype, head_dim, head_dim / group_size, [&](auto layout) {
         using L = decltype(layout);
-        return p.nt == 2 ? launch<L, 2>(a, p, static_cast<cudaStream_t>(stream))
-                         : launch<L, 1>(a, p, static_cast<cudaStream_t>(stream));
+        const auto st = static_cast<cudaStream_t>(stream);
+        if constexpr (std::is_same<typename L::T, __half>::value) {
+            if (p.rows == 4) return launch<L, 1, kFolded>(a, p, st);
+            return p.nt == 2 ? launch<L, 2, kTwice>(a, p, st) : launch<L, 1, kTwice>(a, p, st);
+        } else {
+            return p.nt == 2 ? launch<L, 2, kOnce>(a, p, st) : launch<L, 1, kOnce>(a, p, st);
+        }
     });
 }
 
