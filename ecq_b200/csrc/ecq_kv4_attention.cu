@@ -24,7 +24,7 @@
 // What bounds it: the cache's bytes for long contexts; below that the ~330
 // instructions per 16 tokens and head, and for short ones launches and merges.
 //
-// Layout of the work. The (request, cache head, row tile, 32-token unit) space
+// Layout of the work. The (request, cache head, row tile, unit of 32 or 64 tokens) space
 // is flattened and cut into one even range per CTA (one wave of CTAs), from the
 // lengths on the device, so ragged batches balance and no host knows them.
 // Within a range unit f belongs to warp f % kWarps. Each warp streams its
@@ -48,12 +48,17 @@ using ecq_dev::pdl_wait;
 using ecq_dev::smem_addr;
 
 constexpr int kWarps = 4;
-// A warp takes two blocks of tokens at a time: what it costs to fetch and to
-// wait for them, and the look at the running maximum, are paid once.
-constexpr int kUnit = 2, kUnitTokens = kUnit * kBlockTokens;
 constexpr int kThreads = kWarps * 32;
-// 16-row tiles need the registers of two 8-row ones
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+// Two CTAs of 4 warps: 8 warps with 255 registers each hide their latencies
+// better inside a step than 12 with 168 or 16 with 128 do among themselves (32
+// requests of 4-8k tokens: 58, 65 and 71 us).
+constexpr int kCtasPerSm = 2;
+// Blocks of 16 tokens that a warp takes at a time: what it costs to fetch and
+// to wait for them, and the look at the running maximum, are paid once, and
+// their products are independent (1, 2 and 4 at a time: 71, 65 and 58 us). With
+// four groups, or two row tiles, four blocks do not fit the registers (16
+// requests of 3-6 tokens and four groups: 55 us, with two blocks 48).
+__host__ __device__ constexpr int unit_blocks(int groups, int nt) { return groups <= 2 && nt == 1 ? 4 : 2; }
 // Weights are exp2(score - reference + kLift). The reference is raised when a
 // score passes it by more than kSlack, so few blocks raise it and the others
 // need no reduction over their tokens. The lift keeps the weights of keys far
@@ -70,9 +75,9 @@ enum Weights { kOnce, kTwice, kFolded };
 template <int NT, int W>
 __host__ __device__ constexpr int tile_rows() { return W == kFolded ? 4 : 8 * NT; }
 
-__host__ __device__ constexpr int ring_slots(int dim, int groups, int besides) {
-    const int room = 74 * 1024 - kWarps * 8 * (dim + 4) * 4 - besides;
-    const int n = room / (kWarps * kUnit * block_bytes(dim, groups));
+__host__ __device__ constexpr int ring_slots(int dim, int groups, int unit, int besides) {
+    const int room = 110 * 1024 - kWarps * 8 * (dim + 4) * 4 - besides;
+    const int n = room / (kWarps * unit * block_bytes(dim, groups));
     return n < 4 ? n : 4;
 }
 
@@ -81,13 +86,14 @@ struct Request {
     int first_q, queries, rows, len, units, tiles, pairs;
 };
 
-template <int TR>  // rows per tile
+template <int TR, int kUnit>  // rows per tile, blocks per unit
 __device__ __forceinline__ Request request(const Args& a, int b) {
     const Range x = range_of(a, b);
     Request r = {x.first_q, x.queries, x.rows > a.most_rows ? 0 : x.rows, x.len, 0, 0, 0};
     r.tiles = (r.rows + TR - 1) / TR;
     r.pairs = r.tiles * a.kv_heads;
     // a request without keys has one (empty) unit, so that its rows are written
+    constexpr int kUnitTokens = kUnit * kBlockTokens;
     r.units = r.rows ? max((r.len + kUnitTokens - 1) / kUnitTokens, 1) : 0;
     return r;
 }
@@ -329,10 +335,10 @@ __device__ __forceinline__ uint32_t neg2(uint32_t a) {
 
 // A unit's blocks at shared address at; first[u]: the request's token that
 // block u starts with (used with kMask; beyond all limits: leave it out).
-template <int D, int G, int NT, bool kMask, int kWeights>
+template <int D, int G, int NT, int U, bool kMask, int kWeights>
 __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
-                                       const int (&first)[kUnit]) {
-    constexpr int U = kUnit, W = D / 32, BB = block_bytes(D, G);
+                                       const int (&first)[U]) {
+    constexpr int W = D / 32, BB = block_bytes(D, G);
     const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
     float s[U][NT][4];
 #pragma unroll
@@ -547,8 +553,9 @@ template <int D, int TR>
 __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
 template <typename T, int D, int G, int NT, bool kPairs, int kWeights>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(const Args a, const int tiles) {
-    constexpr int TR = tile_rows<NT, kWeights>(), NS = ring_slots(D, G, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G),
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const Args a, const int tiles) {
+    constexpr int kUnit = unit_blocks(G, NT), kUnitTokens = kUnit * kBlockTokens;
+    constexpr int TR = tile_rows<NT, kWeights>(), NS = ring_slots(D, G, kUnit, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G),
                   UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         b = pair / (a.kv_heads * tiles);
         head = pair / tiles - b * a.kv_heads;
         tile = pair % tiles;
-        rq = request<TR>(a, b);
+        rq = request<TR, kUnit>(a, b);
         // more queries than the call said: their rows are not computed
         if (tile == tiles - 1 && rq.tiles > tiles && threadIdx.x == 0) raise_status(a.status, ECQ_STATUS_BADARG);
         if (tile >= rq.tiles) return;  // the whole cluster
@@ -587,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         long long total = 0, weight = 0;
         Request own = {};
         for (int r = threadIdx.x; r < a.batch; r += kThreads) {
-            own = request<TR>(a, r);
+            own = request<TR, kUnit>(a, r);
             weight = static_cast<long long>(own.units) * own.pairs;
             total += weight;
         }
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             if (a.batch > kThreads) {  // more than one round: not the last one's any more
                 weight = 0;
                 if (r < a.batch) {
-                    own = request<TR>(a, r);
+                    own = request<TR, kUnit>(a, r);
                     weight = static_cast<long long>(own.units) * own.pairs;
                 }
             }
@@ -657,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     Request fr = rq;
     const int32_t* f_row = a.table + fb * a.table_stride;
     const uint8_t* f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
+    constexpr uint32_t kAll = (1u << kUnit) - 1u;
     uint32_t f_bad = 0;  // a bit per ring slot and block: its page number is out of range
     int f_slot = 0;
     auto look = [&]() {  // the pages of the next unit, one fetch ahead of their use
@@ -672,21 +680,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
                             f_left = 0;
                             return;
                         }
-                        fr = request<TR>(a, fb);
+                        fr = request<TR, kUnit>(a, fb);
                     } while (fr.units == 0);
                     f_row = a.table + fb * a.table_stride;
                 }
                 f_src = a.pages + static_cast<int64_t>(f_head) * page_bytes;
             }
         }
-        if (shift) {  // a page has the whole unit
+        if (kBlockTokens << shift >= kUnitTokens) {  // a page has the whole unit
             f_page[0] = -1;  // nothing there: the one unit of a request without keys
             if (fr.len) f_page[0] = __ldg(f_row + (f_unit * kUnit >> shift)) & INT32_MAX;
         } else {
 #pragma unroll
             for (int u = 0; u < kUnit; ++u) {
                 f_page[u] = -1;
-                if ((f_unit * kUnit + u) * kBlockTokens < fr.len) f_page[u] = __ldg(f_row + f_unit * kUnit + u) & INT32_MAX;
+                if ((f_unit * kUnit + u) * kBlockTokens < fr.len)
+                    f_page[u] = __ldg(f_row + ((f_unit * kUnit + u) >> shift)) & INT32_MAX;
             }
         }
     };
@@ -694,8 +703,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
     auto fetch = [&]() {
         if (f_left <= 0) return;
         const uint32_t bar = bars + 8 * f_slot, dst = ring + f_slot * UB;
-        f_bad &= ~(3u << 2 * f_slot);
-        if (shift && static_cast<uint32_t>(f_page[0]) < a.n_pages) {
+        f_bad &= ~(kAll << kUnit * f_slot);
+        const bool one_page = kBlockTokens << shift >= kUnitTokens;
+        if (one_page && static_cast<uint32_t>(f_page[0]) < a.n_pages) {
             if (lane == 0) {
                 ecq_dev::mbar_expect_tx(bar, UB);
                 ecq_dev::bulk_copy_g2s(dst, f_src + f_page[0] * pool_row + ((f_unit * kUnit) & ((1 << shift) - 1)) * BB, UB, bar);
@@ -704,15 +714,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             uint32_t there = 0;
 #pragma unroll
             for (int u = 0; u < kUnit; ++u) {
-                const int page = shift ? f_page[0] : f_page[u];
+                const int page = one_page ? f_page[0] : f_page[u];
                 if (page >= 0 && page < a.n_pages) there |= 1u << u;
-                else if (page >= 0) f_bad |= 1u << (2 * f_slot + u);
+                else if (page >= 0) f_bad |= 1u << (kUnit * f_slot + u);
             }
             if (lane == 0) {
                 ecq_dev::mbar_expect_tx(bar, __popc(there) * BB);
 #pragma unroll
                 for (int u = 0; u < kUnit; ++u)
-                    if (there >> u & 1u) ecq_dev::bulk_copy_g2s(dst + u * BB, f_src + f_page[u] * pool_row, BB, bar);
+                    if (there >> u & 1u)
+                        ecq_dev::bulk_copy_g2s(dst + u * BB, f_src + f_page[u] * pool_row + ((f_unit * kUnit + u) & ((1 << shift) - 1)) * BB,
+                                               BB, bar);
                 if (f_bad) raise_status(a.status, ECQ_STATUS_BADARG);
             }
         }
@@ -764,16 +776,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
         while (i < n) {
             int first[kUnit] = {};
 #pragma unroll 1
-            while (i < min(n, seen) && !(f_bad >> 2 * slot & 3u)) {
+            while (i < min(n, seen) && !(f_bad >> kUnit * slot & kAll)) {
                 if (!wait()) break;
-                blocks<D, G, NT, false, kWeights>(st, rows, me, ring + slot * UB, first);
+                blocks<D, G, NT, kUnit, false, kWeights>(st, rows, me, ring + slot * UB, first);
                 done();
             }
             if (i >= n || !wait()) break;
 #pragma unroll
             for (int u = 0; u < kUnit; ++u)
-                first[u] = f_bad >> (2 * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
-            blocks<D, G, NT, true, kWeights>(st, rows, me, ring + slot * UB, first);
+                first[u] = f_bad >> (kUnit * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
+            blocks<D, G, NT, kUnit, true, kWeights>(st, rows, me, ring + slot * UB, first);
             done();
         }
         // the next segment's rows are on their way while the warps join
@@ -791,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attention_kernel(co
             if (head == 0 && tile == 0) {
                 do {
                     if (++b >= a.batch) break;
-                    rq = request<TR>(a, b);
+                    rq = request<TR, kUnit>(a, b);
                 } while (rq.units == 0);
                 if (b >= a.batch) late = true;
             }
@@ -975,7 +987,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
         s_l[deal][row] = L;
     }
     __syncthreads();
-    const Request rq = request<TR>(a, cut.x);
+    const Request rq = request<TR, 1>(a, cut.x);
     if (rq.rows == 0) return;
     const int head = cut.y / rq.tiles, tile = cut.y - head * rq.tiles;
     const int tr = threadIdx.x >> 5, qr = tile * TR + tr;
@@ -999,7 +1011,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
     store<T, V>(out_row<T>(a, rq.first_q, head, qr) + V * lane, val);
 }
 
-int grid_ctas(int nt) { return ctas_per_sm(nt) * ecq_dev::sm_count_cached(); }
+int grid_ctas() { return kCtasPerSm * ecq_dev::sm_count_cached(); }
 
 // Requests with up to so many rows (queries times heads that share a cache
 // head) are streamed by attention_kernel, those with more are the prompt
@@ -1014,8 +1026,7 @@ int stream_rows(int batch, int kv_heads) {
     return rows > 32 ? static_cast<int>(rows) : 32;
 }
 
-// 16-row tiles (one pass over the keys for twice the rows, at two thirds of the
-// warps) where 8-row tiles would be even in number: 128 pairs of 4096 tokens,
+// 16-row tiles (one pass over the keys for twice the rows) where 8-row tiles would be even in number: 128 pairs of 4096 tokens,
 // 16 rows 49 against 54 us, 32 rows 77 against 89, but 24 rows 77 against 71.
 int row_tiles_of_8(int share, int max_q) {
     return (static_cast<int64_t>(share) * max_q + 7) / 8 % 2 == 0 ? 2 : 1;
@@ -1026,9 +1037,9 @@ int row_tiles_of_8(int share, int max_q) {
 // the price of a look at all lengths, and of a second kernel that joins what
 // was cut. Clusters have neither, and are taken where that counts: all of them
 // fit on the GPU at once, and the longest request that the tables have room for
-// is a few rounds of its cluster's warps (7b step, 32 pairs of up to 66 units:
+// is a few steps of its cluster's warps (7b step, 32 pairs of up to 2112 tokens:
 // 14.4 us with ranges, 10.5 with clusters).
-constexpr int kMostRounds = 6;
+constexpr int kMostTokens = 192;  // per warp
 struct Plan {
     int most_rows;  // of a request that is streamed
     bool prompts;   // some may have more
@@ -1047,29 +1058,28 @@ Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page
     p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8 * p.nt;
     p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.tiles;
-    const int64_t units = static_cast<int64_t>(max_pages) * page_size / kUnitTokens + 1;
     p.ranks = kMostRanks;
-    while (p.ranks && pairs * p.ranks > grid_ctas(p.nt)) p.ranks /= 2;
-    if (units > static_cast<int64_t>(kMostRounds) * p.ranks * kWarps) p.ranks = 0;
+    while (p.ranks && pairs * p.ranks > grid_ctas()) p.ranks /= 2;
+    if (static_cast<int64_t>(max_pages) * page_size > kMostTokens * p.ranks * kWarps) p.ranks = 0;
     return p;
 }
 
 template <typename L, int NT, int W>
 int32_t launch(const Args& a, const Plan& plan, cudaStream_t stream) {
     using T = typename L::T;
-    constexpr int UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = tile_rows<NT, W>() * (L::D + 4) * 4;
+    constexpr int kUnit = unit_blocks(L::G, NT), UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = tile_rows<NT, W>() * (L::D + 4) * 4;
     if (plan.ranks) {
-        constexpr int smem = kWarps * ring_slots(L::D, L::G, part) * UB + join + part;
+        constexpr int smem = kWarps * ring_slots(L::D, L::G, kUnit, part) * UB + join + part;
         const auto kernel = attention_kernel<T, L::D, L::G, NT, true, W>;
         if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
         const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * plan.tiles * plan.ranks);
         return result(
             ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, plan.ranks, a, plan.tiles));
     }
-    constexpr int smem = kWarps * ring_slots(L::D, L::G, 0) * UB + join;
+    constexpr int smem = kWarps * ring_slots(L::D, L::G, kUnit, 0) * UB + join;
     const auto kernel = attention_kernel<T, L::D, L::G, NT, false, W>;
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
-    const dim3 grid(grid_ctas(NT));
+    const dim3 grid(grid_ctas());
     cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a, 0);
     if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, tile_rows<NT, W>()>, grid, dim3(kJoinWarps * 32), 0, stream, a);
     return result(rc);
@@ -1086,7 +1096,7 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
     // the same clusters or ranges for both types: tiles of 4 rows are taken where there is one tile of 8
     const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size, ECQ_KV4_BF16);
-    return p.ranks ? 0 : grid_ctas(p.nt) * (16 + 2 * 4 * 8ll * p.nt * (head_dim + 2));
+    return p.ranks ? 0 : grid_ctas() * (16 + 2 * 4 * 8ll * p.nt * (head_dim + 2));
 }
 
 int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -1118,7 +1128,7 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     a.lens = static_cast<const int32_t*>(seq_lens);
     a.starts = static_cast<const int32_t*>(q_starts);
     a.cuts = static_cast<int4*>(workspace);
-    a.parts = reinterpret_cast<float*>(a.cuts + grid_ctas(p.nt));
+    a.parts = reinterpret_cast<float*>(a.cuts + grid_ctas());
     a.status = static_cast<int32_t*>(status);
     a.q_token = q_token_stride;
     a.q_head = q_head_stride;
