@@ -16,13 +16,16 @@
 // For fp16 outputs p and p s are fp16 twice (value and remainder: 22 bits), so
 // V's side keeps fp32 accuracy. With up to 4 rows the remainders take the
 // columns that would be idle: rows n and n + 4 of the narrow side are one row
-// (32 requests of 4-8k tokens, heads shared by 4: 70 -> 65 us). For bf16 they
+// (7 % on a decode step of 32 requests). For bf16 they
 // are fp16 once: 2^-12 of each weight beside the output's 2^-9, for 30
 // instructions fewer of 330. q is scaled to its row's largest power of two and
 // exact in fp16.
 //
-// What bounds it: the cache's bytes for long contexts; below that the ~330
-// instructions per 16 tokens and head, and for short ones launches and merges.
+// What bounds it: the ~265 instructions per 16 tokens and head, issued by 8
+// warps per SM, and for short contexts launches and joins. Measured: 32 requests
+// of 4-8k tokens, 8 cache heads shared by 4: 58 us, 3.9 TB/s of the 6.55 that a
+// copy reaches; one request of 131071 tokens, shared by 8: 40 us, 3.8 TB/s; 32
+// heads of 2049 tokens: 8.8 us, 1.0 TB/s.
 //
 // Layout of the work. The (request, cache head, row tile, unit of 32 or 64 tokens) space
 // is flattened and cut into one even range per CTA (one wave of CTAs), from the
@@ -56,9 +59,13 @@ constexpr int kCtasPerSm = 2;
 // Blocks of 16 tokens that a warp takes at a time: what it costs to fetch and
 // to wait for them, and the look at the running maximum, are paid once, and
 // their products are independent (1, 2 and 4 at a time: 71, 65 and 58 us). With
-// four groups, or two row tiles, four blocks do not fit the registers (16
+// four groups four blocks do not fit the registers (16
 // requests of 3-6 tokens and four groups: 55 us, with two blocks 48).
-__host__ __device__ constexpr int unit_blocks(int groups, int nt) { return groups <= 2 && nt == 1 ? 4 : 2; }
+__host__ __device__ constexpr int unit_blocks(int groups) { return groups <= 2 ? 4 : 2; }
+// Row tiles of 8 that a warp takes at once. Two of them are one pass over the
+// keys for 16 rows, but leave registers for two blocks a step only, and took as
+// long (128 pairs of 4096 tokens, 16 rows: 49.6 against 47.4 us).
+constexpr int NT = 1;
 // Weights are exp2(score - reference + kLift). The reference is raised when a
 // score passes it by more than kSlack, so few blocks raise it and the others
 // need no reduction over their tokens. The lift keeps the weights of keys far
@@ -72,7 +79,7 @@ constexpr int kMostRanks = 8;  // CTAs that share a pair
 
 // How the weights are held: once, twice, or twice in the columns of a row.
 enum Weights { kOnce, kTwice, kFolded };
-template <int NT, int W>
+template <int W>
 __host__ __device__ constexpr int tile_rows() { return W == kFolded ? 4 : 8 * NT; }
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups, int unit, int besides) {
@@ -174,7 +181,7 @@ __device__ __forceinline__ void load(float (&x)[V], const float* p) {
     }
 }
 // The query rows of one tile as B operands, and what their scores need.
-template <int D, int G, int NT>
+template <int D, int G>
 struct Rows {
     uint32_t b[NT][D / 16][2];
     uint32_t sums[NT][2];  // B operand that takes (scale, zero) pairs: (0, sum of the group's q), high and low part
@@ -185,7 +192,7 @@ struct Rows {
 
 // A lane's share of the tile's rows as they lie in memory: the loads are issued
 // early and set_rows makes the operands of them.
-template <typename T, int D, int NT, int W>
+template <typename T, int D, int W>
 __device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& a, const Request& rq, int head, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
 #pragma unroll
@@ -201,8 +208,8 @@ __device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& 
     }
 }
 
-template <typename T, int D, int G, int NT, int W>
-__device__ __forceinline__ void set_rows(Rows<D, G, NT>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
+template <typename T, int D, int G, int W>
+__device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
                                          const Request& rq, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
     R.least = rq.len;
@@ -277,7 +284,7 @@ __device__ __forceinline__ void set_rows(Rows<D, G, NT>& R, const uint4 (&raw)[N
 }
 
 // Running softmax of one warp over its blocks.
-template <int D, int G, int NT>
+template <int D, int G>
 struct State {
     float o[NT][D / 16][4];
     float sums[NT][2];  // columns 2t, 2t + 1; lanes of row r < G: sum p zero of group r; of row G: sum p
@@ -335,8 +342,8 @@ __device__ __forceinline__ uint32_t neg2(uint32_t a) {
 
 // A unit's blocks at shared address at; first[u]: the request's token that
 // block u starts with (used with kMask; beyond all limits: leave it out).
-template <int D, int G, int NT, int U, bool kMask, int kWeights>
-__device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>& R, const Lane<D, G>& me, uint32_t at,
+template <int D, int G, int U, bool kMask, int kWeights>
+__device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, const Lane<D, G>& me, uint32_t at,
                                        const int (&first)[U]) {
     constexpr int W = D / 32, BB = block_bytes(D, G);
     const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
@@ -552,10 +559,10 @@ __device__ __forceinline__ void blocks(State<D, G, NT>& S, const Rows<D, G, NT>&
 template <int D, int TR>
 __host__ __device__ constexpr int part_floats() { return TR * (D + 2); }
 
-template <typename T, int D, int G, int NT, bool kPairs, int kWeights>
+template <typename T, int D, int G, bool kPairs, int kWeights>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const Args a, const int tiles) {
-    constexpr int kUnit = unit_blocks(G, NT), kUnitTokens = kUnit * kBlockTokens;
-    constexpr int TR = tile_rows<NT, kWeights>(), NS = ring_slots(D, G, kUnit, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G),
+    constexpr int kUnit = unit_blocks(G), kUnitTokens = kUnit * kBlockTokens;
+    constexpr int TR = tile_rows<kWeights>(), NS = ring_slots(D, G, kUnit, kPairs ? TR * (D + 4) * 4 : 0), BB = block_bytes(D, G),
                   UB = kUnit * BB, OS = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kWarps];
@@ -658,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
     const Request rq0 = rq;
     const int head0 = head, tile0 = tile;
     uint4 raw[NT][D / 32];
-    load_rows<T, D, NT, kWeights>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
+    load_rows<T, D, kWeights>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
     int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + mine, f_page[kUnit];
     int f_left = range > mine ? static_cast<int>((range - mine + step - 1) / step) : 0;
     Request fr = rq;
@@ -742,13 +749,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
     int slot = 0;
     uint32_t phase = 0;
     bool late = false;  // a copy did not come: nothing more is fetched or read
-    Rows<D, G, NT> rows;
-    State<D, G, NT> st;
+    Rows<D, G> rows;
+    State<D, G> st;
     const Lane<D, G> me;
 #pragma unroll 1
     for (long long f = 0; f < range;) {
         const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), range - f));
-        set_rows<T, D, G, NT, kWeights>(rows, raw, a, rq, tile);
+        set_rows<T, D, G, kWeights>(rows, raw, a, rq, tile);
         st.reset();
         // this warp's first unit in [f, f + n)
         int i = kPairs ? mine : (warp - static_cast<int>(f % kWarps) + kWarps) % kWarps;
@@ -778,14 +785,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
 #pragma unroll 1
             while (i < min(n, seen) && !(f_bad >> kUnit * slot & kAll)) {
                 if (!wait()) break;
-                blocks<D, G, NT, kUnit, false, kWeights>(st, rows, me, ring + slot * UB, first);
+                blocks<D, G, kUnit, false, kWeights>(st, rows, me, ring + slot * UB, first);
                 done();
             }
             if (i >= n || !wait()) break;
 #pragma unroll
             for (int u = 0; u < kUnit; ++u)
                 first[u] = f_bad >> (kUnit * slot + u) & 1u ? INT32_MAX - kUnitTokens : (unit0 + i) * kUnitTokens + u * kBlockTokens;
-            blocks<D, G, NT, kUnit, true, kWeights>(st, rows, me, ring + slot * UB, first);
+            blocks<D, G, kUnit, true, kWeights>(st, rows, me, ring + slot * UB, first);
             done();
         }
         // the next segment's rows are on their way while the warps join
@@ -808,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
                 if (b >= a.batch) late = true;
             }
             if (late) f = range;
-            else load_rows<T, D, NT, kWeights>(raw, a, rq, head, tile);
+            else load_rows<T, D, kWeights>(raw, a, rq, head, tile);
         }
         float* part = kPairs ? s_part : a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
         if (!kPairs && starts && !ends && threadIdx.x == 0) {
@@ -1019,17 +1026,11 @@ int grid_ctas() { return kCtasPerSm * ecq_dev::sm_count_cached(); }
 // kernel the same wherever it is, the prompt kernel works by 256 rows of a pair
 // on one SM: many pairs fill the GPU with those, few do not. Measured (us,
 // stream / prompt kernel, shared by 4): 128 pairs of 4096 tokens 32 rows
-// 77 / 85, 48 rows 108 / 86; 32 pairs of 8192 96 rows 103 / 146; 8 pairs of
-// 65536 256 rows 456 / 1139: they meet at about 4500 rows of all pairs.
+// 79 / 85; 32 pairs of 8192 96 rows 106 / 146; 8 pairs of 65536 256 rows
+// 481 / 1139: they meet at about 4500 rows of all pairs.
 int stream_rows(int batch, int kv_heads) {
     const int64_t rows = 4500 / (static_cast<int64_t>(batch) * kv_heads);
     return rows > 32 ? static_cast<int>(rows) : 32;
-}
-
-// 16-row tiles (one pass over the keys for twice the rows) where 8-row tiles would be even in number: 128 pairs of 4096 tokens,
-// 16 rows 49 against 54 us, 32 rows 77 against 89, but 24 rows 77 against 71.
-int row_tiles_of_8(int share, int max_q) {
-    return (static_cast<int64_t>(share) * max_q + 7) / 8 % 2 == 0 ? 2 : 1;
 }
 
 // CTAs of a cluster for each (request, head, tile); 0: ranges instead. Ranges
@@ -1043,7 +1044,6 @@ constexpr int kMostTokens = 192;  // per warp
 struct Plan {
     int most_rows;  // of a request that is streamed
     bool prompts;   // some may have more
-    int nt;         // 8-row tiles as one
     int rows;       // of a tile
     int tiles;      // of a streamed request at most
     int ranks;      // CTAs of a cluster; 0: ranges
@@ -1054,8 +1054,7 @@ Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page
     p.most_rows = stream_rows(batch, kv_heads);
     p.prompts = rows > p.most_rows;
     if (!p.prompts) p.most_rows = INT32_MAX;
-    p.nt = row_tiles_of_8(share, max_q);
-    p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8 * p.nt;
+    p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8 * NT;
     p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.tiles;
     p.ranks = kMostRanks;
@@ -1064,24 +1063,24 @@ Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page
     return p;
 }
 
-template <typename L, int NT, int W>
+template <typename L, int W>
 int32_t launch(const Args& a, const Plan& plan, cudaStream_t stream) {
     using T = typename L::T;
-    constexpr int kUnit = unit_blocks(L::G, NT), UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = tile_rows<NT, W>() * (L::D + 4) * 4;
+    constexpr int kUnit = unit_blocks(L::G), UB = kUnit * block_bytes(L::D, L::G), join = kWarps * 8 * (L::D + 4) * 4, part = tile_rows<W>() * (L::D + 4) * 4;
     if (plan.ranks) {
         constexpr int smem = kWarps * ring_slots(L::D, L::G, kUnit, part) * UB + join + part;
-        const auto kernel = attention_kernel<T, L::D, L::G, NT, true, W>;
+        const auto kernel = attention_kernel<T, L::D, L::G, true, W>;
         if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
         const unsigned ctas = static_cast<unsigned>(a.batch * a.kv_heads * plan.tiles * plan.ranks);
         return result(
             ecq_dev::launch_pdl_cluster(kernel, dim3(ctas), dim3(kThreads), smem, stream, plan.ranks, a, plan.tiles));
     }
     constexpr int smem = kWarps * ring_slots(L::D, L::G, kUnit, 0) * UB + join;
-    const auto kernel = attention_kernel<T, L::D, L::G, NT, false, W>;
+    const auto kernel = attention_kernel<T, L::D, L::G, false, W>;
     if (!ecq_dev::ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem)) return ECQ_ERR_CUDA;
     const dim3 grid(grid_ctas());
     cudaError_t rc = launch_pdl(kernel, grid, dim3(kThreads), smem, stream, a, 0);
-    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, tile_rows<NT, W>()>, grid, dim3(kJoinWarps * 32), 0, stream, a);
+    if (rc == cudaSuccess) rc = launch_pdl(join_kernel<T, L::D, tile_rows<W>()>, grid, dim3(kJoinWarps * 32), 0, stream, a);
     return result(rc);
 }
 
@@ -1096,7 +1095,7 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
     // the same clusters or ranges for both types: tiles of 4 rows are taken where there is one tile of 8
     const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size, ECQ_KV4_BF16);
-    return p.ranks ? 0 : grid_ctas() * (16 + 2 * 4 * 8ll * p.nt * (head_dim + 2));
+    return p.ranks ? 0 : grid_ctas() * (16 + 2 * 4 * 8ll * NT * (head_dim + 2));
 }
 
 int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -1152,10 +1151,9 @@ int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_
         using L = decltype(layout);
         const auto st = static_cast<cudaStream_t>(stream);
         if constexpr (std::is_same<typename L::T, __half>::value) {
-            if (p.rows == 4) return launch<L, 1, kFolded>(a, p, st);
-            return p.nt == 2 ? launch<L, 2, kTwice>(a, p, st) : launch<L, 1, kTwice>(a, p, st);
+            return p.rows == 4 ? launch<L, kFolded>(a, p, st) : launch<L, kTwice>(a, p, st);
         } else {
-            return p.nt == 2 ? launch<L, 2, kOnce>(a, p, st) : launch<L, 1, kOnce>(a, p, st);
+            return launch<L, kOnce>(a, p, st);
         }
     });
 }
