@@ -102,7 +102,9 @@ int32_t ecq_kv4_gather(void *k, void *v, int32_t dtype, const void *pages, int64
  * contiguous, q 16-byte aligned with strides that are multiples of 8, out
  * 8-byte aligned with multiples of 4. heads / kv_heads is at most 64. A page
  * number outside the pool, or a length beyond the table's row, sets
- * ECQ_STATUS_BADARG and its keys are left out. workspace:
+ * ECQ_STATUS_BADARG and its keys are left out. The same status says that a
+ * request had more than max_q queries and some of its rows were not written.
+ * workspace:
  * ecq_kv4_attention_workspace_bytes, its content does not matter; calls that
  * may overlap need one each. */
 int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
