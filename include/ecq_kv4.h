@@ -27,7 +27,9 @@
  * Stored values: x is clamped to +-65504; zero = fp16(min of the group), scale
  * = fp16((max - min) / 15), code = (x - zero) / scale rounded to nearest even
  * and clamped to 0..15 (0 where scale is 0). A NaN makes its group's scale and
- * zero NaN.
+ * zero NaN. The scale may be rounded up, so that code 15 stands for a little more
+ * than the group's maximum, 65584 at most: read back in fp16 a value of 65520 or
+ * more is infinite.
  */
 #ifndef ECQ_KV4_H
 #define ECQ_KV4_H
@@ -104,6 +106,9 @@ int32_t ecq_kv4_gather(void *k, void *v, int32_t dtype, const void *pages, int64
  * number outside the pool, or a length beyond the table's row, sets
  * ECQ_STATUS_BADARG and its keys are left out. The same status says that a
  * request had more than max_q queries and some of its rows were not written.
+ * Requests with many rows take values of up to +-131008, twice fp16's end and more
+ * than ecq_kv4_append stores: where a pool's bytes stand for more, queries that
+ * see the token get infinities or NaN.
  * workspace:
  * ecq_kv4_attention_workspace_bytes, its content does not matter; calls that
  * may overlap need one each. */
