@@ -71,9 +71,12 @@ constexpr int NT = 1;
 // need no reduction over their tokens. The lift keeps the weights of keys far
 // below the largest (most of a long context) out of fp16's subnormals, whose
 // step of 2^-24 would be felt in sums of thousands of them. weight * scale
-// then overflows fp16 from a scale of 16: that is seen (kDrop).
+// then overflows fp16 from a scale of 16: that is seen, and the unit's weights go
+// in times 2^-13 (any finite scale's product is finite then; weights are at
+// least 2^-24 of the largest that they can be) and its part of o comes out times
+// 2^13. The reference stays: one that moved by less than its own rounding would
+// not be the one that the earlier sums were divided by.
 constexpr float kSlack = 2.f, kLift = 10.f;
-constexpr float kDrop = 10.f;  // the reference goes up by so much where weight * scale is infinite
 constexpr float kNoMax = -1e30f;
 constexpr int kMostRanks = 8;  // CTAs that share a pair
 
@@ -131,11 +134,12 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void add4(float (&o)[4], const float (&t)[4]) {
+// o += t up
+__device__ __forceinline__ void add4(float (&o)[4], const float (&t)[4], uint64_t up) {
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-        const uint64_t x = ecq_dev::add2(ecq_dev::pack2(__float_as_uint(o[i]), __float_as_uint(o[i + 1])),
-                                         ecq_dev::pack2(__float_as_uint(t[i]), __float_as_uint(t[i + 1])));
+        const uint64_t x = ecq_dev::fma2(ecq_dev::pack2(__float_as_uint(t[i]), __float_as_uint(t[i + 1])), up,
+                                         ecq_dev::pack2(__float_as_uint(o[i]), __float_as_uint(o[i + 1])));
         ecq_dev::unpack2(x, o[i], o[i + 1]);
     }
 }
@@ -335,6 +339,10 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t abs2(uint32_t a) {
+    const __half2 r = __habs2(*reinterpret_cast<const __half2*>(&a));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t neg2(uint32_t a) {
     const __half2 r = __hneg2(*reinterpret_cast<const __half2*>(&a));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -421,9 +429,11 @@ __device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, cons
             }
         }
     }
-    uint32_t hi[U][NT][G][2], lo[U][NT][G][2];
-    for (int drops = 0;; ++drops) {
-        uint32_t ph[U][NT][2], pl[U][NT][2], most = 0u;
+    uint32_t ph[U][NT][2], pl[U][NT][2], hi[U][NT][G][2], lo[U][NT][G][2];
+    // the weights and their products with V's scales, those of kDown times 2^-13; the largest of them
+    auto weights = [&](auto down) {
+        constexpr bool kDown = decltype(down)::value;
+        uint32_t most = 0u;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -451,9 +461,10 @@ __device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, cons
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
-                        const uint32_t w = ph[u][nt][i];
-                        uint32_t h = mul2(w, sc);
-                        uint32_t l = kWeights != kOnce ? fma2h(pl[u][nt][i], sc, fma2h(w, sc, neg2(h))) : 0u;
+                        constexpr uint32_t kScale = 0x08000800u;  // 2^-13
+                        const uint32_t w = kDown ? mul2(ph[u][nt][i], kScale) : ph[u][nt][i];
+                        uint32_t h = mul2(w, sc), l = 0u;
+                        if (kWeights != kOnce) l = fma2h(kDown ? mul2(pl[u][nt][i], kScale) : pl[u][nt][i], sc, fma2h(w, sc, neg2(h)));
                         if (kMask) {  // weight 0: 0, whatever the scale is
                             const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
                             h &= keep;
@@ -461,58 +472,49 @@ __device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, cons
                         }
                         hi[u][nt][g][i] = kWeights == kFolded && r >= 4 ? l : h;
                         lo[u][nt][g][i] = l;
-                        most = max2(most, h);  // not negative, and a NaN passes by
+                        most = max2(most, abs2(h));  // a NaN passes by
                     }
                 }
         }
-        // two drops bring any finite scale's product below fp16's end; a scale that is infinite stays so
-        if (drops == 2 || !__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
-            // rows of A: the groups' zeros, then ones (the sum of the weights)
-            float sums[NT][4];
+        return most;
+    };
+    const uint32_t most = weights(std::false_type());
+    uint64_t up = 0x3f8000003f800000ull;
+    if (__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
+        weights(std::true_type());
+        up = 0x4600000046000000ull;  // 2^13
+    }
+    // rows of A: the groups' zeros, then ones (the sum of the weights)
+    float sums[NT][4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint32_t za[2][1], zb[2][1], z[2];
-                lds<1, 0>(za[0], at + u * BB + me.v_pair);
-                lds<1, 16 * G>(zb[0], at + u * BB + me.v_pair);
-                lds<1, 32 * G>(za[1], at + u * BB + me.v_pair);
-                lds<1, 48 * G>(zb[1], at + u * BB + me.v_pair);
+    for (int u = 0; u < U; ++u) {
+        uint32_t za[2][1], zb[2][1], z[2];
+        lds<1, 0>(za[0], at + u * BB + me.v_pair);
+        lds<1, 16 * G>(zb[0], at + u * BB + me.v_pair);
+        lds<1, 32 * G>(za[1], at + u * BB + me.v_pair);
+        lds<1, 48 * G>(zb[1], at + u * BB + me.v_pair);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    z[i] = __byte_perm(za[i][0], zb[i][0], 0x7632);
-                    if (kMask) {  // where a zero is not finite its scale is not either, and that reaches the rows that see the token
-                        if ((z[i] & 0x7c00u) == 0x7c00u) z[i] &= 0xffff0000u;
-                        if ((z[i] & 0x7c000000u) == 0x7c000000u) z[i] &= 0xffffu;
-                    }
-                    z[i] = r == G ? 0x3c003c00u : z[i];
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const bool rest = kWeights == kFolded && r >= 4;
-                    const uint32_t p0 = rest ? pl[u][nt][0] : ph[u][nt][0], p1 = rest ? pl[u][nt][1] : ph[u][nt][1];
-                    if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
-                    else mma(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
-                    if (kWeights == kTwice) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
-                }
+        for (int i = 0; i < 2; ++i) {
+            z[i] = __byte_perm(za[i][0], zb[i][0], 0x7632);
+            if (kMask) {  // where a zero is not finite its scale is not either, and that reaches the rows that see the token
+                if ((z[i] & 0x7c00u) == 0x7c00u) z[i] &= 0xffff0000u;
+                if ((z[i] & 0x7c000000u) == 0x7c000000u) z[i] &= 0xffffu;
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                S.sums[nt][0] += sums[nt][0];
-                S.sums[nt][1] += sums[nt][1];
-            }
-            break;
+            z[i] = r == G ? 0x3c003c00u : z[i];
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            const bool rest = kWeights == kFolded && r >= 4;
+            const uint32_t p0 = rest ? pl[u][nt][0] : ph[u][nt][0], p1 = rest ? pl[u][nt][1] : ph[u][nt][1];
+            if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
+            else mma(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
+            if (kWeights == kTwice) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
+        }
+    }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                S.m[nt][c] += kDrop;
-                S.sums[nt][c] *= 0.0009765625f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    S.o[nt][i][c] *= 0.0009765625f;
-                    S.o[nt][i][c + 2] *= 0.0009765625f;
-                }
-            }
+    for (int nt = 0; nt < NT; ++nt) {
+        S.sums[nt][0] += sums[nt][0];
+        S.sums[nt][1] += sums[nt][1];
     }
     // The unit's part of o starts from 0 and is added with a rounded fp32 sum: codes are 0..15 and the zeros take about 7.5
     // of that away again, so what a running sum loses to the tensor core's truncation would be many times as much in o.
@@ -552,7 +554,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, cons
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) add4(S.o[nt][4 * w + 2 * half + j], t[j][nt]);
+                for (int nt = 0; nt < NT; ++nt) add4(S.o[nt][4 * w + 2 * half + j], t[j][nt], up);
         }
 }
 

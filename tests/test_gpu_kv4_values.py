@@ -85,3 +85,34 @@ def test_bytes_far_past_the_end_of_fp16_stay_with_the_rows_that_see_them():
         assert torch.equal(got[:first], want[:first])
         if v:
             assert bool(got[first:, :, :32].isnan().all()) and torch.equal(got[first:, :, 32:], want[first:, :, 32:])
+
+
+# -- weights times scales past fp16's end ---------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,g", LAYOUTS)
+@pytest.mark.parametrize("share", [1, 4, 9])
+@pytest.mark.parametrize("score", [1.0, 2.0 ** 20, 2.0 ** 25])
+def test_large_values_after_small_ones(dtype, dim, g, share, score):
+    """One key for all tokens, so the mean of the values, of which every other
+    256 tokens' are large: a warp's sums of small ones meet weights that their
+    scales carry out of fp16, at references of which 10 is less than a step."""
+    heads, n, page = 32, 2500, 64
+    k = torch.ones(n, heads, dim, device="cuda")
+    big = (torch.arange(n, device="cuda") // 256 % 2 == 1)[:, None, None]
+    v = torch.where(big, 20000.0, 2000.0) * randn(n, heads, dim, seed=dim)
+    if dtype == torch.float16:
+        k *= max(1.0, score / 1024)
+    pages, table = store(k.to(dtype), v.clamp(-60000, 60000).to(dtype), page, g)
+    wide = torch.full((1, 2000), -1, dtype=torch.int32, device="cuda")  # room for far more: ranges
+    wide[:, :table.shape[1]] = table
+    q = torch.full((1, heads * share, dim), (score if dtype == torch.bfloat16 else min(score, 1024.0)) * 1.3125 / dim ** 0.5, device="cuda").to(dtype)
+    value = torch.from_numpy(decode(pages, dim, g)[1][1]).cuda()[:n]
+    want = value.mean(0).repeat_interleave(share, 0)[None]
+    # equal weights stay equal. A weight's product with a scale is rounded to fp16, once for bf16: 2^-11 of what it adds,
+    # evenly and independently: codes times scales of at most twice the largest value, over n tokens (six times the root mean
+    # square). fp32 sums of n such terms: 2^-24 sqrt(n) of the largest
+    tol = want.abs() * torch.finfo(dtype).eps / 2 + (6 * 2.0 ** -11 / 3 ** 0.5 * n ** -0.5 + 2.0 ** -24 * n ** 0.5) * 2 * value.abs().max()
+    for tb in (wide, table):
+        got = ecq.kv4_attention(q, pages, tb, i32([n]), group_size=g)
+        assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
