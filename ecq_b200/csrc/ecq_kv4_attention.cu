@@ -77,7 +77,6 @@ constexpr int NT = 1;
 // 2^13. The reference stays: one that moved by less than its own rounding would
 // not be the one that the earlier sums were divided by.
 constexpr float kSlack = 2.f, kLift = 10.f;
-constexpr float kNoMax = -1e30f;
 constexpr int kMostRanks = 8;  // CTAs that share a pair
 
 // How the weights are held: once, twice, or twice in the columns of a row.
@@ -189,7 +188,8 @@ template <int D, int G>
 struct Rows {
     uint32_t b[NT][D / 16][2];
     uint32_t sums[NT][2];  // B operand that takes (scale, zero) pairs: (0, sum of the group's q), high and low part
-    float factor[NT][2];   // scale log2(e) 2^24 / the row's power of two
+    float factor[NT][2];   // scale log2(e) 2^24 / the row's power of two, less where scores are huge (raise_far)
+    uint32_t own;          // where that is in shared memory as it was
     int limit[NT][2];      // keys that the column's row sees
     int least;             // the smallest limit of rows that exist
 };
@@ -214,7 +214,7 @@ __device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& 
 
 template <typename T, int D, int G, int W>
 __device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
-                                         const Request& rq, int tile) {
+                                         const Request& rq, int tile, float (*own)[2]) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
     R.least = rq.len;
 #pragma unroll
@@ -284,7 +284,10 @@ __device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D
             R.factor[nt][c] = __shfl_sync(0xffffffffu, factor, from);
             R.limit[nt][c] = __shfl_sync(0xffffffffu, limit, from);
         }
+        if (n == 0) own[nt * 4 + t][0] = R.factor[nt][0], own[nt * 4 + t][1] = R.factor[nt][1];
     }
+    R.own = smem_addr(own) + 8 * t;
+    __syncwarp();
 }
 
 // Running softmax of one warp over its blocks.
@@ -293,7 +296,9 @@ struct State {
     float o[NT][D / 16][4];
     float sums[NT][2];  // columns 2t, 2t + 1; lanes of row r < G: sum p zero of group r; of row G: sum p
     float m[NT][2];
+    bool far;  // some row's factor has gone down
     __device__ __forceinline__ void reset() {
+        far = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -351,7 +356,7 @@ __device__ __forceinline__ uint32_t neg2(uint32_t a) {
 // A unit's blocks at shared address at; first[u]: the request's token that
 // block u starts with (used with kMask; beyond all limits: leave it out).
 template <int D, int G, int U, bool kMask, int kWeights>
-__device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, const Lane<D, G>& me, uint32_t at,
+__device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane<D, G>& me, uint32_t at,
                                        const int (&first)[U]) {
     constexpr int W = D / 32, BB = block_bytes(D, G);
     const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
@@ -410,16 +415,30 @@ __device__ __forceinline__ void blocks(State<D, G>& S, const Rows<D, G>& R, cons
             top[c] = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
             for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][nt][c], s[u][nt][c + 2]));
-            top[c] *= R.factor[nt][c];
         }
-        if (__any_sync(0xffffffffu, top[0] > S.m[nt][0] + (kSlack + kLift) || top[1] > S.m[nt][1] + (kSlack + kLift))) {
+        if (__any_sync(0xffffffffu, fmaf(top[0], R.factor[nt][0], -S.m[nt][0]) > kSlack + kLift ||
+                                        fmaf(top[1], R.factor[nt][1], -S.m[nt][1]) > kSlack + kLift)) {
+            float held[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float x = fmaxf(top[c] - kLift, S.m[nt][c]);
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                const float keep = exp2_fast(S.m[nt][c] - x);
-                S.m[nt][c] = x;
+                for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+                held[c] = S.m[nt][c];
+                S.m[nt][c] = fmaxf(fmaf(top[c], R.factor[nt][c], -kLift), held[c]);
+            }
+            if (S.far || __any_sync(0xffffffffu, fmaxf(fabsf(S.m[nt][0]), fabsf(S.m[nt][1])) > kNear)) {
+                uint32_t own[2];
+                lds<2, 0>(own, R.own + 32 * nt);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (S.m[nt][c] > held[c])
+                        raise_far(S.m[nt][c], held[c], R.factor[nt][c], top[c], __uint_as_float(own[c]), kLift);
+                S.far = S.far || __any_sync(0xffffffffu, R.factor[nt][0] != __uint_as_float(own[0]) ||
+                                                             R.factor[nt][1] != __uint_as_float(own[1]));
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float keep = exp2_fast(held[c] - S.m[nt][c]);
                 S.sums[nt][c] *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
@@ -573,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
     __shared__ Request s_own;
     __shared__ uint64_t s_bar[kWarps][NS];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
+    __shared__ __align__(8) float s_factor[kWarps][NT * 4][2];  // the rows' factors
     float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * UB);
     float* s_part = s_o + kWarps * 8 * OS;  // kPairs: this CTA's part of the pair
     const int lane = threadIdx.x & 31, cta = blockIdx.x;
@@ -757,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
 #pragma unroll 1
     for (long long f = 0; f < range;) {
         const int n = static_cast<int>(min(static_cast<long long>(rq.units - unit0), range - f));
-        set_rows<T, D, G, kWeights>(rows, raw, a, rq, tile);
+        set_rows<T, D, G, kWeights>(rows, raw, a, rq, tile, s_factor[warp]);
         st.reset();
         // this warp's first unit in [f, f + n)
         int i = kPairs ? mine : (warp - static_cast<int>(f % kWarps) + kWarps) % kWarps;
@@ -835,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
                 float z[G];
 #pragma unroll
                 for (int g = 0; g < G; ++g) z[g] = __shfl_sync(0xffffffffu, st.sums[nt][c], 4 * g + t);
-                if (r == 0) s_m[warp][2 * t + c] = st.m[nt][c];
+                if (r == 0) s_m[warp][2 * t + c] = st.far ? reference(st.m[nt][c], rows.factor[nt][c], s_factor[warp][nt * 4 + t][c]) : st.m[nt][c];
                 if (r == G) s_l[warp][2 * t + c] = st.sums[nt][c];
                 float* dst = s_o + (warp * 8 + 2 * t + c) * OS + r;
 #pragma unroll

@@ -3,6 +3,8 @@
 // launch of the one for prompts.
 #pragma once
 
+#include <float.h>
+
 #include "ecq_kv4.cuh"
 
 namespace ecq_kv4 {
@@ -48,6 +50,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// A row's weights are exp2(score * factor - m), where the reference m is `lift` below the row's largest product. The
+// products are exact and m is a float: from 2^27 on m's rounding would carry weights out of fp16, or all of them to 0. So
+// rows with such products have a factor that is less by a power of two than their own, and a lift of kFarLift,
+// with which m is exact: what fp32 tells apart is then still 4 and more apart, and that is less than its error.
+constexpr float kFarLift = 8.f;
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ int power_of(float x) { return (__float_as_int(x) >> 23 & 255) - 127; }
+
+constexpr float kNoMax = -FLT_MAX;       // m of a row without scores: below them all
+constexpr float kNear = 33554432.f;      // 2^25: m of rows with less is what the plain form makes it
+
+// Raising m for a new largest score, top: m = max(top factor - lift, held), and exp2(held - m) is what earlier weights are
+// to be multiplied by. This puts that right for a row that is raised where the new m is beyond kNear, or the factor has gone
+// down already.
+__device__ __forceinline__ void raise_far(float& m, float& held, float& factor, float top, float own, float lift) {
+    const float held_lift = factor == own ? lift : kFarLift;
+    const int over = max(power_of(top * own) - 26, 0);
+    const float f = own * power2(-over);
+    held = (held + held_lift) * power2(power_of(f) - power_of(factor)) - held_lift;
+    m = fmaf(top, f, over ? -kFarLift : -lift);
+    factor = f;
+}
+// m as it compares with those of other parts of the row, whose factors may differ.
+__device__ __forceinline__ float reference(float m, float factor, float own) {
+    return factor == own ? m : (m + kFarLift) * power2(power_of(own) - power_of(factor));
 }
 __device__ __forceinline__ uint32_t h2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);

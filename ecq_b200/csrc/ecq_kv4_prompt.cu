@@ -70,7 +70,6 @@ constexpr uint32_t kTmemColumns = 512;
 // P is exp2(score - reference + kLift), at most 2^15; the lift keeps the weights of keys far below the largest out of
 // fp16's subnormals
 constexpr float kSlack = 8.f, kLift = 7.f;
-constexpr float kNoMax = -1e30f;
 
 template <int D, int G>
 struct Smem {
@@ -395,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             if (lane == 0) mbar_arrive(bars + offsetof(Control, rows) + 8 * x);
             wait(bars + offsetof(Control, rows) + 8 * x, 0);
         }
-        const float factor = *reinterpret_cast<volatile float*>(&ctl.factor[here]);
+        float factor = *reinterpret_cast<volatile float*>(&ctl.factor[here]);
         if (x == 0 && ok) {  // this thread's half of the row's channels to tensor memory
 #pragma unroll
             for (int part = 0; part < D / 64; ++part) {
@@ -414,7 +413,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         }
         float m = kNoMax;
         uint64_t l[2] = {0ull, 0ull};  // two pairs of sums
-        const uint64_t f2x = ecq_dev::pack2(__float_as_uint(factor), __float_as_uint(factor));
         const uint32_t pair = (bars + offsetof(Control, pair) + 8 * (x * 4 + (warp & 3)));
         int j = 0;
 #pragma unroll 1
@@ -438,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             for (int k = 0; k < 4; ++k) t[k] = __uint_as_float(s[k]);
 #pragma unroll
             for (int k = 4; k < kHalf; ++k) t[k & 3] = fmaxf(t[k & 3], __uint_as_float(s[k]));
-            float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * factor;
+            float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
             volatile float* tops = &ctl.top[j & 1][0][0];
             tops[h * 2 * kRows + here] = top;
             __syncwarp();
@@ -446,9 +444,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             if (!wait(pair, j & 1)) break;
             top = fmaxf(top, tops[(h ^ 1) * 2 * kRows + here]);
             bool emptied = j == 0;  // P and O are not in use by the last step's product
-            if (__any_sync(0xffffffffu, top > m + (kSlack + kLift))) {
-                const float next = fmaxf(top - kLift, m), keep = exp2_fast(m - next);
-                m = next;
+            if (__any_sync(0xffffffffu, fmaf(top, factor, -m) > kSlack + kLift)) {
+                float held = m;
+                m = fmaxf(fmaf(top, factor, -kLift), held);
+                const bool far = (fabsf(m) > kNear && m != kNoMax) || (fabsf(held) > kNear && held != kNoMax);
+                if (__any_sync(0xffffffffu, far) && m > held)
+                    raise_far(m, held, factor, top, *reinterpret_cast<volatile float*>(&ctl.factor[here]), kLift);
+                const float keep = exp2_fast(held - m);
                 const uint64_t k2 = ecq_dev::pack2(__float_as_uint(keep), __float_as_uint(keep));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) l[u] = ecq_dev::fma2(l[u], k2, 0ull);
@@ -467,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                     }
                 }
             }
+            const uint64_t f2x = ecq_dev::pack2(__float_as_uint(factor), __float_as_uint(factor));
             const uint64_t m2 = ecq_dev::pack2(__float_as_uint(-m), __float_as_uint(-m));
 #pragma unroll
             for (int k = 0; k < kHalf; k += 2) {

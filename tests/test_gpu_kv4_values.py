@@ -116,3 +116,93 @@ def test_large_values_after_small_ones(dtype, dim, g, share, score):
     for tb in (wide, table):
         got = ecq.kv4_attention(q, pages, tb, i32([n]), group_size=g)
         assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+
+
+# -- scores of any size -------------------------------------------------------------
+
+FORMS = [(1, 4, 1, 1), (1, 4, 1, 5000), (2, 9, 3, 1), (64, 2, 60, 1)]  # heads, share, queries, room in the table: streamed (clusters, ranges, two tiles), prompt
+
+
+def one_hot(heads, share, new, room, dtype, dim, exponents, sign, seed):
+    """Queries of one direction and many sizes, keys of which token 5 is the
+    best by far: each output is that token's value."""
+    n, g, page = 100, 32, 16
+    way = torch.randint(1, 9, (dim,), generator=torch.Generator().manual_seed(seed)).cuda().float()
+    k, v = randn(n, heads, dim, seed=seed).abs() + 1, randn(n, heads, dim, seed=seed + 1)
+    k[5] = 8.0 if sign > 0 else 0.125
+    pages, table = store(k.to(dtype), v.to(dtype), page, g)
+    wide = torch.full((1, max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    rows = new * heads * share
+    size = sign * 2.0 ** torch.tensor([exponents[i % len(exponents)] for i in range(rows)], dtype=torch.float64, device="cuda")
+    q = (size[:, None] * way.double()).view(new, heads * share, dim).to(dtype)
+    assert bool(q.isfinite().all())
+    got = ecq.kv4_attention(q, pages, wide, i32([n]), i32([0, new]), new, group_size=g)
+    want = torch.from_numpy(decode(pages, dim, g)[1][1]).cuda()[5].repeat_interleave(share, 0).expand(new, -1, -1)
+    # the other keys' weights are 0 in float64 too. V and the weight are rounded to fp16 at most, or the weight times V's
+    # scale, which a code of up to 15 makes 2^-11 of the group's range, twice the largest value; then the output.
+    err = (got.double() - want).abs()
+    assert bool((err <= want.abs() * torch.finfo(dtype).eps / 2 + 3 * 2.0 ** -11 * want.abs().max()).all()), float(err.max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype,exponents", [(torch.float16, (6, 9, 12)), (torch.bfloat16, (16, 18, 20, 21)), (torch.bfloat16, (30, 60, 80, 90)), (torch.bfloat16, (96, 99, 102))])
+def test_scores_that_fp32_cannot_tell_from_their_neighbours(dim, form, dtype, exponents):
+    one_hot(*form, dtype, dim, exponents, 1.0, 7)
+    one_hot(*form, dtype, dim, exponents, -1.0, 9)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("exponent", range(0, 29, 2))
+def test_large_scores_that_are_equal(form, dtype, exponent):
+    """One key for all tokens: the mean of the values that a query sees, however
+    large the score (2^exponent times 16 to 30) is."""
+    heads, share, new, room = form
+    n, dim, g, page = 90, 64, 32, 16
+    k = torch.ones(n, heads, dim, device="cuda")
+    if dtype == torch.float16:
+        k *= 2.0 ** max(0, exponent - 13)
+        exponent = min(exponent, 13)
+    pages, table = store(k.to(dtype), randn(n, heads, dim, seed=exponent).to(dtype), page, g)
+    wide = torch.full((1, max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    # odd multiples, so that the products with log2(e) are none that fp32 holds exactly
+    q = (2.0 ** exponent * (16 + torch.arange(new * heads * share, device="cuda") % 15)[:, None].expand(-1, dim) / 8).view(new, heads * share, dim).to(dtype)
+    got = ecq.kv4_attention(q, pages, wide, i32([n]), i32([0, new]), new, group_size=g)
+    v = torch.from_numpy(decode(pages, dim, g)[1][1]).cuda()[:n]
+    mean = v.cumsum(0)[n - new:] / torch.arange(n - new + 1, n + 1, device="cuda")[:, None, None]
+    want = mean.repeat_interleave(share, 1)
+    # equal weights in fp16 are equal; V (and V's scale times a weight) is off by 2^-11 of the largest, and the output is rounded
+    tol = want.abs() * torch.finfo(dtype).eps / 2 + 3 * 2.0 ** -11 * v.abs().max()
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("first", [0, 70])
+def test_moderate_scores_beside_huge_negative_ones(form, dtype, first):
+    # tokens from `first` on, 20 of them, are out of reach; the others' softmax is as without them
+    heads, share, new, room = form
+    n, dim, g, page = 150, 64, 32, 16
+    k, v = randn(n, heads, dim, seed=1), randn(n, heads, dim, seed=2)
+    k[:, :, 0] = 0.0
+    k[first:first + 20, :, 0] = -60000.0
+    pages, table = store(k.to(dtype), v.to(dtype), page, g)
+    wide = torch.full((1, max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = randn(new, heads * share, dim, seed=3)
+    q[..., 0] = 2000.0
+    q = q.to(dtype)
+    got = ecq.kv4_attention(q, pages, wide, i32([n]), i32([0, new]), new, group_size=g)
+    (_, kk), (_, vv) = decode(pages, dim, g)
+    seen = torch.arange(n, device="cuda") <= n - new + torch.arange(new, device="cuda")[:, None]
+    seen &= (torch.arange(n, device="cuda") < first) | (torch.arange(n, device="cuda") >= first + 20)
+    kk, vv = (torch.from_numpy(x[:n]).cuda().repeat_interleave(share, 1) for x in (kk, vv))
+    s = torch.einsum("ihd,jhd->hij", q.double(), kk) * dim ** -0.5
+    want = torch.einsum("hij,jhd->ihd", torch.softmax(s.masked_fill(~seen, -float("inf")), -1), vv)
+    # The other channels' |q| |k| come to under 128, over 8: with K off by 2^-11 of itself a score is off by 16 2^-11 and an
+    # output by twice that of |v|; V and weights (codes times scales: twice the largest |v|) are off by 2^-11 each.
+    tol = want.abs() * torch.finfo(dtype).eps / 2 + (2 * 16 + 4) * 2.0 ** -11 * vv.abs().max()
+    assert bool(((got.double() - want).abs() <= tol).all())
