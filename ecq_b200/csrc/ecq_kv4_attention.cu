@@ -240,7 +240,11 @@ __device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D
         // their bits in fp16. A negative scale turns the row's sign; with none every score is 0.
         const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
         float up = __int_as_float((14 - ex + 127) << 23);
+        // the products reach 2^14 (128 channels of 65504 times 2^15, times 2^-24): a factor of up to 2^112 keeps scores
+        // finite. What a larger one would tell apart (nonzero differences of products are 2^-72 and more) this one does.
+        constexpr float kMostFactor = 5.192296858534828e33f;
         float factor = fabsf(a.scale) * 1.4426950408889634f * (__int_as_float((ex - 14 + 127) << 23) * 16777216.f);
+        if (factor > kMostFactor) factor = kMostFactor;
         if (a.scale < 0.f) up = -up;
         if (factor == 0.f) {
             up = 0.f;

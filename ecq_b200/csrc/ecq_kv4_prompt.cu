@@ -376,6 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                 const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
                 float up = __int_as_float((10 - ex + 127) << 23);
                 float f = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 9 + 127) << 23);  // K is halved
+                // the products reach 2^34 (128 channels of 65504 times 2^11): a factor of up to 2^93 keeps scores
+                // finite, and tells apart all that a larger one would (nonzero differences are 2^-48 and more)
+                constexpr float kMostFactor = 9.903520314283042e27f;
+                if (f > kMostFactor) f = kMostFactor;
                 if (a.scale < 0.f) up = -up;
                 if (f == 0.f) {
                     up = 0.f;

@@ -206,3 +206,10 @@ def test_moderate_scores_beside_huge_negative_ones(form, dtype, first):
     # output by twice that of |v|; V and weights (codes times scales: twice the largest |v|) are off by 2^-11 each.
     tol = want.abs() * torch.finfo(dtype).eps / 2 + (2 * 16 + 4) * 2.0 ** -11 * vv.abs().max()
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_queries_of_any_size(dim, form, sign):
+    one_hot(*form, torch.bfloat16, dim, [124, 122, 119, 116, 114, 110, 104, 100, 95, 60, 20], sign, 7)
