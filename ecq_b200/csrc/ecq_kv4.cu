@@ -130,17 +130,19 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     bad = __syncthreads_or(bad || sum.tokens > max_tokens);
     const bool dry = !bad && pages_sum > count;
     ecq_dev::cluster_sync();
-    const int tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads;
+    // unsigned: the counts are below 2^31, so an index that has gone past its end by a stride is below 2^32
+    const unsigned tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads;
+    const unsigned n = batch, most = max_tokens;
     if (bad || dry) {
         if (tid == 0) {
             raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
             *count_out = count;
         }
-        for (int b = tid; b <= batch; b += threads) {
+        for (unsigned b = tid; b <= n; b += threads) {
             q_starts[b] = 0;
-            if (b < batch) lens_out[b] = s_len[b];
+            if (b < n) lens_out[b] = s_len[b];
         }
-        for (int i = tid; i < max_tokens; i += threads) {
+        for (unsigned i = tid; i < most; i += threads) {
             slots[i] = -1;
             positions[i] = -1;
         }
@@ -148,25 +150,26 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     }
     const int total = static_cast<int>(sum.tokens), pages = static_cast<int>(pages_sum);
     if (tid == 0) *count_out = count - pages;
-    for (int b = tid; b <= batch; b += threads) {
-        const int start = b < batch ? s_tok[b] : total;
+    for (unsigned b = tid; b <= n; b += threads) {
+        const int start = b < n ? s_tok[b] : total;
         q_starts[b] = start;
-        if (b < batch) lens_out[b] = s_len[b] + ((b + 1 < batch ? s_tok[b + 1] : total) - start);
+        if (b < n) lens_out[b] = s_len[b] + ((b + 1 < n ? s_tok[b + 1] : total) - start);
     }
-    for (int j = tid; j < pages; j += threads) {
-        const int b = owner(s_page, batch, j);
+    for (unsigned j0 = tid; j0 < static_cast<unsigned>(pages); j0 += threads) {
+        const int j = static_cast<int>(j0), b = owner(s_page, batch, j);
         const int held = (s_len[b] + page_size - 1) >> page_shift;
         table[b * table_stride + held + (j - s_page[b])] = free_pages[count - 1 - j];
     }
     // a thread takes kRun tokens in a row: one search, and mostly one page, for all of them
-    for (int i0 = tid * kRun; i0 < max_tokens; i0 += threads * kRun) {
+    for (unsigned i0 = tid * kRun; i0 < most; i0 += threads * kRun) {
         int b = 0, held = 0, next = -1, page = -1, have = -1;
-        if (i0 < total) b = owner(s_tok, batch, i0);
+        if (i0 < static_cast<unsigned>(total)) b = owner(s_tok, batch, static_cast<int>(i0));
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const int i = i0 + k;
+            const unsigned at_token = i0 + k;
+            const int i = static_cast<int>(at_token);
             int slot = -1, pos = -1;
-            if (i < total) {
+            if (at_token < static_cast<unsigned>(total)) {
                 if (i >= next) {  // the first token, or the next request that has any
                     while ((b + 1 < batch ? s_tok[b + 1] : total) <= i) ++b;
                     next = b + 1 < batch ? s_tok[b + 1] : total;
@@ -183,9 +186,9 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
                 const long long at = (static_cast<long long>(page) << page_shift) + (pos & (page_size - 1));
                 slot = page < 0 || at > 0x7fffffffll ? -1 : static_cast<int>(at);
             }
-            if (i < max_tokens) {
-                slots[i] = slot;
-                positions[i] = pos;
+            if (at_token < most) {
+                slots[at_token] = slot;
+                positions[at_token] = pos;
             }
         }
     }
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
     bad = __syncthreads_or(bad);
     const bool full = !bad && pages_sum + count > free_capacity;
     ecq_dev::cluster_sync();
-    const int tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads;
+    const unsigned tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads, n = batch;  // as above
     if (bad || full) {
         if (tid == 0) {
             raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
@@ -236,18 +239,18 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
         }
         // done requests' lengths were read by this thread's own CTA: take them from the input again
         if (lens_out != lens_in)
-            for (int b = tid; b < batch; b += threads) lens_out[b] = lens_in[b];
+            for (unsigned b = tid; b < n; b += threads) lens_out[b] = lens_in[b];
         return;
     }
     const int pages = static_cast<int>(pages_sum);
     if (tid == 0) *count_out = count + pages;
-    for (int b = tid; b < batch; b += threads) lens_out[b] = s_len[b];
-    for (int j0 = tid * kRun; j0 < pages; j0 += threads * kRun) {
-        int b = owner(s_page, batch, j0);
+    for (unsigned b = tid; b < n; b += threads) lens_out[b] = s_len[b];
+    for (unsigned j0 = tid * kRun; j0 < static_cast<unsigned>(pages); j0 += threads * kRun) {
+        int b = owner(s_page, batch, static_cast<int>(j0));
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const int j = j0 + k;
-            if (j < pages) {
+            const int j = static_cast<int>(j0 + k);
+            if (j0 + k < static_cast<unsigned>(pages)) {
                 while (b + 1 < batch && s_page[b + 1] <= j) ++b;  // the last request that starts at or before j: the one with it
                 free_pages[count + j] = table[b * table_stride + (j - s_page[b])];
             }
@@ -333,11 +336,12 @@ template <int D, int kPer>
 struct RowLane {
     static constexpr int kUnit = D / 4;  // lanes per token and head
     static constexpr int kTokens = kRowThreads / kUnit;
-    int token, c;  // channels 8c .. 8c + 7
+    unsigned token;  // below 2^32 behind the last of 2^31 - 1 tokens too
+    int c;           // channels 8c .. 8c + 7
     bool is_v;
     __device__ __forceinline__ RowLane() {
         const int l = threadIdx.x % kUnit;
-        token = static_cast<int>(blockIdx.x) * (kTokens * kPer) + threadIdx.x / kUnit;
+        token = blockIdx.x * (kTokens * kPer) + threadIdx.x / kUnit;
         is_v = l >= D / 8;
         c = l % (D / 8);
     }
@@ -348,8 +352,8 @@ __device__ __forceinline__ void row_slots(int (&slot)[kPer], const RowLane<D, kP
                                           int64_t n_slots, int32_t* status) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int token = me.token + i * me.kTokens;
-        slot[i] = token < tokens ? slots[token] : -1;
+        const unsigned token = me.token + i * me.kTokens;
+        slot[i] = token < static_cast<unsigned>(tokens) ? slots[token] : -1;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, 
             const uint32_t c = (x >> (4 * i)) & 15u;
             f[i] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, p.x, p.y);
         }
-        if (me.token + n * me.kTokens < tokens)
+        if (me.token + n * me.kTokens < static_cast<unsigned>(tokens))
             *reinterpret_cast<uint4*>(dst + n * me.kTokens * step) =
                 make_uint4(from_float2<T>(f[0], f[1]), from_float2<T>(f[2], f[3]), from_float2<T>(f[4], f[5]),
                            from_float2<T>(f[6], f[7]));
@@ -505,7 +509,7 @@ int rows_per_thread(int tokens, int kv_heads, int head_dim) {
 }
 dim3 row_grid(int tokens, int kv_heads, int head_dim, int per) {
     const int block = kRowThreads / (head_dim / 4) * per;
-    return dim3((tokens + block - 1) / block, kv_heads);
+    return dim3((static_cast<unsigned>(tokens) + block - 1) / block, kv_heads);
 }
 
 bool table_args_ok(int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_size, int32_t free_capacity) {
