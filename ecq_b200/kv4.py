@@ -67,6 +67,12 @@ def _on(device: int, fn, *args) -> int:
         return fn(*args, _raw_stream(device))
 
 
+def _fits(name: str, n: int, least: int = 0) -> None:
+    """Counts are 32-bit integers in the library, and ctypes cuts larger ones off."""
+    if not least <= n < 1 << 31:
+        raise ValueError(f"{name} must be at least {least} and below 2^31, not {n}")
+
+
 def _int32(name: str, t: torch.Tensor, n: int | None = None) -> None:
     if t.dtype != _I32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 with one dimension")
@@ -151,6 +157,8 @@ def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     filled with -1 behind the last, so a captured step keeps its shapes. All
     or nothing: if pages, room or lengths do not suffice nothing changes, every
     slot is -1 and ``status`` says so."""
+    _fits("max_tokens", max_tokens)
+    _fits("page_size", page_size)
     device = _device(seq_lens, "new_lens block_table free_pages free_count seq_lens_out free_count_out status", new_lens,
                      block_table, free_pages, free_count, seq_lens_out, free_count_out, status)
     batch = seq_lens.shape[0] if seq_lens.dim() else 0
@@ -159,8 +167,6 @@ def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     _int32("free_pages", free_pages)
     _int32("free_count", free_count, 1)
     stride, cols = _table(block_table, batch)
-    if max_tokens < 0:
-        raise ValueError("max_tokens is negative")
     out = torch.empty(2 * batch + 2 + 2 * max_tokens, dtype=_I32, device=seq_lens.device)
     starts, slots, positions, lens_out, count_out = out.split_with_sizes((batch + 1, max_tokens, max_tokens, batch, 1))
     if seq_lens_out is not None:
@@ -184,6 +190,7 @@ def kv4_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.T
     """Push the pages of the requests where ``done`` (bool [batch]) on
     free_pages (in place) and set their lengths to 0. Returns the lengths and
     the count of free pages, as new tensors or in the ``_out`` ones."""
+    _fits("page_size", page_size)
     device = _device(seq_lens, "done block_table free_pages free_count seq_lens_out free_count_out status", done,
                      block_table, free_pages, free_count, seq_lens_out, free_count_out, status)
     batch = seq_lens.shape[0] if seq_lens.dim() else 0
@@ -220,6 +227,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slots: tor
     _, v_token, v_head = _rows("v", v)
     if k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v must have one shape and type")
+    _fits("the number of tokens", k.shape[0])
     device = _device(k, "v pages slots status", v, pages, slots, status)
     tokens, heads, dim = k.shape
     page_size = _page_size(pages, dim, group_size)
@@ -266,6 +274,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     by default. Rows that see nothing (length 0) are 0; rows at or behind
     q_starts[-1] are left as they were in ``out``."""
     code, q_token, q_head = _rows("q", q)
+    _fits("max_q", max_q, 1)
     device = _device(q, "pages block_table seq_lens q_starts out status", pages, block_table, seq_lens, q_starts, out, status)
     tokens, heads, dim = q.shape
     page_size = _page_size(pages, dim, group_size)
@@ -279,8 +288,6 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         _int32("q_starts", q_starts, batch + 1)
     elif tokens != batch or max_q != 1:
         raise ValueError("without q_starts every request has one query")
-    if max_q < 1:
-        raise ValueError("max_q must be at least 1")
     if out is None:
         if q.is_contiguous():
             out = torch.empty_like(q)
