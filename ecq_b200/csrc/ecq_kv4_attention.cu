@@ -722,13 +722,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
         }
         if (kBlockTokens << shift >= kUnitTokens) {  // a page has the whole unit
             f_page[0] = -1;  // nothing there: the one unit of a request without keys
-            if (fr.len) f_page[0] = __ldg(f_row + (f_unit * kUnit >> shift)) & INT32_MAX;
+            if (fr.len) f_page[0] = page_at(f_row + (f_unit * kUnit >> shift));
         } else {
 #pragma unroll
             for (int u = 0; u < kUnit; ++u) {
                 f_page[u] = -1;
                 if ((f_unit * kUnit + u) * kBlockTokens < fr.len)
-                    f_page[u] = __ldg(f_row + ((f_unit * kUnit + u) >> shift)) & INT32_MAX;
+                    f_page[u] = page_at(f_row + ((f_unit * kUnit + u) >> shift));
             }
         }
     };

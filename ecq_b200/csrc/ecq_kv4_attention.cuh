@@ -46,6 +46,11 @@ __device__ __forceinline__ Range range_of(const Args& a, int b) {
     return {lo, hi - lo, (hi - lo) * a.share, max(len, 0)};
 }
 
+// A table's entry; a negative one is as bad as one behind the pool, and -1 is free to mean that there is none.
+__device__ __forceinline__ int page_at(const int32_t* p) {
+    return static_cast<int>(min(static_cast<uint32_t>(__ldg(p)), static_cast<uint32_t>(INT32_MAX)));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

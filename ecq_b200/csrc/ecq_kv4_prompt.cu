@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             const int32_t* row = a.table + b * a.table_stride;
             auto page_of = [&](int j) {  // -1: no such tokens
                 const int blk = j * kTileBlocks + lane;
-                return j < steps && blk * kBlockTokens < rq.len ? __ldg(row + (blk >> shift)) & INT32_MAX : -1;
+                return j < steps && blk * kBlockTokens < rq.len ? page_at(row + (blk >> shift)) : -1;
             };
             constexpr uint32_t kLanes = (1u << kTileBlocks) - 1u;
             int page = page_of(0), j = 0;

@@ -6,7 +6,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import ecq_b200 as ecq  # noqa: E402
-from test_gpu_kv4 import DTYPES, LAYOUTS, check_attention, decode, i32, reference  # noqa: E402
+from test_gpu_kv4 import BADARG, DTYPES, LAYOUTS, check_attention, decode, i32, reference  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -213,3 +213,25 @@ def test_moderate_scores_beside_huge_negative_ones(form, dtype, first):
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 def test_queries_of_any_size(dim, form, sign):
     one_hot(*form, torch.bfloat16, dim, [124, 122, 119, 116, 114, 110, 104, 100, 95, 60, 20], sign, 7)
+
+
+# -- what only the device sees --------------------------------------------------------
+
+@pytest.mark.parametrize("heads,new,room", [(1, 1, 1), (1, 1, 5000), (2, 9, 1), (64, 60, 1)])
+@pytest.mark.parametrize("page,entry", [(16, -1), (64, -1), (16, -2 ** 31), (16, -2 ** 31 + 1), (64, -2 ** 31 + 1), (256, -2 ** 31)])
+def test_negative_page_numbers_are_reported_and_left_out(heads, new, room, page, entry):
+    # the last page of the table is bad: the answer is that of a request without its keys
+    share, dim, g = 2, 64, 32
+    n = 4 * page + 9
+    pages, table = store(randn(n, heads, dim, seed=1).half(), randn(n, heads, dim, seed=2).half(), page, g)
+    wide = torch.full((1, max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q, status = randn(new, heads * share, dim, seed=3).half(), i32([0])
+    bad = wide.clone()
+    bad[0, 4] = entry
+    got = ecq.kv4_attention(q, pages, bad, i32([n]), i32([0, new]), new, group_size=g, status=status)
+    assert status.item() == BADARG
+    for i in range(new):
+        last = min(n - new + i + 1, 4 * page)
+        want = reference(q[i:i + 1], pages, table, [last], [0, 1], page, dim, g)
+        check_attention(got[i:i + 1], *want, torch.float16, new * share > 70)
