@@ -39,11 +39,11 @@ __device__ __forceinline__ Range range_of(const Args& a, int b) {
     }
     int len = a.lens[b];
     const long long room = static_cast<long long>(a.max_pages) << a.page_shift;
-    if (len > room) {
+    if (len < 0 || len > room) {
         raise_status(a.status, ECQ_STATUS_BADARG);
-        len = static_cast<int>(room);
+        len = len < 0 ? 0 : static_cast<int>(room);
     }
-    return {lo, hi - lo, (hi - lo) * a.share, max(len, 0)};
+    return {lo, hi - lo, (hi - lo) * a.share, len};
 }
 
 // A table's entry; a negative one is as bad as one behind the pool, and -1 is free to mean that there is none.

@@ -103,7 +103,7 @@ int32_t ecq_kv4_gather(void *k, void *v, int32_t dtype, const void *pages, int64
  * out: [total_q][heads][head_dim] of dtype, strides in elements, head_dim
  * contiguous, q 16-byte aligned with strides that are multiples of 8, out
  * 8-byte aligned with multiples of 4. heads / kv_heads is at most 64. A page
- * number outside the pool, or a length beyond the table's row, sets
+ * number outside the pool, or a length below 0 or beyond the table's row, sets
  * ECQ_STATUS_BADARG and its keys are left out. The same status says that a
  * request had more than max_q queries and some of its rows were not written.
  * Requests with many rows take values of up to +-131008, twice fp16's end and more

@@ -235,3 +235,18 @@ def test_negative_page_numbers_are_reported_and_left_out(heads, new, room, page,
         last = min(n - new + i + 1, 4 * page)
         want = reference(q[i:i + 1], pages, table, [last], [0, 1], page, dim, g)
         check_attention(got[i:i + 1], *want, torch.float16, new * share > 70)
+
+
+@pytest.mark.parametrize("heads,new,room", [(1, 1, 1), (1, 1, 5000), (64, 60, 1)])
+@pytest.mark.parametrize("length", [-1, -2 ** 31])
+def test_negative_lengths_are_reported_and_their_rows_zero(heads, new, room, length):
+    dim, g, n = 64, 32, 70
+    pages, table = store(randn(n, heads, dim, seed=1).half(), randn(n, heads, dim, seed=2).half(), 16, g)
+    wide = torch.full((2, max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q, status = randn(2 * new, 2 * heads, dim, seed=3).half(), i32([0])
+    starts = i32([0, new, 2 * new])
+    want = ecq.kv4_attention(q, pages, wide, i32([n, 0]), starts, new, group_size=g, status=status)
+    assert status.item() == 0
+    got = ecq.kv4_attention(q, pages, wide, i32([n, length]), starts, new, group_size=g, status=status)
+    assert status.item() == BADARG and torch.equal(got, want) and not bool(got[new:].any())
