@@ -83,6 +83,11 @@ __device__ __forceinline__ int owner(const int* start, int n, int i) {
     return lo;
 }
 
+// A page number whose slots are no int32.
+__device__ __forceinline__ bool bad_page(int32_t page, int page_shift) {
+    return static_cast<uint32_t>(page) > static_cast<uint32_t>(INT32_MAX >> page_shift);
+}
+
 __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     const int32_t* lens_in, const int32_t* __restrict__ new_lens, int32_t* lens_out, int32_t* table,
     int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_shift, const int32_t* __restrict__ free_pages,
@@ -92,6 +97,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     int32_t* s_len = sm;
     int32_t* s_tok = sm + batch;      // tokens before request b
     int32_t* s_page = s_tok + batch;  // new pages before request b
+    int32_t* s_part = s_page + batch;  // its last page, where new tokens go on in that
     __shared__ long long w_tok[kTableThreads / 32];
     __shared__ int w_pg[kTableThreads / 32];
     pdl_launch_dependents();
@@ -102,10 +108,17 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     Totals sum = {0, 0};
     long long pages_sum = 0;
     bool bad = count < 0 || count > free_capacity;
+    // the first pages to be popped, on their way while the lengths are scanned
+    int32_t first_page[kRun];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        const int j = k * kTableThreads + threadIdx.x;
+        first_page[k] = !bad && j < count ? free_pages[count - 1 - j] : 0;
+    }
     for (int base = 0; base < batch; base += kTableThreads) {
         const int b = base + threadIdx.x;
         long long tok = 0;
-        int pg = 0, len = 0;
+        int pg = 0, len = 0, part = 0;
         if (b < batch) {
             len = lens_in[b];
             const int add = new_lens[b];
@@ -115,17 +128,26 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
                 tok = add;
                 // room < 2^31 (checked on the host), so the sums fit
                 pg = ((len + add + page_size - 1) >> page_shift) - ((len + page_size - 1) >> page_shift);
+                if (add && (len & (page_size - 1))) part = table[b * table_stride + (len >> page_shift)];
             }
         }
         const Totals all = block_exclusive(tok, pg, w_tok, w_pg);
+        bad |= bad_page(part, page_shift);
         if (b < batch) {
             s_len[b] = len;
+            s_part[b] = part;
             // beyond 2^31 the call is refused below and nothing uses these
             s_tok[b] = static_cast<int>(min(sum.tokens + tok, 0x7fffffffll));
             s_page[b] = static_cast<int>(min(pages_sum + pg, 0x7fffffffll));
         }
         sum.tokens += all.tokens;
         pages_sum += all.pages;
+    }
+    if (pages_sum <= count) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) bad |= k * kTableThreads + static_cast<int>(threadIdx.x) < pages_sum && bad_page(first_page[k], page_shift);
+        for (unsigned j = threadIdx.x + kRun * kTableThreads; j < static_cast<unsigned>(pages_sum); j += kTableThreads)
+            bad |= bad_page(free_pages[count - 1 - static_cast<int>(j)], page_shift);
     }
     bad = __syncthreads_or(bad || sum.tokens > max_tokens);
     const bool dry = !bad && pages_sum > count;
@@ -181,10 +203,9 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
                 if (col != have) {
                     have = col;
                     // a page of this step comes off the stack again: the table entry is another thread's write
-                    page = col < held ? table[b * table_stride + col] : free_pages[count - 1 - (s_page[b] + col - held)];
+                    page = col < held ? s_part[b] : free_pages[count - 1 - (s_page[b] + col - held)];
                 }
-                const long long at = (static_cast<long long>(page) << page_shift) + (pos & (page_size - 1));
-                slot = page < 0 || at > 0x7fffffffll ? -1 : static_cast<int>(at);
+                slot = (page << page_shift) + (pos & (page_size - 1));
             }
             if (at_token < most) {
                 slots[at_token] = slot;
@@ -529,7 +550,7 @@ unsigned table_ctas(int64_t outputs, bool in_place) {
 
 cudaError_t allow(const void* fn, size_t smem) {
     if (smem <= 48 * 1024) return cudaSuccess;
-    return ecq_dev::ensure_smem_limit(fn, 112 * 1024) ? cudaSuccess : cudaErrorInvalidValue;
+    return ecq_dev::ensure_smem_limit(fn, 16 * ECQ_KV4_MAX_BATCH) ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -551,7 +572,7 @@ int32_t ecq_kv4_extend(const void* seq_lens, const void* new_lens, void* seq_len
         return ECQ_ERR_ARG;
     if (!table_args_ok(table_stride, max_pages, batch, page_size, free_capacity)) return ECQ_ERR_ARG;
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
-    const size_t smem = static_cast<size_t>(batch) * 12;
+    const size_t smem = static_cast<size_t>(batch) * 16;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(extend_kernel), smem); rc != cudaSuccess) return result(rc);
     const unsigned ctas = table_ctas(static_cast<int64_t>(max_tokens) + batch,
                                      seq_lens == seq_lens_out || free_count == free_count_out);

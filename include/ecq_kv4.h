@@ -61,9 +61,11 @@ int64_t ecq_kv4_page_bytes(int32_t head_dim, int32_t page_size, int32_t group_si
  *   *free_count_out = what is left on the stack
  * seq_lens_out may be seq_lens and free_count_out free_count; no other pair may
  * overlap. All or nothing: where a length is negative or too long for its table
- * row, the new tokens are more than max_tokens (ECQ_STATUS_BADARG) or the
- * pages do not suffice (ECQ_STATUS_NO_PAGES), lengths, count and table stay as
- * they were, q_starts is all 0 and slots and positions all -1. */
+ * row, the new tokens are more than max_tokens, a page that would be popped or
+ * that a request goes on in is negative or has slots of 2^31 and more
+ * (ECQ_STATUS_BADARG) or the pages do not suffice (ECQ_STATUS_NO_PAGES),
+ * lengths, count and table stay as they were, q_starts is all 0 and slots and
+ * positions all -1. */
 int32_t ecq_kv4_extend(const void *seq_lens, const void *new_lens, void *seq_lens_out, void *block_table,
                        int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_size,
                        const void *free_pages, int32_t free_capacity, const void *free_count, void *free_count_out,

@@ -29,6 +29,7 @@ MOST = 2 ** 31 - 1
 def test_extend_with_the_most_tokens(refused):
     need(24)
     table, status = torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), i32([0])
+    table[0, 0] = 9
     st = ecq.kv4_extend(i32([3, 0]), i32([9, -1 if refused else 20]), table, i32([7, 6, 5, 4]), i32([4]), 16, MOST, status=status)
     assert status.item() == (BADARG if refused else 0)
     n = 0 if refused else 29
@@ -37,6 +38,7 @@ def test_extend_with_the_most_tokens(refused):
         assert x[n:].amax().item() == -1 and x[n:].amin().item() == -1
     if not refused:
         assert st.positions[:29].tolist() == list(range(3, 12)) + list(range(20))
+        assert st.slots[:9].tolist() == [9 * 16 + i for i in range(3, 12)]
         assert st.slots[9:29].tolist() == [4 * 16 + i for i in range(16)] + [5 * 16 + i for i in range(4)]
 
 
@@ -49,3 +51,41 @@ def test_append_of_the_most_tokens():
     ecq.kv4_append(k, (-k[:1]).expand(MOST, 1, 64), pages, slots, status=status)
     got, neg = ecq.kv4_gather(pages, i32([20, 3, 4]), 64)
     assert status.item() == 0 and bool(got[0].any()) and torch.equal(got[0], got[1]) and torch.equal(neg[0], neg[1]) and not bool(got[2].any())
+
+
+TOO_LARGE = 2 ** 31 // 16  # the first page of 16 tokens whose slots are no int32
+
+
+@pytest.mark.parametrize("page", [-1, -2 ** 31, TOO_LARGE, 2 ** 31 - 1])
+@pytest.mark.parametrize("batch,in_place", [(3, False), (3, True), (700, False), (700, True)])
+@pytest.mark.parametrize("where", ["held", "first popped", "last popped"])
+def test_extend_refuses_bad_pages(page, batch, in_place, where):
+    cols, each = 6, 3
+    lens = [5] + [16] * (batch - 1)              # request 0 goes on in its first page, the others start new ones
+    new = [2] + [16 * each] * (batch - 1)
+    table = torch.arange(batch * cols, dtype=torch.int32, device="cuda").view(batch, cols).contiguous()
+    pops = each * (batch - 1)
+    free = torch.arange(pops + 4, dtype=torch.int32, device="cuda")
+    status, ln, ct = i32([0]), i32(lens), i32([pops + 4])
+    kw = dict(status=status, seq_lens_out=ln, free_count_out=ct) if in_place else dict(status=status)
+    pad = sum(new) + 3
+    ok = table.clone()
+    if where == "held":
+        table[0, 0] = page
+    else:
+        free[-1 if where == "first popped" else 4] = page
+    free[:4] = -1                                # not popped: not looked at
+    table[1:, 0] = -1                            # full: not looked at either
+    keep, stack = table.clone(), free.clone()
+    st = ecq.kv4_extend(ln, i32(new), table, free, ct, 16, pad, **kw)
+    assert status.item() == BADARG
+    assert st.seq_lens.tolist() == lens and st.free_count.item() == pops + 4 and torch.equal(table, keep) and torch.equal(free, stack)
+    assert not bool(st.q_starts.any()) and bool((st.slots == -1).all()) and bool((st.positions == -1).all())
+    # the same with a good page
+    status.zero_()
+    table[0, 0] = ok[0, 0]
+    free[4:] = torch.arange(4, pops + 4, dtype=torch.int32, device="cuda")
+    st = ecq.kv4_extend(ln, i32(new), table, free, ct, 16, pad, **kw)
+    assert status.item() == 0 and st.free_count.item() == 4
+    assert st.slots[:2].tolist() == [5, 6] and bool((st.slots[:-3] >= 0).all())
+    assert st.seq_lens.tolist() == [a + b for a, b in zip(lens, new)]
