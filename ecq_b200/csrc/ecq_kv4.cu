@@ -107,13 +107,14 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     const int page_size = 1 << page_shift;
     Totals sum = {0, 0};
     long long pages_sum = 0;
-    bool bad = count < 0 || count > free_capacity;
+    const bool stack = count >= 0 && count <= free_capacity;
+    bool bad = !stack;
     // the first pages to be popped, on their way while the lengths are scanned
     int32_t first_page[kRun];
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
         const int j = k * kTableThreads + threadIdx.x;
-        first_page[k] = !bad && j < count ? free_pages[count - 1 - j] : 0;
+        first_page[k] = stack && j < count ? free_pages[count - 1 - j] : 0;
     }
     for (int base = 0; base < batch; base += kTableThreads) {
         const int b = base + threadIdx.x;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
         sum.tokens += all.tokens;
         pages_sum += all.pages;
     }
-    if (pages_sum <= count) {
+    if (stack && sum.tokens <= max_tokens && pages_sum <= count) {  // (the pages of more tokens may not fit an int)
 #pragma unroll
         for (int k = 0; k < kRun; ++k) bad |= k * kTableThreads + static_cast<int>(threadIdx.x) < pages_sum && bad_page(first_page[k], page_shift);
         for (unsigned j = threadIdx.x + kRun * kTableThreads; j < static_cast<unsigned>(pages_sum); j += kTableThreads)

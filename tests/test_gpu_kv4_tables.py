@@ -89,3 +89,20 @@ def test_extend_refuses_bad_pages(page, batch, in_place, where):
     assert status.item() == 0 and st.free_count.item() == 4
     assert st.slots[:2].tolist() == [5, 6] and bool((st.slots[:-3] >= 0).all())
     assert st.seq_lens.tolist() == [a + b for a, b in zip(lens, new)]
+
+
+@pytest.mark.parametrize("count", [-1, -2 ** 31, 101, 2 ** 31 - 1])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_count_that_the_stack_cannot_have(count, in_place):
+    # more pages asked for than the first ones that are looked at: nothing behind the stack is read
+    batch, cols = 700, 5
+    table = torch.arange(batch * cols, dtype=torch.int32, device="cuda").view(batch, cols).contiguous()
+    keep, status, ln, ct = table.clone(), i32([0]), i32([0] * batch), i32([count])
+    kw = dict(status=status, seq_lens_out=ln, free_count_out=ct) if in_place else dict(status=status)
+    st = ecq.kv4_extend(ln, i32([80] * batch), table, torch.arange(100, dtype=torch.int32, device="cuda"), ct, 16, 80 * batch, **kw)
+    assert status.item() == BADARG and torch.equal(table, keep) and st.free_count.item() == count
+    assert not bool(st.seq_lens.any()) and not bool(st.q_starts.any()) and bool((st.slots == -1).all())
+    status.zero_()
+    _, got = ecq.kv4_release(torch.ones(batch, dtype=torch.bool, device="cuda"), i32([80] * batch), table,
+                             torch.arange(100, dtype=torch.int32, device="cuda"), i32([count]), 16, status=status)
+    assert status.item() == BADARG and got.item() == count
