@@ -23,22 +23,25 @@ using ecq_dev::pdl_wait;
 // parts keeps anything from being written before every CTA has read; otherwise
 // there are more of them. Work per token and per
 // page is found by a binary search in the scanned starts, so one request with
-// all the tokens is spread like many with few. Bound by launch and barrier
-// latency.
+// all the tokens is spread like many with few. Release is one CTA or one cluster
+// in any case: whether all of its pages were good decides what it says. Bound by
+// launch and barrier latency: one token of 17 requests 4.5 us, 512 prompts of up
+// to 255 tokens 6.0 us, 17 requests released 2.6 us, 256 of 512 with up to 512
+// pages 5.9 us.
 // ---------------------------------------------------------------------------
 constexpr int kTableThreads = 512;
 constexpr int kRun = 4;  // outputs that a thread takes in a row
 
 struct Totals {
-    long long tokens;  // sums of 2^13 lengths below 2^31
-    int pages;
+    long long first;  // tokens, or pages that are given back: of 2^13 requests below 2^31 each
+    int second;       // new pages, or parts of those
 };
 
-// Exclusive sums over the CTA of (tokens, pages); returns the totals.
-__device__ __forceinline__ Totals block_exclusive(long long& tokens, int& pages, long long* s_tok, int* s_pg) {
+// Exclusive sums over the CTA of two counts; returns the totals.
+__device__ __forceinline__ Totals block_exclusive(long long& first, int& second, long long* s_tok, int* s_pg) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long t = tokens;
-    int p = pages;
+    long long t = first;
+    int p = second;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long tt = __shfl_up_sync(0xffffffffu, t, o);
@@ -60,14 +63,14 @@ __device__ __forceinline__ Totals block_exclusive(long long& tokens, int& pages,
 #pragma unroll
     for (int w = 0; w < kTableThreads / 32; ++w) {
         if (w == warp) {
-            bt = all.tokens;
-            bp = all.pages;
+            bt = all.first;
+            bp = all.second;
         }
-        all.tokens += s_tok[w];
-        all.pages += s_pg[w];
+        all.first += s_tok[w];
+        all.second += s_pg[w];
     }
-    tokens = bt + t - tokens;
-    pages = bp + p - pages;
+    first = bt + t - first;
+    second = bp + p - second;
     return all;
 }
 
@@ -105,8 +108,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     const int32_t count = *count_in;
     const long long room = static_cast<long long>(max_pages) << page_shift;
     const int page_size = 1 << page_shift;
-    Totals sum = {0, 0};
-    long long pages_sum = 0;
+    long long tokens_sum = 0, pages_sum = 0;
     const bool stack = count >= 0 && count <= free_capacity;
     bool bad = !stack;
     // the first pages to be popped, on their way while the lengths are scanned
@@ -138,19 +140,19 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
             s_len[b] = len;
             s_part[b] = part;
             // beyond 2^31 the call is refused below and nothing uses these
-            s_tok[b] = static_cast<int>(min(sum.tokens + tok, 0x7fffffffll));
+            s_tok[b] = static_cast<int>(min(tokens_sum + tok, 0x7fffffffll));
             s_page[b] = static_cast<int>(min(pages_sum + pg, 0x7fffffffll));
         }
-        sum.tokens += all.tokens;
-        pages_sum += all.pages;
+        tokens_sum += all.first;
+        pages_sum += all.second;
     }
-    if (stack && sum.tokens <= max_tokens && pages_sum <= count) {  // (the pages of more tokens may not fit an int)
+    if (stack && tokens_sum <= max_tokens && pages_sum <= count) {  // (the pages of more tokens may not fit an int)
 #pragma unroll
         for (int k = 0; k < kRun; ++k) bad |= k * kTableThreads + static_cast<int>(threadIdx.x) < pages_sum && bad_page(first_page[k], page_shift);
         for (unsigned j = threadIdx.x + kRun * kTableThreads; j < static_cast<unsigned>(pages_sum); j += kTableThreads)
             bad |= bad_page(free_pages[count - 1 - static_cast<int>(j)], page_shift);
     }
-    bad = __syncthreads_or(bad || sum.tokens > max_tokens);
+    bad = __syncthreads_or(bad || tokens_sum > max_tokens);
     const bool dry = !bad && pages_sum > count;
     ecq_dev::cluster_sync();
     // unsigned: the counts are below 2^31, so an index that has gone past its end by a stride is below 2^32
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
         }
         return;
     }
-    const int total = static_cast<int>(sum.tokens), pages = static_cast<int>(pages_sum);
+    const int total = static_cast<int>(tokens_sum), pages = static_cast<int>(pages_sum);
     if (tid == 0) *count_out = count - pages;
     for (unsigned b = tid; b <= n; b += threads) {
         const int start = b < n ? s_tok[b] : total;
@@ -216,6 +218,9 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(
     }
 }
 
+// One CTA or one cluster. The pages are written behind the stack's end first, where nothing is yet, and looked at on the
+// way; lengths and count say so only if all of them were good.
+constexpr int kPart = 256;  // pages that a warp takes at a time
 __global__ void __launch_bounds__(kTableThreads) release_kernel(
     const uint8_t* __restrict__ done, const int32_t* lens_in, int32_t* lens_out, const int32_t* __restrict__ table,
     int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_shift, int32_t* __restrict__ free_pages,
@@ -223,61 +228,74 @@ __global__ void __launch_bounds__(kTableThreads) release_kernel(
     extern __shared__ int32_t sm[];
     int32_t* s_len = sm;              // length after the call
     int32_t* s_page = sm + batch;     // pages given back before request b
+    int32_t* s_part = s_page + batch;  // parts of up to kPart pages before it
     __shared__ long long w_tok[kTableThreads / 32];
     __shared__ int w_pg[kTableThreads / 32];
+    __shared__ float s_bad;           // this CTA found something wrong
     pdl_launch_dependents();
     pdl_wait();
     const int32_t count = *count_in;
     const int page_size = 1 << page_shift;
-    long long pages_sum = 0;
+    long long pages_sum = 0, parts_sum = 0;
     bool bad = count < 0 || count > free_capacity;
     for (int base = 0; base < batch; base += kTableThreads) {
         const int b = base + threadIdx.x;
-        long long none = 0;
-        int pg = 0, len = 0;
+        long long pg = 0;
+        int parts = 0, len = 0;
         bool give = false;
         if (b < batch) {
             len = lens_in[b];
             give = done[b] != 0;
             const long long held = (static_cast<long long>(len) + page_size - 1) >> page_shift;
             if (len < 0 || held > max_pages) bad = true;
-            else if (give) pg = static_cast<int>(held);
+            else if (give) pg = held;
         }
-        const Totals all = block_exclusive(none, pg, w_tok, w_pg);
+        parts = static_cast<int>((pg + kPart - 1) / kPart);
+        const Totals all = block_exclusive(pg, parts, w_tok, w_pg);
         if (b < batch) {
             s_len[b] = give ? 0 : len;
             s_page[b] = static_cast<int>(min(pages_sum + pg, 0x7fffffffll));
+            s_part[b] = static_cast<int>(parts_sum + parts);
         }
-        pages_sum += all.pages;
+        pages_sum += all.first;
+        parts_sum += all.second;
     }
     bad = __syncthreads_or(bad);
-    const bool full = !bad && pages_sum + count > free_capacity;
-    ecq_dev::cluster_sync();
-    const unsigned tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads, n = batch;  // as above
-    if (bad || full) {
-        if (tid == 0) {
-            raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
-            *count_out = count;
-        }
-        // done requests' lengths were read by this thread's own CTA: take them from the input again
-        if (lens_out != lens_in)
-            for (unsigned b = tid; b < n; b += threads) lens_out[b] = lens_in[b];
-        return;
-    }
-    const int pages = static_cast<int>(pages_sum);
-    if (tid == 0) *count_out = count + pages;
-    for (unsigned b = tid; b < n; b += threads) lens_out[b] = s_len[b];
-    for (unsigned j0 = tid * kRun; j0 < static_cast<unsigned>(pages); j0 += threads * kRun) {
-        int b = owner(s_page, batch, static_cast<int>(j0));
+    const bool full = pages_sum + count > free_capacity;
+    // unsigned, as above
+    const unsigned tid = blockIdx.x * kTableThreads + threadIdx.x, threads = gridDim.x * kTableThreads, n = batch;
+    const int pages = bad || full ? 0 : static_cast<int>(pages_sum), parts = bad || full ? 0 : static_cast<int>(parts_sum);
+    const int lane = threadIdx.x & 31;
+    for (int i = tid >> 5; i < parts; i += threads >> 5) {  // a warp takes a part of a request's pages
+        const int b = owner(s_part, batch, i), first = (i - s_part[b]) * kPart + lane;
+        const int held = (b + 1 < batch ? s_page[b + 1] : pages) - s_page[b];
+        const int32_t* from = table + b * table_stride;
+        int32_t* to = free_pages + count + s_page[b];
+        int32_t page[kPart / 32];
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) {
-            const int j = static_cast<int>(j0 + k);
-            if (j0 + k < static_cast<unsigned>(pages)) {
-                while (b + 1 < batch && s_page[b + 1] <= j) ++b;  // the last request that starts at or before j: the one with it
-                free_pages[count + j] = table[b * table_stride + (j - s_page[b])];
-            }
+        for (int k = 0; k < kPart / 32; ++k) page[k] = first + 32 * k < held ? from[first + 32 * k] : 0;
+#pragma unroll
+        for (int k = 0; k < kPart / 32; ++k) {
+            bad |= bad_page(page[k], page_shift);
+            if (first + 32 * k < held) to[first + 32 * k] = page[k];
         }
     }
+    bad = __syncthreads_or(bad);
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) s_bad = bad ? 1.f : 0.f;
+        ecq_dev::cluster_sync();  // every CTA has read the lengths and the count, too
+        for (unsigned r = 0; r < gridDim.x; ++r) bad |= ecq_dev::ld_cluster_f32(&s_bad, r) != 0.f;
+        ecq_dev::cluster_arrive();
+    }
+    if (tid == 0) {
+        if (bad || full) raise_status(status, bad ? ECQ_STATUS_BADARG : ECQ_STATUS_NO_PAGES);
+        *count_out = count + (bad ? 0 : pages);
+    }
+    for (unsigned b = tid; b < n; b += threads) {
+        if (!bad && !full) lens_out[b] = s_len[b];
+        else if (lens_out != lens_in) lens_out[b] = lens_in[b];
+    }
+    if (gridDim.x > 1) ecq_dev::cluster_wait();  // no CTA leaves while another reads its flag
 }
 
 // ---------------------------------------------------------------------------
@@ -595,12 +613,12 @@ int32_t ecq_kv4_release(const void* done, const void* seq_lens, void* seq_lens_o
         return ECQ_ERR_ARG;
     if (!table_args_ok(table_stride, max_pages, batch, page_size, free_capacity)) return ECQ_ERR_ARG;
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
-    const size_t smem = static_cast<size_t>(batch) * 8;
+    const size_t smem = static_cast<size_t>(batch) * 12;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(release_kernel), smem); rc != cudaSuccess) return result(rc);
-    const unsigned ctas = table_ctas(static_cast<int64_t>(batch) * max_pages / 2,
-                                     seq_lens == seq_lens_out || free_count == free_count_out);
+    // a cluster where the warps of one CTA would take more than a part each, should half of the pages come back
+    const unsigned ctas = static_cast<int64_t>(batch) * max_pages / 2 > kTableThreads / 32 * kPart ? 8 : 1;
     return result(launch_pdl_cluster(release_kernel, dim3(ctas), dim3(kTableThreads), smem,
-                                     static_cast<cudaStream_t>(stream), ctas < 8 ? ctas : 8, static_cast<const uint8_t*>(done),
+                                     static_cast<cudaStream_t>(stream), ctas, static_cast<const uint8_t*>(done),
                                      static_cast<const int32_t*>(seq_lens), static_cast<int32_t*>(seq_lens_out),
                                      static_cast<const int32_t*>(block_table), table_stride, max_pages, batch,
                                      log2i(page_size), static_cast<int32_t*>(free_pages), free_capacity,

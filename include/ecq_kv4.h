@@ -74,7 +74,8 @@ int32_t ecq_kv4_extend(const void *seq_lens, const void *new_lens, void *seq_len
 /* Gives the pages of the requests with done[b] != 0 (uint8) back: pushed on
  * free_pages in the order of requests and columns, their lengths set to 0. The
  * table's entries stay (a length of 0 makes them unused). All or nothing as
- * above; ECQ_STATUS_NO_PAGES where the stack (free_capacity) has no room. */
+ * above, bad pages among those to be pushed included; ECQ_STATUS_NO_PAGES where
+ * the stack (free_capacity) has no room. */
 int32_t ecq_kv4_release(const void *done, const void *seq_lens, void *seq_lens_out, const void *block_table,
                         int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_size, void *free_pages,
                         int32_t free_capacity, const void *free_count, void *free_count_out, void *status,

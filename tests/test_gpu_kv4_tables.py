@@ -106,3 +106,29 @@ def test_a_count_that_the_stack_cannot_have(count, in_place):
     _, got = ecq.kv4_release(torch.ones(batch, dtype=torch.bool, device="cuda"), i32([80] * batch), table,
                              torch.arange(100, dtype=torch.int32, device="cuda"), i32([count]), 16, status=status)
     assert status.item() == BADARG and got.item() == count
+
+
+@pytest.mark.parametrize("page", [-1, -2 ** 31, TOO_LARGE])
+@pytest.mark.parametrize("batch,cols", [(3, 6), (700, 6), (40, 700)])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("last", [False, True])
+def test_release_refuses_bad_pages(page, batch, cols, in_place, last):
+    lens = [16 * cols - 3 - b % 5 for b in range(batch)]
+    done = [b % 2 == 0 for b in range(batch)]
+    who = max(b for b in range(batch) if done[b]) if last else 0
+    table = torch.arange(batch * cols, dtype=torch.int32, device="cuda").view(batch, cols).contiguous()
+    table[1] = -1                                    # not done: not looked at
+    good = int(table[who, cols - 1 if last else 0])
+    table[who, cols - 1 if last else 0] = page
+    room = batch * cols + 2
+    free = torch.full((room,), -5, dtype=torch.int32, device="cuda")
+    status, ln, ct, flags = i32([0]), i32(lens), i32([2]), torch.tensor(done, device="cuda")
+    kw = dict(status=status, seq_lens_out=ln, free_count_out=ct) if in_place else dict(status=status)
+    got = ecq.kv4_release(flags, ln, table, free, ct, 16, **kw)
+    assert status.item() == BADARG and got[0].tolist() == lens and got[1].item() == 2 and bool((free[:2] == -5).all())  # behind the stack's end anything may be
+    status.zero_()
+    table[who, cols - 1 if last else 0] = good
+    got = ecq.kv4_release(flags, ln, table, free, ct, 16, **kw)
+    pages = [p for b in range(batch) if done[b] for p in range(b * cols, (b + 1) * cols)]
+    assert status.item() == 0 and got[1].item() == 2 + len(pages) and free[2:2 + len(pages)].tolist() == pages
+    assert got[0].tolist() == [0 if d else n for n, d in zip(lens, done)]
