@@ -840,8 +840,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
                 } while (rq.units == 0);
                 if (b >= a.batch) late = true;
             }
-            if (late) f = range;
-            else load_rows<T, D, kWeights>(raw, a, rq, head, tile);
+            if (!late) load_rows<T, D, kWeights>(raw, a, rq, head, tile);
         }
         float* part = kPairs ? s_part : a.parts + (2 * static_cast<size_t>(cta) + starts) * part_floats<D, TR>();
         if (!kPairs && starts && !ends && threadIdx.x == 0) {
@@ -907,7 +906,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
                     }
                 }
             }
-            __syncthreads();
+            // a warp that gave up takes the others with it: they would wait for it at the next segment's barriers
+            if (nt + 1 < NT) __syncthreads();
+            else if (__syncthreads_or(late)) late = true, f = range;
         }
     }
     if constexpr (kPairs) {
