@@ -29,9 +29,10 @@ from ._lib import EcqError, check, lib
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _I32 = torch.int32
 _U8 = torch.uint8
-# the current stream's handle and the current device, without objects for them
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# the current stream's handle and the current device, without objects for them (a torch without CUDA has neither, and no
+# tensor that would get here)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 class KV4Step(NamedTuple):

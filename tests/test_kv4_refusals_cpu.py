@@ -1,4 +1,8 @@
 """More refusals of the 4-bit KV cache's entry points that need no device."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -24,3 +28,13 @@ def test_counts_that_are_no_32_bit_integers(n):
     for call in calls:
         with pytest.raises(ValueError, match="2\\^31"):
             call()
+
+
+def test_import_with_a_torch_without_cuda():
+    code = ("import torch\n"
+            "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    delattr(torch._C, name)\n"
+            "import ecq_b200.model, ecq_b200 as ecq\n"
+            "assert ecq.kv4_pages(1, 1, 64, device='cpu').numel()\n")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0, run.stderr
