@@ -15,6 +15,9 @@ tensors. Calls run on the current stream of the tensors' device, allocate only
 their results and workspaces (from torch's allocator, so they can be captured
 into CUDA graphs) and do not synchronise. Bad values that only the device sees
 set bits of the ``status`` word.
+
+The calls are for inference: the cache's bytes carry no gradient to k and v, and
+a backward pass through ``kv4_attention`` to its q raises.
 """
 from __future__ import annotations
 
@@ -260,6 +263,20 @@ def kv4_gather(pages: torch.Tensor, slots: torch.Tensor, head_dim: int, *, group
     return k, v
 
 
+class _NoBackward(torch.autograd.Function):
+    """kv4_attention of a q that requires a gradient: the same output, which says so when one is asked for."""
+
+    @staticmethod
+    def forward(ctx, q, out, call):
+        if out is not None:
+            ctx.mark_dirty(out)
+        return call(q, out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("kv4_attention has no backward pass: call it under torch.no_grad() or with q.detach()")
+
+
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                   q_starts: torch.Tensor | None = None, max_q: int = 1, *, group_size: int = 64,
                   scale: float | None = None, out: torch.Tensor | None = None,
@@ -274,6 +291,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     their request, each sees the tokens up to its own. scale: 1 / sqrt(head_dim)
     by default. Rows that see nothing (length 0) are 0; rows at or behind
     q_starts[-1] are left as they were in ``out``."""
+    if q.requires_grad and torch.is_grad_enabled():
+        return _NoBackward.apply(q, out, lambda q, out: kv4_attention(
+            q, pages, block_table, seq_lens, q_starts, max_q, group_size=group_size, scale=scale, out=out, status=status))
     code, q_token, q_head = _rows("q", q)
     _fits("max_q", max_q, 1)
     device = _device(q, "pages block_table seq_lens q_starts out status", pages, block_table, seq_lens, q_starts, out, status)
