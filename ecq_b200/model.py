@@ -155,14 +155,19 @@ class Llama7BDecoder:
         (where it was measured faster), the second above.
         kv_cache: "fp16" holds the cache as [heads, tokens, head_dim] rows for
         these; "int4" holds it in 4 bits (ecq_b200.kv4: pages of 64 tokens, a
-        scale and a zero per 64 channels) and runs its attention."""
+        scale and a zero per 64 channels) and runs its attention, which
+        leaves nothing to choose (attention stays "auto")."""
         self.cfg = cfg = cfg or Llama7BConfig()
         if attention not in ("ecq", "sdpa", "auto"):
             raise ValueError("attention is 'ecq', 'sdpa' or 'auto'")
-        if attention == "auto":
-            attention = "ecq" if cfg.heads // tp <= ECQ_ATTENTION_MAX_HEADS else "sdpa"
         if kv_cache not in ("fp16", "int4"):
             raise ValueError("kv_cache is 'fp16' or 'int4'")
+        if kv_cache == "int4":
+            if attention != "auto":
+                raise ValueError(f"attention {attention!r} is of the fp16 cache: kv_cache 'int4' has its own")
+            attention = "kv4"
+        elif attention == "auto":
+            attention = "ecq" if cfg.heads // tp <= ECQ_ATTENTION_MAX_HEADS else "sdpa"
         self.kv_cache = kv_cache
         self.attention = attention
         self.dev = torch.device(device or "cuda")

@@ -38,3 +38,12 @@ def test_import_with_a_torch_without_cuda():
             "assert ecq.kv4_pages(1, 1, 64, device='cpu').numel()\n")
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=Path(__file__).resolve().parents[1])
     assert run.returncode == 0, run.stderr
+
+
+@pytest.mark.parametrize("attention", ["ecq", "sdpa"])
+def test_the_decoder_with_a_4bit_cache_has_no_choice_of_attention(attention):
+    from ecq_b200.model import Llama7BConfig, Llama7BDecoder
+
+    cfg = Llama7BConfig(layers=1, hidden=512, heads=4, head_dim=128, mlp=1024, vocab=1000, kv_len=16)
+    with pytest.raises(ValueError, match="int4"):
+        Llama7BDecoder(cfg, device="cpu", kv_cache="int4", attention=attention)
