@@ -134,6 +134,10 @@ def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
     if t.dim() != 3 or code is None:
         raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, head_dim]")
     token, head, last = t.stride()
+    if t.shape[0] == 1:  # a dimension of one entry has no stride to speak of
+        token = 0
+    if t.shape[1] == 1:
+        head = 0
     if t.numel() and (last != 1 or token % 8 or head % 8 or t.data_ptr() % 16):
         raise ValueError(f"{name}: head_dim must be contiguous, rows 16-byte aligned")
     return code, token, head
@@ -319,6 +323,10 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must have q's shape and type")
         o_token, o_head, last = out.stride()
+        if tokens == 1:
+            o_token = 0
+        if heads == 1:
+            o_head = 0
         if out.numel() and (last != 1 or o_token % 4 or o_head % 4 or out.data_ptr() % 8):
             raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
     need = _workspace_bytes(batch, heads, kv_heads, dim, max_q, cols, page_size, device)

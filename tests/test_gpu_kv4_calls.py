@@ -28,3 +28,28 @@ def test_a_gradient_that_attention_does_not_have_is_said(given):
     assert w.grad is None
     with torch.no_grad():
         assert not ecq.kv4_attention(q * w, pages, table, i32([40, 17]), group_size=32).requires_grad
+
+
+@pytest.mark.parametrize("odd", [1, 4, 68])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_strides_of_dimensions_with_one_entry_do_not_matter(odd, dim):
+    # one token out of a fused projection whose width is no multiple of 8, and one head of one
+    pages, table = fill([40], 2, dim, 32, 16, 1)
+    x = torch.randn(8 * dim, device="cuda").half()
+    q = x[:4 * dim].view(1, 4, dim)
+    k, v = x[4 * dim:6 * dim].view(1, 2, dim), x[6 * dim:].view(1, 2, dim)
+    want = ecq.kv4_attention(q, pages, table, i32([40]), group_size=32)
+    as_odd = lambda t, at: x.as_strided(t.shape, (8 * dim + odd, dim, 1), at)  # noqa: E731
+    out = torch.zeros(9 * dim, device="cuda", dtype=torch.float16).as_strided(q.shape, (8 * dim + odd, dim, 1))
+    got = ecq.kv4_attention(as_odd(q, 0), pages, table, i32([40]), group_size=32, out=out)
+    assert torch.equal(got, want) and torch.equal(out, want)
+    a, b = pages.clone(), pages.clone()
+    ecq.kv4_append(k, v, a, i32([5]), group_size=32)
+    ecq.kv4_append(as_odd(k, 4 * dim), as_odd(v, 6 * dim), b, i32([5]), group_size=32)
+    assert torch.equal(a, b)
+    pool = ecq.kv4_pages(1, 1, dim, 16, 32)
+    ecq.kv4_append(x.as_strided((3, 1, dim), (2 * dim, odd, 1)), x.as_strided((3, 1, dim), (2 * dim, odd, 1), dim), pool, i32([0, 1, 2]), group_size=32)
+    want = ecq.kv4_attention(x.view(4, 2, dim)[:3, :1].contiguous(), pool, i32([[0], [0], [0]]), i32([3, 3, 3]), group_size=32)
+    got = ecq.kv4_attention(x.as_strided((3, 1, dim), (2 * dim, odd, 1)), pool, i32([[0], [0], [0]]), i32([3, 3, 3]), group_size=32,
+                            out=torch.zeros(6 * dim, device="cuda", dtype=torch.float16).as_strided((3, 1, dim), (2 * dim, odd, 1)))
+    assert torch.equal(got, want)
