@@ -160,7 +160,8 @@ def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     by new_lens[b] tokens (int32 [batch]). Pages that it did not have yet are
     popped off the end of free_pages[:free_count] into its row of block_table
     (in place); lengths and count come back as new tensors, or in
-    ``seq_lens_out`` / ``free_count_out``, which may be the inputs. At most
+    ``seq_lens_out`` / ``free_count_out``, which may be seq_lens / free_count
+    themselves and share memory with nothing else. At most
     ``max_tokens`` new tokens: ``slots`` and ``positions`` have that length,
     filled with -1 behind the last, so a captured step keeps its shapes. All
     or nothing: if pages, room or lengths do not suffice nothing changes, every
@@ -329,6 +330,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
             o_head = 0
         if out.numel() and (last != 1 or o_token % 4 or o_head % 4 or out.data_ptr() % 8):
             raise ValueError("out: head_dim must be contiguous, rows 8-byte aligned")
+        if (tokens > 1 and o_token < dim) or (heads > 1 and o_head < dim):
+            raise ValueError("out: rows share memory")
     need = _workspace_bytes(batch, heads, kv_heads, dim, max_q, cols, page_size, device)
     ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
     check(_on(device, lib().ecq_kv4_attention, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, code,

@@ -53,3 +53,12 @@ def test_strides_of_dimensions_with_one_entry_do_not_matter(odd, dim):
     got = ecq.kv4_attention(x.as_strided((3, 1, dim), (2 * dim, odd, 1)), pool, i32([[0], [0], [0]]), i32([3, 3, 3]), group_size=32,
                             out=torch.zeros(6 * dim, device="cuda", dtype=torch.float16).as_strided((3, 1, dim), (2 * dim, odd, 1)))
     assert torch.equal(got, want)
+
+
+def test_an_output_whose_rows_share_memory_is_refused():
+    pages, table = fill([40, 17], 2, 64, 32, 16, 1)
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    for out in (torch.zeros(1, 4, 64, device="cuda").half().expand(2, 4, 64), torch.zeros(2, 1, 64, device="cuda").half().expand(2, 4, 64),
+                torch.zeros(1000, device="cuda").half().as_strided((2, 4, 64), (32, 128, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            ecq.kv4_attention(q, pages, table, i32([40, 17]), group_size=32, out=out)
