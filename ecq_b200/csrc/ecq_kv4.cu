@@ -558,6 +558,30 @@ bool table_args_ok(int64_t table_stride, int32_t max_pages, int32_t batch, int32
     return static_cast<int64_t>(max_pages) * page_size < (1ll << 31) - 256;
 }
 
+// Whether n bytes at a and m at b share any.
+bool shares(const void* a, int64_t n, const void* b, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < static_cast<uintptr_t>(n) : x - y < static_cast<uintptr_t>(m);
+}
+// Lengths and count that are written must be apart from all that is read and written, but for the inputs that they may be.
+struct Span {
+    const void* at;
+    int64_t bytes;
+};
+template <size_t N>
+bool outputs_apart(const void* lens, const void* lens_out, const void* count, const void* count_out, int32_t batch,
+                   const Span (&others)[N]) {
+    const int64_t n = 4ll * batch;
+    if (shares(lens_out, n, count_out, 4) || shares(lens_out, n, count, 4) || shares(count_out, 4, lens, n)) return false;
+    if ((lens_out != lens && shares(lens_out, n, lens, n)) || (count_out != count && shares(count_out, 4, count, 4))) return false;
+    for (const Span& s : others)
+        if (s.bytes && (shares(lens_out, n, s.at, s.bytes) || shares(count_out, 4, s.at, s.bytes))) return false;
+    return true;
+}
+int64_t table_bytes(int64_t table_stride, int32_t max_pages, int32_t batch) {
+    return 4 * ((batch - 1) * table_stride + max_pages);
+}
+
 // CTAs for so many outputs, kRun to a thread: one, a cluster, or (not in
 // place) several clusters.
 unsigned table_ctas(int64_t outputs, bool in_place) {
@@ -591,6 +615,10 @@ int32_t ecq_kv4_extend(const void* seq_lens, const void* new_lens, void* seq_len
         return ECQ_ERR_ARG;
     if (!table_args_ok(table_stride, max_pages, batch, page_size, free_capacity)) return ECQ_ERR_ARG;
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
+    const Span others[] = {{new_lens, 4ll * batch}, {block_table, table_bytes(table_stride, max_pages, batch)},
+                           {free_pages, 4ll * free_capacity}, {q_starts, 4ll * batch + 4}, {slots, 4ll * max_tokens},
+                           {positions, 4ll * max_tokens}};
+    if (!outputs_apart(seq_lens, seq_lens_out, free_count, free_count_out, batch, others)) return ECQ_ERR_ARG;
     const size_t smem = static_cast<size_t>(batch) * 16;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(extend_kernel), smem); rc != cudaSuccess) return result(rc);
     const unsigned ctas = table_ctas(static_cast<int64_t>(max_tokens) + batch,
@@ -613,6 +641,8 @@ int32_t ecq_kv4_release(const void* done, const void* seq_lens, void* seq_lens_o
         return ECQ_ERR_ARG;
     if (!table_args_ok(table_stride, max_pages, batch, page_size, free_capacity)) return ECQ_ERR_ARG;
     if (batch > ECQ_KV4_MAX_BATCH) return ECQ_ERR_UNSUPPORTED;
+    const Span others[] = {{done, batch}, {block_table, table_bytes(table_stride, max_pages, batch)}, {free_pages, 4ll * free_capacity}};
+    if (!outputs_apart(seq_lens, seq_lens_out, free_count, free_count_out, batch, others)) return ECQ_ERR_ARG;
     const size_t smem = static_cast<size_t>(batch) * 12;
     if (cudaError_t rc = allow(reinterpret_cast<const void*>(release_kernel), smem); rc != cudaSuccess) return result(rc);
     // a cluster where the warps of one CTA would take more than a part each, should half of the pages come back

@@ -60,7 +60,7 @@ int64_t ecq_kv4_page_bytes(int32_t head_dim, int32_t page_size, int32_t group_si
  *     and its position in its request; -1 for q_starts[batch] <= i < max_tokens
  *   *free_count_out = what is left on the stack
  * seq_lens_out may be seq_lens and free_count_out free_count; no other pair may
- * overlap. All or nothing: where a length is negative or too long for its table
+ * overlap (refused, for these two). All or nothing: where a length is negative or too long for its table
  * row, the new tokens are more than max_tokens, a page that would be popped or
  * that a request goes on in is negative or has slots of 2^31 and more
  * (ECQ_STATUS_BADARG) or the pages do not suffice (ECQ_STATUS_NO_PAGES),

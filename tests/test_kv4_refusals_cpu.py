@@ -8,6 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import ecq_b200 as ecq  # noqa: E402
+from ecq_b200 import _lib  # noqa: E402
 
 
 def i32(*s):
@@ -47,3 +48,36 @@ def test_the_decoder_with_a_4bit_cache_has_no_choice_of_attention(attention):
     cfg = Llama7BConfig(layers=1, hidden=512, heads=4, head_dim=128, mlp=1024, vocab=1000, kv_len=16)
     with pytest.raises(ValueError, match="int4"):
         Llama7BDecoder(cfg, device="cpu", kv_cache="int4", attention=attention)
+
+
+# the C ABI's pointers are looked at but not dereferenced before a call is refused
+AT = dict(lens=0x10000, new=0x20000, lens_out=0x30000, table=0x40000, free=0x50000, count=0x60000, count_out=0x70000, starts=0x80000,
+          slots=0x90000, positions=0xa0000, done=0xb0000)
+
+
+@pytest.mark.parametrize("out,what,shift", [
+    ("lens_out", "new", 0), ("lens_out", "new", 76), ("lens_out", "new", -76), ("lens_out", "lens", 4), ("lens_out", "lens", -4),
+    ("lens_out", "table", 0), ("lens_out", "table", 4 * 100 - 4), ("lens_out", "free", 4 * 49), ("lens_out", "count", -76), ("lens_out", "starts", 80),
+    ("lens_out", "slots", 0), ("lens_out", "positions", 16), ("lens_out", "count_out", 0), ("count_out", "lens", 40), ("count_out", "new", 76),
+    ("count_out", "table", 8), ("count_out", "free", 4 * 49), ("count_out", "starts", 80), ("count_out", "slots", 4), ("count_out", "count", 2)])
+def test_lengths_and_count_that_share_memory_with_something_else(out, what, shift):
+    # 20 requests with 5 columns, a stack of 50, 7 tokens
+    a = dict(AT)
+    a[out] = a[what] + shift
+    L = _lib.lib()
+    extend = L.ecq_kv4_extend(a["lens"], a["new"], a["lens_out"], a["table"], 5, 5, 20, 16, a["free"], 50, a["count"], a["count_out"],
+                              a["starts"], a["slots"], a["positions"], 7, None, None)
+    assert extend == -1
+    if what in ("lens", "table", "free", "count", "count_out"):
+        assert L.ecq_kv4_release(a["done"], a["lens"], a["lens_out"], a["table"], 5, 5, 20, 16, a["free"], 50, a["count"], a["count_out"],
+                                 None, None) == -1
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls would run")
+@pytest.mark.parametrize("out,what,shift", [("lens_out", "lens", 0), ("lens_out", "new", 80), ("lens_out", "new", -80), ("lens_out", "table", 400),
+                                            ("count_out", "count", 0), ("count_out", "slots", 28), ("count_out", "free", -4)])
+def test_lengths_and_count_beside_other_memory_are_not_refused(out, what, shift):
+    a = dict(AT)
+    a[out] = a[what] + shift
+    assert _lib.lib().ecq_kv4_extend(a["lens"], a["new"], a["lens_out"], a["table"], 5, 5, 20, 16, a["free"], 50, a["count"], a["count_out"],
+                                     a["starts"], a["slots"], a["positions"], 7, None, None) != -1
