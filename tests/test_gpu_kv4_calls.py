@@ -62,3 +62,20 @@ def test_an_output_whose_rows_share_memory_is_refused():
                 torch.zeros(1000, device="cuda").half().as_strided((2, 4, 64), (32, 128, 1))):
         with pytest.raises(ValueError, match="share memory"):
             ecq.kv4_attention(q, pages, table, i32([40, 17]), group_size=32, out=out)
+
+
+@pytest.mark.parametrize("tp", [2, 4])
+def test_the_decoders_ranks_hold_their_heads_of_the_4bit_cache(tp):
+    from ecq_b200.model import Llama7BConfig, Llama7BDecoder
+
+    cfg = Llama7BConfig(layers=2, hidden=2048, heads=16, head_dim=128, mlp=2048, vocab=1000, kv_len=100)
+    whole = Llama7BDecoder(cfg, tp=1, seed=5, kv_cache="int4").cache
+    for rank in range(tp):
+        mine = Llama7BDecoder(cfg, tp=tp, rank=rank, seed=5, exchange="nccl", kv_cache="int4").cache
+        assert torch.equal(mine.block_table, whole.block_table) and torch.equal(mine.seq_lens, whole.seq_lens)
+        n = cfg.heads // tp
+        q = torch.randn(1, cfg.heads, 128, device="cuda").half()
+        for layer in range(cfg.layers):
+            assert torch.equal(mine.pages[layer], whole.pages[layer][:, rank * n:(rank + 1) * n])
+            mine.attention(layer, q[:, rank * n:(rank + 1) * n])
+        mine.check()

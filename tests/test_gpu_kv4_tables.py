@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import ecq_b200 as ecq  # noqa: E402
-from test_gpu_kv4 import BADARG, i32  # noqa: E402
+from test_gpu_kv4 import BADARG, Model, i32  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -132,3 +132,34 @@ def test_release_refuses_bad_pages(page, batch, cols, in_place, last):
     pages = [p for b in range(batch) if done[b] for p in range(b * cols, (b + 1) * cols)]
     assert status.item() == 0 and got[1].item() == 2 + len(pages) and free[2:2 + len(pages)].tolist() == pages
     assert got[0].tolist() == [0 if d else n for n, d in zip(lens, done)]
+
+
+@pytest.mark.parametrize("batch,page,most", [(1, 16, 1), (1, 64, 5000), (17, 16, 40), (512, 32, 70), (513, 16, 3), (1100, 256, 30),
+                                             (700, 16, 400), (8192, 16, 2)])
+def test_extend_and_release_in_place_over_many_steps(batch, page, most):
+    """As a cache calls them: lengths and count in place, on a cluster of CTAs where there is much to write."""
+    rng = random.Random(batch + page)
+    cols = -(-3 * most // page) + 1
+    n_pages = batch * cols
+    m = Model(batch, cols, page, n_pages)
+    lens, count, free, status = i32([0] * batch), i32([n_pages]), i32(m.free), i32([0])
+    table = torch.full((batch, cols), -1, dtype=torch.int32, device="cuda")
+    for step in range(6):
+        new = [rng.choice([0, 1, rng.randint(0, most)]) if n + most <= cols * page else 0 for n in m.lens]
+        if step == 0:
+            new[-1] = most
+        pad = sum(new) + rng.randint(0, 5)
+        starts, slots, pos = m.extend(new)
+        st = ecq.kv4_extend(lens, i32(new), table, free, count, page, pad, status=status, seq_lens_out=lens, free_count_out=count)
+        assert st.seq_lens is lens and lens.tolist() == m.lens and st.q_starts.tolist() == starts
+        assert st.slots.tolist() == slots + [-1] * (pad - len(slots)) and st.positions.tolist() == pos + [-1] * (pad - len(pos))
+        assert count.item() == len(m.free)
+        got = table.cpu().numpy()
+        for b, row in enumerate(m.rows):
+            assert got[b, :len(row)].tolist() == row
+        done = [rng.random() < 0.4 for _ in range(batch)]
+        m.release(done)
+        ecq.kv4_release(torch.tensor(done, device="cuda"), lens, table, free, count, page, status=status, seq_lens_out=lens,
+                        free_count_out=count)
+        assert lens.tolist() == m.lens and count.item() == len(m.free) and free[:len(m.free)].tolist() == m.free
+    assert sorted([p for r in m.rows for p in r] + m.free) == list(range(n_pages)) and status.item() == 0

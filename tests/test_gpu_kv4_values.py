@@ -1,12 +1,14 @@
 """Attention over the 4-bit KV cache where values, scores or lengths are at the
-ends of their ranges."""
+ends of their ranges, and with a bound on the error that one key too many or too
+few does not pass."""
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import ecq_b200 as ecq  # noqa: E402
-from test_gpu_kv4 import BADARG, DTYPES, LAYOUTS, check_attention, decode, i32, reference  # noqa: E402
+from kv4_checks import bounds, errors, within  # noqa: E402
+from test_gpu_kv4 import BADARG, DTYPES, LAYOUTS, check_attention, decode, fill, i32, reference  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -250,3 +252,38 @@ def test_negative_lengths_are_reported_and_their_rows_zero(heads, new, room, len
     assert status.item() == 0
     got = ecq.kv4_attention(q, pages, wide, i32([n, length]), starts, new, group_size=g, status=status)
     assert status.item() == BADARG and torch.equal(got, want) and not bool(got[new:].any())
+
+
+# -- one key too many or too few ------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,g", LAYOUTS)
+@pytest.mark.parametrize("lens,new,heads,share,page", [
+    ([1500], [130], 80, 8, 64), ([300, 5, 64], [257, 1, 64], 64, 2, 16), ([128, 129, 191, 192, 193], [128, 65, 100, 64, 193], 64, 1, 32),
+    ([2500, 700], [300, 400], 8, 4, 256)])                                # prompts
+def test_prompts_see_all_their_keys_and_no_others(dtype, dim, g, lens, new, heads, share, page):
+    exactly(lens, new, heads, share, dim, g, page, dtype, 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,g", LAYOUTS)
+@pytest.mark.parametrize("lens,new,heads,share,page,room", [
+    ([2049], [1], 8, 1, 64, 1), ([700, 64, 65, 999], [1, 1, 1, 1], 2, 7, 16, 1), ([6000, 129], [1, 1], 2, 4, 64, 2000),
+    ([1500, 400, 64], [6, 3, 5], 8, 4, 32, 1), ([1500, 400, 640], [6, 3, 5], 2, 4, 32, 4000)])
+def test_steps_see_all_their_keys_and_no_others(dtype, dim, g, lens, new, heads, share, page, room):
+    exactly(lens, new, heads, share, dim, g, page, dtype, room)
+
+
+def exactly(lens, new, heads, share, dim, g, page, dtype, room):
+    pages, table = fill(lens, heads, dim, g, page, sum(lens), dtype)       # keys and values without a common part
+    wide = torch.full((len(lens), max(room, table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = randn(starts[-1], heads * share, dim, seed=7).to(dtype)
+    got = ecq.kv4_attention(q, pages, wide, i32(lens), i32(starts), max(new), group_size=g)
+    want = reference(q, pages, table, lens, starts, page, dim, g)[0]
+    for b in range(len(lens)):
+        at = slice(starts[b], starts[b + 1])
+        assert within(got[at], want[at], heads, dtype), (b, errors(got[at], want[at], heads), bounds(dtype))
