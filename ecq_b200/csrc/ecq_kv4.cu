@@ -376,25 +376,24 @@ template <int D, int kPer>
 struct RowLane {
     static constexpr int kUnit = D / 4;  // lanes per token and head
     static constexpr int kTokens = kRowThreads / kUnit;
-    unsigned token;  // below 2^32 behind the last of 2^31 - 1 tokens too
-    int c;           // channels 8c .. 8c + 7
+    int token, c;  // channels 8c .. 8c + 7
+    int left;      // tokens from there on (an index behind 2^31 - 1 of them is no int)
     bool is_v;
-    __device__ __forceinline__ RowLane() {
+    __device__ __forceinline__ RowLane(int tokens) {
         const int l = threadIdx.x % kUnit;
-        token = blockIdx.x * (kTokens * kPer) + threadIdx.x / kUnit;
+        const unsigned first = blockIdx.x * (kTokens * kPer) + threadIdx.x / kUnit;
+        token = static_cast<int>(first);
+        left = first < static_cast<unsigned>(tokens) ? tokens - token : 0;
         is_v = l >= D / 8;
         c = l % (D / 8);
     }
 };
 // The slots of the thread's rows; -1: none. One beyond the pool is reported.
 template <int D, int kPer>
-__device__ __forceinline__ void row_slots(int (&slot)[kPer], const RowLane<D, kPer>& me, const int32_t* slots, int tokens,
+__device__ __forceinline__ void row_slots(int (&slot)[kPer], const RowLane<D, kPer>& me, const int32_t* slots,
                                           int64_t n_slots, int32_t* status) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const unsigned token = me.token + i * me.kTokens;
-        slot[i] = token < static_cast<unsigned>(tokens) ? slots[token] : -1;
-    }
+    for (int i = 0; i < kPer; ++i) slot[i] = i * me.kTokens < me.left ? slots[me.token + i * me.kTokens] : -1;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
         if (slot[i] >= n_slots) {
@@ -426,12 +425,12 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const T* __restrict
                                                             int tokens, int32_t* status) {
     constexpr int kGroupLanes = D / G / 8;
     pdl_launch_dependents();
-    const RowLane<D, kPer> me;
+    const RowLane<D, kPer> me(tokens);
     const int64_t step = me.is_v ? v_token : k_token;
     const T* src = (me.is_v ? v + blockIdx.y * v_head : k + blockIdx.y * k_head) + me.token * step + 8 * me.c;
     pdl_wait();
     int slot[kPer];
-    row_slots(slot, me, slots, tokens, n_slots, status);
+    row_slots(slot, me, slots, n_slots, status);
     uint4 raw[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -506,12 +505,12 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, 
                                                             const int32_t* __restrict__ slots, int tokens,
                                                             int32_t* status) {
     pdl_launch_dependents();
-    const RowLane<D, kPer> me;
+    const RowLane<D, kPer> me(tokens);
     const int64_t step = static_cast<int64_t>(heads) * D;
     T* dst = (me.is_v ? v : k) + me.token * step + blockIdx.y * D + 8 * me.c;
     pdl_wait();
     int slot[kPer];
-    row_slots(slot, me, slots, tokens, n_slots, status);
+    row_slots(slot, me, slots, n_slots, status);
     uint32_t word[kPer], par[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -534,7 +533,7 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(T* __restrict__ k, 
             const uint32_t c = (x >> (4 * i)) & 15u;
             f[i] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, p.x, p.y);
         }
-        if (me.token + n * me.kTokens < static_cast<unsigned>(tokens))
+        if (n * me.kTokens < me.left)
             *reinterpret_cast<uint4*>(dst + n * me.kTokens * step) =
                 make_uint4(from_float2<T>(f[0], f[1]), from_float2<T>(f[2], f[3]), from_float2<T>(f[4], f[5]),
                            from_float2<T>(f[6], f[7]));
