@@ -21,11 +21,14 @@
 // instructions fewer of 330. q is scaled to its row's largest power of two and
 // exact in fp16.
 //
-// What bounds it: the ~265 instructions per 16 tokens and head, issued by 8
-// warps per SM, and for short contexts launches and joins. Measured: 32 requests
-// of 4-8k tokens, 8 cache heads shared by 4: 58 us, 3.9 TB/s of the 6.55 that a
-// copy reaches; one request of 131071 tokens, shared by 8: 40 us, 3.8 TB/s; 32
-// heads of 2049 tokens: 8.8 us, 1.0 TB/s.
+// What bounds it: the latency of instructions that wait for one another, with
+// two warps per scheduler (8 per SM, 255 registers each) to hide it. Of ~267
+// instructions per 16 tokens and head a scheduler issues one in 39 % of the
+// cycles, the ALU is busy in 47 % and the tensor cores in 27 %. For short contexts
+// it is launches and joins. Measured: 32 requests of 4-8k tokens, 8 cache heads
+// shared by 4: 58 us, 3.9 TB/s of the 6.55 that a copy reaches; one request of
+// 131071 tokens, shared by 8: 40 us, 3.8 TB/s; 32 heads of 2049 tokens: 8.9 us,
+// 1.0 TB/s; 16 requests of 3-6 tokens and 1.5-4k keys, 8 shared by 4: 48 us.
 //
 // Layout of the work. The (request, cache head, row tile, unit of 32 or 64 tokens) space
 // is flattened and cut into one even range per CTA (one wave of CTAs), from the
@@ -72,10 +75,10 @@ constexpr int NT = 1;
 // below the largest (most of a long context) out of fp16's subnormals, whose
 // step of 2^-24 would be felt in sums of thousands of them. weight * scale
 // then overflows fp16 from a scale of 16: that is seen, and the unit's weights go
-// in times 2^-13 (any finite scale's product is finite then; weights are at
-// least 2^-24 of the largest that they can be) and its part of o comes out times
-// 2^13. The reference stays: one that moved by less than its own rounding would
-// not be the one that the earlier sums were divided by.
+// in times 2^-13 (at most 2^-1, so any finite scale's product is finite; what
+// fp16 loses of them there is 2^-25) and its part of o comes out times 2^13. The
+// reference stays as it is: raised by less than a step of its own, it would not
+// be what the earlier sums are then multiplied for.
 constexpr float kSlack = 2.f, kLift = 10.f;
 constexpr int kMostRanks = 8;  // CTAs that share a pair
 
@@ -1066,7 +1069,7 @@ int stream_rows(int batch, int kv_heads) {
 // was cut. Clusters have neither, and are taken where that counts: all of them
 // fit on the GPU at once, and the longest request that the tables have room for
 // is a few steps of its cluster's warps (7b step, 32 pairs of up to 2112 tokens:
-// 14.4 us with ranges, 10.5 with clusters).
+// 13.8 us with ranges, 8.9 with clusters).
 constexpr int kMostTokens = 192;  // per warp
 struct Plan {
     int most_rows;  // of a request that is streamed

@@ -28,18 +28,20 @@
 // bits. K and V are halved (scores and outputs are doubled in fp32): a group
 // whose scale was rounded up holds values past fp16's end, up to 65584 where
 // ecq_kv4_append wrote it. Halved they keep fp16's precision; what that costs is
-// one bit of values below 2^-13. What bounds it: instructions and the exponentials (16 a cycle and SM:
-// 1024 cycles a step at D = 128, the products 1152, measured 2170). Measured: 37
+// one bit of values below 2^-13.
+//
+// What bounds it: instructions and the exponentials (16 a cycle and SM: 1024
+// cycles a step at D = 128, the products 1152, measured 2240). Measured: 37
 // heads, 1024 rows and 32768 keys 603 us, 1055 TFLOP/s of 1718; four prompt
-// chunks of 500-632 tokens with 2.5-4k keys, 32 heads 154 us, 950 TFLOP/s: two
+// chunks of 500-632 tokens with 2.5-4k keys, 32 heads 156 us, 934 TFLOP/s: two
 // waves of CTAs, each of which starts and ends alone on its SM.
 //
 // Masks. Keys beyond a row's own are chosen away in S. A V row whose scale or
 // zero is not finite (or whose values leave even the doubled range, as bytes
 // that ecq_kv4_append never writes can) would reach rows that do not see it (0 *
 // NaN), so it enters as 0 and the first such token per group of channels is
-// remembered: rows that see it get NaN there at the end. Keys of a page whose number is bad
-// are left out.
+// remembered: rows that see it get NaN there at the end. Keys of a page whose
+// number is bad are left out.
 //
 // Every wait is bounded and looks at a flag that a wait sets which gave up; all
 // roles then leave, and tensor memory is given back after the products in
