@@ -65,10 +65,10 @@ constexpr int kCtasPerSm = 2;
 // four groups four blocks do not fit the registers (16
 // requests of 3-6 tokens and four groups: 55 us, with two blocks 48).
 __host__ __device__ constexpr int unit_blocks(int groups) { return groups <= 2 ? 4 : 2; }
-// Row tiles of 8 that a warp takes at once. Two of them are one pass over the
-// keys for 16 rows, but leave registers for two blocks a step only, and took as
-// long (128 pairs of 4096 tokens, 16 rows: 49.6 against 47.4 us).
-constexpr int NT = 1;
+// A warp takes one tile of 8 rows. Two at once were one pass over the keys for
+// 16 rows, but left registers for two blocks a step only, and took as long (128
+// pairs of 4096 tokens, 16 rows: 49.6 against 47.4 us).
+constexpr int kTileRows = 8;
 // Weights are exp2(score - reference + kLift). The reference is raised when a
 // score passes it by more than kSlack, so few blocks raise it and the others
 // need no reduction over their tokens. The lift keeps the weights of keys far
@@ -85,7 +85,7 @@ constexpr int kMostRanks = 8;  // CTAs that share a pair
 // How the weights are held: once, twice, or twice in the columns of a row.
 enum Weights { kOnce, kTwice, kFolded };
 template <int W>
-__host__ __device__ constexpr int tile_rows() { return W == kFolded ? 4 : 8 * NT; }
+__host__ __device__ constexpr int tile_rows() { return W == kFolded ? 4 : kTileRows; }
 
 __host__ __device__ constexpr int ring_slots(int dim, int groups, int unit, int besides) {
     const int room = 110 * 1024 - kWarps * 8 * (dim + 4) * 4 - besides;
@@ -189,110 +189,104 @@ __device__ __forceinline__ void load(float (&x)[V], const float* p) {
 // The query rows of one tile as B operands, and what their scores need.
 template <int D, int G>
 struct Rows {
-    uint32_t b[NT][D / 16][2];
-    uint32_t sums[NT][2];  // B operand that takes (scale, zero) pairs: (0, sum of the group's q), high and low part
-    float factor[NT][2];   // scale log2(e) 2^24 / the row's power of two, less where scores are huge (raise_far)
-    uint32_t own;          // where that is in shared memory as it was
-    int limit[NT][2];      // keys that the column's row sees
-    int least;             // the smallest limit of rows that exist
+    uint32_t b[D / 16][2];
+    uint32_t sums[2];  // B operand that takes (scale, zero) pairs: (0, sum of the group's q), high and low part
+    float factor[2];   // scale log2(e) 2^24 / the row's power of two, less where scores are huge (raise_far)
+    uint32_t own;      // where that is in shared memory as it was
+    int limit[2];      // keys that the column's row sees
+    int least;         // the smallest limit of rows that exist
 };
 
 // A lane's share of the tile's rows as they lie in memory: the loads are issued
 // early and set_rows makes the operands of them.
 template <typename T, int D, int W>
-__device__ __forceinline__ void load_rows(uint4 (&raw)[NT][D / 32], const Args& a, const Request& rq, int head, int tile) {
+__device__ __forceinline__ void load_rows(uint4 (&raw)[D / 32], const Args& a, const Request& rq, int head, int tile) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
+    const int row = W == kFolded ? tile * 4 + (n & 3) : tile * 8 + n, i = row / a.share;
+    const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
+                   static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int row = W == kFolded ? tile * 4 + (n & 3) : (tile * NT + nt) * 8 + n, i = row / a.share;
-        const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(rq.first_q + i) * a.q_token +
-                       static_cast<int64_t>(head * a.share + row - i * a.share) * a.q_head + 8 * t;
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-            raw[nt][w] = make_uint4(0, 0, 0, 0);
-            if (row < rq.rows) raw[nt][w] = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
-        }
+    for (int w = 0; w < D / 32; ++w) {
+        raw[w] = make_uint4(0, 0, 0, 0);
+        if (row < rq.rows) raw[w] = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
     }
 }
 
 template <typename T, int D, int G, int W>
-__device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D / 32], const Args& a,
+__device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[D / 32], const Args& a,
                                          const Request& rq, int tile, float (*own)[2]) {
     const int lane = threadIdx.x & 31, t = lane & 3, n = lane >> 2;
     R.least = rq.len;
+    const int row = W == kFolded ? tile * 4 + (n & 3) : tile * 8 + n;
+    const bool in = row < rq.rows;
+    float x[D / 32][8];
+    float top = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int row = W == kFolded ? tile * 4 + (n & 3) : (tile * NT + nt) * 8 + n;
-        const bool in = row < rq.rows;
-        float x[D / 32][8];
-        float top = 0.f;
+    for (int w = 0; w < D / 32; ++w) {
+        const uint32_t us[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-            const uint32_t us[4] = {raw[nt][w].x, raw[nt][w].y, raw[nt][w].z, raw[nt][w].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = cvt2(us[e], T());
-                x[w][2 * e] = f.x;
-                x[w][2 * e + 1] = f.y;
-                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = cvt2(us[e], T());
+            x[w][2 * e] = f.x;
+            x[w][2 * e + 1] = f.y;
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // rows are brought to [2^14, 2^15): elements down to 2^-28 of the largest, and a sixteenth of them, keep
-        // their bits in fp16. A negative scale turns the row's sign; with none every score is 0.
-        const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
-        float up = __int_as_float((14 - ex + 127) << 23);
-        // the products reach 2^14 (128 channels of 65504 times 2^15, times 2^-24): a factor of up to 2^112 keeps scores
-        // finite. What a larger one would tell apart (nonzero differences of products are 2^-72 and more) this one does.
-        constexpr float kMostFactor = 5.192296858534828e33f;
-        float factor = fabsf(a.scale) * 1.4426950408889634f * (__int_as_float((ex - 14 + 127) << 23) * 16777216.f);
-        if (factor > kMostFactor) factor = kMostFactor;
-        if (a.scale < 0.f) up = -up;
-        if (factor == 0.f) {
-            up = 0.f;
-            factor = 1.f;
-        }
-        float sums[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) sums[g] = 0.f;
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[w][e] = __half2float(__float2half_rn(x[w][e] * up));
-                sums[w * 32 * G / D] += x[w][e];
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                R.b[nt][2 * w + h][0] = h2(x[w][2 * h], x[w][4 + 2 * h]);
-                R.b[nt][2 * w + h][1] = h2(x[w][1 + 2 * h] * 0.0625f, x[w][5 + 2 * h] * 0.0625f);
-            }
-        }
-        // query i sees keys up to len - queries + i
-        const int limit = in ? rq.len - rq.queries + row / a.share + 1 : rq.len;
-        int least = max(limit, 0);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-        R.least = min(R.least, least);
-        float mine = 0.f;  // lane t has group t's sum (at most 2^22), times 2^-24
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
-            if (t == g) mine = sums[g] * 5.9604644775390625e-8f;
-        }
-        const float high = __half2float(__float2half_rn(mine));
-        R.sums[nt][0] = h2(0.f, high);
-        R.sums[nt][1] = h2(0.f, mine - high);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {  // column 2t + c is row 2t + c of the tile: lane 4 (2t + c) has it
-            const int from = 4 * (2 * t + c);
-            R.factor[nt][c] = __shfl_sync(0xffffffffu, factor, from);
-            R.limit[nt][c] = __shfl_sync(0xffffffffu, limit, from);
-        }
-        if (n == 0) own[nt * 4 + t][0] = R.factor[nt][0], own[nt * 4 + t][1] = R.factor[nt][1];
     }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // rows are brought to [2^14, 2^15): elements down to 2^-28 of the largest, and a sixteenth of them, keep
+    // their bits in fp16. A negative scale turns the row's sign; with none every score is 0.
+    const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
+    float up = __int_as_float((14 - ex + 127) << 23);
+    // the products reach 2^14 (128 channels of 65504 times 2^15, times 2^-24): a factor of up to 2^112 keeps scores
+    // finite. What a larger one would tell apart (nonzero differences of products are 2^-72 and more) this one does.
+    constexpr float kMostFactor = 5.192296858534828e33f;
+    float factor = fabsf(a.scale) * 1.4426950408889634f * (__int_as_float((ex - 14 + 127) << 23) * 16777216.f);
+    if (factor > kMostFactor) factor = kMostFactor;
+    if (a.scale < 0.f) up = -up;
+    if (factor == 0.f) {
+        up = 0.f;
+        factor = 1.f;
+    }
+    float sums[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) sums[g] = 0.f;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[w][e] = __half2float(__float2half_rn(x[w][e] * up));
+            sums[w * 32 * G / D] += x[w][e];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            R.b[2 * w + h][0] = h2(x[w][2 * h], x[w][4 + 2 * h]);
+            R.b[2 * w + h][1] = h2(x[w][1 + 2 * h] * 0.0625f, x[w][5 + 2 * h] * 0.0625f);
+        }
+    }
+    // query i sees keys up to len - queries + i
+    const int limit = in ? rq.len - rq.queries + row / a.share + 1 : rq.len;
+    int least = max(limit, 0);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+    R.least = min(R.least, least);
+    float mine = 0.f;  // lane t has group t's sum (at most 2^22), times 2^-24
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        if (t == g) mine = sums[g] * 5.9604644775390625e-8f;
+    }
+    const float high = __half2float(__float2half_rn(mine));
+    R.sums[0] = h2(0.f, high);
+    R.sums[1] = h2(0.f, mine - high);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {  // column 2t + c is row 2t + c of the tile: lane 4 (2t + c) has it
+        const int from = 4 * (2 * t + c);
+        R.factor[c] = __shfl_sync(0xffffffffu, factor, from);
+        R.limit[c] = __shfl_sync(0xffffffffu, limit, from);
+    }
+    if (n == 0) own[t][0] = R.factor[0], own[t][1] = R.factor[1];
     R.own = smem_addr(own) + 8 * t;
     __syncwarp();
 }
@@ -300,21 +294,18 @@ __device__ __forceinline__ void set_rows(Rows<D, G>& R, const uint4 (&raw)[NT][D
 // Running softmax of one warp over its blocks.
 template <int D, int G>
 struct State {
-    float o[NT][D / 16][4];
-    float sums[NT][2];  // columns 2t, 2t + 1; lanes of row r < G: sum p zero of group r; of row G: sum p
-    float m[NT][2];
+    float o[D / 16][4];
+    float sums[2];  // columns 2t, 2t + 1; lanes of row r < G: sum p zero of group r; of row G: sum p
+    float m[2];
     bool far;  // some row's factor has gone down
     __device__ __forceinline__ void reset() {
         far = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
-            sums[nt][0] = sums[nt][1] = 0.f;
-            m[nt][0] = m[nt][1] = kNoMax;
-        }
+            for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+        sums[0] = sums[1] = 0.f;
+        m[0] = m[1] = kNoMax;
     }
 };
 
@@ -367,7 +358,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
                                        const int (&first)[U]) {
     constexpr int W = D / 32, BB = block_bytes(D, G);
     const int r = (threadIdx.x & 31) >> 2, tok = token_of(r);
-    float s[U][NT][4];
+    float s[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         uint32_t k0[W], k1[W], kp[2][G], pair[2][1];
@@ -380,20 +371,15 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
         // sum over the groups of zero * (sum of q): the pairs (scale, zero) as they lie are an A operand (lanes past the
         // last group meet zeros in B). Then, per group, the codes.
         constexpr int A = G > 2 ? G : 2;  // accumulators: neighbouring steps go to different ones
-        float acc[NT][A][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-            mma_first(s[u][nt], pair[0][0], pair[1][0], pair[0][0], pair[1][0], R.sums[nt][0], R.sums[nt][1]);
+        float acc[A][4];
+        mma_first(s[u], pair[0][0], pair[1][0], pair[0][0], pair[1][0], R.sums[0], R.sums[1]);
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) {
             const int n = i % A, step = n * (2 * W / A) + i / A, w = step / 2, h = step % 2;
             const uint32_t x0 = h ? k0[w] >> 8 : k0[w], x1 = h ? k1[w] >> 8 : k1[w];
             const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (i < A) mma_first(acc[nt][n], a0, a1, a2, a3, R.b[nt][step][0], R.b[nt][step][1]);
-                else mma(acc[nt][n], a0, a1, a2, a3, R.b[nt][step][0], R.b[nt][step][1]);
-            }
+            if (i < A) mma_first(acc[n], a0, a1, a2, a3, R.b[step][0], R.b[step][1]);
+            else mma(acc[n], a0, a1, a2, a3, R.b[step][0], R.b[step][1]);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -401,61 +387,52 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
             for (int n = 0; n < A; ++n) {
                 const float scale = f2(kp[i][n * G / A]).x;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) s[u][nt][2 * i + c] = fmaf(scale, acc[nt][n][2 * i + c], s[u][nt][2 * i + c]);
+                for (int c = 0; c < 2; ++c) s[u][2 * i + c] = fmaf(scale, acc[n][2 * i + c], s[u][2 * i + c]);
             }
         if (kMask) {
             // a token out of sight, or behind the last, may hold anything: it is chosen away, not computed away
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (first[u] + tok + 8 * (c >> 1) >= R.limit[nt][c & 1]) s[u][nt][c] = -INFINITY;
+            for (int c = 0; c < 4; ++c)
+                if (first[u] + tok + 8 * (c >> 1) >= R.limit[c & 1]) s[u][c] = -INFINITY;
         }
     }
+    float top[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float top[2];
+    for (int c = 0; c < 2; ++c) {
+        top[c] = fmaxf(s[0][c], s[0][c + 2]);
+#pragma unroll
+        for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][c], s[u][c + 2]));
+    }
+    if (__any_sync(0xffffffffu, fmaf(top[0], R.factor[0], -S.m[0]) > kSlack + kLift ||
+                                    fmaf(top[1], R.factor[1], -S.m[1]) > kSlack + kLift)) {
+        float held[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            top[c] = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
-            for (int u = 1; u < U; ++u) top[c] = fmaxf(top[c], fmaxf(s[u][nt][c], s[u][nt][c + 2]));
+            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+            held[c] = S.m[c];
+            S.m[c] = fmaxf(fmaf(top[c], R.factor[c], -kLift), held[c]);
         }
-        if (__any_sync(0xffffffffu, fmaf(top[0], R.factor[nt][0], -S.m[nt][0]) > kSlack + kLift ||
-                                        fmaf(top[1], R.factor[nt][1], -S.m[nt][1]) > kSlack + kLift)) {
-            float held[2];
+        if (S.far || __any_sync(0xffffffffu, fmaxf(fabsf(S.m[0]), fabsf(S.m[1])) > kNear)) {
+            uint32_t own[2];
+            lds<2, 0>(own, R.own);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 2; ++c)
+                if (S.m[c] > held[c]) raise_far(S.m[c], held[c], R.factor[c], top[c], __uint_as_float(own[c]), kLift);
+            S.far = S.far || __any_sync(0xffffffffu, R.factor[0] != __uint_as_float(own[0]) || R.factor[1] != __uint_as_float(own[1]));
+        }
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-                held[c] = S.m[nt][c];
-                S.m[nt][c] = fmaxf(fmaf(top[c], R.factor[nt][c], -kLift), held[c]);
-            }
-            if (S.far || __any_sync(0xffffffffu, fmaxf(fabsf(S.m[nt][0]), fabsf(S.m[nt][1])) > kNear)) {
-                uint32_t own[2];
-                lds<2, 0>(own, R.own + 32 * nt);
+        for (int c = 0; c < 2; ++c) {
+            const float keep = exp2_fast(held[c] - S.m[c]);
+            S.sums[c] *= keep;
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    if (S.m[nt][c] > held[c])
-                        raise_far(S.m[nt][c], held[c], R.factor[nt][c], top[c], __uint_as_float(own[c]), kLift);
-                S.far = S.far || __any_sync(0xffffffffu, R.factor[nt][0] != __uint_as_float(own[0]) ||
-                                                             R.factor[nt][1] != __uint_as_float(own[1]));
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float keep = exp2_fast(held[c] - S.m[nt][c]);
-                S.sums[nt][c] *= keep;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    S.o[nt][i][c] *= keep;
-                    S.o[nt][i][c + 2] *= keep;
-                }
+            for (int i = 0; i < D / 16; ++i) {
+                S.o[i][c] *= keep;
+                S.o[i][c + 2] *= keep;
             }
         }
     }
-    uint32_t ph[U][NT][2], pl[U][NT][2], hi[U][NT][G][2], lo[U][NT][G][2];
+    uint32_t ph[U][2], pl[U][2], hi[U][G][2], lo[U][G][2];
     // the weights and their products with V's scales, those of kDown times 2^-13; the largest of them
     auto weights = [&](auto down) {
         constexpr bool kDown = decltype(down)::value;
@@ -463,17 +440,15 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int i = 0; i < 2; ++i) {
+                float p[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float p[2];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) p[c] = exp2_fast(fmaf(s[u][nt][2 * i + c], R.factor[nt][c], -S.m[nt][c]));
-                    const uint32_t x = h2(p[0], p[1]);
-                    const float2 back = f2(x);
-                    ph[u][nt][i] = transpose(x);
-                    if (kWeights != kOnce) pl[u][nt][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
-                }
+                for (int c = 0; c < 2; ++c) p[c] = exp2_fast(fmaf(s[u][2 * i + c], R.factor[c], -S.m[c]));
+                const uint32_t x = h2(p[0], p[1]);
+                const float2 back = f2(x);
+                ph[u][i] = transpose(x);
+                if (kWeights != kOnce) pl[u][i] = transpose(h2(p[0] - back.x, p[1] - back.y));
+            }
             uint32_t sa[2][G], sb[2][G];
             lds<G, 0>(sa[0], at + u * BB + me.v_params);
             lds<G, 16 * G>(sb[0], at + u * BB + me.v_params);
@@ -484,22 +459,19 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     const uint32_t sc = __byte_perm(sa[i][g], sb[i][g], 0x5410);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
-                        constexpr uint32_t kScale = 0x08000800u;  // 2^-13
-                        const uint32_t w = kDown ? mul2(ph[u][nt][i], kScale) : ph[u][nt][i];
-                        uint32_t h = mul2(w, sc), l = 0u;
-                        if (kWeights != kOnce) l = fma2h(kDown ? mul2(pl[u][nt][i], kScale) : pl[u][nt][i], sc, fma2h(w, sc, neg2(h)));
-                        if (kMask) {  // weight 0: 0, whatever the scale is
-                            const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
-                            h &= keep;
-                            l &= keep;
-                        }
-                        hi[u][nt][g][i] = kWeights == kFolded && r >= 4 ? l : h;
-                        lo[u][nt][g][i] = l;
-                        most = max2(most, abs2(h));  // a NaN passes by
+                    // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
+                    constexpr uint32_t kScale = 0x08000800u;  // 2^-13
+                    const uint32_t w = kDown ? mul2(ph[u][i], kScale) : ph[u][i];
+                    uint32_t h = mul2(w, sc), l = 0u;
+                    if (kWeights != kOnce) l = fma2h(kDown ? mul2(pl[u][i], kScale) : pl[u][i], sc, fma2h(w, sc, neg2(h)));
+                    if (kMask) {  // weight 0: 0, whatever the scale is
+                        const uint32_t keep = (w & 0xffffu ? 0xffffu : 0u) | (w & 0xffff0000u ? 0xffff0000u : 0u);
+                        h &= keep;
+                        l &= keep;
                     }
+                    hi[u][g][i] = kWeights == kFolded && r >= 4 ? l : h;
+                    lo[u][g][i] = l;
+                    most = max2(most, abs2(h));  // a NaN passes by
                 }
         }
         return most;
@@ -511,7 +483,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
         up = 0x4600000046000000ull;  // 2^13
     }
     // rows of A: the groups' zeros, then ones (the sum of the weights)
-    float sums[NT][4];
+    float sums[4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         uint32_t za[2][1], zb[2][1], z[2];
@@ -528,20 +500,14 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
             }
             z[i] = r == G ? 0x3c003c00u : z[i];
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const bool rest = kWeights == kFolded && r >= 4;
-            const uint32_t p0 = rest ? pl[u][nt][0] : ph[u][nt][0], p1 = rest ? pl[u][nt][1] : ph[u][nt][1];
-            if (u == 0) mma_first(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
-            else mma(sums[nt], z[0], 0u, z[1], 0u, p0, p1);
-            if (kWeights == kTwice) mma(sums[nt], z[0], 0u, z[1], 0u, pl[u][nt][0], pl[u][nt][1]);
-        }
+        const bool rest = kWeights == kFolded && r >= 4;
+        const uint32_t p0 = rest ? pl[u][0] : ph[u][0], p1 = rest ? pl[u][1] : ph[u][1];
+        if (u == 0) mma_first(sums, z[0], 0u, z[1], 0u, p0, p1);
+        else mma(sums, z[0], 0u, z[1], 0u, p0, p1);
+        if (kWeights == kTwice) mma(sums, z[0], 0u, z[1], 0u, pl[u][0], pl[u][1]);
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        S.sums[nt][0] += sums[nt][0];
-        S.sums[nt][1] += sums[nt][1];
-    }
+    S.sums[0] += sums[0];
+    S.sums[1] += sums[1];
     // The unit's part of o starts from 0 and is added with a rounded fp32 sum: codes are 0..15 and the zeros take about 7.5
     // of that away again, so what a running sum loses to the tensor core's truncation would be many times as much in o.
     constexpr int VW = D / 64;  // words of a lane's chunk of a V row
@@ -558,7 +524,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const uint32_t pick = half ? 0x7632u : 0x5410u;
-            float t[2][NT][4];
+            float t[2][4];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t x = __byte_perm(v[u][0][w], v[u][1][w], pick), y = __byte_perm(v[u][2][w], v[u][3][w], pick);
@@ -569,18 +535,14 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
                         const int g = (4 * w + 2 * half + j) * 16 * G / D;
                         const uint32_t xs = j ? x >> 8 : x, ys = j ? y >> 8 : y;
                         const uint32_t a0 = xs & 0x000f000fu, a1 = xs & 0x00f000f0u, a2 = ys & 0x000f000fu, a3 = ys & 0x00f000f0u;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t(&p)[2] = part ? lo[u][nt][g] : hi[u][nt][g];
-                            if (u == 0 && part == 0) mma_first(t[j][nt], a0, a1, a2, a3, p[0], p[1]);
-                            else mma(t[j][nt], a0, a1, a2, a3, p[0], p[1]);
-                        }
+                        const uint32_t(&p)[2] = part ? lo[u][g] : hi[u][g];
+                        if (u == 0 && part == 0) mma_first(t[j], a0, a1, a2, a3, p[0], p[1]);
+                        else mma(t[j], a0, a1, a2, a3, p[0], p[1]);
                     }
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) add4(S.o[nt][4 * w + 2 * half + j], t[j][nt], up);
+                add4(S.o[4 * w + 2 * half + j], t[j], up);
         }
 }
 
@@ -599,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
     __shared__ Request s_own;
     __shared__ uint64_t s_bar[kWarps][NS];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-    __shared__ __align__(8) float s_factor[kWarps][NT * 4][2];  // the rows' factors
+    __shared__ __align__(8) float s_factor[kWarps][4][2];  // the rows' factors
     float* s_o = reinterpret_cast<float*>(smem + kWarps * NS * UB);
     float* s_part = s_o + kWarps * 8 * OS;  // kPairs: this CTA's part of the pair
     const int lane = threadIdx.x & 31, cta = blockIdx.x;
@@ -693,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
     const int64_t pool_row = static_cast<int64_t>(page_bytes) * a.kv_heads;
     const Request rq0 = rq;
     const int head0 = head, tile0 = tile;
-    uint4 raw[NT][D / 32];
+    uint4 raw[D / 32];
     load_rows<T, D, kWeights>(raw, a, rq, head, tile);  // before the ring's copies fill the memory's queues
     int fb = b, f_head = head, f_tile = tile, f_unit = unit0 + mine, f_page[kUnit];
     int f_left = range > mine ? static_cast<int>((range - mine + step - 1) / step) : 0;
@@ -853,66 +815,62 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_kernel(const A
             a.cuts[cta] = make_int4(b_now, head_now * now.tiles + tile_now, static_cast<int>(more), 0);
         }
         constexpr int V = D / 32;
+        const int t = lane & 3, r = lane >> 2;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int t = lane & 3, r = lane >> 2;
+        for (int c = 0; c < 2; ++c) {
+            float z[G];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float z[G];
+            for (int g = 0; g < G; ++g) z[g] = __shfl_sync(0xffffffffu, st.sums[c], 4 * g + t);
+            if (r == 0) s_m[warp][2 * t + c] = st.far ? reference(st.m[c], rows.factor[c], s_factor[warp][t][c]) : st.m[c];
+            if (r == G) s_l[warp][2 * t + c] = st.sums[c];
+            float* dst = s_o + (warp * 8 + 2 * t + c) * OS + r;
 #pragma unroll
-                for (int g = 0; g < G; ++g) z[g] = __shfl_sync(0xffffffffu, st.sums[nt][c], 4 * g + t);
-                if (r == 0) s_m[warp][2 * t + c] = st.far ? reference(st.m[nt][c], rows.factor[nt][c], s_factor[warp][nt * 4 + t][c]) : st.m[nt][c];
-                if (r == G) s_l[warp][2 * t + c] = st.sums[nt][c];
-                float* dst = s_o + (warp * 8 + 2 * t + c) * OS + r;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    dst[16 * i] = fmaf(st.o[nt][i][c], 16777216.f, z[i * 16 * G / D]);
-                    dst[16 * i + 8] = fmaf(st.o[nt][i][c + 2], 1048576.f, z[i * 16 * G / D]);
-                }
+            for (int i = 0; i < D / 16; ++i) {
+                dst[16 * i] = fmaf(st.o[i][c], 16777216.f, z[i * 16 * G / D]);
+                dst[16 * i + 8] = fmaf(st.o[i][c + 2], 1048576.f, z[i * 16 * G / D]);
             }
-            __syncthreads();
-#pragma unroll
-            for (int row = warp; row < (TR < 8 ? TR : 8); row += kWarps) {
-                float M = kNoMax, L = 0.f, o[V];
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[v] = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float k = exp2_fast(s_m[w][row] - M);
-                    float x[V], l = s_l[w][row];
-                    load<V>(x, s_o + (w * 8 + row) * OS + V * lane);
-                    if (kWeights == kFolded) {
-                        float y[V];
-                        load<V>(y, s_o + (w * 8 + row + 4) * OS + V * lane);
-                        l += s_l[w][row + 4];
-#pragma unroll
-                        for (int v = 0; v < V; ++v) x[v] += y[v];
-                    }
-                    L = fmaf(k, l, L);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) o[v] = fmaf(k, x[v], o[v]);
-                }
-                const int tr = nt * 8 + row, qr = tile_now * TR + tr;
-                if (qr >= now.rows) continue;
-                if (!kPairs && starts && ends) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) o[v] = L == 0.f ? 0.f : o[v] / L;
-                    store<T, V>(out_row<T>(a, now.first_q, head_now, qr) + V * lane, o);
-                } else {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) part[TR * 2 + tr * D + V * lane + v] = o[v];
-                    if (lane == 0) {
-                        part[2 * tr] = M;
-                        part[2 * tr + 1] = L;
-                    }
-                }
-            }
-            // a warp that gave up takes the others with it: they would wait for it at the next segment's barriers
-            if (nt + 1 < NT) __syncthreads();
-            else if (__syncthreads_or(late)) late = true, f = range;
         }
+        __syncthreads();
+#pragma unroll
+        for (int tr = warp; tr < TR; tr += kWarps) {
+            float M = kNoMax, L = 0.f, o[V];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][tr]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float k = exp2_fast(s_m[w][tr] - M);
+                float x[V], l = s_l[w][tr];
+                load<V>(x, s_o + (w * 8 + tr) * OS + V * lane);
+                if (kWeights == kFolded) {
+                    float y[V];
+                    load<V>(y, s_o + (w * 8 + tr + 4) * OS + V * lane);
+                    l += s_l[w][tr + 4];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[v] += y[v];
+                }
+                L = fmaf(k, l, L);
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = fmaf(k, x[v], o[v]);
+            }
+            const int qr = tile_now * TR + tr;
+            if (qr >= now.rows) continue;
+            if (!kPairs && starts && ends) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = L == 0.f ? 0.f : o[v] / L;
+                store<T, V>(out_row<T>(a, now.first_q, head_now, qr) + V * lane, o);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) part[TR * 2 + tr * D + V * lane + v] = o[v];
+                if (lane == 0) {
+                    part[2 * tr] = M;
+                    part[2 * tr + 1] = L;
+                }
+            }
+        }
+        // a warp that gave up takes the others with it: they would wait for it at the next segment's barriers
+        if (__syncthreads_or(late)) late = true, f = range;
     }
     if constexpr (kPairs) {
         // the cluster's parts: rank r joins rows r, r + ranks, ...
@@ -1084,7 +1042,7 @@ Plan plan(int batch, int kv_heads, int share, int max_q, int max_pages, int page
     p.most_rows = stream_rows(batch, kv_heads);
     p.prompts = rows > p.most_rows;
     if (!p.prompts) p.most_rows = INT32_MAX;
-    p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8 * NT;
+    p.rows = rows <= 4 && dtype == ECQ_KV4_F16 ? 4 : 8;
     p.tiles = static_cast<int>(((rows < p.most_rows ? rows : p.most_rows) + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.tiles;
     p.ranks = kMostRanks;
@@ -1125,7 +1083,7 @@ int64_t ecq_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t 
     if (!sizes_ok(head_dim, page_size, 32) || heads / kv_heads > 64) return ECQ_ERR_UNSUPPORTED;
     // the same clusters or ranges for both types: tiles of 4 rows are taken where there is one tile of 8
     const Plan p = plan(batch, kv_heads, heads / kv_heads, max_q, max_pages, page_size, ECQ_KV4_BF16);
-    return p.ranks ? 0 : grid_ctas() * (16 + 2 * 4 * 8ll * NT * (head_dim + 2));
+    return p.ranks ? 0 : grid_ctas() * (16 + 2 * 4 * 8ll * (head_dim + 2));
 }
 
 int32_t ecq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
