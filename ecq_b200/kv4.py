@@ -17,7 +17,8 @@ into CUDA graphs) and do not synchronise. Bad values that only the device sees
 set bits of the ``status`` word.
 
 The calls are for inference: the cache's bytes carry no gradient to k and v, and
-a backward pass through ``kv4_attention`` to its q raises.
+a backward pass through a result of ``kv4_attention`` to its q raises. What is
+written into a tensor that the caller gives (``out``) carries none either.
 """
 from __future__ import annotations
 
@@ -272,10 +273,8 @@ class _NoBackward(torch.autograd.Function):
     """kv4_attention of a q that requires a gradient: the same output, which says so when one is asked for."""
 
     @staticmethod
-    def forward(ctx, q, out, call):
-        if out is not None:
-            ctx.mark_dirty(out)
-        return call(q, out)
+    def forward(ctx, q, call):
+        return call(q)
 
     @staticmethod
     def backward(ctx, grad):
@@ -296,9 +295,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     their request, each sees the tokens up to its own. scale: 1 / sqrt(head_dim)
     by default. Rows that see nothing (length 0) are 0; rows at or behind
     q_starts[-1] are left as they were in ``out``."""
-    if q.requires_grad and torch.is_grad_enabled():
-        return _NoBackward.apply(q, out, lambda q, out: kv4_attention(
-            q, pages, block_table, seq_lens, q_starts, max_q, group_size=group_size, scale=scale, out=out, status=status))
+    if q.requires_grad and out is None and torch.is_grad_enabled():
+        return _NoBackward.apply(q, lambda q: kv4_attention(
+            q, pages, block_table, seq_lens, q_starts, max_q, group_size=group_size, scale=scale, status=status))
     code, q_token, q_head = _rows("q", q)
     _fits("max_q", max_q, 1)
     device = _device(q, "pages block_table seq_lens q_starts out status", pages, block_table, seq_lens, q_starts, out, status)

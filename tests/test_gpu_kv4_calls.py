@@ -14,20 +14,25 @@ def cuda():
         pytest.skip("no CUDA device")
 
 
-@pytest.mark.parametrize("given", [False, True])
-def test_a_gradient_that_attention_does_not_have_is_said(given):
+def test_a_gradient_that_attention_does_not_have_is_said():
     pages, table = fill([40, 17], 2, 64, 32, 16, 1)
     q = torch.randn(2, 4, 64, device="cuda").half()
     want = ecq.kv4_attention(q, pages, table, i32([40, 17]), group_size=32)
     w = torch.ones(64, device="cuda", dtype=torch.float16, requires_grad=True)
-    out = torch.full_like(q, 7.0) if given else None
-    got = ecq.kv4_attention(q * w, pages, table, i32([40, 17]), group_size=32, out=out)
-    assert torch.equal(got, want) and got.requires_grad and (not given or got.data_ptr() == out.data_ptr())
+    got = ecq.kv4_attention(q * w, pages, table, i32([40, 17]), group_size=32)
+    assert torch.equal(got, want) and got.requires_grad
     with pytest.raises(RuntimeError, match="no backward"):
         got.float().sum().backward()
     assert w.grad is None
     with torch.no_grad():
         assert not ecq.kv4_attention(q * w, pages, table, i32([40, 17]), group_size=32).requires_grad
+    # a buffer that is used again stays a buffer
+    buf = torch.zeros(5, 4, 64, dtype=torch.float16, device="cuda")
+    with torch.no_grad():
+        view = buf[1:3]
+    for out in (buf[:2], view, buf[3:]):
+        got = ecq.kv4_attention(q * w, pages, table, i32([40, 17]), group_size=32, out=out)
+        assert torch.equal(got, want) and torch.equal(out, want) and not got.requires_grad and not buf.requires_grad
 
 
 @pytest.mark.parametrize("odd", [1, 4, 68])
