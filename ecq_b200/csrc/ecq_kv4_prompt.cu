@@ -7,8 +7,8 @@
 //            (cp.async.bulk, a lane per block, its page number read one step
 //            ahead);
 //   decoders four warps turn codes into fp16 K [64 x D] and four into V^T [D x
-//            64], in the tensor core's K-major, no-swizzle layout: half of code *
-//            scale + zero, rounded once to fp16, shared by all 256 rows;
+//            64], in the tensor core's K-major, no-swizzle layout: code * scale +
+//            zero, rounded once to fp16, shared by all 256 rows;
 //   MMA      one warp issues S = Q K^T and O += P V for both tiles;
 //   softmax  eight warps per tile, two threads per row with 32 keys each: S from
 //            tensor memory (its place is free for the next step's scores at
@@ -25,22 +25,20 @@
 //
 // fp16 for K, V and P costs a relative 2^-12 on average of each, next to the
 // output's own rounding; q is brought to its row's power of two and keeps its
-// bits. K and V are halved (scores and outputs are doubled in fp32): a group
-// whose scale was rounded up holds values past fp16's end, up to 65584 where
-// ecq_kv4_append wrote it. Halved they keep fp16's precision; what that costs is
-// one bit of values below 2^-13.
+// bits. A group whose scale was rounded up holds values past fp16's end, up to
+// 65584 where ecq_kv4_append wrote it: they count as 65504 (2^-9 less at most),
+// which a look at code 15's value of each group finds.
 //
 // What bounds it: instructions and the exponentials (16 a cycle and SM: 1024
-// cycles a step at D = 128, the products 1152, measured 2240). Measured: 37
-// heads, 1024 rows and 32768 keys 603 us, 1055 TFLOP/s of 1718; four prompt
-// chunks of 500-632 tokens with 2.5-4k keys, 32 heads 156 us, 934 TFLOP/s: two
+// cycles a step at D = 128, the products 1152, measured 2250). Measured: 37
+// heads, 1024 rows and 32768 keys 606 us, 1050 TFLOP/s of 1718; four prompt
+// chunks of 500-632 tokens with 2.5-4k keys, 32 heads 158 us, 922 TFLOP/s: two
 // waves of CTAs, each of which starts and ends alone on its SM.
 //
 // Masks. Keys beyond a row's own are chosen away in S. A V row whose scale or
-// zero is not finite (or whose values leave even the doubled range, as bytes
-// that ecq_kv4_append never writes can) would reach rows that do not see it (0 *
-// NaN), so it enters as 0 and the first such token per group of channels is
-// remembered: rows that see it get NaN there at the end. Keys of a page whose
+// zero is not finite would reach rows that do not see it (0 * NaN), so it
+// enters as 0 and the first such token per group of channels is remembered:
+// rows that see it get NaN there at the end. Keys of a page whose
 // number is bad are left out.
 //
 // Every wait is bounded and looks at a flag that a wait sets which gave up; all
@@ -218,20 +216,29 @@ __device__ __forceinline__ uint32_t hfma(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
-__device__ __forceinline__ uint32_t hmul(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t hadd(uint32_t a, uint32_t b) {
     uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// Half of code * scale + zero of the nibbles at bits 0..3 (low) or 4..7 of both
-// halves of x, where half_zero is zero / 2: a nibble in the mantissa of 1024 is
-// 1024 + code (or 1024 + 16 code), the fma that makes code / 2 of it is exact, and
-// the second one rounds once.
-__device__ __forceinline__ uint32_t value_low(uint32_t x, uint32_t scale, uint32_t half_zero) {
-    return hfma(hfma((x & 0x000f000fu) | 0x64006400u, 0x38003800u, 0xe000e000u), scale, half_zero);
+// Held to +-65504; a NaN stays one.
+__device__ __forceinline__ uint32_t hold(uint32_t x) {
+    asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7bff7bffu));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfbfffbffu));
+    return x;
 }
-__device__ __forceinline__ uint32_t value_high(uint32_t x, uint32_t scale, uint32_t half_zero) {
-    return hfma(hfma((x & 0x00f000f0u) | 0x64006400u, 0x28002800u, 0xd000d000u), scale, half_zero);
+// 0 where both halves of x are finite (their products with 0, summed up), else NaN in one of them
+__device__ __forceinline__ uint32_t not_finite(uint32_t x, uint32_t before) { return hfma(x, 0u, before); }
+__device__ __forceinline__ bool any_nan(uint32_t probe) { return (probe & 0x7fff7fffu) != 0u; }
+constexpr uint32_t kTop = 0x4b804b80u;  // 15, twice: a group's values are finite where its first and its last are
+// code * scale + zero of the nibbles at bits 0..3 (low) or 4..7 of both halves
+// of x: a nibble in the mantissa of 1024 is 1024 + code (or 1024 + 16 code),
+// what takes that off is exact, and the fma rounds once.
+__device__ __forceinline__ uint32_t value_low(uint32_t x, uint32_t scale, uint32_t zero) {
+    return hfma(hadd((x & 0x000f000fu) | 0x64006400u, 0xe400e400u), scale, zero);
+}
+__device__ __forceinline__ uint32_t value_high(uint32_t x, uint32_t scale, uint32_t zero) {
+    return hfma(hfma((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u), scale, zero);
 }
 
 template <typename T, int D, int G>
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                 for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const int ex = top == 0.f ? 0 : max((__float_as_int(top) >> 23) - 127, -100);
                 float up = __int_as_float((10 - ex + 127) << 23);
-                float f = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 9 + 127) << 23);  // K is halved
+                float f = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((ex - 10 + 127) << 23);
                 // the products reach 2^34 (128 channels of 65504 times 2^11): a factor of up to 2^93 keeps scores
                 // finite, and tells apart all that a larger one would (nonzero differences are 2^-48 and more)
                 constexpr float kMostFactor = 9.903520314283042e27f;
@@ -514,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             after_sync();
         }
         if (ok) {
-            const float inv = sum == 0.f ? 0.f : 2.f / sum;  // V is halved
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             // this warp's 32 rows and half of the channels through its part of the tile's q (no product reads that any
             // more), so that rows are stored together
             constexpr int kBytesRow = D, kChunks = kBytesRow / 16;
@@ -574,23 +581,35 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                         w[half][0] = u.x, w[half][1] = u.y;
                     }
 #pragma unroll
-                    for (int g = 0; g < G; ++g) p[half][g] = hmul(lds1(from_p + off + half * 2 * BB + 4 * g), 0x38003c00u);  // zero / 2
+                    for (int g = 0; g < G; ++g) p[half][g] = lds1(from_p + off + half * 2 * BB + 4 * g);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive((bars + offsetof(Control, packed_empty) + 8 * (slot)));
                 if (j >= 2 && !__all_sync(0xffffffffu, wait_for((bars + offsetof(Control, k_empty) + 8 * (stage)), ((j >> 1) - 1) & 1, gave_up, a.status)))
                     break;
+                uint32_t probe = 0u;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t dst = to + stage * S::kBytesK + half * 512;
+                for (int g = 0; g < G; ++g)
+                    probe = not_finite(hfma(__byte_perm(p[0][g], p[1][g], 0x5410), kTop, __byte_perm(p[0][g], p[1][g], 0x7632)), probe);
+                auto store = [&](auto held) {
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {
-                        const uint32_t pg = p[half][q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
-                        const uint32_t u = w[half][q], y = u >> 8;
-                        sts4(dst + 4 * q * S::kLboK, value_low(u, sc, z), value_high(u, sc, z), value_low(y, sc, z),
-                             value_high(y, sc, z));
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t dst = to + stage * S::kBytesK + half * 512;
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            const uint32_t pg = p[half][q * 32 * G / D], sc = __byte_perm(pg, pg, 0x1010), z = __byte_perm(pg, pg, 0x3232);
+                            const uint32_t u = w[half][q], y = u >> 8;
+                            uint32_t v[4] = {value_low(u, sc, z), value_high(u, sc, z), value_low(y, sc, z), value_high(y, sc, z)};
+                            if (decltype(held)::value && !any_nan(not_finite(pg, 0u))) {  // what is not finite itself stays so
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] = hold(v[i]);
+                            }
+                            sts4(dst + 4 * q * S::kLboK, v[0], v[1], v[2], v[3]);
+                        }
                     }
-                }
+                };
+                if (any_nan(probe)) store(std::true_type());
+                else store(std::false_type());
                 fence_proxy_async();
                 mbar_arrive((bars + offsetof(Control, k_full) + 8 * (stage)));
             }
@@ -625,6 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                 const bool ragged = (j + 1) * kKeys > rq.len || hidden;
                 if (has) {
                     uint32_t sc[kGroups][4], z[kGroups][4];
+                    bool past = false;  // values past fp16's end
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
                         if (ragged) {
@@ -632,27 +652,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                             for (int k = 0; k < 8; ++k)
                                 if (j * kKeys + kc * 8 + k >= rq.len || (hidden >> (kc / 2) & 1u)) p[g][k] = 0u;
                         }
-                        // half of code 15's value: where it is finite, those of all codes are
-                        constexpr uint32_t kTop = 0x47804780u;  // 7.5
-                        uint32_t probe = 0u;  // stays 0, or is NaN once something is not finite
+                        uint32_t probe = 0u;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             sc[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x5410);
-                            z[g][k] = hmul(__byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x7632), 0x38003800u);
-                            probe = hfma(hfma(sc[g][k], kTop, z[g][k]), 0u, probe);
+                            z[g][k] = __byte_perm(p[g][2 * k], p[g][2 * k + 1], 0x7632);
+                            probe = not_finite(hfma(sc[g][k], kTop, z[g][k]), probe);
                         }
-                        if (probe & 0x7fff7fffu) {
+                        if (any_nan(probe)) {
+                            past = true;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t top = hfma(sc[g][k], kTop, z[g][k]);
-#pragma unroll
-                                for (int i = 0; i < 2; ++i)
-                                    if ((top >> 16 * i & 0x7c00u) == 0x7c00u) {
-                                        sc[g][k] &= i ? 0xffffu : 0xffff0000u;
-                                        z[g][k] &= i ? 0xffffu : 0xffff0000u;
-                                        atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + 2 * k + i);
-                                    }
-                            }
+                            for (int k = 0; k < 8; ++k)
+                                if (any_nan(not_finite(p[g][k], 0u))) {
+                                    sc[g][k / 2] &= k & 1 ? 0xffffu : 0xffff0000u;
+                                    z[g][k / 2] &= k & 1 ? 0xffffu : 0xffff0000u;
+                                    atomicMin(&ctl.poison[g0 + g], j * kKeys + kc * 8 + k);
+                                }
                         }
                     }
                     const uint32_t dst = to + stage * S::kBytesV;
@@ -667,6 +682,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                             v[1][k] = value_high(both, sc[g][k], z[g][k]);
                             v[2][k] = value_low(y, sc[g][k], z[g][k]);
                             v[3][k] = value_high(y, sc[g][k], z[g][k]);
+                        }
+                        if (past) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e / 4][e % 4] = hold(v[e / 4][e % 4]);
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) sts4(dst + (4 * h + e) * 128, v[e][0], v[e][1], v[e][2], v[e][3]);

@@ -75,7 +75,8 @@ int32_t ecq_kv4_extend(const void *seq_lens, const void *new_lens, void *seq_len
  * free_pages in the order of requests and columns, their lengths set to 0. The
  * table's entries stay (a length of 0 makes them unused). All or nothing as
  * above, bad pages among those to be pushed included; ECQ_STATUS_NO_PAGES where
- * the stack (free_capacity) has no room. */
+ * the stack (free_capacity) has no room. What lies behind the stack's end may be
+ * overwritten in any case. */
 int32_t ecq_kv4_release(const void *done, const void *seq_lens, void *seq_lens_out, const void *block_table,
                         int64_t table_stride, int32_t max_pages, int32_t batch, int32_t page_size, void *free_pages,
                         int32_t free_capacity, const void *free_count, void *free_count_out, void *status,
@@ -109,9 +110,8 @@ int32_t ecq_kv4_gather(void *k, void *v, int32_t dtype, const void *pages, int64
  * number outside the pool, or a length below 0 or beyond the table's row, sets
  * ECQ_STATUS_BADARG and its keys are left out. The same status says that a
  * request had more than max_q queries and some of its rows were not written.
- * Requests with many rows take values of up to +-131008, twice fp16's end and more
- * than ecq_kv4_append stores: where a pool's bytes stand for more, queries that
- * see the token get infinities or NaN.
+ * For requests with many rows K and V are rounded to fp16, and values past its
+ * end (65520 to 65584 as ecq_kv4_append stores them) count as +-65504.
  * workspace:
  * ecq_kv4_attention_workspace_bytes, its content does not matter; calls that
  * may overlap need one each. */
