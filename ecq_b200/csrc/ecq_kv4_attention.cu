@@ -75,8 +75,9 @@ constexpr int kTileRows = 8;
 // below the largest (most of a long context) out of fp16's subnormals, whose
 // step of 2^-24 would be felt in sums of thousands of them. weight * scale
 // then overflows fp16 from a scale of 16: that is seen, and the unit's weights go
-// in times 2^-13 (at most 2^-1, so any finite scale's product is finite; what
-// fp16 loses of them there is 2^-25) and its part of o comes out times 2^13. The
+// in times 2^-15 (at most 2^-1 then, for a weight is up to 2^14 where the
+// reference's own step is 8: any finite scale's product is finite; what fp16
+// loses of them there is 2^-25) and its part of o comes out times 2^15. The
 // reference stays as it is: raised by less than a step of its own, it would not
 // be what the earlier sums are then multiplied for.
 constexpr float kSlack = 2.f, kLift = 10.f;
@@ -433,7 +434,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
         }
     }
     uint32_t ph[U][2], pl[U][2], hi[U][G][2], lo[U][G][2];
-    // the weights and their products with V's scales, those of kDown times 2^-13; the largest of them
+    // the weights and their products with V's scales, those of kDown times 2^-15; the largest of them
     auto weights = [&](auto down) {
         constexpr bool kDown = decltype(down)::value;
         uint32_t most = 0u;
@@ -460,7 +461,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
                 for (int g = 0; g < G; ++g) {
                     const uint32_t sc = __byte_perm(sa[i][g], sb[i][g], 0x5410);
                     // (weight * scale) in two parts: the product, and what its rounding lost (exact) with the weight's rest
-                    constexpr uint32_t kScale = 0x08000800u;  // 2^-13
+                    constexpr uint32_t kScale = 0x02000200u;  // 2^-15
                     const uint32_t w = kDown ? mul2(ph[u][i], kScale) : ph[u][i];
                     uint32_t h = mul2(w, sc), l = 0u;
                     if (kWeights != kOnce) l = fma2h(kDown ? mul2(pl[u][i], kScale) : pl[u][i], sc, fma2h(w, sc, neg2(h)));
@@ -480,7 +481,7 @@ __device__ __forceinline__ void blocks(State<D, G>& S, Rows<D, G>& R, const Lane
     uint64_t up = 0x3f8000003f800000ull;
     if (__any_sync(0xffffffffu, (most & 0xffffu) == 0x7c00u || most >> 16 == 0x7c00u)) {
         weights(std::true_type());
-        up = 0x4600000046000000ull;  // 2^13
+        up = 0x4700000047000000ull;  // 2^15
     }
     // rows of A: the groups' zeros, then ones (the sum of the weights)
     float sums[4];

@@ -295,3 +295,28 @@ def exactly(lens, new, heads, share, dim, g, page, dtype, room):
     for b in range(len(lens)):
         at = slice(starts[b], starts[b + 1])
         assert within(got[at], want[at], heads, dtype), (b, errors(got[at], want[at], heads), bounds(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("share", [1, 4, 9])
+def test_the_largest_scales_at_large_scores(dtype, share):
+    """Bytes that kv4_append never writes: scales near fp16's end, codes of 1, at
+    references whose step is 8, so that weights are up to 2^14."""
+    heads, n, dim, g = 2, 64, 64, 32
+    k = torch.full((n, heads, dim), 1024.0, device="cuda").to(dtype)
+    pages, table = store(k, randn(n, heads, dim, seed=1).to(dtype), 16, g)
+    blocks = pages.view(-1, heads, 16 * 64 + 256)
+    blocks[:, :, 512:1024] = 0x11                                                 # V codes
+    par = blocks[:, :, 1152:].contiguous().view(torch.float16).view(-1, heads, 16, 2, 2)
+    par[..., 0], par[..., 1] = 60000.0, -60000.0 + 32 * torch.arange(16, device="cuda")[:, None]
+    blocks[:, :, 1152:] = par.view(torch.uint8).view(-1, heads, 128)
+    value = torch.from_numpy(decode(pages, dim, g)[1][1]).cuda()
+    # scores whose products lie 3.4 and more above a multiple of 8: with the reference 10 below, rounded, weights are 2^13.4 to 2^14
+    for size in (5792.0, 6208.0, 7040.0, 8704.0, 10240.0):
+        q = torch.full((1, heads * share, dim), size, device="cuda").to(dtype)
+        got = ecq.kv4_attention(q, pages, table, i32([n]), group_size=g)
+        want = value.mean(0).repeat_interleave(share, 0)[None]
+        # a weight times a scale: rounded to fp16 once for bf16; else its rest too, of 2^-12 times 2^-15 2^13, to 2^-25: 2^-23 of
+        # the weight, and that product to 2^-11 of itself: under 2^-20 together, of 60000
+        tol = want.abs() * torch.finfo(dtype).eps / 2 + 60000 * (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -20)
+        assert bool(((got.double() - want).abs() <= tol).all()), (size, float((got.double() - want).abs().max()))
