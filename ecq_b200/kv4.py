@@ -165,8 +165,9 @@ def kv4_extend(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     themselves and share memory with nothing else. At most
     ``max_tokens`` new tokens: ``slots`` and ``positions`` have that length,
     filled with -1 behind the last, so a captured step keeps its shapes. All
-    or nothing: if pages, room or lengths do not suffice nothing changes, every
-    slot is -1 and ``status`` says so."""
+    or nothing: if pages, room or lengths do not suffice, or a page that a request
+    goes on in or would get has no slots in int32, nothing changes, every slot is
+    -1 and ``status`` says so."""
     _fits("max_tokens", max_tokens)
     _fits("page_size", page_size)
     device = _device(seq_lens, "new_lens block_table free_pages free_count seq_lens_out free_count_out status", new_lens,
@@ -199,7 +200,8 @@ def kv4_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.T
                 status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Push the pages of the requests where ``done`` (bool [batch]) on
     free_pages (in place) and set their lengths to 0. Returns the lengths and
-    the count of free pages, as new tensors or in the ``_out`` ones."""
+    the count of free pages, as new tensors or in the ``_out`` ones. All or
+    nothing, as ``kv4_extend``; what lies behind the stack's end may change."""
     _fits("page_size", page_size)
     device = _device(seq_lens, "done block_table free_pages free_count seq_lens_out free_count_out status", done,
                      block_table, free_pages, free_count, seq_lens_out, free_count_out, status)
@@ -294,7 +296,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     whose, at most max_q for one request; None: one each. They are the last of
     their request, each sees the tokens up to its own. scale: 1 / sqrt(head_dim)
     by default. Rows that see nothing (length 0) are 0; rows at or behind
-    q_starts[-1] are left as they were in ``out``."""
+    q_starts[-1] are left as they were in ``out``, whose rows must not share
+    memory."""
     if q.requires_grad and out is None and torch.is_grad_enabled():
         return _NoBackward.apply(q, lambda q: kv4_attention(
             q, pages, block_table, seq_lens, q_starts, max_q, group_size=group_size, scale=scale, status=status))
